@@ -390,11 +390,84 @@ int mmuon_butterfly_linear_fwd(const mmuon_butterfly_args* a, void* stream);
 int mmuon_butterfly_linear_bwd(const mmuon_butterfly_args* a, void* stream);
 size_t mmuon_butterfly_linear_workspace(const mmuon_butterfly_args* a);
 
+/* The two ends of a language model around its Monarch layers: the head with its
+   loss, and the token embedding.  Their (vocab, width) gradients are the AdamW
+   group's largest (lm_head.weight, transformer.wte.weight). */
+
+/* Softmax cross entropy of a linear head.  x (tokens, width) and w (vocab, width)
+   bf16, logits = x . w^T in fp32:
+     nll[t] = logsumexp(logits[t]) - logits[t][target[t]], 0 where target[t] ==
+     ignore_index, NaN where it is neither that nor in [0, vocab);
+     loss = sum of nll (MMUON_CE_SUM), divided by the number of targets that are
+     not ignored (MMUON_CE_MEAN; NaN if there is none).
+   Gradients (mmuon_ce_fwd_bwd): dx and dw of sum over t of g[t] nll[t], g = grad
+   where given, else that of loss (1 with MMUON_CE_NONE).
+   No logits are kept: the loss alone keeps two floats per token and 128 of the
+   vocabulary; the gradients take piece_tokens tokens at a time and keep 16 bits
+   per logit of the piece in the workspace. */
+enum { MMUON_CE_NONE = 0, MMUON_CE_MEAN = 1, MMUON_CE_SUM = 2 };
+typedef struct mmuon_ce_args {
+  int64_t tokens;         /* 0 <= tokens < 2^24 */
+  int64_t vocab;          /* 1 <= vocab < 2^22, any number */
+  int32_t width;          /* a positive multiple of 8 */
+  int32_t dtype;          /* MMUON_BF16 */
+  int32_t reduction;      /* MMUON_CE_* */
+  int32_t reserved;       /* 0 */
+  int64_t ignore_index;
+  int64_t x_stride;       /* elements from one row to the next, a multiple of 8 */
+  int64_t w_stride;
+  int64_t piece_tokens;   /* >= 1 */
+  const void* x;          /* rows 16-B aligned */
+  const void* w;
+  const int64_t* target;  /* (tokens) */
+  const float* grad;      /* (tokens) or null */
+  float* nll;             /* out (tokens), or null */
+  float* loss;            /* out (1); null with MMUON_CE_NONE */
+  void* dx;               /* out (tokens, width), contiguous; or null */
+  void* dw;               /* out (vocab, width), contiguous; or null */
+  void* workspace;        /* mmuon_ce_workspace() bytes, 256-B aligned */
+  size_t workspace_bytes;
+} mmuon_ce_args;
+int mmuon_ce_fwd(const mmuon_ce_args* a, void* stream);
+int mmuon_ce_fwd_bwd(const mmuon_ce_args* a, void* stream);
+/* Workspace bytes of a call with these sizes and this piece (train: of mmuon_ce_fwd_bwd;
+   nll null counts it in). */
+size_t mmuon_ce_workspace(const mmuon_ce_args* a, int32_t train);
+/* x *= *factor (device), bf16, numel a multiple of 8; writes nothing where *factor == 1. */
+int mmuon_scale_bf16(void* x, int64_t numel, const float* factor, void* stream);
+
+/* Token embedding: out[t] = scale * w[index[t]] (fp32 product, one rounding), NaN where
+   index[t] is not in [0, vocab).  Gradient of the table: dw[v] = scale * sum of dout[t]
+   over the t with index[t] == v (fp32 sums in a fixed order, one rounding), every row
+   written, zeros where no token has it; ids outside [0, vocab) and padding_idx take
+   no gradient (padding_idx < 0: none). */
+typedef struct mmuon_embedding_args {
+  int64_t tokens;         /* 0 <= tokens < 2^31 */
+  int64_t vocab;          /* 1 <= vocab < 2^31 */
+  int32_t width;          /* any positive number */
+  int32_t dtype;          /* MMUON_BF16 or MMUON_F32: w, out, dout, dw */
+  float scale;
+  int32_t reserved;       /* 0 */
+  int64_t padding_idx;
+  int64_t w_stride;       /* elements from one row to the next */
+  int64_t dout_stride;
+  const int64_t* index;   /* (tokens) */
+  const void* w;          /* forward in (vocab, width) */
+  void* out;              /* forward out (tokens, width), contiguous */
+  const void* dout;       /* backward in (tokens, width) */
+  void* dw;               /* backward out (vocab, width), contiguous */
+  void* workspace;        /* backward: mmuon_embedding_workspace() bytes, 256-B aligned */
+  size_t workspace_bytes;
+} mmuon_embedding_args;
+int mmuon_embedding_fwd(const mmuon_embedding_args* a, void* stream);
+int mmuon_embedding_bwd(const mmuon_embedding_args* a, void* stream);
+size_t mmuon_embedding_workspace(const mmuon_embedding_args* a);
+
 /* Thread-local message of the last failing call ("" if none). */
 const char* mmuon_last_error(void);
 
 /* ABI version: bumped on any change to this header. */
-#define MMUON_ABI_VERSION 8
+#define MMUON_ABI_VERSION 9
 int mmuon_abi_version(void);
 
 #ifdef __cplusplus

@@ -12,7 +12,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(os.environ.get("MMUON_LIB", Path(__file__).resolve().parent / "libmmuon.so"))
-ABI_VERSION = 8
+ABI_VERSION = 9
 # the layer's torch operator; the name carries the ABI, so that one built for another is never loaded (once loaded,
 # its registrations stay for the life of the process)
 TORCH_LIB_PATH = Path(__file__).resolve().parent / f"libmmuon_torch.{ABI_VERSION}.so"
@@ -26,6 +26,8 @@ NS_HOLD_LAST = 4
 NSOP_SYRK, NSOP_POLY, NSOP_PX, NSOP_PX_APPLY, NSOP_SYMM = 0, 1, 2, 3, 4
 NSB_X0, NSB_X1, NSB_A, NSB_P, NSB_X0_S0, NSB_X0_S1, NSB_X1_S0, NSB_X1_S1, NSB_PARAM = range(9)
 NOALLOC_SCRATCH_FLOATS = 1 << 20
+# cross entropy reductions (MMUON_CE_*)
+CE_NONE, CE_MEAN, CE_SUM = 0, 1, 2
 
 _DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float8_e4m3fn: F8E4M3, torch.float8_e5m2: F8E5M2}
 FP8_DTYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
@@ -106,6 +108,23 @@ class ButterflyArgs(C.Structure):
                 ("dw2", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class CeArgs(C.Structure):
+    _fields_ = [("tokens", C.c_int64), ("vocab", C.c_int64), ("width", C.c_int32), ("dtype", C.c_int32),
+                ("reduction", C.c_int32), ("reserved", C.c_int32), ("ignore_index", C.c_int64),
+                ("x_stride", C.c_int64), ("w_stride", C.c_int64), ("piece_tokens", C.c_int64),
+                ("x", C.c_void_p), ("w", C.c_void_p), ("target", C.c_void_p), ("grad", C.c_void_p),
+                ("nll", C.c_void_p), ("loss", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class EmbeddingArgs(C.Structure):
+    _fields_ = [("tokens", C.c_int64), ("vocab", C.c_int64), ("width", C.c_int32), ("dtype", C.c_int32),
+                ("scale", C.c_float), ("reserved", C.c_int32), ("padding_idx", C.c_int64), ("w_stride", C.c_int64),
+                ("dout_stride", C.c_int64), ("index", C.c_void_p), ("w", C.c_void_p), ("out", C.c_void_p),
+                ("dout", C.c_void_p), ("dw", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "mmuon_abi_version": (C.c_int, []),
@@ -136,6 +155,13 @@ SIGNATURES = {
     "mmuon_butterfly_linear_fwd": (C.c_int, [C.POINTER(ButterflyArgs), C.c_void_p]),
     "mmuon_butterfly_linear_bwd": (C.c_int, [C.POINTER(ButterflyArgs), C.c_void_p]),
     "mmuon_butterfly_linear_workspace": (C.c_size_t, [C.POINTER(ButterflyArgs)]),
+    "mmuon_ce_fwd": (C.c_int, [C.POINTER(CeArgs), C.c_void_p]),
+    "mmuon_ce_fwd_bwd": (C.c_int, [C.POINTER(CeArgs), C.c_void_p]),
+    "mmuon_ce_workspace": (C.c_size_t, [C.POINTER(CeArgs), C.c_int32]),
+    "mmuon_embedding_fwd": (C.c_int, [C.POINTER(EmbeddingArgs), C.c_void_p]),
+    "mmuon_embedding_bwd": (C.c_int, [C.POINTER(EmbeddingArgs), C.c_void_p]),
+    "mmuon_embedding_workspace": (C.c_size_t, [C.POINTER(EmbeddingArgs)]),
+    "mmuon_scale_bf16": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
 }
 
 _lib = None

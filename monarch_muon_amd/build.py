@@ -2,7 +2,7 @@
 
 ``python -m monarch_muon_amd.build`` compiles every ``csrc/*.hip`` to an object
 in parallel and links the shared library next to this file, and beside it
-``libmmuon_torch.<ABI>.so``, the layer's native torch operator (``csrc/torch_ops.cpp``,
+``libmmuon_torch.<ABI>.so``, the native torch operators (``csrc/torch_*.cpp``,
 host code only).  hipcc cross-compiles for gfx950 without a GPU.  ``build_probe()`` builds the
 bench-only HBM streaming probe (``bench_probe.hip`` beside ``bench.py``) into a
 library of its own, apart from the optimizer's.
@@ -58,11 +58,11 @@ def _build_torch_ops() -> None:
     cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1",
            "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-isystem", str(inc / "include"), "-isystem", str(inc / "include/torch/csrc/api/include"),
-           "-isystem", str(rocm / "include"), "-isystem", "/opt/rocm/include", str(CSRC / "torch_ops.cpp"),
+           "-isystem", str(rocm / "include"), "-isystem", "/opt/rocm/include", *map(str, sorted(CSRC.glob("*.cpp"))),
            "-o", str(tmp), f"-L{inc / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"torch_ops.cpp failed:\n{r.stdout}{r.stderr}")
+        raise RuntimeError(f"the torch operators failed:\n{r.stdout}{r.stderr}")
     os.replace(tmp, TORCH_LIB)
     for old in HERE.glob("libmmuon_torch*.so"):   # built for another ABI: never loaded again
         if old != TORCH_LIB:

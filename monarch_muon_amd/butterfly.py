@@ -132,16 +132,19 @@ butterfly_blk_op.register_autograd(_backward, setup_context=_setup_context)
 # operator's first launch (_bind), so a process may build it, or name another, after the import.
 _BOUND = ("mmuon_butterfly_linear_fwd", "mmuon_butterfly_linear_bwd", "mmuon_butterfly_linear_workspace",
           "mmuon_last_error")
+_BOUND_LM = ("mmuon_ce_fwd", "mmuon_ce_fwd_bwd", "mmuon_ce_workspace", "mmuon_scale_bf16", "mmuon_embedding_fwd",
+             "mmuon_embedding_bwd", "mmuon_embedding_workspace")
 _linear_op = _torch_lib = None
 
 
 @C.CFUNCTYPE(C.c_int)
 def _bind() -> int:
-    """Give the operator the functions of the library that ``_abi`` loads (called by the operator, any thread)."""
+    """Give the operators the functions of the library that ``_abi`` loads (called by an operator, any thread)."""
     try:
         lib = _abi.lib()
-        return _torch_lib.mmuon_torch_bind(lib.mmuon_abi_version(),
-                                           *(C.cast(getattr(lib, name), C.c_void_p) for name in _BOUND))
+        version = lib.mmuon_abi_version()
+        lm, blk = ([C.cast(getattr(lib, name), C.c_void_p) for name in names] for names in (_BOUND_LM, _BOUND))
+        return _torch_lib.mmuon_torch_bind_lm(version, *lm) or _torch_lib.mmuon_torch_bind(version, *blk)
     except Exception as e:
         _torch_lib.mmuon_torch_refuse(str(e).encode())
         return -1

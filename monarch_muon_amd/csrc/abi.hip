@@ -620,3 +620,116 @@ int mmuon_butterfly_bwd(const mmuon_butterfly_args* a, void* stream) {
 }
 
 }  // extern "C"
+
+namespace {
+
+int check_ce(const mmuon_ce_args* a, bool train) {
+  if (a == nullptr) return fail(MMUON_EINVAL, "null cross entropy arguments");
+  if (a->dtype != MMUON_BF16) return fail(MMUON_EINVAL, "cross entropy: dtype must be MMUON_BF16 (got %d)", a->dtype);
+  if (a->tokens < 0 || a->tokens >= (int64_t(1) << 24))
+    return fail(MMUON_ERANGE, "cross entropy: tokens must be in [0, 2^24) (got %lld)", (long long)a->tokens);
+  if (a->vocab < 1 || a->vocab >= (int64_t(1) << 22))
+    return fail(MMUON_ERANGE, "cross entropy: vocab must be in [1, 2^22) (got %lld)", (long long)a->vocab);
+  if (a->width <= 0 || a->width % 8)
+    return fail(MMUON_EINVAL, "cross entropy: width must be a positive multiple of 8 (got %d)", a->width);
+  if (a->reduction < MMUON_CE_NONE || a->reduction > MMUON_CE_SUM)
+    return fail(MMUON_EINVAL, "cross entropy: unknown reduction %d", a->reduction);
+  if (a->piece_tokens < 1) return fail(MMUON_EINVAL, "cross entropy: piece_tokens must be positive");
+  for (const int64_t stride : {a->x_stride, a->w_stride}) {
+    if (stride < 0 || stride % 8)
+      return fail(MMUON_EINVAL, "cross entropy: row strides must be multiples of 8 elements (got %lld)", (long long)stride);
+    // per-lane offsets of a tile (256 rows) stay below 2^31
+    if (stride >= (int64_t(1) << 22) || a->width >= (1 << 22))
+      return fail(MMUON_ERANGE, "cross entropy: rows beyond the kernels' 32-bit tile offsets");
+  }
+  const auto bad = [&](const void* p, bool per_token) { return (p == nullptr && !(per_token && a->tokens == 0)) || !aligned16(p); };
+  if (bad(a->x, true) || bad(a->w, false)) return fail(MMUON_EINVAL, "cross entropy: null or unaligned x or w");
+  if (a->target == nullptr && a->tokens > 0) return fail(MMUON_EINVAL, "cross entropy: null target");
+  if (a->reduction == MMUON_CE_NONE ? a->nll == nullptr && a->tokens > 0 : a->loss == nullptr)
+    return fail(MMUON_EINVAL, "cross entropy: nowhere to write the loss");
+  if (train && (!aligned16(a->dx) || !aligned16(a->dw))) return fail(MMUON_EINVAL, "cross entropy: unaligned dx or dw");
+  if (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 255) != 0)
+    return fail(MMUON_EINVAL, "cross entropy: workspace must be 256-B aligned");
+  const size_t need = mmuon::ce_workspace(*a, train);
+  if (a->workspace_bytes < need)
+    return fail(MMUON_EINVAL, "cross entropy: workspace of %zu bytes, %zu needed", a->workspace_bytes, need);
+  return MMUON_OK;
+}
+
+int check_embedding(const mmuon_embedding_args* a, bool bwd) {
+  if (a == nullptr) return fail(MMUON_EINVAL, "null embedding arguments");
+  if (a->dtype != MMUON_BF16 && a->dtype != MMUON_F32)
+    return fail(MMUON_EINVAL, "embedding: dtype must be MMUON_BF16 or MMUON_F32 (got %d)", a->dtype);
+  const int64_t most = int64_t(1) << 31;
+  if (a->tokens < 0 || a->tokens >= most || a->vocab < 1 || a->vocab >= most)
+    return fail(MMUON_ERANGE, "embedding: tokens (%lld) and vocab (%lld) must be below 2^31", (long long)a->tokens,
+                (long long)a->vocab);
+  if (a->width <= 0) return fail(MMUON_EINVAL, "embedding: width must be positive (got %d)", a->width);
+  if ((bwd ? a->dout_stride : a->w_stride) < 0) return fail(MMUON_EINVAL, "embedding: negative row stride");
+  const uintptr_t mask = uintptr_t(dtype_size(a->dtype)) - 1;
+  const auto bad = [&](const void* p, bool per_token) {
+    return (p == nullptr && !(per_token && a->tokens == 0)) || (reinterpret_cast<uintptr_t>(p) & mask) != 0;
+  };
+  if (a->index == nullptr && a->tokens > 0) return fail(MMUON_EINVAL, "embedding: null index");
+  if (!bwd) {
+    if (bad(a->w, false) || bad(a->out, true)) return fail(MMUON_EINVAL, "embedding: null or unaligned w or out");
+    return MMUON_OK;
+  }
+  if (bad(a->dout, true) || bad(a->dw, false)) return fail(MMUON_EINVAL, "embedding: null or unaligned dout or dw");
+  if (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 255) != 0)
+    return fail(MMUON_EINVAL, "embedding: workspace must be 256-B aligned");
+  if (a->workspace_bytes < mmuon::embedding_workspace(*a))
+    return fail(MMUON_EINVAL, "embedding: workspace of %zu bytes, %zu needed", a->workspace_bytes,
+                mmuon::embedding_workspace(*a));
+  return MMUON_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mmuon_ce_workspace(const mmuon_ce_args* a, int32_t train) {
+  if (a == nullptr || a->tokens < 0 || a->tokens >= (int64_t(1) << 24) || a->vocab < 1 ||
+      a->vocab >= (int64_t(1) << 22) || a->width <= 0 || a->piece_tokens < 1)
+    return 0;
+  return mmuon::ce_workspace(*a, train != 0);
+}
+
+int mmuon_ce_fwd(const mmuon_ce_args* a, void* stream) {
+  if (int rc = check_ce(a, false)) return rc;
+  mmuon::launch_ce(*a, false, static_cast<hipStream_t>(stream));
+  return check_launch("cross entropy forward");
+}
+
+int mmuon_ce_fwd_bwd(const mmuon_ce_args* a, void* stream) {
+  if (int rc = check_ce(a, true)) return rc;
+  mmuon::launch_ce(*a, true, static_cast<hipStream_t>(stream));
+  return check_launch("cross entropy forward and backward");
+}
+
+int mmuon_scale_bf16(void* x, int64_t numel, const float* factor, void* stream) {
+  if (numel < 0 || numel % 8) return fail(MMUON_EINVAL, "scale: numel must be a multiple of 8 (got %lld)", (long long)numel);
+  if (numel == 0) return MMUON_OK;
+  if (x == nullptr || !aligned16(x) || factor == nullptr) return fail(MMUON_EINVAL, "scale: null or unaligned pointer");
+  mmuon::launch_ce_scale(x, numel, factor, static_cast<hipStream_t>(stream));
+  return check_launch("scale");
+}
+
+size_t mmuon_embedding_workspace(const mmuon_embedding_args* a) {
+  if (a == nullptr || a->tokens < 0 || a->tokens >= (int64_t(1) << 31)) return 0;
+  return mmuon::embedding_workspace(*a);
+}
+
+int mmuon_embedding_fwd(const mmuon_embedding_args* a, void* stream) {
+  if (int rc = check_embedding(a, false)) return rc;
+  mmuon::launch_embedding_fwd(*a, static_cast<hipStream_t>(stream));
+  return check_launch("embedding forward");
+}
+
+int mmuon_embedding_bwd(const mmuon_embedding_args* a, void* stream) {
+  if (int rc = check_embedding(a, true)) return rc;
+  mmuon::launch_embedding_bwd(*a, static_cast<hipStream_t>(stream));
+  return check_launch("embedding backward");
+}
+
+}  // extern "C"

@@ -91,6 +91,16 @@ size_t butterfly_linear_workspace(const mmuon_butterfly_args& a);
 int launch_butterfly_fwd(const mmuon_butterfly_args& a, bool features, hipStream_t s);
 int launch_butterfly_bwd(const mmuon_butterfly_args& a, bool features, hipStream_t s);
 
+// Cross entropy of a linear head ---------------------------------------------------
+size_t ce_workspace(const mmuon_ce_args& a, bool train);
+int launch_ce(const mmuon_ce_args& a, bool train, hipStream_t s);
+int launch_ce_scale(void* x, int64_t numel, const float* factor, hipStream_t s);
+
+// Token embedding ------------------------------------------------------------------
+size_t embedding_workspace(const mmuon_embedding_args& a);
+int launch_embedding_fwd(const mmuon_embedding_args& a, hipStream_t s);
+int launch_embedding_bwd(const mmuon_embedding_args& a, hipStream_t s);
+
 // Gradient-clipping coefficient of a launch (gscale: device pointer, or null
 // when not clipping), read once per thread: the per-element form would test
 // the pointer in every element (a branch each) and, after the thread's first

@@ -10,35 +10,22 @@
 // The library's functions are bound at the first launch (loader, mmuon_torch_bind) to the
 // ones that monarch_muon_amd/_abi.py loads, so MMUON_LIB selects them here too; a library of
 // another ABI than this file was compiled with is refused.
-#include <ATen/ATen.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/library.h>
+#include "torch_common.hpp"
 
 #include <algorithm>
-#include <atomic>
 #include <mutex>
 #include <string>
 #include <tuple>
 
-#include "../../include/mmuon.h"
+namespace mmuon_torch {
+
+Abi abi;
+std::atomic<bool> bound{false};
 
 namespace {
-
-using at::Tensor;
-using Pair = std::tuple<Tensor, Tensor>;
-using Triple = std::tuple<Tensor, Tensor, Tensor>;
-
-struct Abi {
-  int (*fwd)(const mmuon_butterfly_args*, void*) = nullptr;
-  int (*bwd)(const mmuon_butterfly_args*, void*) = nullptr;
-  size_t (*workspace)(const mmuon_butterfly_args*) = nullptr;
-  const char* (*last_error)() = nullptr;
-} abi;
-std::atomic<bool> bound{false};
 int (*loader)() = nullptr;         // loads the library and binds it; 0 where it did
 thread_local std::string refusal;  // why it did not
+}  // namespace
 
 void bind_library() {
   if (bound.load(std::memory_order_acquire)) return;
@@ -46,13 +33,19 @@ void bind_library() {
   TORCH_CHECK(loader != nullptr && loader() == 0, refusal);
 }
 
-void check_rc(int rc, const char* what) {
-  TORCH_CHECK(rc == 0, what, " failed (code ", rc, "): ", abi.last_error());
+Tensor dense_aligned(const Tensor& t) {
+  const Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 == 0 ? c : c.clone();
 }
 
-void require_cuda(const Tensor& t) {
-  TORCH_CHECK(t.is_cuda(), "libmmuon kernels need tensors on a ROCm GPU (no CPU path)");
-}
+}  // namespace mmuon_torch
+
+using namespace mmuon_torch;
+
+namespace {
+
+using Pair = std::tuple<Tensor, Tensor>;
+using Triple = std::tuple<Tensor, Tensor, Tensor>;
 
 mmuon_butterfly_args make_args(const Tensor& x2, const Tensor& w1, const Tensor& w2) {
   for (const Tensor* t : {&x2, &w1, &w2}) require_cuda(*t);
@@ -83,15 +76,6 @@ mmuon_butterfly_args make_args(const Tensor& x2, const Tensor& w1, const Tensor&
   a.w2 = w2.data_ptr();
   return a;
 }
-
-// The kernels read rows of 16-B chunks.  A gradient may be a contiguous view at any element
-// (one of the parts that torch.cat's backward hands out): such a one is copied.
-Tensor dense_aligned(const Tensor& t) {
-  const Tensor c = t.contiguous();
-  return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 == 0 ? c : c.clone();
-}
-
-void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
 Pair linear_impl(const Tensor& x, const Tensor& w1_, const Tensor& w2_) {
   const Tensor x2 = x.contiguous(), w1 = w1_.contiguous(), w2 = w2_.contiguous();
@@ -182,10 +166,6 @@ struct LinearBwdFn : torch::autograd::Function<LinearBwdFn> {
   }
 };
 
-bool any_requires_grad(std::initializer_list<const Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return false;
-  return std::any_of(ts.begin(), ts.end(), [](const Tensor* t) { return t->requires_grad(); });
-}
 Pair linear_autograd(const Tensor& x2, const Tensor& w1, const Tensor& w2) {
   if (any_requires_grad({&x2, &w1, &w2})) {
     const variable_list r = LinearFn::apply(x2, w1, w2);
@@ -222,6 +202,21 @@ TORCH_LIBRARY_IMPL(mmuon, Autograd, m) {
 }
 
 extern "C" {
+
+// The functions of the language-model operators (torch_lm.cpp), given before mmuon_torch_bind
+// declares the library bound.
+int mmuon_torch_bind_lm(int version, void* ce_fwd, void* ce_fwd_bwd, void* ce_workspace, void* scale, void* emb_fwd,
+                        void* emb_bwd, void* emb_workspace) {
+  if (version != MMUON_ABI_VERSION || bound) return 0;  // mmuon_torch_bind says so
+  abi.ce_fwd = reinterpret_cast<decltype(abi.ce_fwd)>(ce_fwd);
+  abi.ce_fwd_bwd = reinterpret_cast<decltype(abi.ce_fwd_bwd)>(ce_fwd_bwd);
+  abi.ce_workspace = reinterpret_cast<decltype(abi.ce_workspace)>(ce_workspace);
+  abi.scale = reinterpret_cast<decltype(abi.scale)>(scale);
+  abi.emb_fwd = reinterpret_cast<decltype(abi.emb_fwd)>(emb_fwd);
+  abi.emb_bwd = reinterpret_cast<decltype(abi.emb_bwd)>(emb_bwd);
+  abi.emb_workspace = reinterpret_cast<decltype(abi.emb_workspace)>(emb_workspace);
+  return 0;
+}
 
 void mmuon_torch_set_loader(int (*fn)()) { loader = fn; }
 

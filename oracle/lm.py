@@ -1,0 +1,69 @@
+"""Plain float64 forms of the language-model ends (test infrastructure): the head's cross entropy with its gradients
+and the embedding with its gradient, and how far a kernel that computes them with the stated roundings may be off.
+
+Roundings of ``linear_cross_entropy``: bf16 products summed in fp32 (unit roundoff 2^-24 per step), p from a 16-bit
+code (relative 2^-11 ln 2 at most, zero below 2^-64 of a part's maximum), dl and the results rounded to bf16 (2^-8)."""
+from __future__ import annotations
+
+import torch
+
+U32, UBF = 2.0 ** -24, 2.0 ** -8
+UCODE = 2.0 ** -11 * 0.6932
+
+
+def cross_entropy(x, w, target, ignore_index=-100, reduction="mean", grad=None):
+    """(loss, dx, dw, bounds): float64 on the CPU; ``bounds`` = (of loss, dx, dw) elementwise."""
+    x, w = x.double().cpu(), w.double().cpu()
+    target = target.cpu().long()
+    T, D = x.shape
+    V = w.shape[0]
+    keep = target != ignore_index
+    xk, yk = x[keep], target[keep]
+    n = len(yk)
+    l = xk @ w.T
+    lse = torch.logsumexp(l, 1)
+    nll = torch.zeros(T, dtype=torch.float64)
+    ly = l.gather(1, yk[:, None])[:, 0]
+    nll[keep] = lse - ly
+    # a logit: D fp32 roundings of partial sums no larger than sum |x w|; log2 e, its power, the sum over V in
+    # parts, the logarithm
+    size = (xk.abs() @ w.abs().T).amax(1) if n else torch.zeros(0, dtype=torch.float64)
+    err = U32 * (2 * (D + 4) * size + 4 * lse.abs() + V ** 0.5 + 40)
+    tol = torch.zeros(T, dtype=torch.float64)
+    tol[keep] = err
+    if grad is not None:
+        g = grad.double().cpu()[keep]
+    elif reduction == "mean":
+        g = torch.full((n,), 1.0 / n if n else 0.0, dtype=torch.float64)
+    else:
+        g = torch.ones(n, dtype=torch.float64)
+    p = (l - lse[:, None]).exp()
+    dl = p.clone()
+    dl[torch.arange(n), yk] -= 1
+    dl = dl * g[:, None]
+    # p: its logit and lse, its code, bf16; the target's entry p - 1 has the error of p by nll
+    rel = UCODE + UBF + 2 * err[:, None] + 2.0 ** -18
+    off = dl.abs() * rel + (p * g.abs()[:, None]) * (2 * err[:, None] + 4 * U32) + g.abs()[:, None] * 1e-19
+    dx, dxt = torch.zeros_like(x), torch.zeros_like(x)
+    dx[keep] = dl @ w
+    dxt[keep] = off @ w.abs() + 2 * V * U32 * (dl.abs() @ w.abs())
+    dw = dl.T @ xk
+    dwt = off.T @ xk.abs() + 2 * (n + 1) * U32 * (dl.abs().T @ xk.abs())
+    loss, lt = {"none": (nll, tol),
+                "sum": (nll.sum(), tol.sum() + 2 * (T + 20) * U32 * nll.abs().sum()),
+                "mean": (nll.sum() / n if n else nll.sum() * float("nan"),
+                         (tol.sum() + 2 * (T + 20) * U32 * nll.abs().sum()) / max(n, 1))}[reduction]
+    return loss, dx, dw, (lt, dxt + 1.01 * UBF * dx.abs() + 1e-37, dwt + 1.01 * UBF * dw.abs() + 1e-37)
+
+
+def embedding_grad(dout, index, vocab, scale=1.0, padding_idx=None):
+    """(dw, bound of an fp32 sum in any order before the last rounding), float64 on the CPU."""
+    dout, index = dout.double().cpu().reshape(index.numel(), -1), index.cpu().long().reshape(-1)
+    keep = (index >= 0) & (index < vocab)
+    if padding_idx is not None:
+        keep &= index != padding_idx
+    dw = torch.zeros(vocab, dout.shape[1], dtype=torch.float64)
+    dw.index_add_(0, index[keep], dout[keep])
+    size = torch.zeros_like(dw).index_add_(0, index[keep], dout[keep].abs())
+    count = torch.bincount(index[keep], minlength=vocab).double()
+    return dw * scale, (count + 2)[:, None] * U32 * size * abs(scale)
