@@ -442,8 +442,8 @@ int mmuon_scale_bf16(void* x, int64_t numel, const float* factor, void* stream);
    written, zeros where no token has it; ids outside [0, vocab) and padding_idx take
    no gradient (padding_idx < 0: none). */
 typedef struct mmuon_embedding_args {
-  int64_t tokens;         /* 0 <= tokens < 2^31 */
-  int64_t vocab;          /* 1 <= vocab < 2^31 */
+  int64_t tokens;         /* 0 <= tokens < 2^26 */
+  int64_t vocab;          /* 1 <= vocab < 2^24 */
   int32_t width;          /* any positive number */
   int32_t dtype;          /* MMUON_BF16 or MMUON_F32: w, out, dout, dw */
   float scale;

@@ -660,10 +660,9 @@ int check_embedding(const mmuon_embedding_args* a, bool bwd) {
   if (a == nullptr) return fail(MMUON_EINVAL, "null embedding arguments");
   if (a->dtype != MMUON_BF16 && a->dtype != MMUON_F32)
     return fail(MMUON_EINVAL, "embedding: dtype must be MMUON_BF16 or MMUON_F32 (got %d)", a->dtype);
-  const int64_t most = int64_t(1) << 31;
-  if (a->tokens < 0 || a->tokens >= most || a->vocab < 1 || a->vocab >= most)
-    return fail(MMUON_ERANGE, "embedding: tokens (%lld) and vocab (%lld) must be below 2^31", (long long)a->tokens,
-                (long long)a->vocab);
+  if (a->tokens < 0 || a->tokens >= (int64_t(1) << 26) || a->vocab < 1 || a->vocab >= (int64_t(1) << 24))
+    return fail(MMUON_ERANGE, "embedding: tokens (%lld) must be below 2^26 and vocab (%lld) in [1, 2^24)",
+                (long long)a->tokens, (long long)a->vocab);
   if (a->width <= 0) return fail(MMUON_EINVAL, "embedding: width must be positive (got %d)", a->width);
   if ((bwd ? a->dout_stride : a->w_stride) < 0) return fail(MMUON_EINVAL, "embedding: negative row stride");
   const uintptr_t mask = uintptr_t(dtype_size(a->dtype)) - 1;
@@ -716,7 +715,9 @@ int mmuon_scale_bf16(void* x, int64_t numel, const float* factor, void* stream) 
 }
 
 size_t mmuon_embedding_workspace(const mmuon_embedding_args* a) {
-  if (a == nullptr || a->tokens < 0 || a->tokens >= (int64_t(1) << 31)) return 0;
+  if (a == nullptr || a->tokens < 0 || a->tokens >= (int64_t(1) << 26) || a->vocab < 1 ||
+      a->vocab >= (int64_t(1) << 24) || a->width <= 0)
+    return 0;
   return mmuon::embedding_workspace(*a);
 }
 

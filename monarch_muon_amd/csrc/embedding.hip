@@ -2,12 +2,14 @@
 //
 //   out[t] = scale w[i_t]            dw[v] = scale sum over t with i_t = v of dout[t]
 //
-// The gradient is dense, one launch, and does not depend on timing: rows are dealt to
-// classes (row v to class v % C), one workgroup each.  A workgroup reads all ids, places
-// the positions of its rows in token order (counts per row and wave, then a stable rank),
-// and writes its rows: zeros, or the fp32 sum of the row's gradients in token order,
-// rounded once.  Common words have neighbouring ids, so the rows of a class are far apart.
+// The gradient is dense and does not depend on timing: rows are dealt to classes (row v to
+// class v % C), one workgroup each.  A workgroup reads all ids, places the positions of its
+// rows in token order (counts per row and wave, then a stable rank), and writes zeros to the
+// rows that no token has.  Common words have neighbouring ids, so the rows of a class are far
+// apart.  A second launch sums the positions in fp32, SEG to a wave whatever rows they are
+// of; a third joins the pieces of rows that lie in several SEGs, in order.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 #include "kernels.hpp"
@@ -46,92 +48,226 @@ __global__ __launch_bounds__(256) void embed_lookup(mmuon_embedding_args a, int 
   }
 }
 
-constexpr int GT = 1024, GW = GT / 64;  // threads and waves of a gradient workgroup
-constexpr int MAX_ROWS = 1024;          // rows of a class
+constexpr int SEG = 32;  // positions that one wave sums
 
-template <class T, int N>
-__global__ __launch_bounds__(GT) void embed_grad(mmuon_embedding_args a, int log2c, int* order) {
-  __shared__ int at[GW][MAX_ROWS];     // counts, then the next place, of a row's positions in a wave's tokens
-  __shared__ int first[MAX_ROWS + 1];  // the row's first place
-  __shared__ int below[GW], wsum[GW];
+// The positions that have a gradient, class after class, row after row, in token order: the
+// token and the row of each, at a row's first one how many it has, and how many there are.
+struct GradSpace {
+  int* token;
+  int* row;
+  int* count;
+  int* all;
+  float* sums;  // of the pieces of rows that lie in several SEGs: two for each SEG
+};
+
+// WAVES waves, ROWS rows of a class at most, LIST ids of a class that a wave keeps from its scan
+template <class T, int N, int WAVES, int ROWS, int LIST>
+__global__ __launch_bounds__(64 * WAVES) void embed_rows(mmuon_embedding_args a, int log2c, GradSpace space) {
+  constexpr int NTH = 64 * WAVES;
+  static_assert(ROWS % NTH == 0 || NTH % ROWS == 0, "rows are scanned by whole workgroups");
+  __shared__ int at[WAVES][ROWS];     // counts, then the next place, of a row's positions in a wave's tokens
+  __shared__ int first[ROWS + 1];     // the row's first place
+  __shared__ uint32_t kept[WAVES][LIST];  // ids of the class: row << 22 | token of the run
+  __shared__ int below[WAVES], wsum[WAVES];
   const int c = blockIdx.x, C = 1 << log2c;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rows = int((a.vocab - c + C - 1) >> log2c);
-  for (int i = threadIdx.x; i < GW * MAX_ROWS; i += GT) (&at[0][0])[i] = 0;
+  const uint64_t before = (uint64_t(1) << lane) - 1;
+  for (int i = threadIdx.x; i < WAVES * rows; i += NTH) at[i / rows][i % rows] = 0;
   __syncthreads();
   // a wave's tokens: a run of whole 64s
-  const int64_t run = (a.tokens + 64 * GW - 1) / (64 * GW) * 64, t0 = wave * run, t1 = min(a.tokens, t0 + run);
-  const auto row_of = [&](int64_t t, int& less) {  // the token's row of this class, or -1
-    const int64_t v = t < t1 ? a.index[t] : -1;
+  const int64_t run = (a.tokens + NTH - 1) / NTH * 64, t0 = wave * run, t1 = min(a.tokens, t0 + run);
+  int less = 0, found = 0;
+  const auto row_of = [&](int64_t v) {  // the id's row of this class, or -1
     if (v < 0 || v >= a.vocab || v == a.padding_idx) return -1;
     less += int(v & (C - 1)) < c;
     return int(v & (C - 1)) == c ? int(v >> log2c) : -1;
   };
-  int less = 0;
-#pragma unroll 4
-  for (int64_t t = t0 + lane; t < t1; t += 64) {
-    const int r = row_of(t, less);
-    if (r >= 0) atomicAdd(&at[wave][r], 1);
+  constexpr int U = 8;
+  for (int64_t t = t0; t < t1; t += 64 * U) {
+    int64_t v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = t + u * 64 + lane < t1 ? a.index[t + u * 64 + lane] : -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = row_of(v[u]);
+      const uint64_t hit = __ballot(r >= 0);
+      if (r >= 0) {
+        atomicAdd(&at[wave][r], 1);
+        const int j = found + __popcll(hit & before);
+        if (j < LIST) kept[wave][j] = uint32_t(r) << 22 | uint32_t(t - t0 + u * 64 + lane);
+      }
+      found += __popcll(hit);
+    }
   }
   less = wave_isum(less);
   if (lane == 0) below[wave] = less;
   __syncthreads();
   // places: class after class, row after row, wave after wave
-  int n = 0;
-  if (threadIdx.x < rows)
-    for (int w = 0; w < GW; ++w) n += at[w][threadIdx.x];
-  int incl = n;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(incl, o, 64);
-    if (lane >= o) incl += u;
-  }
-  if (lane == 63) wsum[wave] = incl;
-  __syncthreads();
   int base = 0;
-  for (int w = 0; w < GW; ++w) base += below[w] + (w < wave ? wsum[w] : 0);
-  first[threadIdx.x] = base + incl - n;
-  if (threadIdx.x == GT - 1) first[GT] = base + incl;
-  int place = base + incl - n;
-  for (int w = 0; w < GW; ++w) {
-    const int k = at[w][threadIdx.x];
-    at[w][threadIdx.x] = place;
-    place += k;
+  for (int w = 0; w < WAVES; ++w) base += below[w];
+  for (int r0 = 0; r0 < rows; r0 += NTH) {
+    const int r = r0 + threadIdx.x;
+    int n = 0;
+    if (r < rows)
+      for (int w = 0; w < WAVES; ++w) n += at[w][r];
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += u;
+    }
+    if (lane == 63) wsum[wave] = incl;
+    __syncthreads();
+    int place = base + incl - n;
+    for (int w = 0; w < WAVES; ++w) {
+      place += w < wave ? wsum[w] : 0;
+      base += wsum[w];
+    }
+    if (r < rows) {
+      first[r] = place;
+      if (n > 0) space.count[place] = n;
+      for (int w = 0; w < WAVES; ++w) {
+        const int k = at[w][r];
+        at[w][r] = place;
+        place += k;
+      }
+    }
+    __syncthreads();
   }
-  __syncthreads();
+  if (threadIdx.x == 0) {
+    first[rows] = base;
+    if (c == int(gridDim.x) - 1) *space.all = base;
+  }
+  // positions, row by row of 64 tokens, in lane order
   volatile int* next = at[wave];  // one lane's store is another's next load
-  for (int64_t t = t0; t < t1; t += 64) {
-    const int r = row_of(t + lane, less);
+  const auto put = [&](int r, int64_t t) {
     uint64_t left = __ballot(r >= 0);
-    while (left != 0) {  // row by row of these 64 tokens, in lane order
-      const int lead = __ffsll(static_cast<unsigned long long>(left)) - 1;
-      const uint64_t same = __ballot(r >= 0 && r == __shfl(r, lead, 64));
-      const int p = next[__shfl(r, lead, 64)];
-      if (same >> lane & 1) order[p + __popcll(same & ((uint64_t(1) << lane) - 1))] = int(t + lane);
-      if (lane == lead) next[r] = p + __popcll(same);
+    while (left != 0) {
+      const int lead = __ffsll(static_cast<unsigned long long>(left)) - 1, row = __shfl(r, lead, 64);
+      const uint64_t same = __ballot(r == row);
+      const int p = next[row];
+      if (r == row) {
+        space.token[p + __popcll(same & before)] = int(t);
+        space.row[p + __popcll(same & before)] = row * C + c;
+      }
+      if (lane == lead) next[row] = p + __popcll(same);
       left &= ~same;
     }
+  };
+  if (found <= LIST) {
+    for (int j = 0; j < found; j += 64) {
+      const uint32_t k = j + lane < found ? kept[wave][j + lane] : 0;
+      put(j + lane < found ? int(k >> 22) : -1, t0 + (k & ((1u << 22) - 1)));
+    }
+  } else {
+    for (int64_t t = t0; t < t1; t += 64) put(row_of(t + lane < t1 ? a.index[t + lane] : -1), t + lane);
   }
   __syncthreads();
-  const auto* dout = static_cast<const typename T::storage*>(a.dout);
-  for (int r = wave; r < rows; r += GW) {
-    const int p0 = first[r], p1 = first[r + 1];
-    auto* dst = static_cast<typename T::storage*>(a.dw) + (int64_t(r) * C + c) * a.width;
-    for (int col = lane * N; col < a.width; col += 64 * N) {
-      float s[N];
+  // the rows that no token has
+  const float zero[N] = {};
+  const int chunks = (a.width + 64 * N - 1) / (64 * N);
+  for (int task = wave; task < rows * chunks; task += WAVES) {
+    const int r = task / chunks, col = (task - r * chunks) * 64 * N + lane * N;
+    if (first[r + 1] == first[r] && col < a.width)
+      store_n<T, N>(static_cast<typename T::storage*>(a.dw) + (int64_t(r) * C + c) * a.width + col, zero);
+  }
+}
+
+// Sums in fp32: a wave takes 64 N columns of SEG positions, eight loads in flight, and writes
+// the rows that end in it; a row's piece that goes on, or began before, is left in sums (the
+// first piece of SEG i in 2 i, the last in 2 i + 1).
+template <class T, int N>
+__global__ __launch_bounds__(256) void embed_sum(mmuon_embedding_args a, GradSpace space) {
+  const int all = *space.all;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int chunks = (a.width + 64 * N - 1) / (64 * N);
+  const int64_t item = int64_t(blockIdx.x) * 4 + wave;
+  const int seg = int(item / chunks), col = int(item - int64_t(seg) * chunks) * 64 * N + lane * N;
+  const int p0 = seg * SEG, n = min(SEG, all - p0);
+  if (n <= 0) return;
+  // lanes 0 .. n - 1: the positions; lane n: the one after, lane 63: the one before (rows only)
+  const int at = lane <= n ? p0 + lane : p0 - 1;
+  const bool is = (lane <= n || lane == 63) && at >= 0 && at < all;
+  const int token = is && lane < n ? space.token[at] : 0, row = is ? space.row[at] : -1;
+  const int after = __shfl_down(row, 1, 64);  // (all lanes take part)
+  const uint64_t ends = __ballot(lane < n && row != after);
+  const bool began = __builtin_amdgcn_readlane(row, 63) == __builtin_amdgcn_readlane(row, 0);  // before this SEG
+  if (col >= a.width) return;
+  const auto* dout = static_cast<const typename T::storage*>(a.dout) + col;
+  float s[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) s[k] = 0.f;
+  bool first = true;
+  const auto piece = [&](int slot) { store_n<F32T, N>(space.sums + (int64_t(seg) * 2 + slot) * a.width + col, s); };
+  constexpr int U = 8;
+  for (int p = 0; p < n; p += U) {
+    float x[U][N];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      load_n<T, N>(dout + __builtin_amdgcn_readlane(token, min(p + u, n - 1)) * a.dout_stride, x[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (p + u >= n) break;
+#pragma unroll
+      for (int k = 0; k < N; ++k) s[k] += x[u][k];
+      if (!(ends >> (p + u) & 1)) continue;
+      if (first && began) {
+        piece(0);
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) s[k] *= a.scale;
+        store_n<T, N>(static_cast<typename T::storage*>(a.dw) + int64_t(__builtin_amdgcn_readlane(row, p + u)) * a.width + col, s);
+      }
+      first = false;
 #pragma unroll
       for (int k = 0; k < N; ++k) s[k] = 0.f;
-#pragma unroll 4
-      for (int p = p0; p < p1; ++p) {
-        float x[N];
-        load_n<T, N>(dout + order[p] * a.dout_stride + col, x);
-#pragma unroll
-        for (int k = 0; k < N; ++k) s[k] += x[k];
-      }
-#pragma unroll
-      for (int k = 0; k < N; ++k) s[k] *= a.scale;
-      store_n<T, N>(dst + col, s);
     }
+  }
+  if (!(ends >> (n - 1) & 1)) piece(first ? 0 : 1);  // goes on in the next SEG
+}
+
+// The rows that lie in several SEGs: a workgroup sums 32 N columns of the row that goes on from
+// its SEG, if it begins there; 8 runs of the row's pieces side by side, joined in order.
+template <class T, int N>
+__global__ __launch_bounds__(256) void embed_join(mmuon_embedding_args a, GradSpace space) {
+  constexpr int LANES = 32, RUNS = 256 / LANES, SLICE = LANES * N;
+  __shared__ float sums[RUNS][SLICE];
+  const int all = *space.all, slices = (a.width + SLICE - 1) / SLICE;
+  const int seg = blockIdx.x / slices, slice = blockIdx.x % slices, p0 = seg * SEG;
+  if (p0 + SEG >= all) return;
+  const int r = space.row[p0 + SEG];
+  if (space.row[p0 + SEG - 1] != r) return;
+  const int lead = threadIdx.x & (SEG - 1);  // the row's first position, among this SEG's
+  const uint64_t mine = __ballot(space.row[p0 + lead] == r);
+  const int f = p0 + __ffsll(static_cast<unsigned long long>(mine)) - 1;
+  if (f == p0 && p0 > 0 && space.row[p0 - 1] == r) return;  // began before
+  const int pieces = (f + space.count[f] - 1) / SEG - seg + 1;
+  const int run = threadIdx.x / LANES, lane = threadIdx.x % LANES, col = slice * SLICE + lane * N;
+  const int each = (pieces + RUNS - 1) / RUNS, k1 = min((run + 1) * each, pieces);
+  float s[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) s[k] = 0.f;
+  if (col < a.width) {
+#pragma unroll 8
+    for (int i = run * each; i < k1; ++i) {
+      // the row is the last of its first SEG and the first of the others
+      const int slot = 2 * (seg + i) + (i == 0 && f > p0 ? 1 : 0);
+      float x[N];
+      load_n<F32T, N>(space.sums + int64_t(slot) * a.width + col, x);
+#pragma unroll
+      for (int k = 0; k < N; ++k) s[k] += x[k];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) sums[run][lane * N + k] = s[k];
+  __syncthreads();
+  auto* dst = static_cast<typename T::storage*>(a.dw) + int64_t(r) * a.width + slice * SLICE;
+  for (int e = threadIdx.x; e < min(SLICE, a.width - slice * SLICE); e += 256) {
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < RUNS; ++k) v += sums[k][e];
+    T::store(dst, e, v * a.scale);
   }
 }
 
@@ -151,27 +287,62 @@ void lookup(const mmuon_embedding_args& a, hipStream_t s) {
   else hipLaunchKernelGGL((embed_lookup<T, 1>), grid, block, 0, s, a, lanes);
 }
 
-// Classes: a power of two, at most MAX_ROWS rows each; 256, one workgroup per CU, where
-// that suffices
-int log2_classes(int64_t vocab) {
-  int l = 8;
-  while ((vocab + (int64_t(1) << l) - 1) >> l > MAX_ROWS) ++l;
+// Classes: a power of two.  Many small workgroups (2048, eight per CU) where the ids are few
+// enough for each to read them all; else 256, or what 1024 rows of a class need.
+constexpr int64_t FEW_IDS = 4096;
+int log2_classes(int64_t tokens, int64_t vocab) {
+  int l = tokens <= FEW_IDS ? 11 : 8;
+  const int most = tokens <= FEW_IDS ? 256 : 1024;
+  while ((vocab + (int64_t(1) << l) - 1) >> l > most) ++l;
+  while (l > 0 && int64_t(1) << (l - 1) >= vocab) --l;
   return l;
+}
+
+struct GradLayout {
+  size_t token, row, count, all, total;  // the sums come first
+};
+GradLayout grad_layout(int64_t tokens, int64_t width) {
+  GradLayout l;
+  const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  l.token = up(size_t(tokens > SEG ? (tokens + SEG - 1) / SEG : 0) * 2 * width * 4);
+  l.row = l.token + up(size_t(tokens) * 4);
+  l.count = l.row + up(size_t(tokens) * 4);
+  l.all = l.count + up(size_t(tokens) * 4);
+  l.total = l.all + 256;
+  return l;
+}
+
+template <class T, int N>
+void gradient_n(const mmuon_embedding_args& a, hipStream_t s) {
+  const int l = log2_classes(a.tokens, a.vocab);
+  const int classes = int(std::min<int64_t>(int64_t(1) << l, a.vocab));
+  const GradLayout at = grad_layout(a.tokens, a.width);
+  char* ws = static_cast<char*>(a.workspace);
+  const GradSpace space{reinterpret_cast<int*>(ws + at.token), reinterpret_cast<int*>(ws + at.row),
+                        reinterpret_cast<int*>(ws + at.count), reinterpret_cast<int*>(ws + at.all),
+                        reinterpret_cast<float*>(ws)};
+  if (a.tokens <= FEW_IDS)
+    hipLaunchKernelGGL((embed_rows<T, N, 4, 256, 64>), dim3(classes), dim3(256), 0, s, a, l, space);
+  else hipLaunchKernelGGL((embed_rows<T, N, 16, 1024, 512>), dim3(classes), dim3(1024), 0, s, a, l, space);
+  if (a.tokens == 0) return;
+  const int64_t segs = (a.tokens + SEG - 1) / SEG, waves = segs * ((a.width + 64 * N - 1) / (64 * N));
+  hipLaunchKernelGGL((embed_sum<T, N>), dim3(unsigned((waves + 3) / 4)), dim3(256), 0, s, a, space);
+  if (segs > 1)
+    hipLaunchKernelGGL((embed_join<T, N>), dim3(unsigned((segs - 1) * ((a.width + 32 * N - 1) / (32 * N)))), dim3(256),
+                       0, s, a, space);
 }
 
 template <class T>
 void gradient(const mmuon_embedding_args& a, hipStream_t s) {
-  const bool vec = whole_chunks(a.dout, a.dout_stride, a.width) && whole_chunks(a.dw, a.width, a.width);
-  const int l = log2_classes(a.vocab);
-  const dim3 grid(unsigned(std::min<int64_t>(int64_t(1) << l, a.vocab))), block(GT);
-  int* order = static_cast<int*>(a.workspace);
-  if (vec) hipLaunchKernelGGL((embed_grad<T, 8>), grid, block, 0, s, a, l, order);
-  else hipLaunchKernelGGL((embed_grad<T, 1>), grid, block, 0, s, a, l, order);
+  if (whole_chunks(a.dout, a.dout_stride, a.width) && whole_chunks(a.dw, a.width, a.width)) gradient_n<T, 8>(a, s);
+  else gradient_n<T, 1>(a, s);
 }
 
 }  // namespace
 
-size_t embedding_workspace(const mmuon_embedding_args& a) { return size_t(std::max<int64_t>(a.tokens, 1)) * 4; }
+size_t embedding_workspace(const mmuon_embedding_args& a) {
+  return grad_layout(a.tokens, a.width).total;
+}
 
 int launch_embedding_fwd(const mmuon_embedding_args& a, hipStream_t s) {
   if (a.tokens == 0) return 0;

@@ -124,7 +124,7 @@ def test_entry_points_validate_before_launching():
     emb = dict(tokens=4, vocab=100, width=7, dtype=_abi.F32, scale=1.0, padding_idx=-1, w_stride=7, dout_stride=7,
                index=4096, w=8192, out=12288, dout=16384, dw=20480, workspace=32768, workspace_bytes=0)
     for change, code, message in [({}, -1, b"workspace of"), ({"dtype": _abi.F8E4M3}, -1, b"dtype"),
-                                  ({"tokens": 1 << 31}, -3, b"2^31"), ({"vocab": 0}, -3, b"vocab"),
+                                  ({"tokens": 1 << 26}, -3, b"2^26"), ({"vocab": 0}, -3, b"vocab"),
                                   ({"width": 0}, -1, b"width"), ({"dout": 16386}, -1, b"unaligned"),
                                   ({"index": None}, -1, b"index"), ({"dout_stride": -7}, -1, b"stride")]:
         assert lib.mmuon_embedding_bwd(C.byref(_abi.EmbeddingArgs(**{**emb, **change})), None) == code, change
