@@ -433,8 +433,9 @@ int mmuon_ce_fwd_bwd(const mmuon_ce_args* a, void* stream);
 /* Workspace bytes of a call with these sizes and this piece (train: of mmuon_ce_fwd_bwd;
    nll null counts it in). */
 size_t mmuon_ce_workspace(const mmuon_ce_args* a, int32_t train);
-/* x *= *factor (device), bf16, numel a multiple of 8; writes nothing where *factor == 1. */
-int mmuon_scale_bf16(void* x, int64_t numel, const float* factor, void* stream);
+/* x and y (either may be empty) *= *factor (device), bf16, nx and ny multiples of 8; writes
+   nothing where *factor == 1. */
+int mmuon_scale_bf16(void* x, int64_t nx, void* y, int64_t ny, const float* factor, void* stream);
 
 /* Token embedding: out[t] = scale * w[index[t]] (fp32 product, one rounding), NaN where
    index[t] is not in [0, vocab).  Gradient of the table: dw[v] = scale * sum of dout[t]

@@ -161,7 +161,7 @@ SIGNATURES = {
     "mmuon_embedding_fwd": (C.c_int, [C.POINTER(EmbeddingArgs), C.c_void_p]),
     "mmuon_embedding_bwd": (C.c_int, [C.POINTER(EmbeddingArgs), C.c_void_p]),
     "mmuon_embedding_workspace": (C.c_size_t, [C.POINTER(EmbeddingArgs)]),
-    "mmuon_scale_bf16": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
+    "mmuon_scale_bf16": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
 }
 
 _lib = None

@@ -706,11 +706,12 @@ int mmuon_ce_fwd_bwd(const mmuon_ce_args* a, void* stream) {
   return check_launch("cross entropy forward and backward");
 }
 
-int mmuon_scale_bf16(void* x, int64_t numel, const float* factor, void* stream) {
-  if (numel < 0 || numel % 8) return fail(MMUON_EINVAL, "scale: numel must be a multiple of 8 (got %lld)", (long long)numel);
-  if (numel == 0) return MMUON_OK;
-  if (x == nullptr || !aligned16(x) || factor == nullptr) return fail(MMUON_EINVAL, "scale: null or unaligned pointer");
-  mmuon::launch_ce_scale(x, numel, factor, static_cast<hipStream_t>(stream));
+int mmuon_scale_bf16(void* x, int64_t nx, void* y, int64_t ny, const float* factor, void* stream) {
+  if (nx < 0 || nx % 8 || ny < 0 || ny % 8)
+    return fail(MMUON_EINVAL, "scale: sizes must be multiples of 8 (got %lld, %lld)", (long long)nx, (long long)ny);
+  if ((nx > 0 && x == nullptr) || (ny > 0 && y == nullptr) || !aligned16(x) || !aligned16(y) || factor == nullptr)
+    return fail(MMUON_EINVAL, "scale: null or unaligned pointer");
+  mmuon::launch_ce_scale(x, nx, y, ny, factor, static_cast<hipStream_t>(stream));
   return check_launch("scale");
 }
 

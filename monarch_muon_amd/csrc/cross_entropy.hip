@@ -40,16 +40,16 @@ constexpr int CODE_ZERO = 65535;                 // p = 0
 enum {
   EP_STATS = 0,  // logits: statistics of each part, the targets' logits
   EP_CODES = 1,  // the same, and the codes
-  EP_ROWS = 2,   // bf16 result, rows = columns of the tile
-  EP_FRAG = 3    // fp32 accumulators in fragment order (a split of K, or a piece of the tokens)
+  EP_ROWS = 2    // bf16 result, rows = columns of the tile; or fp32 accumulators of a part of K
 };
 
 // D (M x N) = A (M x K) B^T (N x K), where N (logits, dx) or K (dw) are the piece's tokens:
 // compact tokens t0 .. of *count, at most `piece`.
 struct HeadGemm {
   GOp a, b;
-  int M, N, K, S, kchunk;
+  int M, N, K;
   int tiles_m, tiles_n;
+  int full, S;                   // tiles from `full` on are split over K in S
   const int* count;
   int t0, piece, tokens;
   const char* x;                 // x itself, read instead of the gathered rows where no token is ignored
@@ -62,68 +62,316 @@ struct HeadGemm {
   const uint16_t* w;
   int64_t wstride;
   int64_t vocab;
-  float* frag;                   // EP_FRAG: BM x BN floats per virtual tile
-  const float* start;            // accumulators to start from, same order; or null
+  float* frag;                   // accumulators in fragment order: BM x BN floats per virtual tile,
+  int frag_first;                //   from this one on
+  bool start;                    // they are what the sums begin with (a later piece of the tokens)
+  bool keep;                     // they are kept for the next piece, of every tile
   uint16_t* codes;               // EP_CODES: [token][ldc]
   int64_t ldc;
   float2* parts;                 // [token][nparts]: maximum (base 2), sum of 2^(l - maximum)
   int nparts;
   const int64_t* target;         // of the compact tokens of the piece
+  const float* nll;              // dw: sums the loss too, or null
+  float* loss;
+  int mean;
   float* tlogit;                 // [token]
-  __device__ __forceinline__ int live() const { return min(max(*count - t0, 0), piece); }
-  __device__ __forceinline__ int total() const { return tiles_m * tiles_n * S; }
 };
 
-// Virtual tile -> (split, tile row, tile column).  Each XCD (v % 8) takes a contiguous run
-// of tiles; the tiles of a run are numbered in patches PATCH tile columns wide, so the 32
-// tiles that an XCD's CUs hold at a time share 4 column and 8 row operand bands.
+// The sizes that the number of compact tokens decides
+struct HeadSize {
+  int N, K, tiles_m, tiles_n, full, splits;  // unsplit tiles, and parts of the others
+  int S, kchunk;                             // K of a part
+  bool all;                                  // no token is ignored
+  // virtual tiles: both dealt to the XCDs by themselves
+  __device__ __forceinline__ int vfull() const { return (full + 7) / 8 * 8; }
+  __device__ __forceinline__ int vtiles() const { return vfull() + (splits + 7) / 8 * 8; }
+};
+enum { X_IS_A = 0, X_IS_B = 1, X_IS_NONE = 2 };  // which operand x is: of dw, of the logits, of dx
+template <class GE, int X>
+__device__ __forceinline__ HeadSize head_size(const HeadGemm& a) {
+  // (no list: every token of the piece)
+  const int count = a.count != nullptr ? *a.count : a.tokens, n = min(max(count - a.t0, 0), a.piece);
+  HeadSize z;
+  z.N = X == X_IS_A ? a.N : n;
+  z.K = X == X_IS_A ? n : a.K;
+  z.tiles_m = a.tiles_m;
+  z.tiles_n = X == X_IS_A ? a.tiles_n : (n + GE::BN - 1) / GE::BN;
+  z.full = min(a.full, z.tiles_m * z.tiles_n);
+  z.splits = (z.tiles_m * z.tiles_n - z.full) * a.S;
+  z.S = a.S;
+  z.kchunk = ((z.K + a.S - 1) / a.S + BK - 1) / BK * BK;
+  z.all = count == a.tokens;
+  return z;
+}
+
+// The kernel's arguments, read again where they are used: held in scalar registers from the
+// start, they would be spilled around the main loop.
+__device__ __forceinline__ const HeadGemm& late_args() {
+  auto p = (const __attribute__((address_space(4))) void*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const HeadGemm*)p;
+}
+
+// Virtual tile -> tile row and column, part of K.  Each XCD (v % 8) takes a contiguous run of
+// tiles; the tiles of a run are numbered in patches PATCH tile columns wide, so the 32 tiles
+// that an XCD's CUs hold at a time share 4 column and 8 row operand bands.
 constexpr int PATCH = 4;
-__device__ __forceinline__ bool head_tile(const HeadGemm& a, int v, int& sp, int& tm, int& tn, int& idx) {
-  const int total = a.total(), per = (total + 7) >> 3, local = v >> 3;
-  idx = (v & 7) * per + local;
-  if (local >= per || idx >= total) return false;
-  const int plane = a.tiles_m * a.tiles_n;
-  sp = idx / plane;
-  const int t = idx - sp * plane, g = t / (a.tiles_m * PATCH), r = t - g * a.tiles_m * PATCH;
-  const int width = min(PATCH, a.tiles_n - g * PATCH);
-  tm = r / width;
-  tn = g * PATCH + r - tm * width;
-  return true;
+struct HeadTile {
+  int idx;                       // < 0: none
+  int m0, n0, kbeg, kend;
+  bool split;
+  __device__ __forceinline__ int slices() const { return max(kend - kbeg + BK - 1, 0) / BK; }
+};
+__device__ __forceinline__ int2 tile_place(int t, int tiles_m, int tiles_n) {  // (row, column) of tile t
+  const int g = t / (tiles_m * PATCH), r = t - g * tiles_m * PATCH, width = min(PATCH, tiles_n - g * PATCH);
+  const int tm = r / width;
+  return make_int2(tm, g * PATCH + r - tm * width);
+}
+template <class GE>
+__device__ __forceinline__ HeadTile head_tile(const HeadSize& z, int v) {
+  const bool split = v >= z.vfull();
+  const int w = split ? v - z.vfull() : v, n = split ? z.splits : z.full;
+  const int per = (n + 7) >> 3, local = w >> 3, i = (w & 7) * per + local;
+  if (local >= per || i >= n) return HeadTile{-1, 0, 0, 0, 0, split};
+  // part by part: neighbours read the same slices of K
+  const int tail = z.tiles_m * z.tiles_n - z.full, part = split ? i / tail : 0, t = split ? z.full + i - part * tail : i;
+  const int2 at = tile_place(t, z.tiles_m, z.tiles_n);
+  return HeadTile{split ? z.full + (t - z.full) * z.S + part : i, at.x * GE::BM, at.y * GE::BN,
+                  split ? part * z.kchunk : 0, split ? min(z.K, (part + 1) * z.kchunk) : z.K, split};
+}
+
+// The K slices of a workgroup's tiles as one stream through the LDS ring: behind the last
+// slice of a tile come the first of the next, so its operands are on their way while the
+// tile before is finished and stored, and the ring is filled once per launch.  (Filled anew
+// for every tile, with the result staged in it, a tile of 1024 of K took 4 us more of 40.)
+template <class GE, bool AT, bool BT, int X>
+struct Stream {
+  static constexpr int RING = GE::RING, WI = GE::WI, WJ = GE::WJ, NM = WI * WJ, NR = WI + WJ;
+  struct Fr {
+    bf16x8 r[WI];
+    bf16x8 c[WJ];
+  };
+  typedef f32x16 Acc[WI][WJ];
+  // what is loaded next
+  const char *pa, *pb;     // the operands' slices
+  int64_t sa, sb;          // bytes to the next ones
+  int left;                // slices of its tile from it on
+  int v;                   // its virtual tile
+  uint32_t loff[GE::DMA];  // per-lane byte offsets of the loads (OOB: beyond the extent, or no tile left)
+  uint32_t tail[GE::DMA];  // OOB where the load's element lies beyond the last slice's K
+  int wave, lane, wm, wn;
+  char* lds;
+  uint32_t lds0;
+  uint32_t kfrag[BK / 16];
+  uint32_t tfrag_r, tfrag_c;
+
+  __device__ __forceinline__ const uint16_t* slot(uint32_t pos) const {
+    return reinterpret_cast<const uint16_t*>(lds + (pos % RING) * GE::SLOTB);
+  }
+  __device__ __forceinline__ void open(const HeadSize& z) {  // the first tile from v on
+    const int vtiles = z.vtiles();
+    HeadTile t{-1, 0, 0, 0, 0, false};
+    for (; v < vtiles; v += gridDim.x) {
+      t = head_tile<GE>(z, v);
+      if (t.idx >= 0 && t.slices() > 0) break;
+      t.idx = -1;
+    }
+    left = 1;
+    if (t.idx < 0) {  // nothing left: loads that read zeros
+#pragma unroll
+      for (int q = 0; q < GE::DMA; ++q) loff[q] = OOB;
+      v = vtiles - int(gridDim.x);
+      return;
+    }
+    const HeadGemm& a = late_args();
+    GOp oa = a.a, ob = a.b;
+    if (X != X_IS_A) ob.extent = z.N;
+    if (X == X_IS_A && z.all) oa.base = a.x, oa.kstride = a.xstride;
+    if (X == X_IS_B && z.all) ob.base = a.x, ob.mstride = a.xstride;
+    pa = oa.base + mn_off(oa, t.m0) + t.kbeg * oa.kstride;
+    pb = ob.base + mn_off(ob, t.n0) + t.kbeg * ob.kstride;
+    sa = BK * oa.kstride;
+    sb = BK * ob.kstride;
+    left = t.slices();
+    const int rem = t.kend - t.kbeg - (left - 1) * BK;  // K of the last slice
+#pragma unroll
+    for (int q = 0; q < GE::DMA; ++q) {
+      const bool row = q < GE::RL;
+      const int u = row ? GE::RL * wave + q : GE::CL * wave + q - GE::RL;
+      loff[q] = row ? lane_offset<AT>(oa, t.m0, u, lane) : lane_offset<BT>(ob, t.n0, u, lane);
+      const int kd = (row ? AT : BT) ? 16 * (u & 1) + (lane >> 2) : 8 * ((lane & 3) ^ ((lane >> 4) & 3));
+      tail[q] = kd >= rem ? OOB : 0;
+    }
+  }
+  // behind a load: the next slice, of the same tile (!SWITCH: known to be one) or the next
+  template <bool SWITCH>
+  __device__ __forceinline__ void advance(const HeadSize& z) {
+    --left;
+    if (!SWITCH || left > 0) {
+      pa += sa;
+      pb += sb;
+    } else {
+      v += gridDim.x;
+      open(z);
+    }
+  }
+
+  // Load Q (row operand first) of the next slice into the slot of stream position pos.  Load
+  // u of an operand, K form: rows 16 u + lane/4, chunk (lane%4) ^ ((lane>>4)&3); T form: k rows
+  // 16 (u%2) + lane/4, MN 32 (u/2) + 8 (lane%4).  Either lands at byte 1024 u of its slice.
+  template <bool LAST, int Q>
+  __device__ __forceinline__ void issue_one(uint32_t pos) const {
+    constexpr bool ROW = Q < GE::RL;
+    const int u = ROW ? GE::RL * wave + Q : GE::CL * wave + Q - GE::RL;
+    const uint32_t dst = lds0 + (pos % RING) * GE::SLOTB + (ROW ? 0 : GE::RSLB) + u * 1024;
+    bdma16(buffer_rsrc(ROW ? pa : pb), LAST && left == 1 ? loff[Q] | tail[Q] : loff[Q], dst);
+  }
+  template <bool LAST, int Q0, int Q1>
+  __device__ __forceinline__ void issue(uint32_t pos) const {
+    if constexpr (Q0 < Q1) {
+      issue_one<LAST, Q0>(pos);
+      issue<LAST, Q0 + 1, Q1>(pos);
+    }
+  }
+
+  template <int KK, int G>
+  __device__ __forceinline__ void load_one(uint32_t pos, Fr& f) const {
+    const uint16_t* sr = slot(pos);
+    const uint16_t* sc = sr + GE::RSLB / 2;
+    if constexpr (G < WJ)
+      f.c[G] = BT ? frag_rowmajor_tr(sc, tfrag_c + G * 2048, KK) : frag_kmajor(sc, kfrag[KK], (wn * WJ + G) * 32);
+    else
+      f.r[G - WJ] = AT ? frag_rowmajor_tr(sr, tfrag_r + (G - WJ) * 2048, KK)
+                       : frag_kmajor(sr, kfrag[KK], (wm * WI + G - WJ) * 32);
+  }
+  template <int KK, int G0, int G1>
+  __device__ __forceinline__ void load(uint32_t pos, Fr& f) const {
+    if constexpr (G0 < G1) {
+      load_one<KK, G0>(pos, f);
+      load<KK, G0 + 1, G1>(pos, f);
+    }
+  }
+
+  // MFMA g of a k step, with its share of the fragment reads of the next step and, in the
+  // second k step, of the direct loads
+  template <bool LAST, int KK, int g>
+  __device__ __forceinline__ void half(uint32_t pos, const Fr& f, Fr& n, Acc& acc) const {
+    if constexpr (g < NM) {
+      acc[g / WJ][g % WJ] = mfma(f.r[g / WJ], f.c[g % WJ], acc[g / WJ][g % WJ]);
+      if constexpr (KK == 0) {
+        load<1, g * NR / NM, (g + 1) * NR / NM>(pos, n);
+      } else {
+        load<0, g * NR / NM, (g + 1) * NR / NM>(pos + 1, n);
+        issue<LAST, g * GE::DMA / NM, (g + 1) * GE::DMA / NM>(pos + RING - 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      half<LAST, KK, g + 1>(pos, f, n, acc);
+    }
+  }
+  // The slice at stream position pos (fa: its first k step's fragments, then the next slice's).
+  // !LAST: the slice to load is not the last of its tile
+  template <bool LAST>
+  __device__ __forceinline__ void body(const HeadSize& z, uint32_t pos, Fr& fa, Fr& fb, Acc& acc) {
+    half<LAST, 0, 0>(pos, fa, fb, acc);
+    wait_vm<(RING - 3) * GE::DMA>();  // slice pos + 1 landed
+    barrier();
+    // raised wave priority from the barrier to the end of k step 1, so the SIMD's wave still in
+    // this phase wins issue over one already in the next step
+    __builtin_amdgcn_s_setprio(1);
+    half<LAST, 1, 0>(pos, fb, fa, acc);
+    __builtin_amdgcn_s_setprio(0);
+    advance<LAST>(z);
+  }
+  // n slices from stream position pos on
+  __device__ __forceinline__ void run(const HeadSize& z, int n, uint32_t& pos, Fr& fa, Fr& fb, Acc& acc) {
+    while (n > 0) {
+      for (int m = min(n, left - 1); m > 0; --m, --n) body<false>(z, pos++, fa, fb, acc);
+      if (n > 0) {
+        body<true>(z, pos++, fa, fb, acc);
+        --n;
+      }
+    }
+  }
+  __device__ __forceinline__ void fill(const HeadSize& z, Fr& fa) {
+    open(z);
+    for (uint32_t q = 0; q < RING - 1; ++q) {
+      issue<true, 0, GE::DMA>(q);
+      advance<true>(z);
+    }
+    wait_vm<(RING - 2) * GE::DMA>();  // slice 0 landed
+    barrier();
+    load<0, 0, NR>(0, fa);
+  }
+};
+
+// A 32 x 32 MFMA tile as 16-bit values, D[row][column] with a lane = one column, to memory in
+// rows of its columns: w[q] holds rows 8 q + 4 (lane/32) .. + 3 of column lane%32.  Exchanged
+// between halves and between rows of 16 lanes, a lane ends up with eight rows (16 B) of one
+// column and a store of a wave writes 64 B of 16 columns.  fn(column, first row, 16 B)
+template <class Fn>
+__device__ __forceinline__ void store_block(uint2 (&w)[4], int lane, Fn&& fn) {
+  uint32_t x[2][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const auto lo = __builtin_amdgcn_permlane32_swap(w[2 * h].x, w[2 * h + 1].x, false, false);
+    const auto hi = __builtin_amdgcn_permlane32_swap(w[2 * h].y, w[2 * h + 1].y, false, false);
+    x[h][0] = lo[0];
+    x[h][1] = hi[0];
+    x[h][2] = lo[1];
+    x[h][3] = hi[1];
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const auto t = __builtin_amdgcn_permlane16_swap(x[0][k], x[1][k], false, false);
+    x[0][k] = t[0];
+    x[1][k] = t[1];
+  }
+  const int r = lane >> 4, row = ((r & 1) << 1 | r >> 1) * 8;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) fn(h * 16 + (lane & 15), row, make_uint4(x[h][0], x[h][1], x[h][2], x[h][3]));
 }
 
 // Statistics and codes of a tile of logits: rows m0.. are vocabulary, columns n0.. tokens.
 template <class GE, bool CODES>
-__device__ __forceinline__ void loss_epilogue(const HeadGemm& a, char* lds, int m0, int n0,
-                                              f32x16 (&acc)[GE::WI][GE::WJ]) {
+__device__ __forceinline__ void loss_epilogue(const HeadGemm& a, int N, int m0, int n0, f32x16 (&acc)[GE::WI][GE::WJ]) {
   const int tid = fresh_tid();
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / GE::GN, wn = wave % GE::GN;
   constexpr int PW = 32 * GE::WI;               // vocabulary of a part
   const int v0 = m0 + wm * PW, left = a.M - v0;  // rows from `left` on do not exist
   const int half = lane >> 5;
-  if constexpr (CODES) barrier();  // every wave is done with the ring
 #pragma unroll
   for (int j = 0; j < GE::WJ; ++j) {
     const int row = (wn * GE::WJ + j) * 32 + (lane & 31), tok = n0 + row;
-    const bool live = tok < a.N;
+    const bool live = tok < N;
     const int64_t y = live ? a.target[tok] : -1;
     const int64_t rel = y - v0;
     const bool hit = rel >= 0 && rel < PW && rel < left && ((int(rel) >> 2) & 1) == half;
     if (__any(hit)) {
+      // element (rel % 4) + 4 (rel / 8 % 4) + 16 (rel / 32) of the lane's, bit by bit, by masks
+      // (a choice between elements becomes an index, and an index 2048 comparisons)
       const int at = (int(rel) >> 5) * 16 + ((int(rel) >> 3) & 3) * 4 + (int(rel) & 3);
-      float l = 0.f;
+      uint32_t l[GE::WI * 16];
 #pragma unroll
       for (int i = 0; i < GE::WI; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) l = at == i * 16 + r ? acc[i][j][r] : l;
-      if (hit) a.tlogit[tok] = l;
+        for (int r = 0; r < 16; ++r) l[i * 16 + r] = __float_as_uint(acc[i][j][r]);
+#pragma unroll
+      for (int n = GE::WI * 8; n > 0; n /= 2) {
+        const uint32_t upper = at & n ? ~0u : 0u;
+#pragma unroll
+        for (int k = 0; k < n; ++k) l[k] = (l[k + n] & upper) | (l[k] & ~upper);
+      }
+      if (hit) a.tlogit[tok] = __uint_as_float(l[0]);
     }
     if (left < PW) {
+      int limit = left - half * 4;
+      asm volatile("" : "+v"(limit));  // (the comparisons of every j at once would take 128 registers)
 #pragma unroll
       for (int i = 0; i < GE::WI; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (i * 32 + (r >> 2) * 8 + half * 4 + (r & 3) >= left) acc[i][j][r] = -INFINITY;
+          if (i * 32 + (r >> 2) * 8 + (r & 3) >= limit) acc[i][j][r] = -INFINITY;
     }
     float m = -INFINITY;
 #pragma unroll
@@ -134,7 +382,8 @@ __device__ __forceinline__ void loss_epilogue(const HeadGemm& a, char* lds, int 
     const float m2 = m == -INFINITY ? 0.f : m * LOG2E;  // a part that is all -inf: sum 0
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < GE::WI; ++i)
+    for (int i = 0; i < GE::WI; ++i) {
+      uint2 codes[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         float d[4];
@@ -147,24 +396,18 @@ __device__ __forceinline__ void loss_epilogue(const HeadGemm& a, char* lds, int 
           constexpr float K = -1.f / CODE_RANGE;
           const uint32_t lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_u16(d[0] * K, d[1] * K));
           const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_u16(d[2] * K, d[3] * K));
-          const int col = (wm * GE::WI + i) * 32 + q * 8 + half * 4;
-          *reinterpret_cast<uint2*>(lds + GE::tile_at(row, col)) = make_uint2(lo, hi);
+          codes[q] = make_uint2(lo, hi);
         }
       }
+      if constexpr (CODES) {
+        store_block(codes, lane, [&](int c, int r, const uint4& u) {
+          const int t = n0 + (wn * GE::WJ + j) * 32 + c;
+          if (t < N) *reinterpret_cast<uint4*>(a.codes + int64_t(t) * a.ldc + v0 + i * 32 + r) = u;
+        });
+      }
+    }
     s += __shfl_xor(s, 32, 64);
     if (live && half == 0 && left > 0) a.parts[int64_t(tok) * a.nparts + v0 / PW] = make_float2(m2, s);
-  }
-}
-
-// Staged tile -> rows of 16-B chunks: fn(row, first column, chunk)
-template <class GE, class Fn>
-__device__ __forceinline__ void staged_rows(const char* stage, Fn&& fn) {
-  constexpr int CPR = GE::BM / 8;
-  const int tid = fresh_tid();
-#pragma unroll 4
-  for (int it = 0; it < GE::BN * CPR / GE::NTH; ++it) {
-    const int idx = tid + it * GE::NTH, row = idx / CPR, col = idx % CPR * 8;
-    fn(row, col, *reinterpret_cast<const uint4*>(stage + GE::tile_at(row, col)));
   }
 }
 
@@ -180,168 +423,147 @@ __device__ __forceinline__ void add_resid(const HeadGemm& a, int n, int m, float
   v[3] += r * __uint_as_float(u.y & 0xffff0000u);
 }
 
-template <class GE, bool AT, bool BT, int EP>
-__device__ __forceinline__ void head_work(const HeadGemm& a, char* lds, int v) {
-  int sp, tm, tn, idx;
-  if (!head_tile(a, v, sp, tm, tn, idx)) return;
-  const int m0 = tm * GE::BM, n0 = tn * GE::BN;
-  GPipe<GE, AT, BT> p;
+// What becomes of a tile's accumulators
+template <class GE, int EP, int X>
+__device__ __forceinline__ void finish(int N, const HeadTile& t, f32x16 (&acc)[GE::WI][GE::WJ]) {
+  const HeadGemm& a = late_args();
+  const int tid = fresh_tid();
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / GE::GN, wn = wave % GE::GN;
+  if constexpr (EP == EP_ROWS) {
+    // fragment order: float4 q of MFMA tile (i, j) of a wave at 64 lanes x 16 B
+    float* frag = a.frag + ((int64_t(t.idx - a.frag_first) * GE::NW + wave) * (GE::WI * GE::WJ * 16) * 64 + lane * 4);
+    if (a.start) {
+#pragma unroll
+      for (int i = 0; i < GE::WI; ++i)
+#pragma unroll
+        for (int j = 0; j < GE::WJ; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float4 f = *reinterpret_cast<const float4*>(frag + ((i * GE::WJ + j) * 4 + q) * 256);
+            acc[i][j][4 * q] += f.x;
+            acc[i][j][4 * q + 1] += f.y;
+            acc[i][j][4 * q + 2] += f.z;
+            acc[i][j][4 * q + 3] += f.w;
+          }
+    }
+    if (a.keep || t.split) {
+#pragma unroll
+      for (int i = 0; i < GE::WI; ++i)
+#pragma unroll
+        for (int j = 0; j < GE::WJ; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<float4*>(frag + ((i * GE::WJ + j) * 4 + q) * 256) =
+                make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+      return;
+    }
+    const float factor = a.factor != nullptr ? *a.factor : 1.f;
+#pragma unroll
+    for (int j = 0; j < GE::WJ; ++j) {
+      const int n1 = t.n0 + (wn * GE::WJ + j) * 32, n = n1 + (lane & 31);
+#pragma unroll
+      for (int i = 0; i < GE::WI; ++i) {
+        const int m1 = t.m0 + (wm * GE::WI + i) * 32;
+        uint2 w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+          const int m = m1 + q * 8 + (lane >> 5) * 4;
+          if (X == X_IS_NONE && n < N && m < a.M) add_resid(a, n, m, v);
+          w[q] = make_uint2(f2bf2(v[0] * factor, v[1] * factor), f2bf2(v[2] * factor, v[3] * factor));
+        }
+        store_block(w, lane, [&](int c, int r, const uint4& u) {
+          if (n1 + c >= N || m1 + r >= a.M) return;
+          const int row = X == X_IS_NONE ? a.rows[n1 + c] : n1 + c;
+          *reinterpret_cast<uint4*>(a.out + int64_t(row) * a.ostride + int64_t(m1 + r) * 2) = u;
+        });
+      }
+    }
+  } else {
+    loss_epilogue<GE, EP == EP_CODES>(a, N, t.m0, t.n0, acc);
+  }
+}
+
+// Sum of nll, divided by the number of targets that are not ignored where mean (NaN if there
+// is none): each thread's share in order, then a tree (the same order every time for NTH threads)
+template <int NTH>
+__device__ __forceinline__ void sum_loss(const float* nll, int tokens, int count, int mean, float* loss,
+                                         float* scratch) {
+  float s = 0.f;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < tokens; i += NTH) s += nll[i];
+  s = block_sum<NTH>(s, scratch);
+  if (threadIdx.x == 0) *loss = mean ? s / float(count) : s;
+}
+
+template <class GE, bool AT, bool BT, int EP, int X>
+__global__ __launch_bounds__(GE::NTH, GE::PER_CU * GE::NW / 4) void head_gemm(HeadGemm a) {
+  __shared__ __attribute__((aligned(1024))) char lds[GE::LDS];
+  const HeadSize z = head_size<GE, X>(a);
+  const int vtiles = z.vtiles();
+  typedef Stream<GE, AT, BT, X> Pipe;
+  Pipe p;
   p.lane = threadIdx.x & 63;
   p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   p.wm = p.wave / GE::GN;
   p.wn = p.wave % GE::GN;
-  const int kbeg = sp * a.kchunk, kend = min(a.K, kbeg + a.kchunk);
-  p.ak.start(a.a, a.a.base + mn_off(a.a, m0), kbeg);
-  p.bk.start(a.b, a.b.base + mn_off(a.b, n0), kbeg);
-  p.nxt = 0;
-  p.KT = (kend - kbeg + BK - 1) / BK;
-  const int rem = kend - kbeg - (p.KT - 1) * BK;  // K of the last slice
-#pragma unroll
-  for (int q = 0; q < GE::DMA; ++q) {
-    const bool row = q < GE::RL;
-    const int u = row ? GE::RL * p.wave + q : GE::CL * p.wave + q - GE::RL;
-    p.loff[q] = row ? lane_offset<AT>(a.a, m0, u, p.lane) : lane_offset<BT>(a.b, n0, u, p.lane);
-    const int kd = (row ? AT : BT) ? 16 * (u & 1) + (p.lane >> 2) : 8 * ((p.lane & 3) ^ ((p.lane >> 4) & 3));
-    p.tail[q] = kd >= rem ? OOB : 0;
-  }
   p.lds = lds;
   p.lds0 = lds_addr(lds);
 #pragma unroll
   for (int kk = 0; kk < BK / 16; ++kk) p.kfrag[kk] = kmajor_frag_base(kk, p.lane);
   p.tfrag_r = rowmajor_frag_base(p.wm * GE::WI, p.lane);
   p.tfrag_c = rowmajor_frag_base(p.wn * GE::WJ, p.lane);
-  f32x16 acc[GE::WI][GE::WJ];
-  if (p.KT > 0) {
-    p.run(acc);
-  } else {  // an empty piece
+  p.v = blockIdx.x;
+  typename Pipe::Fr fa, fb;
+  p.fill(z, fa);
+  uint32_t pos = 0;
+  for (int v = blockIdx.x; v < vtiles; v += gridDim.x) {
+    const HeadTile t = head_tile<GE>(z, v);
+    if (t.idx < 0) continue;
+    f32x16 acc[GE::WI][GE::WJ];
 #pragma unroll
     for (int i = 0; i < GE::WI; ++i)
 #pragma unroll
       for (int j = 0; j < GE::WJ; ++j) acc[i][j] = f32x16{};
+    p.run(z, t.slices(), pos, fa, fb, acc);
+    finish<GE, EP, X>(z.N, t, acc);
   }
-
-  // fragment order: float4 q of MFMA tile (i, j) of a wave at 64 lanes x 16 B
-  const int64_t f0 = ((int64_t(idx) * GE::NW + p.wave) * (GE::WI * GE::WJ * 16) * 64 + p.lane * 4);
-  if (a.start != nullptr) {
-#pragma unroll
-    for (int i = 0; i < GE::WI; ++i)
-#pragma unroll
-      for (int j = 0; j < GE::WJ; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 t = *reinterpret_cast<const float4*>(a.start + f0 + ((i * GE::WJ + j) * 4 + q) * 256);
-          acc[i][j][4 * q] += t.x;
-          acc[i][j][4 * q + 1] += t.y;
-          acc[i][j][4 * q + 2] += t.z;
-          acc[i][j][4 * q + 3] += t.w;
-        }
-  }
-  if constexpr (EP == EP_FRAG) {
-#pragma unroll
-    for (int i = 0; i < GE::WI; ++i)
-#pragma unroll
-      for (int j = 0; j < GE::WJ; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<float4*>(a.frag + f0 + ((i * GE::WJ + j) * 4 + q) * 256) =
-              make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
-  } else if constexpr (EP == EP_ROWS) {
-    const float factor = a.factor != nullptr ? *a.factor : 1.f;
-#pragma unroll
-    for (int i = 0; i < GE::WI; ++i)
-#pragma unroll
-      for (int j = 0; j < GE::WJ; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-          if (a.resid != nullptr) {
-            const int n = n0 + (p.wn * GE::WJ + j) * 32 + (p.lane & 31);
-            const int m = m0 + (p.wm * GE::WI + i) * 32 + q * 8 + (p.lane >> 5) * 4;
-            if (n < a.N && m < a.M) add_resid(a, n, m, v);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = v[e] * factor;
-        }
+  wait_vm<0>();  // no load is left in flight to LDS that another workgroup may own next
+  // dw sums the loss: the last workgroup has no more tiles than any other
+  if (X == X_IS_A && a.nll != nullptr && blockIdx.x == gridDim.x - 1) {
     barrier();  // every wave is done with the ring
-    stage_acc<GE>(lds, acc);
-    barrier_after_lds_writes();
-    staged_rows<GE>(lds, [&](int r, int c, const uint4& u) {
-      if (n0 + r >= a.N || m0 + c >= a.M) return;
-      const int row = a.rows != nullptr ? a.rows[n0 + r] : n0 + r;
-      *reinterpret_cast<uint4*>(a.out + int64_t(row) * a.ostride + int64_t(m0 + c) * 2) = u;
-    });
-  } else {
-    loss_epilogue<GE, EP == EP_CODES>(a, lds, m0, n0, acc);
-    if constexpr (EP == EP_CODES) {
-      barrier_after_lds_writes();
-      staged_rows<GE>(lds, [&](int r, int c, const uint4& u) {
-        if (n0 + r < a.N) *reinterpret_cast<uint4*>(a.codes + int64_t(n0 + r) * a.ldc + m0 + c) = u;
-      });
-    }
+    sum_loss<GE::NTH>(a.nll, a.tokens, *a.count, a.mean, a.loss, reinterpret_cast<float*>(lds));
   }
 }
 
-// The sizes that the number of compact tokens decides
-enum { X_IS_A = 0, X_IS_B = 1, X_IS_NONE = 2 };  // which operand x is: of dw, of the logits, of dx
+// Sum over the parts of K, in order, of one 32 x 32 MFMA tile of a split tile per workgroup:
+// the fp32 partials in fragment order -> bf16 rows.
 template <class GE, int X>
-__device__ __forceinline__ void settle(HeadGemm& a) {
-  const int n = a.live();
-  if constexpr (X == X_IS_A) {
-    a.K = n;
-    a.kchunk = max(n, 1);
-  } else {
-    a.N = n;
-    a.b.extent = n;
-    a.tiles_n = (n + GE::BN - 1) / GE::BN;
-  }
-  if (X == X_IS_A && *a.count == a.tokens) {
-    a.a.base = a.x;
-    a.a.kstride = a.xstride;
-  }
-  if (X == X_IS_B && *a.count == a.tokens) {
-    a.b.base = a.x;
-    a.b.mstride = a.xstride;
-  }
-}
-
-template <class GE, bool AT, bool BT, int EP, int X>
-__global__ __launch_bounds__(GE::NTH, GE::PER_CU * GE::NW / 4) void head_gemm(HeadGemm a) {
-  __shared__ __attribute__((aligned(1024))) char lds[GE::LDS];
-  settle<GE, X>(a);
-  const int vtiles = (a.total() + 7) / 8 * 8;
-  for (int v = blockIdx.x; v < vtiles; v += gridDim.x) {
-    head_work<GE, AT, BT, EP>(a, lds, v);
-    barrier();  // the staging area is read before the next tile's loads refill the ring
-  }
-}
-
-// Sum over the splits of K, in split order, of one 32 x 32 MFMA tile per workgroup: the
-// fp32 partials in fragment order -> bf16 rows of dx.
-template <class GE>
 __global__ __launch_bounds__(256) void head_join(HeadGemm a) {
   constexpr int PER = GE::NW * GE::WI * GE::WJ;  // MFMA tiles of a tile
-  settle<GE, X_IS_NONE>(a);
-  const int plane = a.tiles_m * a.tiles_n, t = blockIdx.x / PER, in = blockIdx.x % PER;
-  if (t >= plane) return;
-  const int g = t / (a.tiles_m * PATCH), r = t - g * a.tiles_m * PATCH, width = min(PATCH, a.tiles_n - g * PATCH);
-  const int tm = r / width, tn = g * PATCH + r - tm * width;
+  const HeadSize z = head_size<GE, X>(a);
+  const int nth = blockIdx.x / PER, in = blockIdx.x % PER, t = z.full + nth;
+  if (t >= z.tiles_m * z.tiles_n) return;
+  const int2 at = tile_place(t, z.tiles_m, z.tiles_n);
   const int wave = in / (GE::WI * GE::WJ), ij = in % (GE::WI * GE::WJ);
   const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
-  const int m = tm * GE::BM + (wave / GE::GN * GE::WI + ij / GE::WJ) * 32 + q * 8 + (lane >> 5) * 4;
-  const int n = tn * GE::BN + (wave % GE::GN * GE::WJ + ij % GE::WJ) * 32 + (lane & 31);
-  if (m >= a.M || n >= a.N) return;
-  const float* f = a.frag + (int64_t(t) * PER + in) * 1024 + threadIdx.x * 4;
+  const int m = at.x * GE::BM + (wave / GE::GN * GE::WI + ij / GE::WJ) * 32 + q * 8 + (lane >> 5) * 4;
+  const int n = at.y * GE::BN + (wave % GE::GN * GE::WJ + ij % GE::WJ) * 32 + (lane & 31);
+  if (m >= a.M || n >= z.N) return;
+  const float* f = a.frag + (int64_t(z.full + nth * z.S - a.frag_first) * PER + in) * 1024 + threadIdx.x * 4;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < a.S; ++k) {
-    const float4 u = *reinterpret_cast<const float4*>(f + int64_t(k) * plane * PER * 1024);
+#pragma unroll 8
+  for (int k = 0; k < z.S; ++k) {
+    const float4 u = *reinterpret_cast<const float4*>(f + int64_t(k) * PER * 1024);
     v[0] += u.x;
     v[1] += u.y;
     v[2] += u.z;
     v[3] += u.w;
   }
-  add_resid(a, n, m, v);
+  if (X == X_IS_NONE) add_resid(a, n, m, v);
   const float c = a.factor != nullptr ? *a.factor : 1.f;
-  *reinterpret_cast<uint2*>(a.out + int64_t(a.rows[n]) * a.ostride + int64_t(m) * 2) =
+  *reinterpret_cast<uint2*>(a.out + int64_t(X == X_IS_NONE ? a.rows[n] : n) * a.ostride + int64_t(m) * 2) =
       make_uint2(f2bf2(v[0] * c, v[1] * c), f2bf2(v[2] * c, v[3] * c));
 }
 
@@ -358,7 +580,7 @@ struct RowArgs {
   const int* rows;         // the token of a compact token
   const int* count;
   int t0, piece;
-  int64_t vocab;
+  int64_t vocab, ignore;
   const float* grad;       // per token, or null: 1
   float* nll;              // per token
   float* resid;            // per compact token
@@ -369,13 +591,19 @@ struct RowArgs {
 // (one wave where NTHR == 64); valid in every thread.
 template <int NTHR>
 __device__ __forceinline__ float join_parts(const float2* p, int n, float* scratch) {
+  constexpr int U = 4;
   float m = -INFINITY, s = 0.f;
-  for (int i = threadIdx.x % NTHR; i < n; i += NTHR) {
-    const float2 t = p[i];
-    // a part that is empty or all -inf has sum 0 and no maximum
-    const float top = t.y == 0.f ? m : fmaxf(m, t.x);
-    if (top != -INFINITY) s = s * __builtin_amdgcn_exp2f(m - top) + t.y * __builtin_amdgcn_exp2f(t.x - top);
-    else s += t.y;
+  for (int i = threadIdx.x % NTHR; i < n; i += NTHR * U) {
+    float2 t[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) t[u] = i + u * NTHR < n ? p[i + u * NTHR] : make_float2(0.f, 0.f);
+    float top = m;  // a part that is empty or all -inf has sum 0 and no maximum
+#pragma unroll
+    for (int u = 0; u < U; ++u) top = t[u].y == 0.f ? top : fmaxf(top, t[u].x);
+    const bool any = top != -INFINITY;
+    s = any ? s * __builtin_amdgcn_exp2f(m - top) : s;
+#pragma unroll
+    for (int u = 0; u < U; ++u) s += any && t[u].y != 0.f ? t[u].y * __builtin_amdgcn_exp2f(t[u].x - top) : t[u].y;
     m = top;
   }
   float top = wave_max(m);
@@ -402,12 +630,18 @@ __device__ __forceinline__ float token_nll(float lse2, float tlogit, int64_t y, 
   return (lse2 - tlogit * LOG2E) * LN2;
 }
 
-// The loss alone: one wave per token.
+// The loss alone: NTHR threads per token.  Without a list of compact tokens (rows null) every
+// token is one, ignored or not.
+template <int NTHR>
 __global__ __launch_bounds__(256) void head_nll(RowArgs a) {
-  const int tok = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (tok >= a.live()) return;
-  const float lse2 = join_parts<64>(a.parts + int64_t(tok) * a.nparts, a.nparts, nullptr);
-  if ((threadIdx.x & 63) == 0) a.nll[a.rows[tok]] = token_nll(lse2, a.tlogit[tok], a.target[tok], a.vocab);
+  __shared__ float scratch[8];
+  const int tok = blockIdx.x * (256 / NTHR) + threadIdx.x / NTHR;
+  if (tok >= (a.rows != nullptr ? a.live() : a.piece)) return;
+  const float lse2 = join_parts<NTHR>(a.parts + int64_t(tok) * a.nparts, a.nparts, scratch);
+  if (threadIdx.x % NTHR != 0) return;
+  const int64_t y = a.target[tok];
+  const float nll = y == a.ignore ? 0.f : token_nll(lse2, a.tlogit[tok], y, a.vocab);
+  a.nll[a.rows != nullptr ? a.rows[tok] : tok] = nll;
 }
 
 // One workgroup per token: lse, nll, and the row's codes -> dl.
@@ -488,7 +722,8 @@ __global__ __launch_bounds__(1024) void head_compact(const int64_t* target, int 
 }
 
 // One workgroup per row: the piece's rows of x gathered (nothing where no token is ignored),
-// and, with the first piece, the zeros of ignored tokens in dx and nll.
+// and, with the first piece, the zeros of ignored tokens in dx and nll.  head_list: both for
+// one piece of few tokens, each workgroup counting the tokens before its own.
 struct GatherArgs {
   const uint16_t* x;
   int64_t xstride;
@@ -500,33 +735,82 @@ struct GatherArgs {
   int64_t ignore;
   uint16_t* dx;  // or null
   float* nll;
+  int* list_rows;  // head_list: what head_compact writes
+  int64_t* list_target;
+  int* list_count;
+  float* list_inverse;
 };
+__device__ __forceinline__ void copy_row(const GatherArgs& a, int to, int token) {
+  const uint16_t* src = a.x + int64_t(token) * a.xstride;
+  for (int c = threadIdx.x * 8; c < a.width; c += 128 * 8)
+    *reinterpret_cast<uint4*>(a.xc + int64_t(to) * a.width + c) = *reinterpret_cast<const uint4*>(src + c);
+}
+__device__ __forceinline__ void ignored_row(const GatherArgs& a, int token) {
+  if (threadIdx.x == 0) a.nll[token] = 0.f;
+  if (a.dx != nullptr)
+    for (int c = threadIdx.x * 8; c < a.width; c += 128 * 8)
+      *reinterpret_cast<uint4*>(a.dx + int64_t(token) * a.width + c) = make_uint4(0, 0, 0, 0);
+}
 __global__ __launch_bounds__(128) void head_gather(GatherArgs a) {
   const int n = *a.count, j = blockIdx.x;
   if (n == a.tokens) return;
-  if (j < a.piece && a.t0 + j < n) {
-    const uint16_t* src = a.x + int64_t(a.rows[a.t0 + j]) * a.xstride;
-    for (int c = threadIdx.x * 8; c < a.width; c += 128 * 8)
-      *reinterpret_cast<uint4*>(a.xc + int64_t(j) * a.width + c) = *reinterpret_cast<const uint4*>(src + c);
+  if (j < a.piece && a.t0 + j < n) copy_row(a, j, a.rows[a.t0 + j]);
+  if (a.t0 == 0 && j < a.tokens && a.target[j] == a.ignore) ignored_row(a, j);
+}
+constexpr int LIST_TOKENS = 1024;
+__global__ __launch_bounds__(128) void head_list(GatherArgs a) {
+  __shared__ int part[4];
+  const int token = blockIdx.x;
+  int before = 0, all = 0;
+#pragma unroll
+  for (int u = 0; u < LIST_TOKENS / 128; ++u) {
+    const int t = u * 128 + threadIdx.x;
+    const bool is = t < a.tokens && a.target[t] != a.ignore;
+    before += is && t < token;
+    all += is;
   }
-  if (a.t0 == 0 && j < a.tokens && a.target[j] == a.ignore) {
-    if (threadIdx.x == 0) a.nll[j] = 0.f;
-    if (a.dx != nullptr)
-      for (int c = threadIdx.x * 8; c < a.width; c += 128 * 8)
-        *reinterpret_cast<uint4*>(a.dx + int64_t(j) * a.width + c) = make_uint4(0, 0, 0, 0);
+  before = wave_isum(before);
+  all = wave_isum(all);
+  if ((threadIdx.x & 63) == 0) {
+    part[threadIdx.x >> 6] = before;
+    part[2 + (threadIdx.x >> 6)] = all;
   }
+  __syncthreads();
+  before = part[0] + part[1];
+  all = part[2] + part[3];
+  const int64_t y = a.target[token];
+  if (threadIdx.x == 0 && token == 0) {
+    *a.list_count = all;
+    *a.list_inverse = all > 0 ? 1.f / float(all) : 0.f;
+  }
+  if (y == a.ignore) {
+    ignored_row(a, token);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    a.list_rows[before] = token;
+    a.list_target[before] = y;
+  }
+  if (all != a.tokens) copy_row(a, before, token);
 }
 
-// sum of nll, divided by the number of targets that are not ignored where mean (NaN if there
-// is none): each thread's share in order, then a tree (the same order every time)
-__global__ __launch_bounds__(1024) void head_loss(const float* nll, int tokens, const int* count, int mean,
-                                                  float* loss) {
+// The loss without a list: the targets are counted here
+__global__ __launch_bounds__(1024) void head_loss(const float* nll, int tokens, const int* count,
+                                                  const int64_t* target, int64_t ignore, int mean, float* loss) {
   __shared__ float scratch[16];
-  float s = 0.f;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < tokens; i += 1024) s += nll[i];
-  s = block_sum<1024>(s, scratch);
-  if (threadIdx.x == 0) *loss = mean ? s / float(*count) : s;
+  __shared__ int found[16];
+  int c = 0;
+  if (count == nullptr) {
+    for (int i = threadIdx.x; i < tokens; i += 1024) c += target[i] != ignore;
+    c = wave_isum(c);
+    if ((threadIdx.x & 63) == 0) found[threadIdx.x >> 6] = c;
+    c = 0;
+    __syncthreads();
+    for (int w = 0; w < 16; ++w) c += found[w];
+  } else {
+    c = *count;
+  }
+  sum_loss<1024>(nll, tokens, c, mean, loss, scratch);
 }
 
 __global__ __launch_bounds__(256) void head_zero(uint4* x, int64_t chunks) {
@@ -534,56 +818,124 @@ __global__ __launch_bounds__(256) void head_zero(uint4* x, int64_t chunks) {
     x[i] = make_uint4(0, 0, 0, 0);
 }
 
-// x *= *c, in 16-B chunks; nothing is touched where *c == 1
-__global__ __launch_bounds__(256) void head_scale(uint16_t* x, int64_t chunks, const float* c) {
+// x and y *= *c, in 16-B chunks; nothing is touched where *c == 1
+__global__ __launch_bounds__(256) void head_scale(uint16_t* x, int64_t nx, uint16_t* y, int64_t ny, const float* c) {
   const float f = *c;
   if (f == 1.f) return;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < chunks; i += int64_t(gridDim.x) * 256) {
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < nx + ny; i += int64_t(gridDim.x) * 256) {
+    uint16_t* p = i < nx ? x + i * 8 : y + (i - nx) * 8;
     float v[8];
-    Vec8<BF16T>::load(x + i * 8, v);
+    Vec8<BF16T>::load(p, v);
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] *= f;
-    Vec8<BF16T>::store(x + i * 8, v);
+    Vec8<BF16T>::store(p, v);
   }
 }
 
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-typedef Geo<2, 4, 4, 2, 4> H256;  // 256 x 256 tiles, one workgroup per CU
+// Tiles: 256 of the first operand (vocabulary, or width) x 256 or 128 of the second, eight
+// waves, one workgroup per CU
+typedef Geo<2, 4, 4, 2, 4> H256;
+typedef Geo<4, 2, 2, 2, 4> H128;
 
-// M, N, K with all of the piece's tokens valid (settle: the real ones)
-template <class GE>
-void set_tiles(HeadGemm& a, int M, int N, int K, int S) {
+// A product's tile, and the parts of K (S) of the tiles from `full` on.
+struct HeadPlan {
+  bool narrow;  // H128
+  int full, S;
+  int cols() const { return narrow ? 128 : 256; }
+  int part_shift() const { return narrow ? 6 : 7; }  // vocabulary of a wave of the logits
+  int tiles(int64_t m, int64_t n) const { return cdiv(m, 256) * cdiv(n, cols()); }
+  int virtual_tiles(int64_t m, int64_t n) const {
+    const int t = tiles(m, n), f = std::min(full, t);
+    return f + (t - f) * S;
+  }
+  // fp32 accumulators: of the split tiles, or of all
+  size_t frag(int64_t m, int64_t n, bool all) const {
+    return size_t(virtual_tiles(m, n) - (all ? 0 : std::min(full, tiles(m, n)))) * 256 * cols() * 4;
+  }
+};
+
+// Time in ns of a product M x N x K on a 256-CU part (a function of the sizes only, so the order
+// of the sums does not depend on the device): rounds of 256 tiles, each its slices of K at the
+// rate of full rounds and what its start and end cost.  Measured at V = 50304: loss of 4096 x
+// 4096 1.37 ms in 256-wide tiles, 1.80 in 128-wide; 600 x 512 58.6 / 53.7 us, 300 x 4096 198 /
+// 208, 128 x 2048 51 / 47 (x 64-wide 55).
+int64_t round_time(bool narrow, int64_t K) { return narrow ? 1500 + 18 * K : 2500 + 25 * K; }
+int64_t plan_time(const HeadPlan& p, int64_t M, int64_t N, int64_t K) {
+  const int64_t tiles = p.tiles(M, N), full = std::min<int64_t>(p.full, tiles), parts = (tiles - full) * p.S;
+  int64_t t = cdiv(full, 256) * round_time(p.narrow, K) + cdiv(parts, 256) * round_time(p.narrow, cdiv(K, p.S));
+  // the partials' write and read, the join's launch
+  if (parts > 0) t += 5000 + parts * 256 * p.cols() * 8 / 4500;
+  return t;
+}
+constexpr int WHOLE = 1 << 30;  // no tile is split
+
+// The logits: K is not split (a part of a sum has no exponential).
+HeadPlan logits_plan(int64_t T, int64_t D, int64_t V) {
+  const HeadPlan wide{false, WHOLE, 1}, narrow{true, WHOLE, 1};
+  return plan_time(narrow, V, T, D) < plan_time(wide, V, T, D) ? narrow : wide;
+}
+// The gradients: all tiles split (few tokens or a narrow model: dx has few tiles), or those of
+// the last round, that would leave most CUs idle.  At least 256 of K in a part; partials
+// of at most 256 MiB.
+HeadPlan grad_plan(int64_t M, int64_t N, int64_t K, bool narrow_too) {
+  HeadPlan best{false, WHOLE, 1};
+  int64_t best_time = plan_time(best, M, N, K);
+  for (int narrow = 0; narrow <= (narrow_too ? 1 : 0); ++narrow) {
+    const int tiles = HeadPlan{narrow != 0, WHOLE, 1}.tiles(M, N);
+    for (const int full : {WHOLE, 0, tiles / 256 * 256})
+      for (int S = full == WHOLE ? 1 : 2; S <= (full == WHOLE ? 1 : 256) && (S == 1 || K / S >= 256); ++S) {
+        const HeadPlan p{narrow != 0, full, S};
+        if (p.frag(M, N, false) > (size_t(1) << 28)) break;
+        const int64_t t = plan_time(p, M, N, K);
+        if (t < best_time) best = p, best_time = t;
+      }
+  }
+  return best;
+}
+
+// M, N, K with all of the piece's tokens valid (head_size: the real ones)
+void set_tiles(HeadGemm& a, int M, int N, int K, HeadPlan p) {
   a.M = M;
   a.N = N;
   a.K = K;
-  a.kchunk = cdiv(cdiv(K, S), BK) * BK;
-  a.S = cdiv(K, a.kchunk);
-  a.tiles_m = cdiv(M, GE::BM);
-  a.tiles_n = cdiv(N, GE::BN);
+  a.tiles_m = cdiv(M, 256);
+  a.tiles_n = cdiv(N, p.cols());
+  a.full = p.full;
+  a.S = p.S;
 }
 
 template <class GE, bool AT, bool BT, int EP, int X>
-void launch_head(const HeadGemm& a, hipStream_t s) {
-  const int grid = std::min(cdiv(int64_t(a.tiles_m) * a.tiles_n * a.S, 8) * 8, resident_grid(1 << 30) * GE::PER_CU);
+void launch_tile(const HeadGemm& a, int tiles, hipStream_t s) {
+  const int grid = std::min((tiles + 7) / 8 * 8, resident_grid(1 << 30) * GE::PER_CU);
   hipLaunchKernelGGL((head_gemm<GE, AT, BT, EP, X>), dim3(grid), dim3(GE::NTH), 0, s, a);
 }
-
-// Splits of K = V of the dx product: its tiles (tokens x width) may not fill the chip.
-// At least 2048 of K per split.
-int dx_splits(int64_t tokens, int64_t width, int64_t vocab) {
-  const int64_t tiles = cdiv(tokens, 256) * int64_t(cdiv(width, 256));
-  return int(std::max<int64_t>(1, std::min<int64_t>(256 / tiles, vocab / 2048)));
+template <bool AT, bool BT, int EP, int X>
+void launch_head(const HeadGemm& a, HeadPlan p, hipStream_t s) {
+  const int tiles = p.virtual_tiles(a.M, a.N);
+  if (p.narrow) launch_tile<H128, AT, BT, EP, X>(a, tiles, s);
+  else launch_tile<H256, AT, BT, EP, X>(a, tiles, s);
 }
-
-constexpr int PART_SHIFT = 7;  // a wave of the 256-wide tile holds 128 of the vocabulary
+template <class GE, int X>
+void launch_join_tile(const HeadGemm& a, hipStream_t s) {
+  const int split = a.tiles_m * a.tiles_n - a.full;
+  if (split > 0)
+    hipLaunchKernelGGL((head_join<GE, X>), dim3(split * GE::NW * GE::WI * GE::WJ), dim3(256), 0, s, a);
+}
+template <int X>
+void launch_join(const HeadGemm& a, HeadPlan p, hipStream_t s) {
+  if (p.narrow) launch_join_tile<H128, X>(a, s);
+  else launch_join_tile<H256, X>(a, s);
+}
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 struct Layout {
   int64_t piece, ldc;
-  int nparts, splits;
+  int nparts;
+  HeadPlan logits, dx, dw;
   size_t codes, xc, parts, tlogit, resid, dxfrag, dwfrag, nll, rows, compact, count, inverse, total;
 };
 
@@ -592,22 +944,25 @@ Layout head_layout(const mmuon_ce_args& x, bool train) {
   const int64_t T = std::max<int64_t>(x.tokens, 1);
   l.piece = std::min(T, std::max<int64_t>(1, x.piece_tokens));
   l.ldc = int64_t(cdiv(x.vocab, 256)) * 256;
-  l.nparts = cdiv(x.vocab, 1 << PART_SHIFT);
-  l.splits = dx_splits(l.piece, x.width, x.vocab);
+  l.logits = logits_plan(l.piece, x.width, x.vocab);
+  l.dx = grad_plan(x.width, l.piece, x.vocab, true);
+  // (128-wide tiles gained nothing there: 1000 x 512 54 us in 256-wide, 68 in 128-wide)
+  l.dw = grad_plan(x.width, x.vocab, l.piece, false);
+  l.nparts = cdiv(x.vocab, 1 << l.logits.part_shift());
   size_t at = 0;
   const auto take = [&at](size_t n) {
     const size_t here = at;
     at += up256(n);
     return here;
   };
-  const size_t P = size_t(l.piece), tile = 256 * 256 * 4;
+  const size_t P = size_t(l.piece);
   l.codes = take(train ? P * l.ldc * 2 : 0);
   l.xc = take(P * x.width * 2);
   l.parts = take(P * l.nparts * 8);
   l.tlogit = take(P * 4);
   l.resid = take(train ? P * 4 : 0);
-  l.dxfrag = take(train && l.splits > 1 ? tile * l.splits * cdiv(l.piece, 256) * cdiv(x.width, 256) : 0);
-  l.dwfrag = take(train && T > l.piece ? tile * cdiv(x.width, 256) * cdiv(x.vocab, 256) : 0);
+  l.dxfrag = take(train ? l.dx.frag(x.width, l.piece, false) : 0);
+  l.dwfrag = take(train ? l.dw.frag(x.width, x.vocab, T > l.piece) : 0);
   l.nll = take(x.nll == nullptr ? size_t(T) * 4 : 0);
   l.rows = take(size_t(T) * 4);
   l.compact = take(size_t(T) * 8);
@@ -629,12 +984,16 @@ int launch_ce(const mmuon_ce_args& x, bool train, hipStream_t st) {
   int64_t* target = reinterpret_cast<int64_t*>(ws + l.compact);
   int* count = reinterpret_cast<int*>(ws + l.count);
   float* inverse = reinterpret_cast<float*>(ws + l.inverse);
-  const bool mean = x.reduction == MMUON_CE_MEAN;
+  const bool mean = x.reduction == MMUON_CE_MEAN, reduced = x.reduction != MMUON_CE_NONE;
   const int T = int(x.tokens), V = int(x.vocab), P = int(l.piece);
   if (train && x.dw != nullptr && T == 0)
     hipLaunchKernelGGL(head_zero, dim3(1024), dim3(256), 0, st, static_cast<uint4*>(x.dw), x.vocab * x.width / 8);
-  hipLaunchKernelGGL(head_compact, dim3(1), dim3(1024), 0, st, x.target, T, x.ignore_index, rows, target, count,
-                     inverse);
+  // the loss of one column of tiles: leaving tokens out would not make it less
+  const bool list = train || T > 256 || T > P;
+  const bool one = T <= LIST_TOKENS && T <= P;  // head_list
+  if (list && !one)
+    hipLaunchKernelGGL(head_compact, dim3(1), dim3(1024), 0, st, x.target, T, x.ignore_index, rows, target, count,
+                       inverse);
   for (int t0 = 0; t0 < T; t0 += P) {
     const int n = std::min(P, T - t0);
     GatherArgs ga{};
@@ -651,12 +1010,17 @@ int launch_ce(const mmuon_ce_args& x, bool train, hipStream_t st) {
     ga.ignore = x.ignore_index;
     ga.dx = train ? static_cast<uint16_t*>(x.dx) : nullptr;
     ga.nll = nll;
-    hipLaunchKernelGGL(head_gather, dim3(t0 == 0 ? T : n), dim3(128), 0, st, ga);
+    ga.list_rows = rows;
+    ga.list_target = target;
+    ga.list_count = count;
+    ga.list_inverse = inverse;
+    if (list && one) hipLaunchKernelGGL(head_list, dim3(T), dim3(128), 0, st, ga);
+    else if (list) hipLaunchKernelGGL(head_gather, dim3(t0 == 0 ? T : n), dim3(128), 0, st, ga);
 
     HeadGemm f{};  // logits (vocabulary x tokens) = w . x^T
     f.a = make_op(x.w, 0, x.w_stride * 2, 2, V);
     f.b = make_op(ga.xc, 0, int64_t(x.width) * 2, 2, n);
-    f.count = count;
+    f.count = list ? count : nullptr;
     f.t0 = t0;
     f.piece = n;
     f.tokens = T;
@@ -667,30 +1031,32 @@ int launch_ce(const mmuon_ce_args& x, bool train, hipStream_t st) {
     f.ldc = l.ldc;
     f.parts = reinterpret_cast<float2*>(ws + l.parts);
     f.nparts = l.nparts;
-    f.target = target + t0;
+    f.target = list ? target + t0 : x.target;
     f.tlogit = reinterpret_cast<float*>(ws + l.tlogit);
-    set_tiles<H256>(f, V, n, x.width, 1);
-    if (train) launch_head<H256, false, false, EP_CODES, X_IS_B>(f, st);
-    else launch_head<H256, false, false, EP_STATS, X_IS_B>(f, st);
+    set_tiles(f, V, n, x.width, l.logits);
+    if (train) launch_head<false, false, EP_CODES, X_IS_B>(f, l.logits, st);
+    else launch_head<false, false, EP_STATS, X_IS_B>(f, l.logits, st);
 
     RowArgs r{};
     r.codes = f.codes;
     r.ldc = l.ldc;
     r.parts = f.parts;
     r.nparts = l.nparts;
-    r.part_shift = PART_SHIFT;
+    r.part_shift = l.logits.part_shift();
     r.tlogit = f.tlogit;
     r.target = f.target;
-    r.rows = rows + t0;
+    r.rows = list ? rows + t0 : nullptr;
     r.count = count;
     r.t0 = t0;
     r.piece = n;
     r.vocab = V;
+    r.ignore = x.ignore_index;
     r.grad = x.grad;
     r.nll = nll;
     r.resid = reinterpret_cast<float*>(ws + l.resid);
     if (!train) {
-      hipLaunchKernelGGL(head_nll, dim3(cdiv(n, 4)), dim3(256), 0, st, r);
+      if (n <= 2048) hipLaunchKernelGGL(head_nll<256>, dim3(n), dim3(256), 0, st, r);
+      else hipLaunchKernelGGL(head_nll<64>, dim3(cdiv(n, 4)), dim3(256), 0, st, r);
       continue;
     }
     hipLaunchKernelGGL(head_rows, dim3(n), dim3(256), 0, st, r);
@@ -707,14 +1073,10 @@ int launch_ce(const mmuon_ce_args& x, bool train, hipStream_t st) {
       d.w = static_cast<const uint16_t*>(x.w);
       d.wstride = x.w_stride;
       d.frag = reinterpret_cast<float*>(ws + l.dxfrag);
-      set_tiles<H256>(d, x.width, n, V, l.splits);
-      if (d.S > 1) {
-        launch_head<H256, true, false, EP_FRAG, X_IS_NONE>(d, st);
-        hipLaunchKernelGGL(head_join<H256>, dim3(d.tiles_m * d.tiles_n * H256::NW * H256::WI * H256::WJ), dim3(256), 0,
-                           st, d);
-      } else {
-        launch_head<H256, true, false, EP_ROWS, X_IS_NONE>(d, st);
-      }
+      set_tiles(d, x.width, n, V, l.dx);
+      d.frag_first = std::min(d.full, d.tiles_m * d.tiles_n);
+      launch_head<true, false, EP_ROWS, X_IS_NONE>(d, l.dx, st);
+      launch_join<X_IS_NONE>(d, l.dx, st);
     }
     if (x.dw != nullptr) {
       HeadGemm d = f;  // dw^T (width x vocabulary) = x^T dl
@@ -724,22 +1086,30 @@ int launch_ce(const mmuon_ce_args& x, bool train, hipStream_t st) {
       d.ostride = int64_t(x.width) * 2;
       d.factor = factor;
       d.frag = reinterpret_cast<float*>(ws + l.dwfrag);
-      d.start = t0 > 0 ? d.frag : nullptr;
-      set_tiles<H256>(d, x.width, V, n, 1);
-      if (t0 + n < T) launch_head<H256, true, true, EP_FRAG, X_IS_A>(d, st);
-      else launch_head<H256, true, true, EP_ROWS, X_IS_A>(d, st);
+      d.start = t0 > 0;
+      d.keep = t0 + n < T;
+      set_tiles(d, x.width, V, n, l.dw);
+      d.frag_first = T > P ? 0 : std::min(d.full, d.tiles_m * d.tiles_n);
+      if (!d.keep) {
+        d.nll = reduced ? nll : nullptr;
+        d.loss = x.loss;
+        d.mean = mean ? 1 : 0;
+      }
+      launch_head<true, true, EP_ROWS, X_IS_A>(d, l.dw, st);
+      if (!d.keep) launch_join<X_IS_A>(d, l.dw, st);
     }
   }
-  if (x.loss != nullptr && x.reduction != MMUON_CE_NONE)
-    hipLaunchKernelGGL(head_loss, dim3(1), dim3(1024), 0, st, nll, T, count, mean ? 1 : 0, x.loss);
+  if (reduced && !(train && x.dw != nullptr && T > 0))
+    hipLaunchKernelGGL(head_loss, dim3(1), dim3(1024), 0, st, nll, T, list && T > 0 ? count : nullptr, x.target,
+                       x.ignore_index, mean ? 1 : 0, x.loss);
   return 0;
 }
 
-int launch_ce_scale(void* x, int64_t numel, const float* c, hipStream_t st) {
-  const int64_t chunks = numel / 8;
+int launch_ce_scale(void* x, int64_t nx, void* y, int64_t ny, const float* c, hipStream_t st) {
+  const int64_t chunks = (nx + ny) / 8;
   if (chunks > 0)
-    hipLaunchKernelGGL(head_scale, dim3(unsigned(std::min<int64_t>((chunks + 255) / 256, 4096))), dim3(256), 0, st,
-                       static_cast<uint16_t*>(x), chunks, c);
+    hipLaunchKernelGGL(head_scale, dim3(unsigned(std::min<int64_t>((chunks + 255) / 256, 2048))), dim3(256), 0, st,
+                       static_cast<uint16_t*>(x), nx / 8, static_cast<uint16_t*>(y), ny / 8, c);
   return 0;
 }
 

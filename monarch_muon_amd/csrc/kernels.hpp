@@ -94,7 +94,7 @@ int launch_butterfly_bwd(const mmuon_butterfly_args& a, bool features, hipStream
 // Cross entropy of a linear head ---------------------------------------------------
 size_t ce_workspace(const mmuon_ce_args& a, bool train);
 int launch_ce(const mmuon_ce_args& a, bool train, hipStream_t s);
-int launch_ce_scale(void* x, int64_t numel, const float* factor, hipStream_t s);
+int launch_ce_scale(void* x, int64_t nx, void* y, int64_t ny, const float* factor, hipStream_t s);
 
 // Token embedding ------------------------------------------------------------------
 size_t embedding_workspace(const mmuon_embedding_args& a);

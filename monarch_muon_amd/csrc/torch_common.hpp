@@ -25,7 +25,7 @@ struct Abi {
   int (*ce_fwd)(const mmuon_ce_args*, void*) = nullptr;
   int (*ce_fwd_bwd)(const mmuon_ce_args*, void*) = nullptr;
   size_t (*ce_workspace)(const mmuon_ce_args*, int32_t) = nullptr;
-  int (*scale)(void*, int64_t, const float*, void*) = nullptr;
+  int (*scale)(void*, int64_t, void*, int64_t, const float*, void*) = nullptr;
   int (*emb_fwd)(const mmuon_embedding_args*, void*) = nullptr;
   int (*emb_bwd)(const mmuon_embedding_args*, void*) = nullptr;
   size_t (*emb_workspace)(const mmuon_embedding_args*) = nullptr;

@@ -138,17 +138,18 @@ Triple grad_impl(const Tensor& x, const Tensor& w, const Tensor& target, const c
   return {out, dx, dw};
 }
 
-// x *= factor (a float32 scalar on the device)
-void scale_impl(const Tensor& x, const Tensor& factor) {
-  TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16 && factor.scalar_type() == at::kFloat,
-                   "scale_ takes a bfloat16 tensor and a float32 factor");
-  TORCH_CHECK_VALUE(x.is_contiguous() && x.numel() % 8 == 0 && factor.numel() == 1,
-                    "scale_ takes a contiguous tensor of whole 16-byte chunks and one factor");
-  require_one_device({&x, &factor});
+// x and y *= factor (a float32 scalar on the device)
+void scale_impl(const Tensor& x, const Tensor& y, const Tensor& factor) {
+  for (const Tensor* t : {&x, &y}) {
+    TORCH_CHECK_TYPE(t->scalar_type() == at::kBFloat16, "scale_ takes bfloat16 tensors");
+    TORCH_CHECK_VALUE(t->is_contiguous() && t->numel() % 8 == 0, "scale_ takes contiguous tensors of whole 16-byte chunks");
+  }
+  TORCH_CHECK_VALUE(factor.numel() == 1 && factor.scalar_type() == at::kFloat, "scale_ takes one float32 factor");
+  require_one_device({&x, &y, &factor});
   bind_library();
   const c10::DeviceGuard guard(x.device());
-  check_rc(abi.scale(x.data_ptr(), x.numel(), static_cast<const float*>(factor.const_data_ptr()), stream_of(x)),
-           "mmuon_scale_bf16");
+  check_rc(abi.scale(x.data_ptr(), x.numel(), y.data_ptr(), y.numel(),
+                     static_cast<const float*>(factor.const_data_ptr()), stream_of(x)), "mmuon_scale_bf16");
 }
 
 Tensor call_loss(const Tensor& x, const Tensor& w, const Tensor& target, int64_t ignore_index, int64_t reduction,
@@ -166,11 +167,11 @@ Triple call_grad(const Tensor& x, const Tensor& w, const Tensor& target, const c
                                      int64_t, int64_t, bool, bool)>();
   return op.call(x, w, target, grad, ignore_index, reduction, piece, need_dx, need_dw);
 }
-void call_scale(const Tensor& x, const Tensor& factor) {
+void call_scale(const Tensor& x, const Tensor& y, const Tensor& factor) {
   static auto op = c10::Dispatcher::singleton()
                        .findSchemaOrThrow("mmuon::scale_", "")
-                       .typed<void(const Tensor&, const Tensor&)>();
-  op.call(x, factor);
+                       .typed<void(const Tensor&, const Tensor&, const Tensor&)>();
+  op.call(x, y, factor);
 }
 
 struct LossFn : torch::autograd::Function<LossFn> {
@@ -208,9 +209,7 @@ struct LossFn : torch::autograd::Function<LossFn> {
       ctx->saved_data["spent"] = true;
       gx = saved[0];
       gw = saved[1];
-      const Tensor factor = grads[0].to(at::kFloat);
-      if (dx) call_scale(gx, factor);
-      if (dw) call_scale(gw, factor);
+      call_scale(gx, gw, grads[0].to(at::kFloat));
     }
     return {dx ? gx : Tensor(), dw ? gw : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
@@ -346,7 +345,7 @@ TORCH_LIBRARY_FRAGMENT(mmuon, m) {
   m.def("linear_cross_entropy_grad(Tensor x, Tensor weight, Tensor target, Tensor? grad, int ignore_index, int "
         "reduction, int piece_tokens, bool need_dx, bool need_dw) -> (Tensor, Tensor, Tensor)",
         {at::Tag::pt2_compliant_tag});
-  m.def("scale_(Tensor(a!) x, Tensor factor) -> ()", {at::Tag::pt2_compliant_tag});
+  m.def("scale_(Tensor(a!) x, Tensor(b!) y, Tensor factor) -> ()", {at::Tag::pt2_compliant_tag});
   m.def("embedding(Tensor index, Tensor weight, float scale, int padding_idx) -> Tensor",
         {at::Tag::pt2_compliant_tag});
   m.def("embedding_grad(Tensor dout, Tensor index, SymInt vocab, float scale, int padding_idx) -> Tensor",

@@ -36,7 +36,7 @@ def _load() -> None:
                 x.new_empty(x.shape if need_dx else (0,)), weight.new_empty(weight.shape if need_dw else (0,)))
 
     @torch.library.register_fake("mmuon::scale_")
-    def _(x, factor):
+    def _(x, y, factor):
         return None
 
     @torch.library.register_fake("mmuon::embedding")

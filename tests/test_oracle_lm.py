@@ -120,7 +120,8 @@ def test_entry_points_validate_before_launching():
                                   ({"dw": 24584}, -1, b"unaligned dx or dw"), ({"workspace": 32770}, -1, b"256-B")]:
         assert lib.mmuon_ce_fwd_bwd(C.byref(_abi.CeArgs(**{**good, **change})), None) == code, change
         assert message in lib.mmuon_last_error(), (change, lib.mmuon_last_error())
-    assert lib.mmuon_scale_bf16(4096, 12, 8192, None) == -1 and lib.mmuon_scale_bf16(4100, 16, 8192, None) == -1
+    assert lib.mmuon_scale_bf16(4096, 12, None, 0, 8192, None) == lib.mmuon_scale_bf16(4100, 16, None, 0, 8192, None) == -1
+    assert lib.mmuon_scale_bf16(4096, 16, None, 8, 8192, None) == -1
     emb = dict(tokens=4, vocab=100, width=7, dtype=_abi.F32, scale=1.0, padding_idx=-1, w_stride=7, dout_stride=7,
                index=4096, w=8192, out=12288, dout=16384, dw=20480, workspace=32768, workspace_bytes=0)
     for change, code, message in [({}, -1, b"workspace of"), ({"dtype": _abi.F8E4M3}, -1, b"dtype"),
