@@ -6,8 +6,8 @@
 // class v % C), one workgroup each.  A workgroup reads all ids, places the positions of its
 // rows in token order (counts per row and wave, then a stable rank), and writes zeros to the
 // rows that no token has.  Common words have neighbouring ids, so the rows of a class are far
-// apart.  A second launch sums the positions in fp32, SEG to a wave whatever rows they are
-// of; a third joins the pieces of rows that lie in several SEGs, in order.
+// apart.  A second launch sums the positions in fp32, a segment of them to a wave whatever
+// rows they are of; a third joins the pieces of rows that lie in several segments, in order.
 #include <algorithm>
 #include <type_traits>
 
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256) void embed_lookup(mmuon_embedding_args a, int 
   }
 }
 
-constexpr int SEG = 32;  // positions that one wave sums
+constexpr int MAX_SEG = 32;  // positions that one wave sums, at most; 8, 16 or 32 (segment)
 
 // The positions that have a gradient, class after class, row after row, in token order: the
 // token and the row of each, at a row's first one how many it has, and how many there are.
@@ -57,11 +57,12 @@ struct GradSpace {
   int* row;
   int* count;
   int* all;
-  float* sums;  // of the pieces of rows that lie in several SEGs: two for each SEG
+  float* sums;  // of the pieces of rows that lie in several segments: two for each segment
 };
 
-// WAVES waves, ROWS rows of a class at most, LIST ids of a class that a wave keeps from its scan
-template <class T, int N, int WAVES, int ROWS, int LIST>
+// WAVES waves, ROWS rows of a class at most, LIST ids of a class that a wave keeps from its scan;
+// FIRST: zeros to all rows before, not to the empty ones behind
+template <class T, int N, int WAVES, int ROWS, int LIST, bool FIRST>
 __global__ __launch_bounds__(64 * WAVES) void embed_rows(mmuon_embedding_args a, int log2c, GradSpace space) {
   constexpr int NTH = 64 * WAVES;
   static_assert(ROWS % NTH == 0 || NTH % ROWS == 0, "rows are scanned by whole workgroups");
@@ -73,6 +74,17 @@ __global__ __launch_bounds__(64 * WAVES) void embed_rows(mmuon_embedding_args a,
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rows = int((a.vocab - c + C - 1) >> log2c);
   const uint64_t before = (uint64_t(1) << lane) - 1;
+  const auto zero_rows = [&](auto which) {
+    const float zero[N] = {};
+    const int chunks = (a.width + 64 * N - 1) / (64 * N);
+    for (int task = wave; task < rows * chunks; task += WAVES) {
+      const int r = task / chunks, col = (task - r * chunks) * 64 * N + lane * N;
+      if (which(r) && col < a.width)
+        store_n<T, N>(static_cast<typename T::storage*>(a.dw) + (int64_t(r) * C + c) * a.width + col, zero);
+    }
+  };
+  // few ids: most rows are empty, and all zeros are on their way while the ids are read
+  if constexpr (FIRST) zero_rows([](int) { return true; });
   for (int i = threadIdx.x; i < WAVES * rows; i += NTH) at[i / rows][i % rows] = 0;
   __syncthreads();
   // a wave's tokens: a run of whole 64s
@@ -164,27 +176,20 @@ __global__ __launch_bounds__(64 * WAVES) void embed_rows(mmuon_embedding_args a,
     for (int64_t t = t0; t < t1; t += 64) put(row_of(t + lane < t1 ? a.index[t + lane] : -1), t + lane);
   }
   __syncthreads();
-  // the rows that no token has
-  const float zero[N] = {};
-  const int chunks = (a.width + 64 * N - 1) / (64 * N);
-  for (int task = wave; task < rows * chunks; task += WAVES) {
-    const int r = task / chunks, col = (task - r * chunks) * 64 * N + lane * N;
-    if (first[r + 1] == first[r] && col < a.width)
-      store_n<T, N>(static_cast<typename T::storage*>(a.dw) + (int64_t(r) * C + c) * a.width + col, zero);
-  }
+  if constexpr (!FIRST) zero_rows([&](int r) { return first[r + 1] == first[r]; });
 }
 
-// Sums in fp32: a wave takes 64 N columns of SEG positions, eight loads in flight, and writes
+// Sums in fp32: a wave takes 64 N columns of a segment, eight loads in flight, and writes
 // the rows that end in it; a row's piece that goes on, or began before, is left in sums (the
-// first piece of SEG i in 2 i, the last in 2 i + 1).
+// first piece of segment i in 2 i, the last in 2 i + 1).
 template <class T, int N>
-__global__ __launch_bounds__(256) void embed_sum(mmuon_embedding_args a, GradSpace space) {
+__global__ __launch_bounds__(256) void embed_sum(mmuon_embedding_args a, int each, GradSpace space) {
   const int all = *space.all;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int chunks = (a.width + 64 * N - 1) / (64 * N);
   const int64_t item = int64_t(blockIdx.x) * 4 + wave;
   const int seg = int(item / chunks), col = int(item - int64_t(seg) * chunks) * 64 * N + lane * N;
-  const int p0 = seg * SEG, n = min(SEG, all - p0);
+  const int p0 = seg * each, n = min(each, all - p0);
   if (n <= 0) return;
   // lanes 0 .. n - 1: the positions; lane n: the one after, lane 63: the one before (rows only)
   const int at = lane <= n ? p0 + lane : p0 - 1;
@@ -224,25 +229,25 @@ __global__ __launch_bounds__(256) void embed_sum(mmuon_embedding_args a, GradSpa
       for (int k = 0; k < N; ++k) s[k] = 0.f;
     }
   }
-  if (!(ends >> (n - 1) & 1)) piece(first ? 0 : 1);  // goes on in the next SEG
+  if (!(ends >> (n - 1) & 1)) piece(first ? 0 : 1);  // goes on in the next segment
 }
 
-// The rows that lie in several SEGs: a workgroup sums 32 N columns of the row that goes on from
-// its SEG, if it begins there; 8 runs of the row's pieces side by side, joined in order.
+// The rows that lie in several segments: a workgroup sums 32 N columns of the row that goes on
+// from its segment, if it begins there; 8 runs of the row's pieces side by side, joined in order.
 template <class T, int N>
-__global__ __launch_bounds__(256) void embed_join(mmuon_embedding_args a, GradSpace space) {
+__global__ __launch_bounds__(256) void embed_join(mmuon_embedding_args a, int size, GradSpace space) {
   constexpr int LANES = 32, RUNS = 256 / LANES, SLICE = LANES * N;
   __shared__ float sums[RUNS][SLICE];
   const int all = *space.all, slices = (a.width + SLICE - 1) / SLICE;
-  const int seg = blockIdx.x / slices, slice = blockIdx.x % slices, p0 = seg * SEG;
-  if (p0 + SEG >= all) return;
-  const int r = space.row[p0 + SEG];
-  if (space.row[p0 + SEG - 1] != r) return;
-  const int lead = threadIdx.x & (SEG - 1);  // the row's first position, among this SEG's
+  const int seg = blockIdx.x / slices, slice = blockIdx.x % slices, p0 = seg * size;
+  if (p0 + size >= all) return;
+  const int r = space.row[p0 + size];
+  if (space.row[p0 + size - 1] != r) return;
+  const int lead = threadIdx.x & (size - 1);  // the row's first position, among this segment's
   const uint64_t mine = __ballot(space.row[p0 + lead] == r);
   const int f = p0 + __ffsll(static_cast<unsigned long long>(mine)) - 1;
   if (f == p0 && p0 > 0 && space.row[p0 - 1] == r) return;  // began before
-  const int pieces = (f + space.count[f] - 1) / SEG - seg + 1;
+  const int pieces = (f + space.count[f] - 1) / size - seg + 1;
   const int run = threadIdx.x / LANES, lane = threadIdx.x % LANES, col = slice * SLICE + lane * N;
   const int each = (pieces + RUNS - 1) / RUNS, k1 = min((run + 1) * each, pieces);
   float s[N];
@@ -251,7 +256,7 @@ __global__ __launch_bounds__(256) void embed_join(mmuon_embedding_args a, GradSp
   if (col < a.width) {
 #pragma unroll 8
     for (int i = run * each; i < k1; ++i) {
-      // the row is the last of its first SEG and the first of the others
+      // the row is the last of its first segment and the first of the others
       const int slot = 2 * (seg + i) + (i == 0 && f > p0 ? 1 : 0);
       float x[N];
       load_n<F32T, N>(space.sums + int64_t(slot) * a.width + col, x);
@@ -298,13 +303,22 @@ int log2_classes(int64_t tokens, int64_t vocab) {
   return l;
 }
 
+// Positions of a segment: the most that leave eight waves per CU something to sum (1000 tokens
+// of 512 columns: 32 at a time 10.5 us, 8 at a time 5).
+int segment(int64_t tokens, int64_t width, int columns) {
+  int n = MAX_SEG;
+  while (n > 8 && (tokens + n - 1) / n * ((width + columns - 1) / columns) < 2048) n /= 2;
+  return n;
+}
+
 struct GradLayout {
   size_t token, row, count, all, total;  // the sums come first
 };
 GradLayout grad_layout(int64_t tokens, int64_t width) {
   GradLayout l;
   const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  l.token = up(size_t(tokens > SEG ? (tokens + SEG - 1) / SEG : 0) * 2 * width * 4);
+  const int seg = segment(tokens, width, 512);  // (of 64 columns at a time it is no shorter)
+  l.token = up(size_t(tokens > seg ? (tokens + seg - 1) / seg : 0) * 2 * width * 4);
   l.row = l.token + up(size_t(tokens) * 4);
   l.count = l.row + up(size_t(tokens) * 4);
   l.all = l.count + up(size_t(tokens) * 4);
@@ -322,14 +336,15 @@ void gradient_n(const mmuon_embedding_args& a, hipStream_t s) {
                         reinterpret_cast<int*>(ws + at.count), reinterpret_cast<int*>(ws + at.all),
                         reinterpret_cast<float*>(ws)};
   if (a.tokens <= FEW_IDS)
-    hipLaunchKernelGGL((embed_rows<T, N, 4, 256, 64>), dim3(classes), dim3(256), 0, s, a, l, space);
-  else hipLaunchKernelGGL((embed_rows<T, N, 16, 1024, 512>), dim3(classes), dim3(1024), 0, s, a, l, space);
+    hipLaunchKernelGGL((embed_rows<T, N, 4, 256, 64, true>), dim3(classes), dim3(256), 0, s, a, l, space);
+  else hipLaunchKernelGGL((embed_rows<T, N, 16, 1024, 512, false>), dim3(classes), dim3(1024), 0, s, a, l, space);
   if (a.tokens == 0) return;
-  const int64_t segs = (a.tokens + SEG - 1) / SEG, waves = segs * ((a.width + 64 * N - 1) / (64 * N));
-  hipLaunchKernelGGL((embed_sum<T, N>), dim3(unsigned((waves + 3) / 4)), dim3(256), 0, s, a, space);
+  const int seg = segment(a.tokens, a.width, 64 * N);
+  const int64_t segs = (a.tokens + seg - 1) / seg, waves = segs * ((a.width + 64 * N - 1) / (64 * N));
+  hipLaunchKernelGGL((embed_sum<T, N>), dim3(unsigned((waves + 3) / 4)), dim3(256), 0, s, a, seg, space);
   if (segs > 1)
     hipLaunchKernelGGL((embed_join<T, N>), dim3(unsigned((segs - 1) * ((a.width + 32 * N - 1) / (32 * N)))), dim3(256),
-                       0, s, a, space);
+                       0, s, a, seg, space);
 }
 
 template <class T>
