@@ -17,20 +17,49 @@
 namespace mmuon {
 namespace {
 
-// N consecutive elements; N == 1 for rows that are not whole aligned 16-B chunks
+// N consecutive elements: 16 B, or one where rows are not whole aligned 16-B chunks.  (Two
+// 16-B accesses to a lane, 8 floats, leave half of each line to the second: zeros to 50304 x 512
+// floats 23 us, 16 B at a time 18.)
+template <class T>
+constexpr int CHUNK = 16 / int(sizeof(typename T::storage));
 template <class T, int N>
 __device__ __forceinline__ void load_n(const typename T::storage* p, float (&v)[N]) {
-  if constexpr (N == 8) Vec8<T>::load(p, v);
-  else v[0] = T::load(p, 0);
+  if constexpr (N == 8) {
+    Vec8<T>::load(p, v);
+  } else if constexpr (N == 4) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+  } else {
+    v[0] = T::load(p, 0);
+  }
 }
-template <class T, int N>
+template <class T, int N, bool NT = false>
 __device__ __forceinline__ void store_n(typename T::storage* p, const float (&v)[N]) {
-  if constexpr (N == 8) Vec8<T>::store(p, v);
-  else T::store(p, 0, v[0]);
+  if constexpr (N == 1) {
+    T::store(p, 0, v[0]);
+    return;
+  } else {
+    uint4 u;
+    if constexpr (sizeof(typename T::storage) == 2) u = Vec8<T>::pack(v);
+    else u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    if constexpr (NT) store16_nt(p, u);
+    else *reinterpret_cast<uint4*>(p) = u;
+  }
+}
+// fp32 sums of N columns
+template <int N>
+__device__ __forceinline__ void load_sums(const float* p, float (&v)[N]) {
+  if constexpr (N == 8) Vec8<F32T>::load(p, v);
+  else load_n<F32T, N>(p, v);
+}
+template <int N>
+__device__ __forceinline__ void store_sums(float* p, const float (&v)[N]) {
+  if constexpr (N == 8) Vec8<F32T>::store(p, v);
+  else store_n<F32T, N>(p, v);
 }
 
-// `lanes` (a power of two) threads per row
-template <class T, int N>
+// `lanes` (a power of two) threads per row; NT: past the L2s
+template <class T, int N, bool NT>
 __global__ __launch_bounds__(256) void embed_lookup(mmuon_embedding_args a, int lanes) {
   const int64_t t = int64_t(blockIdx.x) * (256 / lanes) + threadIdx.x / lanes;
   if (t >= a.tokens) return;
@@ -44,7 +73,7 @@ __global__ __launch_bounds__(256) void embed_lookup(mmuon_embedding_args a, int 
     load_n<T, N>(src + c, x);
 #pragma unroll
     for (int k = 0; k < N; ++k) x[k] = in ? x[k] * a.scale : NAN;  // no such row: the output shows it
-    store_n<T, N>(dst + c, x);
+    store_n<T, N, NT>(dst + c, x);
   }
 }
 
@@ -63,7 +92,7 @@ struct GradSpace {
 // WAVES waves, ROWS rows of a class at most, LIST ids of a class that a wave keeps from its scan;
 // FIRST: zeros to all rows before, not to the empty ones behind
 template <class T, int N, int WAVES, int ROWS, int LIST, bool FIRST>
-__global__ __launch_bounds__(64 * WAVES) void embed_rows(mmuon_embedding_args a, int log2c, GradSpace space) {
+__global__ __launch_bounds__(64 * WAVES) void embed_rows(mmuon_embedding_args a, int log2c, bool past, GradSpace space) {
   constexpr int NTH = 64 * WAVES;
   static_assert(ROWS % NTH == 0 || NTH % ROWS == 0, "rows are scanned by whole workgroups");
   __shared__ int at[WAVES][ROWS];     // counts, then the next place, of a row's positions in a wave's tokens
@@ -79,8 +108,10 @@ __global__ __launch_bounds__(64 * WAVES) void embed_rows(mmuon_embedding_args a,
     const int chunks = (a.width + 64 * N - 1) / (64 * N);
     for (int task = wave; task < rows * chunks; task += WAVES) {
       const int r = task / chunks, col = (task - r * chunks) * 64 * N + lane * N;
-      if (which(r) && col < a.width)
-        store_n<T, N>(static_cast<typename T::storage*>(a.dw) + (int64_t(r) * C + c) * a.width + col, zero);
+      if (!which(r) || col >= a.width) continue;
+      auto* dst = static_cast<typename T::storage*>(a.dw) + (int64_t(r) * C + c) * a.width + col;
+      if (past) store_n<T, N, true>(dst, zero);
+      else store_n<T, N>(dst, zero);
     }
   };
   // few ids: most rows are empty, and all zeros are on their way while the ids are read
@@ -204,7 +235,7 @@ __global__ __launch_bounds__(256) void embed_sum(mmuon_embedding_args a, int eac
 #pragma unroll
   for (int k = 0; k < N; ++k) s[k] = 0.f;
   bool first = true;
-  const auto piece = [&](int slot) { store_n<F32T, N>(space.sums + (int64_t(seg) * 2 + slot) * a.width + col, s); };
+  const auto piece = [&](int slot) { store_sums<N>(space.sums + (int64_t(seg) * 2 + slot) * a.width + col, s); };
   constexpr int U = 8;
   for (int p = 0; p < n; p += U) {
     float x[U][N];
@@ -259,7 +290,7 @@ __global__ __launch_bounds__(256) void embed_join(mmuon_embedding_args a, int si
       // the row is the last of its first segment and the first of the others
       const int slot = 2 * (seg + i) + (i == 0 && f > p0 ? 1 : 0);
       float x[N];
-      load_n<F32T, N>(space.sums + int64_t(slot) * a.width + col, x);
+      load_sums<N>(space.sums + int64_t(slot) * a.width + col, x);
 #pragma unroll
       for (int k = 0; k < N; ++k) s[k] += x[k];
     }
@@ -281,15 +312,22 @@ bool whole_chunks(const void* base, int64_t stride, int64_t width) {
   return reinterpret_cast<uintptr_t>(base) % 16 == 0 && stride % 8 == 0 && width % 8 == 0;
 }
 
-template <class T>
-void lookup(const mmuon_embedding_args& a, hipStream_t s) {
-  const bool vec = whole_chunks(a.w, a.w_stride, a.width) && whole_chunks(a.out, a.width, a.width);
-  const int chunks = vec ? a.width / 8 : a.width;
+template <class T, int N>
+void lookup_n(const mmuon_embedding_args& a, hipStream_t s) {
+  const int chunks = a.width / N;
   int lanes = 16;  // about four chunks per thread
   while (lanes < 256 && lanes * 4 < chunks) lanes *= 2;
   const dim3 grid(unsigned((a.tokens + 256 / lanes - 1) / (256 / lanes))), block(256);
-  if (vec) hipLaunchKernelGGL((embed_lookup<T, 8>), grid, block, 0, s, a, lanes);
-  else hipLaunchKernelGGL((embed_lookup<T, 1>), grid, block, 0, s, a, lanes);
+  // An output that the L2s (32 MiB) cannot hold is stored past them: 16384 x 4096 in bf16 40.0 ->
+  // 34.0 us, 8192 x 4096 18.7 -> 17.6; a smaller one is read from there by what comes next.
+  if (a.tokens * a.width * int64_t(sizeof(typename T::storage)) > (int64_t(32) << 20))
+    hipLaunchKernelGGL((embed_lookup<T, N, true>), grid, block, 0, s, a, lanes);
+  else hipLaunchKernelGGL((embed_lookup<T, N, false>), grid, block, 0, s, a, lanes);
+}
+template <class T>
+void lookup(const mmuon_embedding_args& a, hipStream_t s) {
+  if (whole_chunks(a.w, a.w_stride, a.width) && whole_chunks(a.out, a.width, a.width)) lookup_n<T, CHUNK<T>>(a, s);
+  else lookup_n<T, 1>(a, s);
 }
 
 // Classes: a power of two.  Many small workgroups (2048, eight per CU) where the ids are few
@@ -317,7 +355,7 @@ struct GradLayout {
 GradLayout grad_layout(int64_t tokens, int64_t width) {
   GradLayout l;
   const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  const int seg = segment(tokens, width, 512);  // (of 64 columns at a time it is no shorter)
+  const int seg = segment(tokens, width, 512);  // (of fewer columns at a time it is no shorter)
   l.token = up(size_t(tokens > seg ? (tokens + seg - 1) / seg : 0) * 2 * width * 4);
   l.row = l.token + up(size_t(tokens) * 4);
   l.count = l.row + up(size_t(tokens) * 4);
@@ -335,9 +373,12 @@ void gradient_n(const mmuon_embedding_args& a, hipStream_t s) {
   const GradSpace space{reinterpret_cast<int*>(ws + at.token), reinterpret_cast<int*>(ws + at.row),
                         reinterpret_cast<int*>(ws + at.count), reinterpret_cast<int*>(ws + at.all),
                         reinterpret_cast<float*>(ws)};
+  // A table that the Infinity Cache (256 MiB) cannot hold gets its zeros past the caches: 16384
+  // tokens of 50304 x 4096 in bf16 135 -> 125 us; 50304 x 512 floats 27 -> 30.
+  const bool past = a.vocab * a.width * int64_t(sizeof(typename T::storage)) > (int64_t(256) << 20);
   if (a.tokens <= FEW_IDS)
-    hipLaunchKernelGGL((embed_rows<T, N, 4, 256, 64, true>), dim3(classes), dim3(256), 0, s, a, l, space);
-  else hipLaunchKernelGGL((embed_rows<T, N, 16, 1024, 512, false>), dim3(classes), dim3(1024), 0, s, a, l, space);
+    hipLaunchKernelGGL((embed_rows<T, N, 4, 256, 64, true>), dim3(classes), dim3(256), 0, s, a, l, past, space);
+  else hipLaunchKernelGGL((embed_rows<T, N, 16, 1024, 512, false>), dim3(classes), dim3(1024), 0, s, a, l, past, space);
   if (a.tokens == 0) return;
   const int seg = segment(a.tokens, a.width, 64 * N);
   const int64_t segs = (a.tokens + seg - 1) / seg, waves = segs * ((a.width + 64 * N - 1) / (64 * N));
@@ -349,7 +390,7 @@ void gradient_n(const mmuon_embedding_args& a, hipStream_t s) {
 
 template <class T>
 void gradient(const mmuon_embedding_args& a, hipStream_t s) {
-  if (whole_chunks(a.dout, a.dout_stride, a.width) && whole_chunks(a.dw, a.width, a.width)) gradient_n<T, 8>(a, s);
+  if (whole_chunks(a.dout, a.dout_stride, a.width) && whole_chunks(a.dw, a.width, a.width)) gradient_n<T, CHUNK<T>>(a, s);
   else gradient_n<T, 1>(a, s);
 }
 
