@@ -40,7 +40,8 @@ constexpr int CODE_ZERO = 65535;                 // p = 0
 enum {
   EP_STATS = 0,  // logits: statistics of each part, the targets' logits
   EP_CODES = 1,  // the same, and the codes
-  EP_ROWS = 2    // bf16 result, rows = columns of the tile; or fp32 accumulators of a part of K
+  EP_ROWS = 2,   // bf16 result, rows = columns of the tile; or fp32 accumulators of a part of K
+  EP_PAST = 3    // the same, rows stored past the caches
 };
 
 // D (M x N) = A (M x K) B^T (N x K), where N (logits, dx) or K (dw) are the piece's tokens:
@@ -430,7 +431,7 @@ __device__ __forceinline__ void finish(int N, const HeadTile& t, f32x16 (&acc)[G
   const int tid = fresh_tid();
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / GE::GN, wn = wave % GE::GN;
-  if constexpr (EP == EP_ROWS) {
+  if constexpr (EP >= EP_ROWS) {
     // fragment order: float4 q of MFMA tile (i, j) of a wave at 64 lanes x 16 B
     float* frag = a.frag + ((int64_t(t.idx - a.frag_first) * GE::NW + wave) * (GE::WI * GE::WJ * 16) * 64 + lane * 4);
     if (a.start) {
@@ -476,7 +477,9 @@ __device__ __forceinline__ void finish(int N, const HeadTile& t, f32x16 (&acc)[G
         store_block(w, lane, [&](int c, int r, const uint4& u) {
           if (n1 + c >= N || m1 + r >= a.M) return;
           const int row = X == X_IS_NONE ? a.rows[n1 + c] : n1 + c;
-          *reinterpret_cast<uint4*>(a.out + int64_t(row) * a.ostride + int64_t(m1 + r) * 2) = u;
+          char* to = a.out + int64_t(row) * a.ostride + int64_t(m1 + r) * 2;
+          if constexpr (EP == EP_PAST) store16_nt(to, u);
+          else *reinterpret_cast<uint4*>(to) = u;
         });
       }
     }
@@ -1086,6 +1089,10 @@ int launch_ce(const mmuon_ce_args& x, bool train, hipStream_t st) {
       d.ostride = int64_t(x.width) * 2;
       d.factor = factor;
       d.frag = reinterpret_cast<float*>(ws + l.dwfrag);
+      // Few tokens: dw is bound by its writes, and one that fills the Infinity Cache leaves past it
+      // (128 tokens of 50304 x 4096 155 -> 115 us, x 2048 87 -> 55, x 1024 35 -> 38; 800 of x 4096
+      // with the other products 1035 -> 1044).
+      const bool past = n <= 512 && x.vocab * x.width * 2 > (int64_t(160) << 20);
       d.start = t0 > 0;
       d.keep = t0 + n < T;
       set_tiles(d, x.width, V, n, l.dw);
@@ -1095,7 +1102,8 @@ int launch_ce(const mmuon_ce_args& x, bool train, hipStream_t st) {
         d.loss = x.loss;
         d.mean = mean ? 1 : 0;
       }
-      launch_head<true, true, EP_ROWS, X_IS_A>(d, l.dw, st);
+      if (past) launch_head<true, true, EP_PAST, X_IS_A>(d, l.dw, st);
+      else launch_head<true, true, EP_ROWS, X_IS_A>(d, l.dw, st);
       if (!d.keep) launch_join<X_IS_A>(d, l.dw, st);
     }
   }
