@@ -334,9 +334,8 @@ __device__ __forceinline__ void store_block(uint2 (&w)[4], int lane, Fn&& fn) {
 
 // Statistics and codes of a tile of logits: rows m0.. are vocabulary, columns n0.. tokens.
 template <class GE, bool CODES>
-__device__ __forceinline__ void loss_epilogue(const HeadGemm& a, int N, int m0, int n0, f32x16 (&acc)[GE::WI][GE::WJ]) {
-  const int tid = fresh_tid();
-  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+__device__ __forceinline__ void loss_epilogue(const HeadGemm& a, int N, int m0, int n0, int wave, int lane,
+                                              f32x16 (&acc)[GE::WI][GE::WJ]) {
   const int wm = wave / GE::GN, wn = wave % GE::GN;
   constexpr int PW = 32 * GE::WI;               // vocabulary of a part
   const int v0 = m0 + wm * PW, left = a.M - v0;  // rows from `left` on do not exist
@@ -424,6 +423,28 @@ __device__ __forceinline__ void add_resid(const HeadGemm& a, int n, int m, float
   v[3] += r * __uint_as_float(u.y & 0xffff0000u);
 }
 
+// Accumulators in fragment order: float4 q of MFMA tile (i, j) of a wave at 64 lanes x 16 B.
+// Where a lane's begin:
+template <class GE>
+__device__ __forceinline__ int64_t fragment(int64_t idx, int wave, int lane) {
+  return (idx * GE::NW + wave) * (GE::WI * GE::WJ * 16 * 64) + lane * 4;
+}
+template <class GE>
+__device__ __forceinline__ void add_fragments(const float* frag, f32x16 (&acc)[GE::WI][GE::WJ]) {
+#pragma unroll
+  for (int i = 0; i < GE::WI; ++i)
+#pragma unroll
+    for (int j = 0; j < GE::WJ; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 f = *reinterpret_cast<const float4*>(frag + ((i * GE::WJ + j) * 4 + q) * 256);
+        acc[i][j][4 * q] += f.x;
+        acc[i][j][4 * q + 1] += f.y;
+        acc[i][j][4 * q + 2] += f.z;
+        acc[i][j][4 * q + 3] += f.w;
+      }
+}
+
 // What becomes of a tile's accumulators
 template <class GE, int EP, int X>
 __device__ __forceinline__ void finish(int N, const HeadTile& t, f32x16 (&acc)[GE::WI][GE::WJ]) {
@@ -431,34 +452,20 @@ __device__ __forceinline__ void finish(int N, const HeadTile& t, f32x16 (&acc)[G
   const int tid = fresh_tid();
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / GE::GN, wn = wave % GE::GN;
+  float* frag = a.frag + fragment<GE>(t.idx - a.frag_first, wave, lane);
+  if (EP >= EP_ROWS && a.start) add_fragments<GE>(frag, acc);
+  if ((EP >= EP_ROWS && a.keep) || t.split) {
+#pragma unroll
+    for (int i = 0; i < GE::WI; ++i)
+#pragma unroll
+      for (int j = 0; j < GE::WJ; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<float4*>(frag + ((i * GE::WJ + j) * 4 + q) * 256) =
+              make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+    return;
+  }
   if constexpr (EP >= EP_ROWS) {
-    // fragment order: float4 q of MFMA tile (i, j) of a wave at 64 lanes x 16 B
-    float* frag = a.frag + ((int64_t(t.idx - a.frag_first) * GE::NW + wave) * (GE::WI * GE::WJ * 16) * 64 + lane * 4);
-    if (a.start) {
-#pragma unroll
-      for (int i = 0; i < GE::WI; ++i)
-#pragma unroll
-        for (int j = 0; j < GE::WJ; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float4 f = *reinterpret_cast<const float4*>(frag + ((i * GE::WJ + j) * 4 + q) * 256);
-            acc[i][j][4 * q] += f.x;
-            acc[i][j][4 * q + 1] += f.y;
-            acc[i][j][4 * q + 2] += f.z;
-            acc[i][j][4 * q + 3] += f.w;
-          }
-    }
-    if (a.keep || t.split) {
-#pragma unroll
-      for (int i = 0; i < GE::WI; ++i)
-#pragma unroll
-        for (int j = 0; j < GE::WJ; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<float4*>(frag + ((i * GE::WJ + j) * 4 + q) * 256) =
-                make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
-      return;
-    }
     const float factor = a.factor != nullptr ? *a.factor : 1.f;
 #pragma unroll
     for (int j = 0; j < GE::WJ; ++j) {
@@ -484,7 +491,7 @@ __device__ __forceinline__ void finish(int N, const HeadTile& t, f32x16 (&acc)[G
       }
     }
   } else {
-    loss_epilogue<GE, EP == EP_CODES>(a, N, t.m0, t.n0, acc);
+    loss_epilogue<GE, EP == EP_CODES>(a, N, t.m0, t.n0, wave, lane, acc);
   }
 }
 
@@ -538,6 +545,24 @@ __global__ __launch_bounds__(GE::NTH, GE::PER_CU * GE::NW / 4) void head_gemm(He
     barrier();  // every wave is done with the ring
     sum_loss<GE::NTH>(a.nll, a.tokens, *a.count, a.mean, a.loss, reinterpret_cast<float*>(lds));
   }
+}
+
+// The split tiles of the logits: a workgroup of one wave sums the parts of what one wave of the
+// product held, in order, and goes on as if it had multiplied.
+template <class GE, int EP>
+__global__ __launch_bounds__(64) void head_logits_join(HeadGemm a) {
+  const HeadSize z = head_size<GE, X_IS_B>(a);
+  const int nth = blockIdx.x / GE::NW, wave = blockIdx.x % GE::NW, lane = threadIdx.x, t = z.full + nth;
+  if (t >= z.tiles_m * z.tiles_n) return;
+  const int2 at = tile_place(t, z.tiles_m, z.tiles_n);
+  f32x16 acc[GE::WI][GE::WJ];
+#pragma unroll
+  for (int i = 0; i < GE::WI; ++i)
+#pragma unroll
+    for (int j = 0; j < GE::WJ; ++j) acc[i][j] = f32x16{};
+  const float* f = a.frag + fragment<GE>(z.full + int64_t(nth) * z.S - a.frag_first, wave, lane);
+  for (int k = 0; k < z.S; ++k) add_fragments<GE>(f + int64_t(k) * GE::BM * GE::BN, acc);
+  loss_epilogue<GE, EP == EP_CODES>(a, z.N, at.x * GE::BM, at.y * GE::BN, wave, lane, acc);
 }
 
 // Sum over the parts of K, in order, of one 32 x 32 MFMA tile of a split tile per workgroup:
@@ -875,15 +900,11 @@ int64_t plan_time(const HeadPlan& p, int64_t M, int64_t N, int64_t K) {
 }
 constexpr int WHOLE = 1 << 30;  // no tile is split
 
-// The logits: K is not split (a part of a sum has no exponential).
-HeadPlan logits_plan(int64_t T, int64_t D, int64_t V) {
-  const HeadPlan wide{false, WHOLE, 1}, narrow{true, WHOLE, 1};
-  return plan_time(narrow, V, T, D) < plan_time(wide, V, T, D) ? narrow : wide;
-}
-// The gradients: all tiles split (few tokens or a narrow model: dx has few tiles), or those of
-// the last round, that would leave most CUs idle.  At least 256 of K in a part; partials
-// of at most 256 MiB.
-HeadPlan grad_plan(int64_t M, int64_t N, int64_t K, bool narrow_too) {
+// All tiles split (few tokens or a narrow model: dx has few tiles), or those of the last round,
+// that would leave most CUs idle.  At least 256 of K in a part; partials of at most 256 MiB.
+// The logits split where that should take 8% off at least (600 tokens of 50304 x 4096 312 ->
+// 273 us, 1000 430 -> 392, x 1024 121 -> 124).
+HeadPlan head_plan(int64_t M, int64_t N, int64_t K, bool narrow_too, bool logits) {
   HeadPlan best{false, WHOLE, 1};
   int64_t best_time = plan_time(best, M, N, K);
   for (int narrow = 0; narrow <= (narrow_too ? 1 : 0); ++narrow) {
@@ -892,7 +913,7 @@ HeadPlan grad_plan(int64_t M, int64_t N, int64_t K, bool narrow_too) {
       for (int S = full == WHOLE ? 1 : 2; S <= (full == WHOLE ? 1 : 256) && (S == 1 || K / S >= 256); ++S) {
         const HeadPlan p{narrow != 0, full, S};
         if (p.frag(M, N, false) > (size_t(1) << 28)) break;
-        const int64_t t = plan_time(p, M, N, K);
+        const int64_t t = plan_time(p, M, N, K) * (logits && full != WHOLE ? 109 : 100) / 100;
         if (t < best_time) best = p, best_time = t;
       }
   }
@@ -933,13 +954,21 @@ void launch_join(const HeadGemm& a, HeadPlan p, hipStream_t s) {
   else launch_join_tile<H256, X>(a, s);
 }
 
+template <int EP>
+void launch_logits(const HeadGemm& a, HeadPlan p, hipStream_t s) {
+  launch_head<false, false, EP, X_IS_B>(a, p, s);
+  const int split = a.tiles_m * a.tiles_n - a.full;
+  if (split > 0 && p.narrow) hipLaunchKernelGGL((head_logits_join<H128, EP>), dim3(split * H128::NW), dim3(64), 0, s, a);
+  else if (split > 0) hipLaunchKernelGGL((head_logits_join<H256, EP>), dim3(split * H256::NW), dim3(64), 0, s, a);
+}
+
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 struct Layout {
   int64_t piece, ldc;
   int nparts;
   HeadPlan logits, dx, dw;
-  size_t codes, xc, parts, tlogit, resid, dxfrag, dwfrag, nll, rows, compact, count, inverse, total;
+  size_t codes, xc, parts, tlogit, resid, frag, dwfrag, nll, rows, compact, count, inverse, total;
 };
 
 Layout head_layout(const mmuon_ce_args& x, bool train) {
@@ -947,10 +976,10 @@ Layout head_layout(const mmuon_ce_args& x, bool train) {
   const int64_t T = std::max<int64_t>(x.tokens, 1);
   l.piece = std::min(T, std::max<int64_t>(1, x.piece_tokens));
   l.ldc = int64_t(cdiv(x.vocab, 256)) * 256;
-  l.logits = logits_plan(l.piece, x.width, x.vocab);
-  l.dx = grad_plan(x.width, l.piece, x.vocab, true);
+  l.logits = head_plan(x.vocab, l.piece, x.width, true, true);
+  l.dx = head_plan(x.width, l.piece, x.vocab, true, false);
   // (128-wide tiles gained nothing there: 1000 x 512 54 us in 256-wide, 68 in 128-wide)
-  l.dw = grad_plan(x.width, x.vocab, l.piece, false);
+  l.dw = head_plan(x.width, x.vocab, l.piece, false, false);
   l.nparts = cdiv(x.vocab, 1 << l.logits.part_shift());
   size_t at = 0;
   const auto take = [&at](size_t n) {
@@ -964,7 +993,7 @@ Layout head_layout(const mmuon_ce_args& x, bool train) {
   l.parts = take(P * l.nparts * 8);
   l.tlogit = take(P * 4);
   l.resid = take(train ? P * 4 : 0);
-  l.dxfrag = take(train ? l.dx.frag(x.width, l.piece, false) : 0);
+  l.frag = take(std::max(l.logits.frag(x.vocab, l.piece, false), train ? l.dx.frag(x.width, l.piece, false) : 0));
   l.dwfrag = take(train ? l.dw.frag(x.width, x.vocab, T > l.piece) : 0);
   l.nll = take(x.nll == nullptr ? size_t(T) * 4 : 0);
   l.rows = take(size_t(T) * 4);
@@ -1037,8 +1066,10 @@ int launch_ce(const mmuon_ce_args& x, bool train, hipStream_t st) {
     f.target = list ? target + t0 : x.target;
     f.tlogit = reinterpret_cast<float*>(ws + l.tlogit);
     set_tiles(f, V, n, x.width, l.logits);
-    if (train) launch_head<false, false, EP_CODES, X_IS_B>(f, l.logits, st);
-    else launch_head<false, false, EP_STATS, X_IS_B>(f, l.logits, st);
+    f.frag = reinterpret_cast<float*>(ws + l.frag);
+    f.frag_first = std::min(f.full, f.tiles_m * f.tiles_n);
+    if (train) launch_logits<EP_CODES>(f, l.logits, st);
+    else launch_logits<EP_STATS>(f, l.logits, st);
 
     RowArgs r{};
     r.codes = f.codes;
@@ -1075,7 +1106,7 @@ int launch_ce(const mmuon_ce_args& x, bool train, hipStream_t st) {
       d.resid = r.resid;
       d.w = static_cast<const uint16_t*>(x.w);
       d.wstride = x.w_stride;
-      d.frag = reinterpret_cast<float*>(ws + l.dxfrag);
+      d.frag = reinterpret_cast<float*>(ws + l.frag);
       set_tiles(d, x.width, n, V, l.dx);
       d.frag_first = std::min(d.full, d.tiles_m * d.tiles_n);
       launch_head<true, false, EP_ROWS, X_IS_NONE>(d, l.dx, st);
