@@ -12,9 +12,10 @@ UCODE = 2.0 ** -11 * 0.6932
 
 
 def cross_entropy(x, w, target, ignore_index=-100, reduction="mean", grad=None):
-    """(loss, dx, dw, bounds): float64 on the CPU; ``bounds`` = (of loss, dx, dw) elementwise."""
-    x, w = x.double().cpu(), w.double().cpu()
-    target = target.cpu().long()
+    """(loss, dx, dw, bounds): float64, where x is; ``bounds`` = (of loss, dx, dw) elementwise."""
+    dev, f64 = x.device, torch.float64
+    x, w = x.double(), w.double().to(dev)
+    target = target.to(dev).long()
     T, D = x.shape
     V = w.shape[0]
     keep = target != ignore_index
@@ -22,24 +23,24 @@ def cross_entropy(x, w, target, ignore_index=-100, reduction="mean", grad=None):
     n = len(yk)
     l = xk @ w.T
     lse = torch.logsumexp(l, 1)
-    nll = torch.zeros(T, dtype=torch.float64)
+    nll = torch.zeros(T, dtype=f64, device=dev)
     ly = l.gather(1, yk[:, None])[:, 0]
     nll[keep] = lse - ly
     # a logit: D fp32 roundings of partial sums no larger than sum |x w|; log2 e, its power, the sum over V in
     # parts, the logarithm
-    size = (xk.abs() @ w.abs().T).amax(1) if n else torch.zeros(0, dtype=torch.float64)
+    size = (xk.abs() @ w.abs().T).amax(1) if n else torch.zeros(0, dtype=f64, device=dev)
     err = U32 * (2 * (D + 4) * size + 4 * lse.abs() + V ** 0.5 + 40)
-    tol = torch.zeros(T, dtype=torch.float64)
+    tol = torch.zeros(T, dtype=f64, device=dev)
     tol[keep] = err
     if grad is not None:
-        g = grad.double().cpu()[keep]
+        g = grad.double().to(dev)[keep]
     elif reduction == "mean":
-        g = torch.full((n,), 1.0 / n if n else 0.0, dtype=torch.float64)
+        g = torch.full((n,), 1.0 / n if n else 0.0, dtype=f64, device=dev)
     else:
-        g = torch.ones(n, dtype=torch.float64)
+        g = torch.ones(n, dtype=f64, device=dev)
     p = (l - lse[:, None]).exp()
     dl = p.clone()
-    dl[torch.arange(n), yk] -= 1
+    dl[torch.arange(n, device=dev), yk] -= 1
     dl = dl * g[:, None]
     # p: its logit and lse, its code, bf16; the target's entry p - 1 has the error of p by nll
     rel = UCODE + UBF + 2 * err[:, None] + 2.0 ** -18

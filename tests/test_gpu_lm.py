@@ -21,10 +21,10 @@ def head(T, D, V, seed=0, ignored=0.0, spread=1.0):
 
 
 def within(got, ref, bound, what):
-    got = got.detach().double().cpu()
+    got = got.detach().double().to(ref.device)
     assert got.shape == ref.shape, what
     assert torch.equal(got.isnan(), ref.isnan()), what
-    off = (got - ref).abs()[~ref.isnan()] - torch.as_tensor(bound).expand_as(ref)[~ref.isnan()]
+    off = (got - ref).abs()[~ref.isnan()] - torch.as_tensor(bound, device=ref.device).expand_as(ref)[~ref.isnan()]
     assert not off.numel() or float(off.max()) <= 0, (what, float(off.max()))
 
 
@@ -67,6 +67,19 @@ def test_head_masks_and_pieces(T, piece, ignored):
     x, w, y = head(T, 64, 777, seed=T, ignored=ignored)
     for reduction in ("mean", "sum"):
         check_head(x.to(DEV), w.to(DEV), y.to(DEV), reduction, piece_tokens=piece)
+
+
+@pytest.mark.parametrize("T, D, V, piece", [
+    (1000, 2048, 16640, None),   # 260 tiles of logits: the last four split over the width, the last tiles of dw too
+    (1100, 1032, 16500, None),   # the same, with edges in every direction
+    (200, 520, 70000, None),     # dx of a few tiles: all split over the vocabulary
+    (128, 2048, 45000, None),    # dw beyond the Infinity Cache's share: stored past it
+    (900, 264, 33000, 400),      # pieces, the last one shorter, dw carried from one to the next
+])
+@pytest.mark.parametrize("ignored", [0.0, 0.4])
+def test_head_splits(T, D, V, piece, ignored):
+    x, w, y = (t.to(DEV) for t in head(T, D, V, seed=T + D, ignored=ignored))
+    check_head(x, w, y, piece_tokens=piece)
 
 
 def test_head_pieces_agree_where_no_sum_crosses_them():
@@ -365,3 +378,20 @@ def test_embedding_in_a_graph_and_on_another_stream():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, torch.autograd.grad(embedding(i, w), w, dy)[0]), seed
+
+
+# ----- together --------------------------------------------------------------------
+def test_example_learns_and_scores():
+    """Embedding, Monarch layers, loss, backward, optimizer, generation of single tokens."""
+    from monarch_muon_amd import example
+    model, losses = example.train(steps=60)
+    assert losses.isfinite().all() and float(losses[0]) > 5.5 and float(losses[-5:].mean()) < 3.0, losses
+    tokens, scores = example.generate(model, 7, 4)
+    assert all(0 <= t < example.VOCAB for t in tokens) and all(-6.3 < s <= 0 for s in scores)
+    # the loss of the example's own calls against the plain form on the same hidden states
+    ids, targets = example.text(torch.Generator().manual_seed(5), DEV)
+    with torch.no_grad():
+        h = model.hidden(ids).reshape(-1, example.WIDTH)
+        got = model.loss(ids, targets)
+    ref, _, _, (bound, _, _) = oracle.cross_entropy(h, model.lm_head.detach(), targets.reshape(-1), ignore_index=example.PAD)
+    within(got, ref, bound, "loss")
