@@ -15,9 +15,9 @@
 // vocabulary that a wave holds, and stores every logit as a 16-bit code: its distance below
 // the part's maximum in base-2 fixed point, step 64 / 65535.  head_rows joins the parts'
 // statistics into lse and turns the codes of a row into bf16 dl where they stand.  A code
-// gives p with a relative error of 3.4e-4 at most, however small p is (2e-3 is bf16's own
-// rounding of dl; bf16 exponentials would round twice); what lies 64 binades below its
-// part's maximum (p < 6e-20) counts as zero.  The target's logit is kept in fp32: the loss
+// gives p with a relative error of 3.4e-4 at most, however small p is, a tenth of bf16's own
+// rounding of dl (exponentials kept in bf16 would be rounded twice); what lies 64 binades
+// below its part's maximum (p < 6e-20) counts as zero.  The target's logit is kept in fp32: the loss
 // and p_y - 1 do not go through a code.  One factor 1 / valid tokens is applied to the
 // fp32 sums of dx and dw and not to dl, and dx adds what bf16 took from its largest term,
 // p_y - 1: with them in dl, its rounding was one for all tokens, up to 2^-8.
@@ -889,7 +889,7 @@ struct HeadPlan {
 // of the sums does not depend on the device): rounds of 256 tiles, each its slices of K at the
 // rate of full rounds and what its start and end cost.  Measured at V = 50304: loss of 4096 x
 // 4096 1.37 ms in 256-wide tiles, 1.80 in 128-wide; 600 x 512 58.6 / 53.7 us, 300 x 4096 198 /
-// 208, 128 x 2048 51 / 47 (x 64-wide 55).
+// 208, 128 x 2048 51 / 47 (64-wide, two workgroups per CU: 55).
 int64_t round_time(bool narrow, int64_t K) { return narrow ? 1500 + 18 * K : 2500 + 25 * K; }
 int64_t plan_time(const HeadPlan& p, int64_t M, int64_t N, int64_t K) {
   const int64_t tiles = p.tiles(M, N), full = std::min<int64_t>(p.full, tiles), parts = (tiles - full) * p.S;

@@ -28,11 +28,11 @@ void require_one_device(std::initializer_list<const Tensor*> ts) {
   }
 }
 
-// Rows of 16-B chunks: the tensor itself where its rows are such, else a copy
+// Rows of 16-B chunks, not too far apart for the kernels' offsets: the tensor itself where its
+// rows are such, else a copy
 Tensor aligned_rows(const Tensor& t) {
-  const bool rows = t.size(1) <= 1 || t.stride(1) == 1;
-  return rows && t.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 ? t
-                                                                                                   : dense_aligned(t);
+  const bool rows = (t.size(1) <= 1 || t.stride(1) == 1) && t.stride(0) % 8 == 0 && t.stride(0) < (int64_t(1) << 22);
+  return rows && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 ? t : dense_aligned(t);
 }
 
 // ---------------------------------------------------------------------------
@@ -57,13 +57,13 @@ void check_head(const Tensor& x, const Tensor& w, const Tensor& target, int64_t 
 
 // Tokens of a piece: as asked, else as many as keep the codes of a piece (2 B per logit)
 // within 1 GiB, in whole 256-token tiles, and pieces of one size.  The loss alone has no
-// codes: 64 times as many.
+// codes: four times as many.
 int64_t piece_of(int64_t tokens, int64_t vocab, int64_t asked, bool train) {
   TORCH_CHECK_VALUE(asked >= 0, "piece_tokens must be positive, got ", asked);
   if (asked > 0) return std::min(asked, std::max<int64_t>(tokens, 1));
   const int64_t row = (vocab + 255) / 256 * 512;
   int64_t most = std::max<int64_t>(256, (int64_t(1) << 30) / row / 256 * 256);
-  if (!train) most *= 64;
+  if (!train) most *= 4;
   if (tokens <= most) return std::max<int64_t>(tokens, 1);
   const int64_t pieces = (tokens + most - 1) / most;
   return ((tokens + pieces - 1) / pieces + 255) / 256 * 256;

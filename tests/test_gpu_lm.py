@@ -95,6 +95,19 @@ def test_head_pieces_agree_where_no_sum_crosses_them():
         assert float((g - grads[0]).float().norm()) <= 2.0 ** -7 * float(grads[0].float().norm())
 
 
+def test_head_offsets_beyond_32_bits():
+    """A piece of 2.4e9 logits against small pieces, and rows of it against the plain form."""
+    x, w, y = (t.to(DEV) for t in head(48000, 8, 50304, seed=30, ignored=0.01))
+    nll = linear_cross_entropy(x, w, y, reduction="none", piece_tokens=48000)
+    assert torch.equal(nll, linear_cross_entropy(x, w, y, reduction="none", piece_tokens=4096))
+    whole = x.clone().requires_grad_()
+    dx, = torch.autograd.grad(linear_cross_entropy(whole, w, y, reduction="sum", piece_tokens=48000), whole)
+    rows = torch.cat([torch.arange(3), torch.arange(47997, 48000)]).to(DEV)
+    loss, rx, _, (lt, xt, _) = oracle.cross_entropy(x[rows], w, y[rows], reduction="none", grad=torch.ones(6))
+    within(nll[rows], loss, lt, "loss")
+    within(dx[rows], rx, xt, "dx")
+
+
 def test_head_empty():
     w = torch.ones(40, 16, device=DEV, dtype=torch.bfloat16, requires_grad=True)
     x = torch.empty(0, 16, device=DEV, dtype=torch.bfloat16, requires_grad=True)
@@ -331,6 +344,19 @@ def test_embedding_shapes_layouts_and_empty():
     for other in (dy.T.contiguous().T, torch.cat([dy, dy], 1)[:, :48], torch.cat([dy.new_zeros(1), dy.reshape(-1)])[1:].view(24, 48)):
         assert torch.equal(torch.autograd.grad(embedding(i, wd), wd, other)[0], ref)
     check_embedding(i, w, dy[:1].expand(24, 48))
+
+
+def test_embedding_offsets_beyond_32_bits():
+    V, D = 1100000, 2048
+    w = torch.zeros(V, D, device=DEV, dtype=torch.bfloat16)
+    i = torch.tensor([0, V - 1, 1048576, V - 1], device=DEV)
+    w[i[:3]] = torch.randn(3, D, device=DEV).bfloat16()
+    assert torch.equal(embedding(i, w), w[i])
+    dy = torch.randn(4, D, device=DEV).bfloat16()
+    wd = w.requires_grad_()
+    dw, = torch.autograd.grad(embedding(i, wd), wd, dy)
+    assert torch.equal(dw[V - 1], (dy[1].float() + dy[3].float()).bfloat16())
+    assert torch.equal(dw[0], dy[0]) and torch.equal(dw[1048576], dy[2]) and int(dw.any(1).sum()) == 3
 
 
 def test_embedding_ids_that_are_no_token():
