@@ -40,8 +40,9 @@ constexpr int CODE_ZERO = 65535;                 // p = 0
 enum {
   EP_STATS = 0,  // logits: statistics of each part, the targets' logits
   EP_CODES = 1,  // the same, and the codes
-  EP_ROWS = 2,   // bf16 result, rows = columns of the tile; or fp32 accumulators of a part of K
-  EP_PAST = 3    // the same, rows stored past the caches
+  EP_CODES_PAST = 2,  // the same, stored past the caches
+  EP_ROWS = 3,   // bf16 result, rows = columns of the tile; or fp32 accumulators of a part of K
+  EP_PAST = 4    // the same, rows stored past the caches
 };
 
 // D (M x N) = A (M x K) B^T (N x K), where N (logits, dx) or K (dw) are the piece's tokens:
@@ -333,7 +334,7 @@ __device__ __forceinline__ void store_block(uint2 (&w)[4], int lane, Fn&& fn) {
 }
 
 // Statistics and codes of a tile of logits: rows m0.. are vocabulary, columns n0.. tokens.
-template <class GE, bool CODES>
+template <class GE, int EP>
 __device__ __forceinline__ void loss_epilogue(const HeadGemm& a, int N, int m0, int n0, int wave, int lane,
                                               f32x16 (&acc)[GE::WI][GE::WJ]) {
   const int wm = wave / GE::GN, wn = wave % GE::GN;
@@ -392,17 +393,20 @@ __device__ __forceinline__ void loss_epilogue(const HeadGemm& a, int N, int m0, 
           d[e] = __builtin_fmaf(acc[i][j][4 * q + e], LOG2E, -m2);
           s += __builtin_amdgcn_exp2f(d[e]);
         }
-        if constexpr (CODES) {
+        if constexpr (EP != EP_STATS) {
           constexpr float K = -1.f / CODE_RANGE;
           const uint32_t lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_u16(d[0] * K, d[1] * K));
           const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_u16(d[2] * K, d[3] * K));
           codes[q] = make_uint2(lo, hi);
         }
       }
-      if constexpr (CODES) {
+      if constexpr (EP != EP_STATS) {
         store_block(codes, lane, [&](int c, int r, const uint4& u) {
           const int t = n0 + (wn * GE::WJ + j) * 32 + c;
-          if (t < N) *reinterpret_cast<uint4*>(a.codes + int64_t(t) * a.ldc + v0 + i * 32 + r) = u;
+          if (t >= N) return;
+          uint16_t* to = a.codes + int64_t(t) * a.ldc + v0 + i * 32 + r;
+          if constexpr (EP == EP_CODES_PAST) store16_nt(to, u);
+          else *reinterpret_cast<uint4*>(to) = u;
         });
       }
     }
@@ -491,7 +495,7 @@ __device__ __forceinline__ void finish(int N, const HeadTile& t, f32x16 (&acc)[G
       }
     }
   } else {
-    loss_epilogue<GE, EP == EP_CODES>(a, N, t.m0, t.n0, wave, lane, acc);
+    loss_epilogue<GE, EP>(a, N, t.m0, t.n0, wave, lane, acc);
   }
 }
 
@@ -562,7 +566,7 @@ __global__ __launch_bounds__(64) void head_logits_join(HeadGemm a) {
     for (int j = 0; j < GE::WJ; ++j) acc[i][j] = f32x16{};
   const float* f = a.frag + fragment<GE>(z.full + int64_t(nth) * z.S - a.frag_first, wave, lane);
   for (int k = 0; k < z.S; ++k) add_fragments<GE>(f + int64_t(k) * GE::BM * GE::BN, acc);
-  loss_epilogue<GE, EP == EP_CODES>(a, z.N, at.x * GE::BM, at.y * GE::BN, wave, lane, acc);
+  loss_epilogue<GE, EP>(a, z.N, at.x * GE::BM, at.y * GE::BN, wave, lane, acc);
 }
 
 // Sum over the parts of K, in order, of one 32 x 32 MFMA tile of a split tile per workgroup:
@@ -672,7 +676,9 @@ __global__ __launch_bounds__(256) void head_nll(RowArgs a) {
   a.nll[a.rows != nullptr ? a.rows[tok] : tok] = nll;
 }
 
-// One workgroup per token: lse, nll, and the row's codes -> dl.
+// One workgroup per token: lse, nll, and the row's codes -> dl.  Bound by its traffic, 4 B per
+// logit: 4096 x 50304 in 149 us, 5.5 TB/s, where a large copy reaches 5.1.
+template <bool PAST>
 __global__ __launch_bounds__(256) void head_rows(RowArgs a) {
   __shared__ float scratch[8];
   const int tok = blockIdx.x;
@@ -692,7 +698,7 @@ __global__ __launch_bounds__(256) void head_rows(RowArgs a) {
   }
   uint16_t* row = a.codes + int64_t(tok) * a.ldc;
   for (int64_t c = threadIdx.x * 8; c < a.ldc; c += 256 * 8) {
-    const uint4 in = *reinterpret_cast<const uint4*>(row + c);
+    const uint4 in = PAST ? load16_nt(row + c) : *reinterpret_cast<const uint4*>(row + c);
     const uint32_t w[4] = {in.x, in.y, in.z, in.w};
     const int part = int(c >> a.part_shift);
     const float top = part < a.nparts ? parts[part].x - lse2 : 0.f;  // beyond: codes of zero
@@ -1068,7 +1074,11 @@ int launch_ce(const mmuon_ce_args& x, bool train, hipStream_t st) {
     set_tiles(f, V, n, x.width, l.logits);
     f.frag = reinterpret_cast<float*>(ws + l.frag);
     f.frag_first = std::min(f.full, f.tiles_m * f.tiles_n);
-    if (train) launch_logits<EP_CODES>(f, l.logits, st);
+    // Codes of twice the Infinity Cache go past it, out and back (6000 tokens of 50304 x 1024 with
+    // gradients 2012 -> 1943 us, 8192 2606 -> 2572; 2000, a cache of them, 698 -> 711)
+    const bool past = int64_t(n) * l.ldc * 2 > (int64_t(512) << 20);
+    if (train && past) launch_logits<EP_CODES_PAST>(f, l.logits, st);
+    else if (train) launch_logits<EP_CODES>(f, l.logits, st);
     else launch_logits<EP_STATS>(f, l.logits, st);
 
     RowArgs r{};
@@ -1093,7 +1103,8 @@ int launch_ce(const mmuon_ce_args& x, bool train, hipStream_t st) {
       else hipLaunchKernelGGL(head_nll<64>, dim3(cdiv(n, 4)), dim3(256), 0, st, r);
       continue;
     }
-    hipLaunchKernelGGL(head_rows, dim3(n), dim3(256), 0, st, r);
+    if (past) hipLaunchKernelGGL(head_rows<true>, dim3(n), dim3(256), 0, st, r);
+    else hipLaunchKernelGGL(head_rows<false>, dim3(n), dim3(256), 0, st, r);
     const float* factor = mean && x.grad == nullptr ? inverse : nullptr;
     if (x.dx != nullptr) {
       HeadGemm d = f;  // dx^T (width x tokens) = w^T dl^T
@@ -1123,7 +1134,7 @@ int launch_ce(const mmuon_ce_args& x, bool train, hipStream_t st) {
       // Few tokens: dw is bound by its writes, and one that fills the Infinity Cache leaves past it
       // (128 tokens of 50304 x 4096 155 -> 115 us, x 2048 87 -> 55, x 1024 35 -> 38; 800 of x 4096
       // with the other products 1035 -> 1044).
-      const bool past = n <= 512 && x.vocab * x.width * 2 > (int64_t(160) << 20);
+      const bool dwpast = n <= 512 && x.vocab * x.width * 2 > (int64_t(160) << 20);
       d.start = t0 > 0;
       d.keep = t0 + n < T;
       set_tiles(d, x.width, V, n, l.dw);
@@ -1133,7 +1144,7 @@ int launch_ce(const mmuon_ce_args& x, bool train, hipStream_t st) {
         d.loss = x.loss;
         d.mean = mean ? 1 : 0;
       }
-      if (past) launch_head<true, true, EP_PAST, X_IS_A>(d, l.dw, st);
+      if (dwpast) launch_head<true, true, EP_PAST, X_IS_A>(d, l.dw, st);
       else launch_head<true, true, EP_ROWS, X_IS_A>(d, l.dw, st);
       if (!d.keep) launch_join<X_IS_A>(d, l.dw, st);
     }
