@@ -870,36 +870,40 @@ __global__ __launch_bounds__(256) void head_scale(uint16_t* x, int64_t nx, uint1
 // Host side
 // ---------------------------------------------------------------------------
 // Tiles: 256 of the first operand (vocabulary, or width) x 256 or 128 of the second, eight
-// waves, one workgroup per CU
+// waves, one workgroup per CU; 128 x 64, four waves, three workgroups per CU
 typedef Geo<2, 4, 4, 2, 4> H256;
 typedef Geo<4, 2, 2, 2, 4> H128;
+typedef Geo<4, 1, 1, 2, 4> H64;
+enum { T256 = 0, T128 = 1, T64 = 2 };
 
 // A product's tile, and the parts of K (S) of the tiles from `full` on.
 struct HeadPlan {
-  bool narrow;  // H128
+  int tile;
   int full, S;
-  int cols() const { return narrow ? 128 : 256; }
-  int part_shift() const { return narrow ? 6 : 7; }  // vocabulary of a wave of the logits
-  int tiles(int64_t m, int64_t n) const { return cdiv(m, 256) * cdiv(n, cols()); }
+  int rows() const { return tile == T64 ? 128 : 256; }
+  int cols() const { return 256 >> tile; }
+  int part_shift() const { return 7 - tile; }  // vocabulary of a wave of the logits
+  int tiles(int64_t m, int64_t n) const { return cdiv(m, rows()) * cdiv(n, cols()); }
   int virtual_tiles(int64_t m, int64_t n) const {
     const int t = tiles(m, n), f = std::min(full, t);
     return f + (t - f) * S;
   }
   // fp32 accumulators: of the split tiles, or of all
   size_t frag(int64_t m, int64_t n, bool all) const {
-    return size_t(virtual_tiles(m, n) - (all ? 0 : std::min(full, tiles(m, n)))) * 256 * cols() * 4;
+    return size_t(virtual_tiles(m, n) - (all ? 0 : std::min(full, tiles(m, n)))) * rows() * cols() * 4;
   }
 };
 
 // Time in ns of a product M x N x K on a 256-CU part (a function of the sizes only, so the order
 // of the sums does not depend on the device): rounds of 256 tiles, each its slices of K at the
 // rate of full rounds and what its start and end cost.  Measured at V = 50304: loss of 4096 x
-// 4096 1.37 ms in 256-wide tiles, 1.80 in 128-wide; 600 x 512 58.6 / 53.7 us, 300 x 4096 198 /
-// 208, 128 x 2048 51 / 47 (64-wide, two workgroups per CU: 55).
+// 4096 1.40 ms in 256-wide tiles, 1.83 in 128-wide; 1000 x 1024 123 / 145 us, 300 x 4096 196 /
+// 213, 600 x 512 59.5 / 60.6, 128 x 2048 50 / 49, 33 x 2048 47 / 41.
 int64_t round_time(bool narrow, int64_t K) { return narrow ? 1500 + 18 * K : 2500 + 25 * K; }
 int64_t plan_time(const HeadPlan& p, int64_t M, int64_t N, int64_t K) {
   const int64_t tiles = p.tiles(M, N), full = std::min<int64_t>(p.full, tiles), parts = (tiles - full) * p.S;
-  int64_t t = cdiv(full, 256) * round_time(p.narrow, K) + cdiv(parts, 256) * round_time(p.narrow, cdiv(K, p.S));
+  const bool narrow = p.tile == T128;
+  int64_t t = cdiv(full, 256) * round_time(narrow, K) + cdiv(parts, 256) * round_time(narrow, cdiv(K, p.S));
   // the partials' write and read, the join's launch
   if (parts > 0) t += 5000 + parts * 256 * p.cols() * 8 / 4500;
   return t;
@@ -911,13 +915,13 @@ constexpr int WHOLE = 1 << 30;  // no tile is split
 // The logits split where that should take 8% off at least (600 tokens of 50304 x 4096 312 ->
 // 273 us, 1000 430 -> 392, x 1024 121 -> 124).
 HeadPlan head_plan(int64_t M, int64_t N, int64_t K, bool narrow_too, bool logits) {
-  HeadPlan best{false, WHOLE, 1};
+  HeadPlan best{T256, WHOLE, 1};
   int64_t best_time = plan_time(best, M, N, K);
-  for (int narrow = 0; narrow <= (narrow_too ? 1 : 0); ++narrow) {
-    const int tiles = HeadPlan{narrow != 0, WHOLE, 1}.tiles(M, N);
+  for (int tile = T256; tile <= (narrow_too ? T128 : T256); ++tile) {
+    const int tiles = HeadPlan{tile, WHOLE, 1}.tiles(M, N);
     for (const int full : {WHOLE, 0, tiles / 256 * 256})
       for (int S = full == WHOLE ? 1 : 2; S <= (full == WHOLE ? 1 : 256) && (S == 1 || K / S >= 256); ++S) {
-        const HeadPlan p{narrow != 0, full, S};
+        const HeadPlan p{tile, full, S};
         if (p.frag(M, N, false) > (size_t(1) << 28)) break;
         const int64_t t = plan_time(p, M, N, K) * (logits && full != WHOLE ? 109 : 100) / 100;
         if (t < best_time) best = p, best_time = t;
@@ -931,7 +935,7 @@ void set_tiles(HeadGemm& a, int M, int N, int K, HeadPlan p) {
   a.M = M;
   a.N = N;
   a.K = K;
-  a.tiles_m = cdiv(M, 256);
+  a.tiles_m = cdiv(M, p.rows());
   a.tiles_n = cdiv(N, p.cols());
   a.full = p.full;
   a.S = p.S;
@@ -945,7 +949,7 @@ void launch_tile(const HeadGemm& a, int tiles, hipStream_t s) {
 template <bool AT, bool BT, int EP, int X>
 void launch_head(const HeadGemm& a, HeadPlan p, hipStream_t s) {
   const int tiles = p.virtual_tiles(a.M, a.N);
-  if (p.narrow) launch_tile<H128, AT, BT, EP, X>(a, tiles, s);
+  if (p.tile == T128) launch_tile<H128, AT, BT, EP, X>(a, tiles, s);
   else launch_tile<H256, AT, BT, EP, X>(a, tiles, s);
 }
 template <class GE, int X>
@@ -956,15 +960,17 @@ void launch_join_tile(const HeadGemm& a, hipStream_t s) {
 }
 template <int X>
 void launch_join(const HeadGemm& a, HeadPlan p, hipStream_t s) {
-  if (p.narrow) launch_join_tile<H128, X>(a, s);
+  if (p.tile == T128) launch_join_tile<H128, X>(a, s);
   else launch_join_tile<H256, X>(a, s);
 }
 
 template <int EP>
 void launch_logits(const HeadGemm& a, HeadPlan p, hipStream_t s) {
+  if constexpr (EP == EP_STATS)
+    if (p.tile == T64) return launch_tile<H64, false, false, EP, X_IS_B>(a, p.virtual_tiles(a.M, a.N), s);
   launch_head<false, false, EP, X_IS_B>(a, p, s);
   const int split = a.tiles_m * a.tiles_n - a.full;
-  if (split > 0 && p.narrow) hipLaunchKernelGGL((head_logits_join<H128, EP>), dim3(split * H128::NW), dim3(64), 0, s, a);
+  if (split > 0 && p.tile == T128) hipLaunchKernelGGL((head_logits_join<H128, EP>), dim3(split * H128::NW), dim3(64), 0, s, a);
   else if (split > 0) hipLaunchKernelGGL((head_logits_join<H256, EP>), dim3(split * H256::NW), dim3(64), 0, s, a);
 }
 
@@ -982,7 +988,10 @@ Layout head_layout(const mmuon_ce_args& x, bool train) {
   const int64_t T = std::max<int64_t>(x.tokens, 1);
   l.piece = std::min(T, std::max<int64_t>(1, x.piece_tokens));
   l.ldc = int64_t(cdiv(x.vocab, 256)) * 256;
-  l.logits = head_plan(x.vocab, l.piece, x.width, true, true);
+  // The loss alone of up to 64 tokens reads the head and little else: small tiles keep every CU
+  // at it (256 x 128: 197 tiles of 50304).  1 token x 4096 103.5 -> 96.8 us, x 1024 27.5 -> 25.6,
+  // 33 x 2048 41.6 -> 40.8, 64 x 512 21.6 -> 20.5, x 4096 106.5 -> 107.5; with gradients no gain.
+  l.logits = !train && l.piece <= 64 ? HeadPlan{T64, WHOLE, 1} : head_plan(x.vocab, l.piece, x.width, true, true);
   l.dx = head_plan(x.width, l.piece, x.vocab, true, false);
   // (128-wide tiles gained nothing there: 1000 x 512 54 us in 256-wide, 68 in 128-wide)
   l.dw = head_plan(x.width, x.vocab, l.piece, false, false);

@@ -51,6 +51,18 @@ def test_head_sizes(T, D, V, reduction):
     check_head(x.to(DEV), w.to(DEV), y.to(DEV), reduction)
 
 
+@pytest.mark.parametrize("T", [1, 32, 64])
+@pytest.mark.parametrize("V", [31, 33, 127, 128, 129, 161, 98400])
+def test_head_small_tiles(T, V):
+    """The loss alone of up to 64 tokens, in tiles of 128 of the vocabulary: its edges, its parts of 32, and more tiles
+    than are resident at a time (769 of them)."""
+    x, w, y = head(T, 40, V, seed=T + V)
+    y[0], y[-1] = 0, V - 1
+    for reduction in ("mean", "none"):
+        ref, _, _, (bound, _, _) = oracle.cross_entropy(x.to(DEV), w.to(DEV), y.to(DEV), -100, reduction)
+        within(linear_cross_entropy(x.to(DEV), w.to(DEV), y.to(DEV), reduction=reduction), ref, bound, reduction)
+
+
 @pytest.mark.parametrize("T, D, V", [(1, 32, 100), (70, 64, 1000), (300, 72, 515)])
 def test_head_per_token(T, D, V):
     x, w, y = head(T, D, V, seed=5, ignored=0.2)
