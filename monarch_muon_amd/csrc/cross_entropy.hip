@@ -21,6 +21,12 @@
 // and p_y - 1 do not go through a code.  One factor 1 / valid tokens is applied to the
 // fp32 sums of dx and dw and not to dl, and dx adds what bf16 took from its largest term,
 // p_y - 1: with them in dl, its rounding was one for all tokens, up to 2^-8.
+//
+// What bounds it, at 4096 tokens of 50304 x 4096: three products of 1.69 TFLOP, 1.42 ms with
+// statistics and codes, 1.23 (dx) and 1.21 (dw), 1.19 to 1.40 PFLOP/s; the matrix cores are 63,
+// 76 and 79% busy at 1.7 to 1.8 GHz, and the package-power limit holds the clock 80% of the
+// time.  One token: the read of the head, 412 MB in 89 us.  Narrow models (16384 tokens x 1024):
+// 10 B of memory traffic per logit (code out, in, dl out, in twice) beside 6144 operations.
 #include <algorithm>
 
 #include "common.hpp"

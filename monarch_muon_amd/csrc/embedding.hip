@@ -90,7 +90,9 @@ struct GradSpace {
 };
 
 // WAVES waves, ROWS rows of a class at most, LIST ids of a class that a wave keeps from its scan;
-// FIRST: zeros to all rows before, not to the empty ones behind
+// FIRST: zeros to all rows before, not to the empty ones behind.  Bound by the zeros (16384 bf16
+// tokens of 50304 x 4096: 80 us for most of 412 MB), then by reading all ids in each of 256
+// workgroups (65536 tokens of 50304 x 1024: 33 us); 1000 tokens of 50304 x 512 floats 19 us.
 template <class T, int N, int WAVES, int ROWS, int LIST, bool FIRST>
 __global__ __launch_bounds__(64 * WAVES) void embed_rows(mmuon_embedding_args a, int log2c, bool past, GradSpace space) {
   constexpr int NTH = 64 * WAVES;
@@ -212,7 +214,8 @@ __global__ __launch_bounds__(64 * WAVES) void embed_rows(mmuon_embedding_args a,
 
 // Sums in fp32: a wave takes 64 N columns of a segment, eight loads in flight, and writes
 // the rows that end in it; a row's piece that goes on, or began before, is left in sums (the
-// first piece of segment i in 2 i, the last in 2 i + 1).
+// first piece of segment i in 2 i, the last in 2 i + 1).  Bound by its reads at random rows: 16384
+// x 4096 in bf16 33 us (5.6 TB/s with the rows it writes), 57344 x 1024 28 us (4.2 of reads alone).
 template <class T, int N>
 __global__ __launch_bounds__(256) void embed_sum(mmuon_embedding_args a, int each, GradSpace space) {
   const int all = *space.all;
@@ -265,6 +268,7 @@ __global__ __launch_bounds__(256) void embed_sum(mmuon_embedding_args a, int eac
 
 // The rows that lie in several segments: a workgroup sums 32 N columns of the row that goes on
 // from its segment, if it begins there; 8 runs of the row's pieces side by side, joined in order.
+// Bound by its latency: 3 to 8 us, where one word is not most of the tokens.
 template <class T, int N>
 __global__ __launch_bounds__(256) void embed_join(mmuon_embedding_args a, int size, GradSpace space) {
   constexpr int LANES = 32, RUNS = 256 / LANES, SLICE = LANES * N;
