@@ -6,8 +6,13 @@
 // A loss that is a scalar makes its gradients in the forward, with the logits at hand, for a
 // gradient of 1; the backward scales them by the one that arrives (on the device; nothing is
 // touched where it is 1).  With a loss per token the backward knows each token's gradient only
-// then, and makes the logits again.
+// then, and makes the logits again.  The loss has no second derivative: what depends on its
+// gradients raises when it is differentiated.  The table's gradient has one.
 #include "torch_common.hpp"
+
+#include <torch/csrc/autograd/engine.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 
 #include <tuple>
 
@@ -174,6 +179,25 @@ void call_scale(const Tensor& x, const Tensor& y, const Tensor& factor) {
   op.call(x, y, factor);
 }
 
+constexpr const char* NO_SECOND = "Trying to backward through mmuon.linear_cross_entropy_grad.default but no autograd "
+                                  "formula was registered.";
+
+// Gradients that the forward made, handed out by the current node of a graph that is kept
+// (create_graph): they depend on the node's inputs and on the gradient that arrived, and a
+// derivative along any of these raises.
+void refuse_derivatives(std::initializer_list<Tensor*> made, const Tensor& arrived) {
+  const std::shared_ptr<torch::autograd::Node> current = torch::autograd::get_current_node();
+  TORCH_CHECK(current != nullptr, NO_SECOND);
+  torch::autograd::edge_list edges = current->next_edges();
+  edges.push_back(torch::autograd::impl::gradient_edge(arrived));
+  const auto error = std::make_shared<torch::autograd::Error>(NO_SECOND, std::move(edges));
+  for (Tensor* t : made) {
+    if (t->numel() == 0) continue;  // not asked for
+    *t = t->detach();
+    torch::autograd::set_history(*t, error);
+  }
+}
+
 struct LossFn : torch::autograd::Function<LossFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& target,
                         int64_t ignore_index, int64_t reduction, int64_t piece) {
@@ -209,11 +233,37 @@ struct LossFn : torch::autograd::Function<LossFn> {
       ctx->saved_data["spent"] = true;
       gx = saved[0];
       gw = saved[1];
-      call_scale(gx, gw, grads[0].to(at::kFloat));
+      {
+        at::AutoDispatchBelowADInplaceOrView below;
+        call_scale(gx, gw, grads[0].to(at::kFloat));
+      }
+      if (at::GradMode::is_enabled()) refuse_derivatives({&gx, &gw}, grads[0]);
     }
     return {dx ? gx : Tensor(), dw ? gw : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
+
+// The gradient has no derivative of its own.
+struct GradFn : torch::autograd::Function<GradFn> {
+  static variable_list forward(AutogradContext*, const Tensor& x, const Tensor& w, const Tensor& target,
+                               const c10::optional<Tensor>& grad, int64_t ignore_index, int64_t reduction,
+                               int64_t piece, bool need_dx, bool need_dw) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [loss, dx, dw] = call_grad(x, w, target, grad, ignore_index, reduction, piece, need_dx, need_dw);
+    return {loss, dx, dw};
+  }
+  static variable_list backward(AutogradContext*, const variable_list&) { TORCH_CHECK(false, NO_SECOND); }
+};
+
+Triple grad_autograd(const Tensor& x, const Tensor& w, const Tensor& target, const c10::optional<Tensor>& grad,
+                     int64_t ignore_index, int64_t reduction, int64_t piece, bool need_dx, bool need_dw) {
+  if (any_requires_grad({&x, &w}) || (grad.has_value() && any_requires_grad({&*grad}))) {
+    const variable_list r = GradFn::apply(x, w, target, grad, ignore_index, reduction, piece, need_dx, need_dw);
+    return {r[0], r[1], r[2]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_grad(x, w, target, grad, ignore_index, reduction, piece, need_dx, need_dw);
+}
 
 Tensor loss_autograd(const Tensor& x, const Tensor& w, const Tensor& target, int64_t ignore_index, int64_t reduction,
                      int64_t piece) {
@@ -312,6 +362,35 @@ Tensor embedding_grad_sym(const Tensor& dout, const Tensor& index, c10::SymInt v
   return embedding_grad_impl(dout, index, vocab.expect_int(), scale, padding_idx);
 }
 
+// The table's gradient is linear in the one that arrives: its derivative by that is the lookup
+// in what arrives here, with zeros where a token took part in nothing.
+struct EmbeddingGradFn : torch::autograd::Function<EmbeddingGradFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& dout, const Tensor& index, c10::SymInt vocab, double scale,
+                        int64_t padding_idx) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({index});
+    ctx->saved_data["vocab"] = vocab;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding_idx"] = padding_idx;
+    return call_embedding_grad(dout, index, vocab, scale, padding_idx);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const Tensor index = ctx->get_saved_variables()[0];
+    const int64_t pad = ctx->saved_data["padding_idx"].toInt();
+    const Tensor rows = call_embedding(index, grads[0], ctx->saved_data["scale"].toDouble(), -1);
+    Tensor none = at::logical_or(index < 0, index >= at::Scalar(ctx->saved_data["vocab"].toSymInt()));
+    if (pad >= 0) none = at::logical_or(none, index == pad);
+    return {rows.masked_fill(none.unsqueeze(-1), 0), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor embedding_grad_autograd(const Tensor& dout, const Tensor& index, c10::SymInt vocab, double scale,
+                               int64_t padding_idx) {
+  if (any_requires_grad({&dout})) return EmbeddingGradFn::apply(dout, index, vocab, scale, padding_idx);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_embedding_grad(dout, index, std::move(vocab), scale, padding_idx);
+}
+
 struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& index, const Tensor& weight, double scale,
                         int64_t padding_idx) {
@@ -360,5 +439,7 @@ TORCH_LIBRARY_IMPL(mmuon, CompositeExplicitAutograd, m) {
 }
 TORCH_LIBRARY_IMPL(mmuon, Autograd, m) {
   m.impl("linear_cross_entropy", loss_autograd);
+  m.impl("linear_cross_entropy_grad", grad_autograd);
   m.impl("embedding", embedding_autograd);
+  m.impl("embedding_grad", embedding_grad_autograd);
 }

@@ -68,7 +68,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     shape of ``target``).
 
     Differentiable in ``x`` and ``weight``.  With "mean" and "sum" the forward makes the gradients, so one backward
-    can be taken of it; with "none" the backward makes the logits again.  ``piece_tokens``: tokens whose logits are
+    can be taken of it; with "none" the backward makes the logits again.  There is no second derivative: one of
+    gradients taken with ``create_graph`` raises.  ``piece_tokens``: tokens whose logits are
     held at a time, 16 bits each; by default as many as fit 1 GiB.
     """
     if _loss_op is None:
@@ -95,7 +96,8 @@ def embedding(index: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
 
     ``index`` int64 or int32, ``weight`` (V, D).  An id outside [0, V) gives a row of NaN.  Differentiable in
     ``weight``: the gradient is dense, the same whatever the timing, each row the float32 sum over its tokens in a
-    fixed order; ids outside [0, V) and ``padding_idx`` (counted from the end where negative) take none.
+    fixed order; ids outside [0, V) and ``padding_idx`` (counted from the end where negative) take none.  The
+    gradient is differentiable in the one that arrives.
     """
     if _embedding_op is None:
         _load()

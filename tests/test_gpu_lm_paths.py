@@ -1,0 +1,42 @@
+"""More of the language-model operators on the GPU against their plain float64 forms: what ordinary calls reach beside
+the sizes and layouts of test_gpu_lm.py."""
+import pytest
+import torch
+
+from monarch_muon_amd import embedding, linear_cross_entropy
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+
+
+# ----- derivatives of gradients ------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_embedding_gradient_derivative(dtype):
+    """The derivative of the table's gradient by the gradient that arrived: scale * up[i], one rounding, and nothing for
+    padding and for ids that are no token, whatever ``up`` holds there."""
+    g = torch.Generator().manual_seed(1)
+    i = torch.tensor([3, 0, 29, -1, 30, 2 ** 40, 3, 7], device=DEV).view(2, 4)
+    w, up = (torch.randn(30, 24, generator=g).to(dtype).to(DEV) for _ in range(2))
+    dout = torch.randn(2, 4, 24, generator=g).to(dtype).to(DEV).requires_grad_()
+    up[7] = float("nan")
+    dw, = torch.autograd.grad(embedding(i, w.requires_grad_(), scale=1.5, padding_idx=7), w, dout, create_graph=True)
+    plain, = torch.autograd.grad(embedding(i, w, scale=1.5, padding_idx=7), w, dout.detach())
+    assert torch.equal(dw, plain)
+    d, = torch.autograd.grad(dw, dout, up)
+    ref = torch.zeros(2, 4, 24, device=DEV)
+    for r, c, v in ((0, 0, 3), (0, 1, 0), (0, 2, 29), (1, 2, 3)):
+        ref[r, c] = up[v].float() * 1.5
+    assert d.dtype == dtype and torch.equal(d, ref.to(dtype))
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_loss_gradient_of_a_kept_graph(reduction):
+    """create_graph changes no value; a derivative of the gradients is refused."""
+    g = torch.Generator().manual_seed(2)
+    x, w = (torch.randn(n, 64, generator=g).bfloat16().to(DEV).requires_grad_() for n in (70, 300))
+    y = torch.randint(0, 300, (70,), generator=g).to(DEV)
+    want = torch.autograd.grad(linear_cross_entropy(x, w, y, reduction=reduction).sum() / 4, (x, w))
+    got = torch.autograd.grad(linear_cross_entropy(x, w, y, reduction=reduction).sum() / 4, (x, w), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    with pytest.raises(RuntimeError, match="no autograd formula"):
+        (got[0].float().square().sum() + w.float().sum()).backward()

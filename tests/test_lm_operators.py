@@ -1,0 +1,80 @@
+"""The language-model operators under torch's autograd, without a GPU: second derivatives on meta tensors."""
+import warnings
+
+import pytest
+import torch
+
+from monarch_muon_amd import embedding, linear_cross_entropy
+
+
+def meta(*shape, dtype=torch.bfloat16):
+    return torch.zeros(shape, dtype=dtype, device="meta")
+
+
+def head(reduction):
+    x, w = meta(6, 16).requires_grad_(), meta(5, 16).requires_grad_()
+    return x, w, linear_cross_entropy(x, w, meta(6, dtype=torch.long), reduction=reduction)
+
+
+# ----- second derivatives ----------------------------------------------------------
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("wrt", ["x", "w", "both", "factor"])
+def test_second_derivative_of_the_loss_is_refused(reduction, wrt):
+    """A gradient taken with create_graph knows that it depends on x, weight and the incoming gradient: a derivative of
+    it raises, also where it is one term beside others that have a derivative of their own."""
+    x, w, loss = head(reduction)
+    factor = meta(dtype=torch.float32).requires_grad_()
+    inputs = {"x": (x,), "w": (w,), "both": (x, w), "factor": (x,)}[wrt]
+    grads = torch.autograd.grad((loss * factor if wrt == "factor" else loss).sum(), inputs, create_graph=True)
+    assert all(g.requires_grad for g in grads)
+    for g in grads:
+        penalty = g.float().square().sum()
+        for target in (x, w, *((factor,) if wrt == "factor" else ())):
+            other = target.float().sum()
+            with pytest.raises(RuntimeError, match="no autograd formula"):
+                torch.autograd.grad(penalty + other, target, retain_graph=True, allow_unused=True)
+
+
+def test_second_derivative_is_refused_by_backward():
+    x, w, loss = head("mean")
+    (g,) = torch.autograd.grad(loss, x, create_graph=True)
+    with pytest.raises(RuntimeError, match="no autograd formula"):
+        (g.float().sum() + w.float().sum()).backward()
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_first_derivatives_carry_no_graph(reduction):
+    """Without create_graph the gradients are plain tensors, and nothing warns."""
+    x, w, loss = head(reduction)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        grads = torch.autograd.grad(loss.sum(), (x, w))
+    assert not any(g.requires_grad for g in grads)
+
+
+def test_gradient_operator_has_no_derivative():
+    """The gradient's own operator, called with tensors that require one."""
+    x, w, _ = head("none")
+    loss, dx, dw = torch.ops.mmuon.linear_cross_entropy_grad(x, w, meta(6, dtype=torch.long), None, -100, 1, 6, True, True)
+    for out in (loss, dx, dw):
+        with pytest.raises(RuntimeError, match="no autograd formula"):
+            torch.autograd.grad(out.float().sum(), x, retain_graph=True)
+
+
+@pytest.mark.parametrize("order", [2, 3])
+def test_embedding_gradient_is_differentiable(order):
+    """The table's gradient is linear in the gradient that arrives: its derivative by that is a lookup, and that of the
+    lookup the table's gradient again."""
+    w = meta(9, 16).requires_grad_()
+    dout = meta(2, 3, 16).requires_grad_()
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        out = embedding(meta(2, 3, dtype=torch.long), w, scale=3.0, padding_idx=4)
+        (dw,) = torch.autograd.grad(out, w, dout, create_graph=True)
+        assert dw.requires_grad
+        up = meta(9, 16).requires_grad_()
+        (d,) = torch.autograd.grad(dw, dout, up, create_graph=True)
+        assert d.shape == dout.shape and d.dtype == dout.dtype
+        if order == 3:
+            (u,) = torch.autograd.grad(d, up, meta(2, 3, 16))
+            assert u.shape == up.shape
