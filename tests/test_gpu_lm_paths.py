@@ -5,6 +5,9 @@ import torch
 
 from monarch_muon_amd import embedding, linear_cross_entropy
 
+from lm_paths import HEAD_PATHS
+from test_gpu_lm import check_head, head
+
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
 
@@ -40,3 +43,13 @@ def test_loss_gradient_of_a_kept_graph(reduction):
     assert all(torch.equal(a, b) for a, b in zip(want, got))
     with pytest.raises(RuntimeError, match="no autograd formula"):
         (got[0].float().square().sum() + w.float().sum()).backward()
+
+
+# ----- tilings of the products -------------------------------------------------------
+@pytest.mark.parametrize("ignored", [0.0, 0.4])
+@pytest.mark.parametrize("size, path", HEAD_PATHS, ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else None)
+def test_head_paths(size, path, ignored):
+    """Each tile and split over K that a product can take, the loss alone and with gradients."""
+    T, D, V, piece = size
+    x, w, y = (t.to(DEV) for t in head(T, D, V, seed=T + V, ignored=ignored))
+    check_head(x, w, y, piece_tokens=piece)
