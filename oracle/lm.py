@@ -68,3 +68,26 @@ def embedding_grad(dout, index, vocab, scale=1.0, padding_idx=None):
     size = torch.zeros_like(dw).index_add_(0, index[keep], dout[keep].abs())
     count = torch.bincount(index[keep], minlength=vocab).double()
     return dw * scale, (count + 2)[:, None] * U32 * size * abs(scale)
+
+
+def head_dx(x, w, target, ignore_index=-100, reduction="mean", grad=None):
+    """(dx, elementwise bound, bound of the norm of the difference) where the target's entry p - 1 of dl reaches dx in
+    fp32: bf16's rounding of it is added back, so it has the error of p by nll alone.  The other entries' roundings
+    differ from one another; the norm of their sum is that of independent errors of at most their size, and with the
+    rounding of the result (its norm known) the two add in squares.  5% for what sums of many thousands may stray."""
+    dev = x.device
+    x64, w64, target = x.double(), w.double().to(dev), target.to(dev).long()
+    _, dx, _, (_, bound, _) = cross_entropy(x, w, target, ignore_index, reduction, grad)
+    keep = target != ignore_index
+    xk, yk = x64[keep], target[keep]
+    n, rows = len(yk), torch.arange(len(yk), device=dev)
+    p = torch.softmax(xk @ w64.T, 1)
+    g = grad.double().to(dev)[keep] if grad is not None else torch.full((n,), 1.0 / n if reduction == "mean" else 1.0,
+                                                                        dtype=torch.float64, device=dev)
+    at_target = (g * (1 - p[rows, yk])).abs()
+    bound[keep] -= (at_target * (UCODE + UBF))[:, None] * w64[yk].abs()
+    dl = p * g[:, None]
+    dl[rows, yk] = 0
+    others = (dl.square() @ w64.square()).sum() * (UBF / 2 + UCODE) ** 2   # (a rounding is half of UBF at most)
+    rounding = (dx.bfloat16().double() - dx).square().sum()
+    return dx, bound, 1.05 * (others + rounding).sqrt()

@@ -6,7 +6,8 @@ import torch
 from monarch_muon_amd import embedding, linear_cross_entropy
 
 from lm_paths import HEAD_PATHS
-from test_gpu_lm import check_head, head
+from oracle import lm as oracle
+from test_gpu_lm import check_head, head, within
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -53,3 +54,21 @@ def test_head_paths(size, path, ignored):
     T, D, V, piece = size
     x, w, y = (t.to(DEV) for t in head(T, D, V, seed=T + V, ignored=ignored))
     check_head(x, w, y, piece_tokens=piece)
+
+
+# ----- what bf16 takes from dl at the target -----------------------------------------
+@pytest.mark.parametrize("reduction, ignored", [("mean", 0.0), ("sum", 0.4), ("none", 0.4)])
+@pytest.mark.parametrize("size", [(129, 256, 1023, None), (600, 776, 2500, None), (200, 520, 70000, None),
+                                  (900, 264, 33000, 400)] + [s for s, _ in HEAD_PATHS],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_dx_has_the_targets_term(size, reduction, ignored):
+    """dx within the bounds that leave no rounding to dl at the target, unsplit, split, masked and in pieces."""
+    T, D, V, piece = size
+    x, w, y = (t.to(DEV) for t in head(T, D, V, seed=T + V, ignored=ignored))
+    up = torch.randn(T, generator=torch.Generator().manual_seed(1)).to(DEV) if reduction == "none" else None
+    dx, bound, norm = oracle.head_dx(x, w, y, reduction=reduction, grad=up)
+    x.requires_grad_()
+    got, = torch.autograd.grad(linear_cross_entropy(x, w, y, reduction=reduction, piece_tokens=piece), x, up)
+    within(got, dx, bound, "dx")
+    off = float((got.double() - dx).norm())
+    assert off <= float(norm), (off / float(norm), off / float(dx.norm()))
