@@ -402,9 +402,10 @@ size_t mmuon_butterfly_linear_workspace(const mmuon_butterfly_args* a);
      not ignored (MMUON_CE_MEAN; NaN if there is none).
    Gradients (mmuon_ce_fwd_bwd): dx and dw of sum over t of g[t] nll[t], g = grad
    where given, else that of loss (1 with MMUON_CE_NONE).
-   No logits are kept: the loss alone keeps two floats per token and 128 of the
-   vocabulary; the gradients take piece_tokens tokens at a time and keep 16 bits
-   per logit of the piece in the workspace. */
+   No logits are kept: the loss alone keeps two floats per token and 32, 64 or 128
+   of the vocabulary; the gradients take piece_tokens tokens at a time and keep 16
+   bits per logit of the piece in the workspace.  Where there are several pieces and
+   dw is wanted, its sums stay there between them: 4 B per element of w. */
 enum { MMUON_CE_NONE = 0, MMUON_CE_MEAN = 1, MMUON_CE_SUM = 2 };
 typedef struct mmuon_ce_args {
   int64_t tokens;         /* 0 <= tokens < 2^24 */
@@ -430,8 +431,9 @@ typedef struct mmuon_ce_args {
 } mmuon_ce_args;
 int mmuon_ce_fwd(const mmuon_ce_args* a, void* stream);
 int mmuon_ce_fwd_bwd(const mmuon_ce_args* a, void* stream);
-/* Workspace bytes of a call with these sizes and this piece (train: of mmuon_ce_fwd_bwd;
-   nll null counts it in). */
+/* Workspace bytes of a call with these sizes, this piece and these outputs (train: of
+   mmuon_ce_fwd_bwd).  Whether a pointer is null counts: nll null counts it in, dx or dw
+   null leaves out what their sums need. */
 size_t mmuon_ce_workspace(const mmuon_ce_args* a, int32_t train);
 /* x and y (either may be empty) *= *factor (device), bf16, nx and ny multiples of 8; writes
    nothing where *factor == 1. */
@@ -468,7 +470,7 @@ size_t mmuon_embedding_workspace(const mmuon_embedding_args* a);
 const char* mmuon_last_error(void);
 
 /* ABI version: bumped on any change to this header. */
-#define MMUON_ABI_VERSION 9
+#define MMUON_ABI_VERSION 10
 int mmuon_abi_version(void);
 
 #ifdef __cplusplus

@@ -12,7 +12,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(os.environ.get("MMUON_LIB", Path(__file__).resolve().parent / "libmmuon.so"))
-ABI_VERSION = 9
+ABI_VERSION = 10
 # the layer's torch operator; the name carries the ABI, so that one built for another is never loaded (once loaded,
 # its registrations stay for the life of the process)
 TORCH_LIB_PATH = Path(__file__).resolve().parent / f"libmmuon_torch.{ABI_VERSION}.so"

@@ -953,8 +953,9 @@ Layout head_layout(const mmuon_ce_args& x, bool train) {
   l.parts = take(P * l.nparts * 8);
   l.tlogit = take(P * 4);
   l.resid = take(train ? P * 4 : 0);
-  l.frag = take(std::max(l.logits.frag(x.vocab, l.piece, false), train ? l.dx.frag(x.width, l.piece, false) : 0));
-  l.dwfrag = take(train ? l.dw.frag(x.width, x.vocab, T > l.piece) : 0);
+  l.frag = take(std::max(l.logits.frag(x.vocab, l.piece, false),
+                         train && x.dx != nullptr ? l.dx.frag(x.width, l.piece, false) : 0));
+  l.dwfrag = take(train && x.dw != nullptr ? l.dw.frag(x.width, x.vocab, T > l.piece) : 0);
   l.nll = take(x.nll == nullptr ? size_t(T) * 4 : 0);
   l.rows = take(size_t(T) * 4);
   l.compact = take(size_t(T) * 8);

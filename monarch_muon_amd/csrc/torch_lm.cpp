@@ -61,9 +61,10 @@ void check_head(const Tensor& x, const Tensor& w, const Tensor& target, int64_t 
 }
 
 // Tokens of a piece: as asked, else as many as keep the codes of a piece (2 B per logit)
-// within 1 GiB, in whole 256-token tiles, and pieces of one size.  The loss alone has no
-// codes: four times as many.
-int64_t piece_of(int64_t tokens, int64_t vocab, int64_t asked, bool train) {
+// within 1 GiB (256 at least), in whole 256-token tiles, and pieces of one size.  The loss
+// alone has no codes: four times as many.  Several pieces keep fp32 sums of dw between them:
+// where one piece of all tokens takes no more memory than those, it is one.
+int64_t piece_of(int64_t tokens, int64_t width, int64_t vocab, int64_t asked, bool train, bool need_dw) {
   TORCH_CHECK_VALUE(asked >= 0, "piece_tokens must be positive, got ", asked);
   if (asked > 0) return std::min(asked, std::max<int64_t>(tokens, 1));
   const int64_t row = (vocab + 255) / 256 * 512;
@@ -71,14 +72,17 @@ int64_t piece_of(int64_t tokens, int64_t vocab, int64_t asked, bool train) {
   if (!train) most *= 4;
   if (tokens <= most) return std::max<int64_t>(tokens, 1);
   const int64_t pieces = (tokens + most - 1) / most;
-  return ((tokens + pieces - 1) / pieces + 255) / 256 * 256;
+  const int64_t piece = ((tokens + pieces - 1) / pieces + 255) / 256 * 256;
+  // codes, gathered rows, statistics (8 B per 64 or 128 of the vocabulary)
+  const int64_t each = row + 2 * width + row / 16;
+  return train && need_dw && (tokens - piece) * each <= 4 * vocab * width ? tokens : piece;
 }
 
 struct HeadCall {
   Tensor x, w, target, grad, ws;
   mmuon_ce_args a{};
   HeadCall(const Tensor& x_, const Tensor& w_, const Tensor& target_, int64_t ignore_index, int64_t reduction,
-           int64_t piece, bool train)
+           int64_t piece, bool train, bool need_dw)
       : x(aligned_rows(x_)), w(aligned_rows(w_)), target(target_.to(at::kLong).contiguous()) {
     a.tokens = x.size(0);
     a.vocab = w.size(0);
@@ -89,7 +93,7 @@ struct HeadCall {
     a.ignore_index = ignore_index;
     a.x_stride = a.tokens > 1 ? x.stride(0) : a.width;
     a.w_stride = a.vocab > 1 ? w.stride(0) : a.width;
-    a.piece_tokens = piece_of(a.tokens, a.vocab, piece, train);
+    a.piece_tokens = piece_of(a.tokens, a.width, a.vocab, piece, train, need_dw);
     a.x = x.const_data_ptr();
     a.w = w.const_data_ptr();
     a.target = static_cast<const int64_t*>(target.const_data_ptr());
@@ -109,7 +113,7 @@ Tensor loss_impl(const Tensor& x, const Tensor& w, const Tensor& target, int64_t
   require_one_device({&x, &w, &target});
   bind_library();
   const c10::DeviceGuard guard(x.device());
-  HeadCall call(x, w, target, ignore_index, reduction, piece, false);
+  HeadCall call(x, w, target, ignore_index, reduction, piece, false, false);
   const bool none = reduction == MMUON_CE_NONE;
   Tensor out = none ? at::empty({x.size(0)}, x.options().dtype(at::kFloat)) : at::empty({}, x.options().dtype(at::kFloat));
   (none ? call.a.nll : call.a.loss) = static_cast<float*>(out.data_ptr());
@@ -127,7 +131,7 @@ Triple grad_impl(const Tensor& x, const Tensor& w, const Tensor& target, const c
                     "grad must hold one float32 per token");
   bind_library();
   const c10::DeviceGuard guard(x.device());
-  HeadCall call(x, w, target, ignore_index, reduction, piece, true);
+  HeadCall call(x, w, target, ignore_index, reduction, piece, true, need_dw);
   const bool none = reduction == MMUON_CE_NONE;
   Tensor out = none ? at::empty({x.size(0)}, x.options().dtype(at::kFloat)) : at::empty({}, x.options().dtype(at::kFloat));
   (none ? call.a.nll : call.a.loss) = static_cast<float*>(out.data_ptr());

@@ -72,3 +72,37 @@ def test_dx_has_the_targets_term(size, reduction, ignored):
     within(got, dx, bound, "dx")
     off = float((got.double() - dx).norm())
     assert off <= float(norm), (off / float(norm), off / float(dx.norm()))
+
+
+# ----- memory ------------------------------------------------------------------------
+def peak(x, w, y, wrt, **kw):
+    """Bytes beyond what stood before, with the gradients."""
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    grads = torch.autograd.grad(linear_cross_entropy(x, w, y, **kw), wrt)
+    torch.cuda.synchronize()
+    return torch.cuda.max_memory_allocated() - before, grads
+
+
+def test_default_piece_counts_the_sums_that_pieces_keep():
+    """6000 tokens of 131072 x 4096: their codes are 1.46 GiB, two pieces' 0.75 and 2 GiB of fp32 sums of dw.  All are
+    one piece where the head is trained; a frozen one takes two, and no sums."""
+    T, D, V = 6000, 4096, 131072
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(T, D, generator=g, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    w = (torch.randn(V, D, generator=g, device=DEV) / 64).bfloat16().requires_grad_()
+    y = torch.randint(0, V, (T,), generator=g, device=DEV)
+    outputs, slack = 2 * D * (T + V), 512 << 20
+    whole, (dx, dw) = peak(x, w, y, (x, w))
+    assert whole <= 2 * T * V + outputs + slack, whole
+    pieces, (px, pw) = peak(x, w, y, (x, w), piece_tokens=3072)
+    assert whole < pieces
+    frozen, (fx,) = peak(x, w.detach(), y, (x,))
+    assert frozen <= (1 << 30) + 2 * D * T + slack, frozen
+    only, (ow,) = peak(x.detach(), w, y, (w,))
+    assert only <= whole
+    # the pieces' sums are of the same terms
+    for a, b in ((px, dx), (fx, dx), (pw, dw), (ow, dw)):
+        assert float((a.float() - b.float()).norm()) <= 2.0 ** -8 * float(b.float().norm())
