@@ -7,7 +7,7 @@ from monarch_muon_amd import embedding, linear_cross_entropy
 
 from lm_paths import HEAD_PATHS
 from oracle import lm as oracle
-from test_gpu_lm import check_head, head, within
+from test_gpu_lm import check_embedding, check_head, head, ids, within
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -106,3 +106,19 @@ def test_default_piece_counts_the_sums_that_pieces_keep():
     # the pieces' sums are of the same terms
     for a, b in ((px, dx), (fx, dx), (pw, dw), (ow, dw)):
         assert float((a.float() - b.float()).norm()) <= 2.0 ** -8 * float(b.float().norm())
+
+
+# ----- rows of whole 16-byte chunks ----------------------------------------------------
+@pytest.mark.parametrize("T, D, V", [(1, 4, 3), (70, 12, 50), (5000, 1028, 300), (300, 516, 1000)])
+def test_float_tables_of_whole_chunks(T, D, V):
+    """float32 rows of 4 mod 8 columns, whole 16-byte chunks: against the plain form, and column by column the same bits
+    as the wider table's, as the same chunks are summed the same way."""
+    g = torch.Generator().manual_seed(T)
+    w, dy = torch.randn(V, D + 4, generator=g).to(DEV), torch.randn(T, D + 4, generator=g).to(DEV)
+    i = ids(T, V, T).to(DEV)
+    check_embedding(i, w[:, :D].contiguous(), dy[:, :D].contiguous(), scale=0.5, pad=V - 1)
+    check_embedding(i, w[:, :D], dy[:, :D])           # rows 4 mod 8 apart where D + 4 is
+    wide, = torch.autograd.grad(embedding(i, w.requires_grad_()), w, dy)
+    table = w.detach()[:, :D].contiguous().requires_grad_()
+    narrow, = torch.autograd.grad(embedding(i, table), table, dy[:, :D].contiguous())
+    assert torch.equal(narrow, wide[:, :D])
