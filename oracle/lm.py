@@ -88,6 +88,6 @@ def head_dx(x, w, target, ignore_index=-100, reduction="mean", grad=None):
     bound[keep] -= (at_target * (UCODE + UBF))[:, None] * w64[yk].abs()
     dl = p * g[:, None]
     dl[rows, yk] = 0
-    others = (dl.square() @ w64.square()).sum() * (UBF / 2 + UCODE) ** 2   # (a rounding is half of UBF at most)
+    others = (dl.square() @ w64.square()).sum() * (UBF + UCODE) ** 2
     rounding = (dx.bfloat16().double() - dx).square().sum()
     return dx, bound, 1.05 * (others + rounding).sqrt()
