@@ -436,7 +436,7 @@ int mmuon_ce_fwd_bwd(const mmuon_ce_args* a, void* stream);
    null leaves out what their sums need. */
 size_t mmuon_ce_workspace(const mmuon_ce_args* a, int32_t train);
 /* x and y (either may be empty) *= *factor (device), bf16, nx and ny multiples of 8; writes
-   nothing where *factor == 1. */
+   nothing where *factor == 1.  Rounded to bf16 again: exact for a power of two. */
 int mmuon_scale_bf16(void* x, int64_t nx, void* y, int64_t ny, const float* factor, void* stream);
 
 /* Token embedding: out[t] = scale * w[index[t]] (fp32 product, one rounding), NaN where

@@ -5,7 +5,9 @@
 //
 // A loss that is a scalar makes its gradients in the forward, with the logits at hand, for a
 // gradient of 1; the backward scales them by the one that arrives (on the device; nothing is
-// touched where it is 1).  With a loss per token the backward knows each token's gradient only
+// touched where it is 1).  They are bf16 by then, so a factor that is no power of two rounds
+// them a second time: kept in fp32 until the backward they would take twice the memory of dx
+// and dw.  With a loss per token the backward knows each token's gradient only
 // then, and makes the logits again.  The loss has no second derivative: what depends on its
 // gradients raises when it is differentiated.  The table's gradient has one.
 #include "torch_common.hpp"

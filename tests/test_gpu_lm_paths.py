@@ -122,3 +122,26 @@ def test_float_tables_of_whole_chunks(T, D, V):
     table = w.detach()[:, :D].contiguous().requires_grad_()
     narrow, = torch.autograd.grad(embedding(i, table), table, dy[:, :D].contiguous())
     assert torch.equal(narrow, wide[:, :D])
+
+
+# ----- the gradient that arrives -------------------------------------------------------
+@pytest.mark.parametrize("factor", [1 / 3, 0.7, -5.0, 2.0 ** -20, 0.0])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_head_upstream_factor(factor, reduction):
+    """Gradients made by the forward, times a factor that arrives later: a second rounding, none for a power of two.
+    With a loss per token the factor is in dl, and the result is rounded once."""
+    x, w, y = (t.to(DEV) for t in head(300, 264, 1000, seed=31, ignored=0.2))
+    _, dx, dw, (_, xt, wt) = oracle.cross_entropy(x, w, y, reduction=reduction)
+    x.requires_grad_(), w.requires_grad_()
+    got = torch.autograd.grad(linear_cross_entropy(x, w, y, reduction=reduction) * factor, (x, w))
+    one = torch.autograd.grad(linear_cross_entropy(x, w, y, reduction=reduction), (x, w))
+    f = float(torch.tensor(factor))
+    for a, b, ref, bound in zip(got, one, (dx, dw), (xt, wt)):
+        assert torch.equal(a, (b.float() * f).bfloat16())
+        within(a, f * ref, abs(f) * bound + 1.01 * oracle.UBF * (f * ref).abs() + 1e-37, "twice rounded")
+    if reduction == "sum":
+        up = torch.full((300,), factor, device=DEV)
+        _, dx, dw, (_, xt, wt) = oracle.cross_entropy(x.detach(), w.detach(), y, reduction="none", grad=up)
+        got = torch.autograd.grad(linear_cross_entropy(x, w, y, reduction="none"), (x, w), up)
+        within(got[0], dx, xt, "dx, rounded once")
+        within(got[1], dw, wt, "dw, rounded once")
