@@ -25,6 +25,7 @@ std::atomic<bool> bound{false};
 namespace {
 int (*loader)() = nullptr;         // loads the library and binds it; 0 where it did
 thread_local std::string refusal;  // why it did not
+std::mutex binding;                // held where abi is written: once bound is set it is only read
 }  // namespace
 
 void bind_library() {
@@ -207,7 +208,9 @@ extern "C" {
 // declares the library bound.
 int mmuon_torch_bind_lm(int version, void* ce_fwd, void* ce_fwd_bwd, void* ce_workspace, void* scale, void* emb_fwd,
                         void* emb_bwd, void* emb_workspace) {
-  if (version != MMUON_ABI_VERSION || bound) return 0;  // mmuon_torch_bind says so
+  if (version != MMUON_ABI_VERSION) return 0;  // mmuon_torch_bind says so
+  const std::lock_guard<std::mutex> lock(binding);
+  if (bound) return 0;  // by another thread's first call
   abi.ce_fwd = reinterpret_cast<decltype(abi.ce_fwd)>(ce_fwd);
   abi.ce_fwd_bwd = reinterpret_cast<decltype(abi.ce_fwd_bwd)>(ce_fwd_bwd);
   abi.ce_workspace = reinterpret_cast<decltype(abi.ce_workspace)>(ce_workspace);
@@ -228,8 +231,7 @@ int mmuon_torch_bind(int version, void* fwd, void* bwd, void* workspace, void* l
               std::to_string(version) + ": build both again with `python -m monarch_muon_amd.build`";
     return -1;
   }
-  static std::mutex mutex;
-  const std::lock_guard<std::mutex> lock(mutex);
+  const std::lock_guard<std::mutex> lock(binding);
   if (bound) return 0;  // by another thread's first call
   abi.fwd = reinterpret_cast<decltype(abi.fwd)>(fwd);
   abi.bwd = reinterpret_cast<decltype(abi.bwd)>(bwd);

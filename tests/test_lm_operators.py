@@ -78,3 +78,26 @@ def test_embedding_gradient_is_differentiable(order):
         if order == 3:
             (u,) = torch.autograd.grad(d, up, meta(2, 3, 16))
             assert u.shape == up.shape
+
+
+# ----- first calls -------------------------------------------------------------------
+def test_first_calls_of_many_threads():
+    """A fresh process whose first calls come from many threads at once: each binds or finds the library bound."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    program = """
+import threading
+from monarch_muon_amd import butterfly
+start, results = threading.Barrier(16), []
+def call():
+    start.wait()
+    results.append(butterfly._bind())
+threads = [threading.Thread(target=call) for _ in range(16)]
+for t in threads: t.start()
+for t in threads: t.join()
+assert results == [0] * 16, results
+"""
+    r = subprocess.run([sys.executable, "-c", program], cwd=Path(__file__).resolve().parent.parent, capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
