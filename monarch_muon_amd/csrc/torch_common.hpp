@@ -51,7 +51,12 @@ Tensor dense_aligned(const Tensor& t);
 
 inline void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
+// Whether a backward is wanted.  None of the operators has a forward-mode derivative: a tangent
+// raises (dropped, it would count as zero).
 inline bool any_requires_grad(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(/*level=*/0).defined(),
+                                "libmmuon operators have no forward-mode derivative");
   if (!at::GradMode::is_enabled()) return false;
   return std::any_of(ts.begin(), ts.end(), [](const Tensor* t) { return t->requires_grad(); });
 }

@@ -4,7 +4,7 @@ import warnings
 import pytest
 import torch
 
-from monarch_muon_amd import embedding, linear_cross_entropy
+from monarch_muon_amd import butterfly_blk, embedding, linear_cross_entropy
 
 
 def meta(*shape, dtype=torch.bfloat16):
@@ -101,3 +101,33 @@ assert results == [0] * 16, results
     r = subprocess.run([sys.executable, "-c", program], cwd=Path(__file__).resolve().parent.parent, capture_output=True,
                        text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+# ----- forward mode ------------------------------------------------------------------
+@pytest.mark.parametrize("call", [
+    lambda t: linear_cross_entropy(t, meta(5, 16), meta(5, dtype=torch.long)),
+    lambda t: linear_cross_entropy(meta(5, 16), t, meta(5, dtype=torch.long), reduction="none"),
+    lambda t: embedding(meta(5, dtype=torch.long), t),
+    lambda t: torch.ops.mmuon.embedding_grad(t, meta(5, dtype=torch.long), 9, 1.0, -1),
+    lambda t: torch.ops.mmuon.linear_cross_entropy_grad(t, meta(5, 16), meta(5, dtype=torch.long), None, -100, 1, 5,
+                                                        True, True)[1],
+    lambda t: butterfly_blk(t, meta(2, 8, 8), meta(2, 8, 8)),
+], ids=["loss by x", "loss by weight", "embedding", "embedding_grad", "loss_grad", "layer"])
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode_is_refused(call, requires_grad):
+    """A tangent that goes in raises; it is not dropped (torch.func.jvp would take that for zero)."""
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(call, (meta(5, 16),), (meta(5, 16),))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(meta(5, 16).requires_grad_(requires_grad), meta(5, 16))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(dual)
+
+
+def test_transforms_are_refused():
+    """torch.func's reverse mode raises; its vmap calls the operator once for each."""
+    y = meta(6, dtype=torch.long)
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.grad(lambda x: linear_cross_entropy(x, meta(5, 16), y))(meta(6, 16))
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.grad(lambda w: embedding(y, w).float().sum())(meta(5, 16))
