@@ -2,6 +2,7 @@
 the sizes and layouts of test_gpu_lm.py."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from monarch_muon_amd import embedding, linear_cross_entropy
 
@@ -145,3 +146,34 @@ def test_head_upstream_factor(factor, reduction):
         got = torch.autograd.grad(linear_cross_entropy(x, w, y, reduction="none"), (x, w), up)
         within(got[0], dx, xt, "dx, rounded once")
         within(got[1], dw, wt, "dw, rounded once")
+
+
+# ----- under torch -------------------------------------------------------------------
+@pytest.mark.parametrize("how", ["compile", "compile_dynamic", "saved_hooks", "checkpoint", "expanded_grad"])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_operators_under_torch(reduction, how):
+    """Embedding and loss traced by torch.compile, with saved-tensor hooks, recomputed by checkpointing and with a
+    gradient that is no dense tensor: the bits of the plain call, with a factor that the backward multiplies in."""
+    g = torch.Generator().manual_seed(4)
+    t, w = ((torch.randn(300, 64, generator=g) / s).bfloat16().to(DEV).requires_grad_() for s in (1, 8))
+    i, y = (torch.randint(0, 300, (90,), generator=g).to(DEV) for _ in range(2))
+    i[5], y[7] = 1, -100
+
+    def step(i, t, w, y):
+        return linear_cross_entropy(embedding(i, t, scale=2.0, padding_idx=1), w, y, reduction=reduction) * 0.3
+    loss = step(i, t, w, y)
+    want = torch.autograd.grad(loss.sum(), (t, w))
+    again = step
+    if how.startswith("compile"):
+        torch._dynamo.reset()
+        again = torch.compile(step, backend="aot_eager", fullgraph=True, dynamic=how.endswith("dynamic"))
+    elif how == "checkpoint":
+        def again(*a):
+            return torch.utils.checkpoint.checkpoint(step, *a, use_reentrant=False)
+    with torch.autograd.graph.saved_tensors_hooks(*((lambda s: s.cpu(), lambda s: s.to(DEV)) if how == "saved_hooks" else
+                                                    (lambda s: s, lambda s: s))):
+        out = again(i, t, w, y)
+    got = torch.autograd.grad(out.sum() if how != "expanded_grad" else out, (t, w),
+                              None if how != "expanded_grad" else torch.ones((), device=DEV).expand(out.shape))
+    assert torch.equal(out, loss) and all(torch.equal(a, b) for a, b in zip(got, want))
+    torch._dynamo.reset()

@@ -131,3 +131,21 @@ def test_transforms_are_refused():
         torch.func.grad(lambda x: linear_cross_entropy(x, meta(5, 16), y))(meta(6, 16))
     with pytest.raises(RuntimeError, match="functorch"):
         torch.func.grad(lambda w: embedding(y, w).float().sum())(meta(5, 16))
+
+
+# ----- tracing -----------------------------------------------------------------------
+@pytest.mark.parametrize("dynamic", [False, True])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_traced_shapes(reduction, dynamic):
+    """torch.compile's tracing of both operators, forward and backward, on meta tensors."""
+    torch._dynamo.reset()
+    step = torch.compile(lambda i, t, w, y: linear_cross_entropy(embedding(i, t, scale=2.0, padding_idx=1), w, y,
+                                                                 reduction=reduction).sum() * 0.3,
+                         backend="aot_eager", fullgraph=True, dynamic=dynamic)
+    for T in (6, 7):
+        t, w = meta(9, 16).requires_grad_(), meta(5, 16).requires_grad_()
+        loss = step(meta(T, dtype=torch.long), t, w, meta(T, dtype=torch.long))
+        assert loss.shape == () and loss.dtype == torch.float32
+        dt, dw = torch.autograd.grad(loss, (t, w))
+        assert dt.shape == t.shape and dw.shape == w.shape
+    torch._dynamo.reset()
