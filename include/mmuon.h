@@ -447,7 +447,7 @@ int mmuon_scale_bf16(void* x, int64_t nx, void* y, int64_t ny, const float* fact
 typedef struct mmuon_embedding_args {
   int64_t tokens;         /* 0 <= tokens < 2^26 */
   int64_t vocab;          /* 1 <= vocab < 2^24 */
-  int32_t width;          /* any positive number */
+  int32_t width;          /* 1 <= width < 2^28, any number */
   int32_t dtype;          /* MMUON_BF16 or MMUON_F32: w, out, dout, dw */
   float scale;
   int32_t reserved;       /* 0 */

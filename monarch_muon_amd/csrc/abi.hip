@@ -664,6 +664,8 @@ int check_embedding(const mmuon_embedding_args* a, bool bwd) {
     return fail(MMUON_ERANGE, "embedding: tokens (%lld) must be below 2^26 and vocab (%lld) in [1, 2^24)",
                 (long long)a->tokens, (long long)a->vocab);
   if (a->width <= 0) return fail(MMUON_EINVAL, "embedding: width must be positive (got %d)", a->width);
+  if (a->width >= (1 << 28))  // a row's columns and those of its last chunk count in 32 bits
+    return fail(MMUON_ERANGE, "embedding: width must be below 2^28 (got %d)", a->width);
   if ((bwd ? a->dout_stride : a->w_stride) < 0) return fail(MMUON_EINVAL, "embedding: negative row stride");
   const uintptr_t mask = uintptr_t(dtype_size(a->dtype)) - 1;
   const auto bad = [&](const void* p, bool per_token) {

@@ -214,17 +214,18 @@ __global__ __launch_bounds__(64 * WAVES) void embed_rows(mmuon_embedding_args a,
 
 // Sums in fp32: a wave takes 64 N columns of a segment, eight loads in flight, and writes
 // the rows that end in it; a row's piece that goes on, or began before, is left in sums (the
-// first piece of segment i in 2 i, the last in 2 i + 1).  Bound by its reads at random rows: 16384
-// x 4096 in bf16 33 us (5.6 TB/s with the rows it writes), 57344 x 1024 28 us (4.2 of reads alone).
+// first piece of segment i in 2 i, the last in 2 i + 1).  Segments seg0 .. seg1 - 1.  Bound by its
+// reads at random rows: 16384 x 4096 in bf16 33 us (5.6 TB/s with the rows it writes), 57344 x 1024
+// 28 us (4.2 of reads alone).
 template <class T, int N>
-__global__ __launch_bounds__(256) void embed_sum(mmuon_embedding_args a, int each, GradSpace space) {
+__global__ __launch_bounds__(256) void embed_sum(mmuon_embedding_args a, int each, int seg0, int seg1, GradSpace space) {
   const int all = *space.all;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int chunks = (a.width + 64 * N - 1) / (64 * N);
   const int64_t item = int64_t(blockIdx.x) * 4 + wave;
-  const int seg = int(item / chunks), col = int(item - int64_t(seg) * chunks) * 64 * N + lane * N;
+  const int s0 = int(item / chunks), seg = seg0 + s0, col = int(item - int64_t(s0) * chunks) * 64 * N + lane * N;
   const int p0 = seg * each, n = min(each, all - p0);
-  if (n <= 0) return;
+  if (seg >= seg1 || n <= 0) return;
   // lanes 0 .. n - 1: the positions; lane n: the one after, lane 63: the one before (rows only)
   const int at = lane <= n ? p0 + lane : p0 - 1;
   const bool is = (lane <= n || lane == 63) && at >= 0 && at < all;
@@ -267,14 +268,14 @@ __global__ __launch_bounds__(256) void embed_sum(mmuon_embedding_args a, int eac
 }
 
 // The rows that lie in several segments: a workgroup sums 32 N columns of the row that goes on
-// from its segment, if it begins there; 8 runs of the row's pieces side by side, joined in order.
-// Bound by its latency: 3 to 8 us, where one word is not most of the tokens.
+// from its segment (seg0 on), if it begins there; 8 runs of the row's pieces side by side, joined
+// in order.  Bound by its latency: 3 to 8 us, where one word is not most of the tokens.
 template <class T, int N>
-__global__ __launch_bounds__(256) void embed_join(mmuon_embedding_args a, int size, GradSpace space) {
+__global__ __launch_bounds__(256) void embed_join(mmuon_embedding_args a, int size, int seg0, GradSpace space) {
   constexpr int LANES = 32, RUNS = 256 / LANES, SLICE = LANES * N;
   __shared__ float sums[RUNS][SLICE];
   const int all = *space.all, slices = (a.width + SLICE - 1) / SLICE;
-  const int seg = blockIdx.x / slices, slice = blockIdx.x % slices, p0 = seg * size;
+  const int seg = seg0 + blockIdx.x / slices, slice = blockIdx.x % slices, p0 = seg * size;
   if (p0 + size >= all) return;
   const int r = space.row[p0 + size];
   if (space.row[p0 + size - 1] != r) return;
@@ -319,17 +320,28 @@ bool whole_chunks(const void* base, int64_t stride, int64_t width) {
   return reinterpret_cast<uintptr_t>(base) % 16 == 0 && stride % CHUNK<T> == 0 && width % CHUNK<T> == 0;
 }
 
+// Workgroups of 256 threads in a launch, which holds fewer than 2^32 threads: more tokens or
+// segments take several
+constexpr int64_t MOST_BLOCKS = int64_t(1) << 23;
+
 template <class T, int N>
 void lookup_n(const mmuon_embedding_args& a, hipStream_t s) {
   const int chunks = a.width / N;
   int lanes = 16;  // about four chunks per thread
   while (lanes < 256 && lanes * 4 < chunks) lanes *= 2;
-  const dim3 grid(unsigned((a.tokens + 256 / lanes - 1) / (256 / lanes))), block(256);
+  const int each = 256 / lanes;
   // An output that the L2s (32 MiB) cannot hold is stored past them: 16384 x 4096 in bf16 40.0 ->
   // 34.0 us, 8192 x 4096 18.7 -> 17.6; a smaller one is read from there by what comes next.
-  if (a.tokens * a.width * int64_t(sizeof(typename T::storage)) > (int64_t(32) << 20))
-    hipLaunchKernelGGL((embed_lookup<T, N, true>), grid, block, 0, s, a, lanes);
-  else hipLaunchKernelGGL((embed_lookup<T, N, false>), grid, block, 0, s, a, lanes);
+  const bool past = a.tokens * a.width * int64_t(sizeof(typename T::storage)) > (int64_t(32) << 20);
+  for (int64_t t = 0; t < a.tokens; t += MOST_BLOCKS * each) {
+    mmuon_embedding_args p = a;
+    p.tokens = std::min(a.tokens - t, MOST_BLOCKS * each);
+    p.index = a.index + t;
+    p.out = static_cast<typename T::storage*>(a.out) + t * a.width;
+    const dim3 grid(unsigned((p.tokens + each - 1) / each)), block(256);
+    if (past) hipLaunchKernelGGL((embed_lookup<T, N, true>), grid, block, 0, s, p, lanes);
+    else hipLaunchKernelGGL((embed_lookup<T, N, false>), grid, block, 0, s, p, lanes);
+  }
 }
 template <class T>
 void lookup(const mmuon_embedding_args& a, hipStream_t s) {
@@ -388,11 +400,19 @@ void gradient_n(const mmuon_embedding_args& a, hipStream_t s) {
   else hipLaunchKernelGGL((embed_rows<T, N, 16, 1024, 512, false>), dim3(classes), dim3(1024), 0, s, a, l, past, space);
   if (a.tokens == 0) return;
   const int seg = segment(a.tokens, a.width, 64 * N);
-  const int64_t segs = (a.tokens + seg - 1) / seg, waves = segs * ((a.width + 64 * N - 1) / (64 * N));
-  hipLaunchKernelGGL((embed_sum<T, N>), dim3(unsigned((waves + 3) / 4)), dim3(256), 0, s, a, seg, space);
-  if (segs > 1)
-    hipLaunchKernelGGL((embed_join<T, N>), dim3(unsigned((segs - 1) * ((a.width + 32 * N - 1) / (32 * N)))), dim3(256),
-                       0, s, a, seg, space);
+  const int segs = int((a.tokens + seg - 1) / seg);
+  const int64_t chunks = (a.width + 64 * N - 1) / (64 * N), slices = (a.width + 32 * N - 1) / (32 * N);
+  const auto launches = [](int n, int64_t each, const auto& fn) {  // n segments of `each` workgroups
+    const int most = int(std::max<int64_t>(1, std::min<int64_t>(n, MOST_BLOCKS / each)));
+    for (int i = 0; i < n; i += most) fn(i, std::min(n, i + most));
+  };
+  launches(segs, (chunks + 3) / 4, [&](int s0, int s1) {
+    hipLaunchKernelGGL((embed_sum<T, N>), dim3(unsigned(((s1 - s0) * chunks + 3) / 4)), dim3(256), 0, s, a, seg, s0, s1,
+                       space);
+  });
+  launches(segs - 1, slices, [&](int s0, int s1) {
+    hipLaunchKernelGGL((embed_join<T, N>), dim3(unsigned((s1 - s0) * slices)), dim3(256), 0, s, a, seg, s0, space);
+  });
 }
 
 template <class T>

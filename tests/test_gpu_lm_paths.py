@@ -177,3 +177,27 @@ def test_operators_under_torch(reduction, how):
                               None if how != "expanded_grad" else torch.ones((), device=DEV).expand(out.shape))
     assert torch.equal(out, loss) and all(torch.equal(a, b) for a, b in zip(got, want))
     torch._dynamo.reset()
+
+
+# ----- more than one launch holds ------------------------------------------------------
+def test_lookup_of_more_threads_than_a_launch_holds():
+    """2^24 tokens and some of 1025 columns, 256 threads each: 2^32 and more threads."""
+    T, D = (1 << 24) + 5, 1025
+    g = torch.Generator(device=DEV).manual_seed(5)
+    w = torch.randn(1000, D, generator=g, device=DEV).bfloat16()
+    i = torch.randint(0, 1000, (T,), generator=g, device=DEV)
+    out = embedding(i, w)
+    for t in range(0, T, 1 << 21):
+        assert torch.equal(out[t:t + (1 << 21)], w[i[t:t + (1 << 21)]]), t
+
+
+def test_gradient_of_more_threads_than_a_launch_holds():
+    """2^26 - 1 tokens of 1025 columns, the most there may be: the sums and their join in several launches.  Small whole
+    numbers, so that every order of the sums is exact."""
+    T, D, V = (1 << 26) - 1, 1025, 1000
+    g = torch.Generator(device=DEV).manual_seed(6)
+    i = torch.randint(0, V, (T,), generator=g, device=DEV)
+    row = torch.randint(-2, 3, (D,), generator=g, device=DEV)
+    count = torch.bincount(i, minlength=V)
+    dw = torch.ops.mmuon.embedding_grad(row.bfloat16().expand(T, D), i, V, 1.0, -1)
+    assert torch.equal(dw, (count[:, None] * row).float().bfloat16())

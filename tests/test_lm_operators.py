@@ -149,3 +149,18 @@ def test_traced_shapes(reduction, dynamic):
         dt, dw = torch.autograd.grad(loss, (t, w))
         assert dt.shape == t.shape and dw.shape == w.shape
     torch._dynamo.reset()
+
+
+# ----- widths ------------------------------------------------------------------------
+def test_widths_that_the_kernels_cannot_count_are_refused():
+    """Columns count in 32 bits, with those of the chunk behind the last: refused before anything is launched."""
+    import ctypes as C
+    from monarch_muon_amd import _abi
+    emb = dict(tokens=4, vocab=100, width=1 << 28, dtype=_abi.F32, scale=1.0, padding_idx=-1, w_stride=1 << 28,
+               dout_stride=1 << 28, index=4096, w=8192, out=12288, dout=16384, dw=20480, workspace=32768,
+               workspace_bytes=1 << 62)
+    lib = _abi.lib()
+    for width in (1 << 28, (1 << 31) - 1):
+        args = C.byref(_abi.EmbeddingArgs(**{**emb, "width": width}))
+        assert lib.mmuon_embedding_fwd(args, None) == lib.mmuon_embedding_bwd(args, None) == -3
+        assert b"2^28" in lib.mmuon_last_error()
