@@ -85,10 +85,10 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         dt = torch.get_autocast_dtype("cuda")
         x, weight = x.to(dt), weight.to(dt)
     shape = target.shape
-    if x.shape[:-1] != shape:
+    if x.dim() == 0 or x.shape[:-1] != shape:
         raise ValueError(f"x {tuple(x.shape)} and target {tuple(shape)} do not match")
     if x.dim() != 2:
-        x, target = x.reshape(-1, x.shape[-1]), target.reshape(-1)
+        x, target = x.reshape(target.numel(), x.shape[-1]), target.reshape(-1)
     out = _loss_op(x, weight, target, ignore_index, _REDUCTIONS[reduction], piece_tokens or 0)
     return out.view(shape) if out.dim() else out
 
@@ -105,7 +105,7 @@ def embedding(index: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     if _embedding_op is None:
         _load()
     pad = -1
-    if padding_idx is not None:
+    if padding_idx is not None and weight.dim() == 2:   # (the operator refuses others)
         rows = weight.shape[0]
         if not -rows <= padding_idx < rows:
             raise ValueError(f"padding_idx {padding_idx} is not one of {rows} rows")

@@ -164,3 +164,16 @@ def test_widths_that_the_kernels_cannot_count_are_refused():
         args = C.byref(_abi.EmbeddingArgs(**{**emb, "width": width}))
         assert lib.mmuon_embedding_fwd(args, None) == lib.mmuon_embedding_bwd(args, None) == -3
         assert b"2^28" in lib.mmuon_last_error()
+
+
+# ----- refusals ----------------------------------------------------------------------
+@pytest.mark.parametrize("call, match", [
+    (lambda: linear_cross_entropy(torch.zeros((), dtype=torch.bfloat16), torch.zeros(5, 16).bfloat16(), torch.tensor(0)),
+     "do not match"),
+    (lambda: linear_cross_entropy(torch.zeros(2, 2, 0).bfloat16(), torch.zeros(5, 0).bfloat16(),
+                                  torch.zeros(2, 2, dtype=torch.long)), "multiple of 8"),
+    (lambda: embedding(torch.zeros(4, dtype=torch.long), torch.zeros(()), padding_idx=0), "expected weight"),
+], ids=["x of no dimension", "x of no columns", "weight of no dimension"])
+def test_shapes_without_columns_are_refused_as_such(call, match):
+    with pytest.raises(ValueError, match=match):
+        call()
