@@ -704,6 +704,7 @@ __global__ __launch_bounds__(256) void head_rows(RowArgs a) {
     a.resid[tok] = term - bf2f(at_target);
   }
   uint16_t* row = a.codes + int64_t(tok) * a.ldc;
+  const float none = lse2 * 0.f;  // a code of zero: p = 0, and no number where the token has no softmax
   for (int64_t c = threadIdx.x * 8; c < a.ldc; c += 256 * 8) {
     const uint4 in = PAST ? load16_nt(row + c) : *reinterpret_cast<const uint4*>(row + c);
     const uint32_t w[4] = {in.x, in.y, in.z, in.w};
@@ -713,8 +714,8 @@ __global__ __launch_bounds__(256) void head_rows(RowArgs a) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const uint32_t lo = w[k] & 0xffff, hi = w[k] >> 16;
-      const float p0 = lo == CODE_ZERO ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(float(lo), -CODE_STEP, top));
-      const float p1 = hi == CODE_ZERO ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(float(hi), -CODE_STEP, top));
+      const float p0 = lo == CODE_ZERO ? none : __builtin_amdgcn_exp2f(__builtin_fmaf(float(lo), -CODE_STEP, top));
+      const float p1 = hi == CODE_ZERO ? none : __builtin_amdgcn_exp2f(__builtin_fmaf(float(hi), -CODE_STEP, top));
       r[k] = f2bf2(g * p0, g * p1);
     }
     if (y >= c && y < c + 8) {

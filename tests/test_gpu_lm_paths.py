@@ -148,6 +148,30 @@ def test_head_upstream_factor(factor, reduction):
         within(got[1], dw, wt, "dw, rounded once")
 
 
+# ----- values beyond the numbers ---------------------------------------------------------
+@pytest.mark.parametrize("where", ["x inf", "x -inf", "x nan", "w inf", "all -inf"])
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_a_token_without_a_softmax_has_no_number_in_its_gradients(where, reduction):
+    """Infinities and NaN among the logits of a token that counts: loss and gradients are NaN where torch's are, in every
+    place, also where a logit is -inf or lies far below an infinite one."""
+    x, w, y = head(70, 64, 300, seed=8)
+    y[y == 9] = 10
+    if where == "all -inf":
+        w[:, 5] = -w[:, 5].abs() - 1
+        x[3, 5] = float("inf")
+    else:
+        (x if where[0] == "x" else w)[(3, 5) if where[0] == "x" else (9, 2)] = float(where[2:])
+    x64, w64 = (t.double().requires_grad_() for t in (x, w))
+    ref = torch.nn.functional.cross_entropy(x64 @ w64.T, y, reduction=reduction)
+    want = torch.autograd.grad(ref.sum(), (x64, w64))
+    x, w = (t.to(DEV).requires_grad_() for t in (x, w))
+    out = linear_cross_entropy(x, w, y.to(DEV), reduction=reduction)
+    got = torch.autograd.grad(out.sum(), (x, w))
+    alone = linear_cross_entropy(x.detach(), w.detach(), y.to(DEV), reduction=reduction)
+    for name, a, b in (("loss", out, ref), ("alone", alone, ref), ("dx", got[0], want[0]), ("dw", got[1], want[1])):
+        assert torch.equal(a.isnan().cpu(), b.isnan()), (name, int(a.isnan().sum()), int(b.isnan().sum()))
+
+
 # ----- under torch -------------------------------------------------------------------
 @pytest.mark.parametrize("how", ["compile", "compile_dynamic", "saved_hooks", "checkpoint", "expanded_grad"])
 @pytest.mark.parametrize("reduction", ["mean", "none"])
