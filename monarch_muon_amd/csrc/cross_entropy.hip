@@ -27,6 +27,8 @@
 // 76 and 79% busy at 1.7 to 1.8 GHz, and the package-power limit holds the clock 80% of the
 // time.  One token: the read of the head, 412 MB in 89 us.  Narrow models (16384 tokens x 1024):
 // 10 B of memory traffic per logit (code out, in, dl out, in twice) beside 6144 operations.
+#include <float.h>
+
 #include <algorithm>
 
 #include "common.hpp"
@@ -387,7 +389,8 @@ __device__ __forceinline__ void loss_epilogue(const HeadGemm& a, int N, int m0, 
 #pragma unroll
       for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
     m = fmaxf(m, __shfl_xor(m, 32, 64));
-    const float m2 = m == -INFINITY ? 0.f : m * LOG2E;  // a part that is all -inf: sum 0
+    // (bounded below: a part that is all -inf, or nearly, has sum 0)
+    const float m2 = fmaxf(m * LOG2E, -FLT_MAX);
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < GE::WI; ++i) {
@@ -418,6 +421,7 @@ __device__ __forceinline__ void loss_epilogue(const HeadGemm& a, int N, int m0, 
       }
     }
     s += __shfl_xor(s, 32, 64);
+    if (m2 == INFINITY) s = NAN;  // beyond what 32 bits hold in base 2 (every distance would be infinite, the sum 0)
     if (live && half == 0 && left > 0) a.parts[int64_t(tok) * a.nparts + v0 / PW] = make_float2(m2, s);
   }
 }

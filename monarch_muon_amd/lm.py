@@ -69,11 +69,15 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
 
     Differentiable in ``x`` and ``weight``.  With "mean" and "sum" the forward makes the gradients, so one backward
     can be taken of it, and a factor that arrives then (``loss / 3``) is multiplied into their bfloat16 values: a second
-    rounding, none for a power of two, and a pass over both where it is not 1.  With "none" the backward makes the logits again.  There is no second derivative: one of
-    gradients taken with ``create_graph`` raises.  ``piece_tokens``: tokens whose logits are
-    held at a time, 16 bits each; by default as many as fit 1 GiB.  Several pieces also hold float32 sums of
-    ``weight``'s gradient, where it is wanted, so a smaller piece can take more memory than one of all tokens (which
-    the default then is).
+    rounding, none for a power of two, and a pass over both where it is not 1.  With "none" the backward makes the
+    logits again.  There is no second derivative: one of gradients taken with ``create_graph`` raises.
+
+    A token with a logit of +inf or NaN, or with none above -inf, has NaN for its loss and gradients; so has one with
+    a logit beyond 2.3e38, which float32 does not hold in base 2.
+
+    ``piece_tokens``: tokens whose logits are held at a time, 16 bits each; by default as many as fit 1 GiB.  Several
+    pieces also hold float32 sums of ``weight``'s gradient, where it is wanted, so a smaller piece can take more memory
+    than one of all tokens (which the default then is).
     """
     if _loss_op is None:
         _load()

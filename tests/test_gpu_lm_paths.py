@@ -172,6 +172,40 @@ def test_a_token_without_a_softmax_has_no_number_in_its_gradients(where, reducti
         assert torch.equal(a.isnan().cpu(), b.isnan()), (name, int(a.isnan().sum()), int(b.isnan().sum()))
 
 
+@pytest.mark.parametrize("T", [3, 70, 300])
+def test_logits_whose_powers_overflow_show(T):
+    """A logit of 2.99e38 is a float32, 1 / ln 2 of it is not: the token's loss and gradients are NaN, not those of a
+    softmax without that word."""
+    x, w, y = head(T, 64, 300, seed=9)
+    w[:, 0], w[200, 0], x[:, 0], x[1, 0] = 0, 2.0 ** 63, 0, 1.7578125 * 2.0 ** 64
+    y[1] = 5
+    x, w, y = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_(), y.to(DEV)
+    row = torch.arange(T, device=DEV) == 1
+    assert torch.equal(linear_cross_entropy(x.detach(), w.detach(), y, reduction="none").isnan(), row)
+    out = linear_cross_entropy(x, w, y, reduction="none")
+    dx, dw = torch.autograd.grad(out.sum(), (x, w))
+    assert torch.equal(out.isnan(), row) and torch.equal(dx.isnan().any(1), row) and dw.isnan().all()
+
+
+def test_words_whose_powers_underflow_have_none():
+    """A part of the vocabulary whose logits are all -2.99e38 counts for nothing, as one whose logits are -inf does."""
+    for low in (2.0 ** 63, float("inf")):
+        x, w, y = head(70, 64, 300, seed=10)
+        x[:, 0], w[:, 0] = 0, 0
+        x[1, 0], w[256:, 0], y[1] = -1.7578125 * 2.0 ** 64, low, 5
+        if low == float("inf"):
+            x[:, 0] = -1        # (0 * inf is no number)
+            y[y >= 256] = 6
+        loss, dx, dw, (lt, xt, wt) = oracle.cross_entropy(x[1:2], w[:256], y[1:2], reduction="none")
+        x, w, y = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_(), y.to(DEV)
+        alone = linear_cross_entropy(x.detach(), w.detach(), y, reduction="none")
+        out = linear_cross_entropy(x, w, y, reduction="none")
+        got, = torch.autograd.grad(out, x, (torch.arange(70, device=DEV) == 1).float())
+        within(alone[1], loss[0], lt[0], "alone")
+        within(out[1], loss[0], lt[0], "loss")
+        within(got[1, 1:], dx[0, 1:], xt[0, 1:], "dx")
+
+
 # ----- under torch -------------------------------------------------------------------
 @pytest.mark.parametrize("how", ["compile", "compile_dynamic", "saved_hooks", "checkpoint", "expanded_grad"])
 @pytest.mark.parametrize("reduction", ["mean", "none"])
