@@ -34,9 +34,11 @@ struct HeadPlan {
 
 // Time in ns of a product M x N x K on a 256-CU part (a function of the sizes only, so the order
 // of the sums does not depend on the device): rounds of 256 tiles, each its slices of K at the
-// rate of full rounds and what its start and end cost.  Measured at V = 50304: loss of 4096 x
-// 4096 1.40 ms in 256-wide tiles, 1.83 in 128-wide; 1000 x 1024 123 / 145 us, 300 x 4096 196 /
-// 213, 600 x 512 59.5 / 60.6, 128 x 2048 50 / 49, 33 x 2048 47 / 41.
+// rate of full rounds and what its start and end cost.  Logits with codes for the gradients end
+// later than that (1000 x 512 90 us, 61 by this): what that costs is not in here.  Measured
+// at V = 50304, the loss alone: 4096 x 4096 1.40 ms in 256-wide tiles, 1.83 in 128-wide; 1000 x
+// 1024 123 / 145 us, 300 x 4096 196 / 213, 600 x 512 59.5 / 60.6, 128 x 2048 50 / 49, 33 x 2048
+// 47 / 41.
 inline int64_t round_time(bool narrow, int64_t K) { return narrow ? 1500 + 18 * K : 2500 + 25 * K; }
 inline int64_t plan_time(const HeadPlan& p, int64_t M, int64_t N, int64_t K) {
   const int64_t tiles = p.tiles(M, N), full = std::min<int64_t>(p.full, tiles), parts = (tiles - full) * p.S;
