@@ -82,7 +82,7 @@ def head_dx(x, w, target, ignore_index=-100, reduction="mean", grad=None):
     xk, yk = x64[keep], target[keep]
     n, rows = len(yk), torch.arange(len(yk), device=dev)
     p = torch.softmax(xk @ w64.T, 1)
-    g = grad.double().to(dev)[keep] if grad is not None else torch.full((n,), 1.0 / n if reduction == "mean" else 1.0,
+    g = grad.double().to(dev)[keep] if grad is not None else torch.full((n,), 1.0 / max(n, 1) if reduction == "mean" else 1.0,
                                                                         dtype=torch.float64, device=dev)
     at_target = (g * (1 - p[rows, yk])).abs()
     bound[keep] -= (at_target * (UCODE + UBF))[:, None] * w64[yk].abs()
