@@ -466,11 +466,79 @@ int mmuon_embedding_fwd(const mmuon_embedding_args* a, void* stream);
 int mmuon_embedding_bwd(const mmuon_embedding_args* a, void* stream);
 size_t mmuon_embedding_workspace(const mmuon_embedding_args* a);
 
+/* What stands between a decoder layer's Monarch projections: the norm with the residual's
+   addition, rotary positions, and differential attention.  The reference takes torch's
+   (pretrain/src/models/llama.py: RMSNorm, apply_rotary_emb, scaled_dot_product_attention). */
+
+/* Root-mean-square norm of rows:
+     h = residual given ? x + residual rounded to dtype : x;
+     y = h * inv * w,  inv = 1 / sqrt(mean of h^2 + eps), fp32, one rounding.
+   With an 8-bit out_dtype, y is codes and scale: for each 128 columns (group 128) or the row
+   (group 0) scale = max |y| / (448 or 57344), 1 where that is 0, and code = y / scale to the
+   nearest even.
+   Backward, from x (the forward's h), inv and dy:
+     dx = inv w dy - h inv^3 mean(w dy h) + dh (of x and of residual alike; dh null: none);
+     dw = sum over rows of dy h inv, fp32 in an order of the sizes alone, one rounding. */
+typedef struct mmuon_norm_args {
+  int64_t rows;           /* 0 <= rows < 2^31 */
+  int32_t width;          /* 1 <= width <= 32768 (bf16), 16384 (fp32), any number */
+  int32_t dtype;          /* MMUON_BF16 or MMUON_F32: x, residual, h, dy, dh, dx */
+  int32_t w_dtype;        /* w, dw: dtype or MMUON_F32 */
+  int32_t out_dtype;      /* y: dtype, MMUON_F8E4M3 or MMUON_F8E5M2 */
+  int32_t group;          /* 128 or 0, with an 8-bit out_dtype */
+  float eps;
+  int64_t x_stride;       /* elements from one row to the next */
+  int64_t residual_stride;
+  int64_t dy_stride;
+  int64_t dh_stride;
+  const void* x;
+  const void* residual;   /* or null */
+  const void* w;          /* (width) */
+  void* h;                /* out (rows, width), contiguous; with residual only, else null */
+  void* y;                /* out (rows, width), contiguous */
+  float* scale;           /* out (rows, ceil(width / 128)) or (rows, 1), with an 8-bit out_dtype */
+  float* inv;             /* forward out (or null), backward in: (rows) */
+  const void* dy;
+  const void* dh;         /* or null */
+  void* dx;               /* out (rows, width), contiguous */
+  void* dw;               /* out (width), or null */
+  void* workspace;        /* backward: mmuon_norm_workspace() bytes, 256-B aligned */
+  size_t workspace_bytes;
+} mmuon_norm_args;
+int mmuon_norm_fwd(const mmuon_norm_args* a, void* stream);
+int mmuon_norm_bwd(const mmuon_norm_args* a, void* stream);
+size_t mmuon_norm_workspace(const mmuon_norm_args* a);
+
+/* Rotary positions of queries (batch, tokens, q_heads, dim) and keys (..., k_heads, dim): the pairs
+   (i, i + part / 2), or interleaved (2 i, 2 i + 1), of each head's first `part` columns are turned
+     (a, b) -> (a c - b s, a s + b c),  c = table[p][i], s = table[p][part / 2 + i],
+   in fp32 with one rounding; the other columns are copied.  p = positions[b][t], or t; a position
+   outside the table gives NaN.  back: by -s, which is the gradient. */
+typedef struct mmuon_rotary_args {
+  int64_t batch;          /* batch * tokens * (q_heads + k_heads) * dim < 2^40, of one sequence < 2^31 */
+  int64_t tokens;
+  int32_t q_heads, k_heads;
+  int32_t dim;            /* 1 <= dim <= 65536 */
+  int32_t part;           /* even, 2 <= part <= dim */
+  int32_t dtype;          /* MMUON_BF16 or MMUON_F32 */
+  int32_t interleaved;
+  int64_t table_rows;
+  int64_t q_stride[3];    /* elements from one sequence, token, head to the next */
+  int64_t k_stride[3];
+  const void* q;
+  const void* k;
+  const float* table;     /* (table_rows, part), contiguous */
+  const int64_t* positions;  /* (batch, tokens), or null */
+  void* q_out;            /* contiguous */
+  void* k_out;
+} mmuon_rotary_args;
+int mmuon_rotary(const mmuon_rotary_args* a, int32_t back, void* stream);
+
 /* Thread-local message of the last failing call ("" if none). */
 const char* mmuon_last_error(void);
 
 /* ABI version: bumped on any change to this header. */
-#define MMUON_ABI_VERSION 10
+#define MMUON_ABI_VERSION 11
 int mmuon_abi_version(void);
 
 #ifdef __cplusplus

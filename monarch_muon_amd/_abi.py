@@ -12,7 +12,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(os.environ.get("MMUON_LIB", Path(__file__).resolve().parent / "libmmuon.so"))
-ABI_VERSION = 10
+ABI_VERSION = 11
 # the layer's torch operator; the name carries the ABI, so that one built for another is never loaded (once loaded,
 # its registrations stay for the life of the process)
 TORCH_LIB_PATH = Path(__file__).resolve().parent / f"libmmuon_torch.{ABI_VERSION}.so"
@@ -125,6 +125,24 @@ class EmbeddingArgs(C.Structure):
                 ("workspace_bytes", C.c_size_t)]
 
 
+class NormArgs(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("width", C.c_int32), ("dtype", C.c_int32), ("w_dtype", C.c_int32),
+                ("out_dtype", C.c_int32), ("group", C.c_int32), ("eps", C.c_float), ("x_stride", C.c_int64),
+                ("residual_stride", C.c_int64), ("dy_stride", C.c_int64), ("dh_stride", C.c_int64),
+                ("x", C.c_void_p), ("residual", C.c_void_p), ("w", C.c_void_p), ("h", C.c_void_p),
+                ("y", C.c_void_p), ("scale", C.c_void_p), ("inv", C.c_void_p), ("dy", C.c_void_p),
+                ("dh", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [("batch", C.c_int64), ("tokens", C.c_int64), ("q_heads", C.c_int32), ("k_heads", C.c_int32),
+                ("dim", C.c_int32), ("part", C.c_int32), ("dtype", C.c_int32), ("interleaved", C.c_int32),
+                ("table_rows", C.c_int64), ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3),
+                ("q", C.c_void_p), ("k", C.c_void_p), ("table", C.c_void_p), ("positions", C.c_void_p),
+                ("q_out", C.c_void_p), ("k_out", C.c_void_p)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "mmuon_abi_version": (C.c_int, []),
@@ -161,6 +179,10 @@ SIGNATURES = {
     "mmuon_embedding_fwd": (C.c_int, [C.POINTER(EmbeddingArgs), C.c_void_p]),
     "mmuon_embedding_bwd": (C.c_int, [C.POINTER(EmbeddingArgs), C.c_void_p]),
     "mmuon_embedding_workspace": (C.c_size_t, [C.POINTER(EmbeddingArgs)]),
+    "mmuon_norm_fwd": (C.c_int, [C.POINTER(NormArgs), C.c_void_p]),
+    "mmuon_norm_bwd": (C.c_int, [C.POINTER(NormArgs), C.c_void_p]),
+    "mmuon_norm_workspace": (C.c_size_t, [C.POINTER(NormArgs)]),
+    "mmuon_rotary": (C.c_int, [C.POINTER(RotaryArgs), C.c_int32, C.c_void_p]),
     "mmuon_scale_bf16": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
 }
 

@@ -134,6 +134,7 @@ _BOUND = ("mmuon_butterfly_linear_fwd", "mmuon_butterfly_linear_bwd", "mmuon_but
           "mmuon_last_error")
 _BOUND_LM = ("mmuon_ce_fwd", "mmuon_ce_fwd_bwd", "mmuon_ce_workspace", "mmuon_scale_bf16", "mmuon_embedding_fwd",
              "mmuon_embedding_bwd", "mmuon_embedding_workspace")
+_BOUND_LAYER = ("mmuon_norm_fwd", "mmuon_norm_bwd", "mmuon_norm_workspace", "mmuon_rotary")
 _linear_op = _torch_lib = None
 
 
@@ -143,8 +144,10 @@ def _bind() -> int:
     try:
         lib = _abi.lib()
         version = lib.mmuon_abi_version()
-        lm, blk = ([C.cast(getattr(lib, name), C.c_void_p) for name in names] for names in (_BOUND_LM, _BOUND))
-        return _torch_lib.mmuon_torch_bind_lm(version, *lm) or _torch_lib.mmuon_torch_bind(version, *blk)
+        lm, layer, blk = ([C.cast(getattr(lib, name), C.c_void_p) for name in names]
+                          for names in (_BOUND_LM, _BOUND_LAYER, _BOUND))
+        return (_torch_lib.mmuon_torch_bind_lm(version, *lm) or _torch_lib.mmuon_torch_bind_layer(version, *layer) or
+                _torch_lib.mmuon_torch_bind(version, *blk))
     except Exception as e:
         _torch_lib.mmuon_torch_refuse(str(e).encode())
         return -1

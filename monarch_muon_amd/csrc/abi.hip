@@ -737,3 +737,104 @@ int mmuon_embedding_bwd(const mmuon_embedding_args* a, void* stream) {
 }
 
 }  // extern "C"
+
+namespace {
+
+// An element's address
+bool misplaced(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t(dtype_size(dtype)) - 1)) != 0; }
+
+bool norm_sizes(const mmuon_norm_args* a) {
+  return a != nullptr && (a->dtype == MMUON_BF16 || a->dtype == MMUON_F32) && a->rows >= 0 &&
+         a->rows < (int64_t(1) << 31) && a->width > 0 && a->width <= (a->dtype == MMUON_BF16 ? 32768 : 16384);
+}
+
+int check_norm(const mmuon_norm_args* a, bool bwd) {
+  if (a == nullptr) return fail(MMUON_EINVAL, "null norm arguments");
+  if (a->dtype != MMUON_BF16 && a->dtype != MMUON_F32)
+    return fail(MMUON_EINVAL, "norm: dtype must be MMUON_BF16 or MMUON_F32 (got %d)", a->dtype);
+  if (a->w_dtype != a->dtype && a->w_dtype != MMUON_F32)
+    return fail(MMUON_EINVAL, "norm: w_dtype must be that of the rows or MMUON_F32 (got %d)", a->w_dtype);
+  if (!norm_sizes(a))
+    return fail(MMUON_ERANGE, "norm: rows (%lld) must be in [0, 2^31) and width (%d) in [1, %d]", (long long)a->rows,
+                a->width, a->dtype == MMUON_BF16 ? 32768 : 16384);
+  if (!(a->eps >= 0.f)) return fail(MMUON_EINVAL, "norm: eps must not be negative (got %g)", a->eps);
+  const bool some = a->rows > 0;
+  const auto bad = [&](const void* p, bool needed) { return (needed && some && p == nullptr) || misplaced(p, a->dtype); };
+  if (a->w == nullptr || misplaced(a->w, a->w_dtype)) return fail(MMUON_EINVAL, "norm: null or unaligned w");
+  if (bad(a->x, true)) return fail(MMUON_EINVAL, "norm: null or unaligned x");
+  if (a->x_stride < 0 || a->residual_stride < 0 || a->dy_stride < 0 || a->dh_stride < 0)
+    return fail(MMUON_EINVAL, "norm: negative row stride");
+  if (misplaced(a->inv, MMUON_F32)) return fail(MMUON_EINVAL, "norm: unaligned inv");
+  if (bwd) {
+    if (bad(a->dy, true) || bad(a->dh, false) || bad(a->dx, true)) return fail(MMUON_EINVAL, "norm: null or unaligned dy, dh or dx");
+    if (a->inv == nullptr && some) return fail(MMUON_EINVAL, "norm: the backward needs the forward's inv");
+    if (misplaced(a->dw, a->w_dtype)) return fail(MMUON_EINVAL, "norm: unaligned dw");
+    if (a->dw == nullptr) return MMUON_OK;
+    const size_t need = mmuon::norm_workspace(*a);
+    if (need > 0 && (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 255) != 0))
+      return fail(MMUON_EINVAL, "norm: workspace must be 256-B aligned");
+    if (a->workspace_bytes < need)
+      return fail(MMUON_EINVAL, "norm: workspace of %zu bytes, %zu needed", a->workspace_bytes, need);
+    return MMUON_OK;
+  }
+  if (bad(a->residual, false) || bad(a->h, false)) return fail(MMUON_EINVAL, "norm: unaligned residual or h");
+  if (is_fp8(a->out_dtype)) {
+    if (a->group != 0 && a->group != 128) return fail(MMUON_EINVAL, "norm: group must be 128, or 0 for the row (got %d)", a->group);
+    if ((some && (a->y == nullptr || a->scale == nullptr)) || misplaced(a->scale, MMUON_F32))
+      return fail(MMUON_EINVAL, "norm: null y or scale, or unaligned scale");
+    return MMUON_OK;
+  }
+  if (a->out_dtype != a->dtype)
+    return fail(MMUON_EINVAL, "norm: out_dtype must be that of the rows or an 8-bit type (got %d)", a->out_dtype);
+  if (bad(a->y, true)) return fail(MMUON_EINVAL, "norm: null or unaligned y");
+  return MMUON_OK;
+}
+
+int check_rotary(const mmuon_rotary_args* a) {
+  if (a == nullptr) return fail(MMUON_EINVAL, "null rotary arguments");
+  if (a->dtype != MMUON_BF16 && a->dtype != MMUON_F32)
+    return fail(MMUON_EINVAL, "rotary: dtype must be MMUON_BF16 or MMUON_F32 (got %d)", a->dtype);
+  if (a->dim < 1 || a->dim > 65536 || a->part < 2 || a->part > a->dim || a->part % 2)
+    return fail(MMUON_EINVAL, "rotary: dim (%d) must be in [1, 65536], part (%d) even and in [2, dim]", a->dim, a->part);
+  if (a->batch < 0 || a->tokens < 0 || a->q_heads < 0 || a->k_heads < 0 || a->table_rows < 0)
+    return fail(MMUON_EINVAL, "rotary: negative size");
+  const double one = double(a->tokens) * (double(a->q_heads) + a->k_heads) * a->dim;
+  if (one >= 2147483648.0 || one * double(a->batch) >= 1099511627776.0 || a->batch >= (int64_t(1) << 31))
+    return fail(MMUON_ERANGE, "rotary: 2^31 elements of a sequence or 2^40 of all are too many");
+  if (a->batch == 0 || a->tokens == 0) return MMUON_OK;
+  if (a->table_rows == 0) return fail(MMUON_EINVAL, "rotary: a table of no positions");
+  for (int i = 0; i < 3; ++i)
+    if (a->q_stride[i] < 0 || a->k_stride[i] < 0) return fail(MMUON_EINVAL, "rotary: negative stride");
+  const auto bad = [&](const void* p, int heads) { return heads > 0 && (p == nullptr || misplaced(p, a->dtype)); };
+  if (bad(a->q, a->q_heads) || bad(a->q_out, a->q_heads) || bad(a->k, a->k_heads) || bad(a->k_out, a->k_heads))
+    return fail(MMUON_EINVAL, "rotary: null or unaligned queries or keys");
+  if (a->table == nullptr || misplaced(a->table, MMUON_F32) || (reinterpret_cast<uintptr_t>(a->positions) & 7) != 0)
+    return fail(MMUON_EINVAL, "rotary: null or unaligned table, or unaligned positions");
+  return MMUON_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mmuon_norm_workspace(const mmuon_norm_args* a) { return norm_sizes(a) ? mmuon::norm_workspace(*a) : 0; }
+
+int mmuon_norm_fwd(const mmuon_norm_args* a, void* stream) {
+  if (int rc = check_norm(a, false)) return rc;
+  mmuon::launch_norm_fwd(*a, static_cast<hipStream_t>(stream));
+  return check_launch("norm forward");
+}
+
+int mmuon_norm_bwd(const mmuon_norm_args* a, void* stream) {
+  if (int rc = check_norm(a, true)) return rc;
+  mmuon::launch_norm_bwd(*a, static_cast<hipStream_t>(stream));
+  return check_launch("norm backward");
+}
+
+int mmuon_rotary(const mmuon_rotary_args* a, int32_t back, void* stream) {
+  if (int rc = check_rotary(a)) return rc;
+  mmuon::launch_rotary(*a, back != 0, static_cast<hipStream_t>(stream));
+  return check_launch("rotary");
+}
+
+}  // extern "C"

@@ -101,6 +101,12 @@ size_t embedding_workspace(const mmuon_embedding_args& a);
 int launch_embedding_fwd(const mmuon_embedding_args& a, hipStream_t s);
 int launch_embedding_bwd(const mmuon_embedding_args& a, hipStream_t s);
 
+// Norm, rotary positions -------------------------------------------------------------
+size_t norm_workspace(const mmuon_norm_args& a);
+int launch_norm_fwd(const mmuon_norm_args& a, hipStream_t s);
+int launch_norm_bwd(const mmuon_norm_args& a, hipStream_t s);
+int launch_rotary(const mmuon_rotary_args& a, bool back, hipStream_t s);
+
 // Gradient-clipping coefficient of a launch (gscale: device pointer, or null
 // when not clipping), read once per thread: the per-element form would test
 // the pointer in every element (a branch each) and, after the thread's first

@@ -29,6 +29,10 @@ struct Abi {
   int (*emb_fwd)(const mmuon_embedding_args*, void*) = nullptr;
   int (*emb_bwd)(const mmuon_embedding_args*, void*) = nullptr;
   size_t (*emb_workspace)(const mmuon_embedding_args*) = nullptr;
+  int (*norm_fwd)(const mmuon_norm_args*, void*) = nullptr;
+  int (*norm_bwd)(const mmuon_norm_args*, void*) = nullptr;
+  size_t (*norm_workspace)(const mmuon_norm_args*) = nullptr;
+  int (*rotary)(const mmuon_rotary_args*, int32_t, void*) = nullptr;
   const char* (*last_error)() = nullptr;
 };
 extern Abi abi;

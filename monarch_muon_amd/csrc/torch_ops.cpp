@@ -221,6 +221,18 @@ int mmuon_torch_bind_lm(int version, void* ce_fwd, void* ce_fwd_bwd, void* ce_wo
   return 0;
 }
 
+// The functions of the operators between a layer's projections (torch_layer.cpp), likewise.
+int mmuon_torch_bind_layer(int version, void* norm_fwd, void* norm_bwd, void* norm_workspace, void* rotary) {
+  if (version != MMUON_ABI_VERSION) return 0;
+  const std::lock_guard<std::mutex> lock(binding);
+  if (bound) return 0;
+  abi.norm_fwd = reinterpret_cast<decltype(abi.norm_fwd)>(norm_fwd);
+  abi.norm_bwd = reinterpret_cast<decltype(abi.norm_bwd)>(norm_bwd);
+  abi.norm_workspace = reinterpret_cast<decltype(abi.norm_workspace)>(norm_workspace);
+  abi.rotary = reinterpret_cast<decltype(abi.rotary)>(rotary);
+  return 0;
+}
+
 void mmuon_torch_set_loader(int (*fn)()) { loader = fn; }
 
 void mmuon_torch_refuse(const char* why) { refusal = why; }
