@@ -534,11 +534,55 @@ typedef struct mmuon_rotary_args {
 } mmuon_rotary_args;
 int mmuon_rotary(const mmuon_rotary_args* a, int32_t back, void* stream);
 
+/* Differential attention.  For each head, maps m = 1, 2 of query and key heads 2 h + m - 1 and
+   2 g + m - 1 (g = h / (heads / kv_heads)), over the keys j that query t of sequence b sees:
+     P_m = softmax over j of scale q_m . k_m[j],  o_m = sum_j P_m[j] v[j],  o = o_1 - lam[h] o_2;
+   0 where a query sees no key.  Key j is seen where j < lengths[b] (all keys without it; a length
+   counts as 0 .. keys) and, if causal, j <= starts[b] + t (lengths[b] - queries + t without it:
+   the queries are the last ones).  Products in bf16, summed in fp32; P rounded to bf16
+   and divided by the sum of the rounded values.
+   With o1, o2 and lse given the forward also leaves what the backward needs.
+   Backward (mmuon_attention_bwd), from the same inputs, o1, o2, lse and dout: dq, dk, dv (zeros
+   where nothing reaches) and dlam, sums in fp32 in an order of the sizes alone. */
+typedef struct mmuon_attention_args {
+  int32_t batch;          /* batch * heads * queries and batch * kv_heads * keys < 2^31 */
+  int32_t queries, keys;
+  int32_t heads, kv_heads;  /* heads a multiple of kv_heads */
+  int32_t dim;            /* of a map's queries and keys, a multiple of 8, at most 128; v has twice as many */
+  int32_t dtype;          /* MMUON_BF16 */
+  int32_t causal;
+  float scale;            /* positive */
+  int32_t lam_stride;     /* 1, or 0: one for all heads */
+  int64_t q_stride[3];    /* elements from one sequence, token, head to the next: multiples of 8; token strides < 2^22 */
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  const void* q;          /* (batch, queries, 2 heads, dim), rows 16-B aligned */
+  const void* k;          /* (batch, keys, 2 kv_heads, dim) */
+  const void* v;          /* (batch, keys, kv_heads, 2 dim) */
+  const float* lam;
+  const int64_t* lengths; /* (batch), or null */
+  const int64_t* starts;  /* (batch), or null */
+  void* o;                /* out (batch, queries, heads, 2 dim), contiguous */
+  float* o1;              /* out, or null: of o's shape, contiguous; backward in */
+  float* o2;
+  float* lse;             /* out, or null: (batch, heads, queries, 2); backward in */
+  const void* dout;       /* backward in: of o's shape, contiguous */
+  void* dq;               /* backward out, contiguous; dq and dlam, or dk and dv, may both be null */
+  void* dk;
+  void* dv;
+  float* dlam;            /* backward out: (heads) */
+  void* workspace;        /* mmuon_attention_workspace() bytes, 256-B aligned */
+  size_t workspace_bytes;
+} mmuon_attention_args;
+int mmuon_attention_fwd(const mmuon_attention_args* a, void* stream);
+int mmuon_attention_bwd(const mmuon_attention_args* a, void* stream);
+size_t mmuon_attention_workspace(const mmuon_attention_args* a, int32_t backward);
+
 /* Thread-local message of the last failing call ("" if none). */
 const char* mmuon_last_error(void);
 
 /* ABI version: bumped on any change to this header. */
-#define MMUON_ABI_VERSION 11
+#define MMUON_ABI_VERSION 12
 int mmuon_abi_version(void);
 
 #ifdef __cplusplus

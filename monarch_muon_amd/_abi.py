@@ -12,7 +12,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(os.environ.get("MMUON_LIB", Path(__file__).resolve().parent / "libmmuon.so"))
-ABI_VERSION = 11
+ABI_VERSION = 12
 # the layer's torch operator; the name carries the ABI, so that one built for another is never loaded (once loaded,
 # its registrations stay for the life of the process)
 TORCH_LIB_PATH = Path(__file__).resolve().parent / f"libmmuon_torch.{ABI_VERSION}.so"
@@ -143,6 +143,17 @@ class RotaryArgs(C.Structure):
                 ("q_out", C.c_void_p), ("k_out", C.c_void_p)]
 
 
+class AttentionArgs(C.Structure):
+    _fields_ = [("batch", C.c_int32), ("queries", C.c_int32), ("keys", C.c_int32), ("heads", C.c_int32),
+                ("kv_heads", C.c_int32), ("dim", C.c_int32), ("dtype", C.c_int32), ("causal", C.c_int32),
+                ("scale", C.c_float), ("lam_stride", C.c_int32), ("q_stride", C.c_int64 * 3),
+                ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("q", C.c_void_p), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("lam", C.c_void_p), ("lengths", C.c_void_p), ("starts", C.c_void_p),
+                ("o", C.c_void_p), ("o1", C.c_void_p), ("o2", C.c_void_p), ("lse", C.c_void_p),
+                ("dout", C.c_void_p), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
+                ("dlam", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "mmuon_abi_version": (C.c_int, []),
@@ -183,6 +194,9 @@ SIGNATURES = {
     "mmuon_norm_bwd": (C.c_int, [C.POINTER(NormArgs), C.c_void_p]),
     "mmuon_norm_workspace": (C.c_size_t, [C.POINTER(NormArgs)]),
     "mmuon_rotary": (C.c_int, [C.POINTER(RotaryArgs), C.c_int32, C.c_void_p]),
+    "mmuon_attention_fwd": (C.c_int, [C.POINTER(AttentionArgs), C.c_void_p]),
+    "mmuon_attention_bwd": (C.c_int, [C.POINTER(AttentionArgs), C.c_void_p]),
+    "mmuon_attention_workspace": (C.c_size_t, [C.POINTER(AttentionArgs), C.c_int32]),
     "mmuon_scale_bf16": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
 }
 

@@ -134,7 +134,8 @@ _BOUND = ("mmuon_butterfly_linear_fwd", "mmuon_butterfly_linear_bwd", "mmuon_but
           "mmuon_last_error")
 _BOUND_LM = ("mmuon_ce_fwd", "mmuon_ce_fwd_bwd", "mmuon_ce_workspace", "mmuon_scale_bf16", "mmuon_embedding_fwd",
              "mmuon_embedding_bwd", "mmuon_embedding_workspace")
-_BOUND_LAYER = ("mmuon_norm_fwd", "mmuon_norm_bwd", "mmuon_norm_workspace", "mmuon_rotary")
+_BOUND_LAYER = ("mmuon_norm_fwd", "mmuon_norm_bwd", "mmuon_norm_workspace", "mmuon_rotary", "mmuon_attention_fwd",
+                "mmuon_attention_bwd", "mmuon_attention_workspace")
 _linear_op = _torch_lib = None
 
 

@@ -813,6 +813,57 @@ int check_rotary(const mmuon_rotary_args* a) {
   return MMUON_OK;
 }
 
+bool attention_sizes(const mmuon_attention_args* a) {
+  return a != nullptr && a->batch >= 0 && a->queries >= 0 && a->keys >= 0 && a->heads >= 0 && a->kv_heads > 0 &&
+         a->heads % a->kv_heads == 0 && a->dim >= 8 && a->dim <= 128 && a->dim % 8 == 0 &&
+         double(a->batch) * a->heads * a->queries < 2147483648.0 && double(a->batch) * a->kv_heads * a->keys < 2147483648.0;
+}
+
+int check_attention(const mmuon_attention_args* a, bool bwd) {
+  if (a == nullptr) return fail(MMUON_EINVAL, "null attention arguments");
+  if (a->dtype != MMUON_BF16) return fail(MMUON_EINVAL, "attention: dtype must be MMUON_BF16 (got %d)", a->dtype);
+  if (a->dim < 8 || a->dim > 128 || a->dim % 8)
+    return fail(MMUON_EINVAL, "attention: dim must be a multiple of 8 of at most 128 (got %d)", a->dim);
+  if (a->heads < 0 || a->kv_heads <= 0 || a->heads % a->kv_heads)
+    return fail(MMUON_EINVAL, "attention: heads (%d) must be a multiple of kv_heads (%d)", a->heads, a->kv_heads);
+  if (!attention_sizes(a))
+    return fail(MMUON_ERANGE, "attention: %d sequences of %d queries and %d keys are negative or too many", a->batch, a->queries, a->keys);
+  if (!(a->scale > 0.f) || !(a->scale <= 3.4e38f))
+    return fail(MMUON_EINVAL, "attention: scale must be positive and finite (got %g)", a->scale);
+  if (a->lam_stride != 0 && a->lam_stride != 1) return fail(MMUON_EINVAL, "attention: lam_stride must be 0 or 1");
+  for (const int64_t* stride : {a->q_stride, a->k_stride, a->v_stride}) {
+    for (int i = 0; i < 3; ++i)
+      if (stride[i] < 0 || stride[i] % 8)
+        return fail(MMUON_EINVAL, "attention: strides must be multiples of 8 elements (got %lld)", (long long)stride[i]);
+    if (stride[1] >= (int64_t(1) << 22))  // a tile's offsets count in 32 bits
+      return fail(MMUON_ERANGE, "attention: tokens %lld elements apart are beyond the kernels' tile offsets", (long long)stride[1]);
+  }
+  const bool queries = a->batch > 0 && a->queries > 0 && a->heads > 0, keys = a->batch > 0 && a->keys > 0;
+  const auto bad = [](const void* p, bool needed) { return (needed && p == nullptr) || !aligned16(p); };
+  if (bad(a->q, queries) || bad(a->k, keys && queries) || bad(a->v, keys && queries))
+    return fail(MMUON_EINVAL, "attention: null or unaligned q, k or v");
+  if ((queries && a->lam == nullptr) || misplaced(a->lam, MMUON_F32)) return fail(MMUON_EINVAL, "attention: null or unaligned lam");
+  if (((reinterpret_cast<uintptr_t>(a->lengths) | reinterpret_cast<uintptr_t>(a->starts)) & 7) != 0)
+    return fail(MMUON_EINVAL, "attention: unaligned lengths or starts");
+  if (bad(a->o1, bwd && queries) || bad(a->o2, bwd && queries) || (bwd && queries && a->lse == nullptr) || misplaced(a->lse, MMUON_F32) ||
+      (a->o1 == nullptr) != (a->o2 == nullptr))
+    return fail(MMUON_EINVAL, "attention: o1, o2 and lse go together, aligned");
+  if (bwd) {
+    if (bad(a->dout, queries) || bad(a->dq, false) || bad(a->dk, false) || bad(a->dv, false) || misplaced(a->dlam, MMUON_F32))
+      return fail(MMUON_EINVAL, "attention: null or unaligned gradients");
+    if ((queries && (a->dq == nullptr) != (a->dlam == nullptr)) || (keys && (a->dk == nullptr) != (a->dv == nullptr)))
+      return fail(MMUON_EINVAL, "attention: dq and dlam, and dk and dv, are made together");
+  } else if (bad(a->o, queries)) {
+    return fail(MMUON_EINVAL, "attention: null or unaligned o");
+  }
+  const size_t need = bwd ? mmuon::attention_backward_workspace(*a) : mmuon::attention_forward_workspace(*a);
+  if (need > 0 && (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 255) != 0))
+    return fail(MMUON_EINVAL, "attention: workspace must be 256-B aligned");
+  if (a->workspace_bytes < need)
+    return fail(MMUON_EINVAL, "attention: workspace of %zu bytes, %zu needed", a->workspace_bytes, need);
+  return MMUON_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -835,6 +886,23 @@ int mmuon_rotary(const mmuon_rotary_args* a, int32_t back, void* stream) {
   if (int rc = check_rotary(a)) return rc;
   mmuon::launch_rotary(*a, back != 0, static_cast<hipStream_t>(stream));
   return check_launch("rotary");
+}
+
+size_t mmuon_attention_workspace(const mmuon_attention_args* a, int32_t backward) {
+  if (!attention_sizes(a)) return 0;
+  return backward ? mmuon::attention_backward_workspace(*a) : mmuon::attention_forward_workspace(*a);
+}
+
+int mmuon_attention_fwd(const mmuon_attention_args* a, void* stream) {
+  if (int rc = check_attention(a, false)) return rc;
+  mmuon::launch_attention_fwd(*a, static_cast<hipStream_t>(stream));
+  return check_launch("attention forward");
+}
+
+int mmuon_attention_bwd(const mmuon_attention_args* a, void* stream) {
+  if (int rc = check_attention(a, true)) return rc;
+  mmuon::launch_attention_bwd(*a, static_cast<hipStream_t>(stream));
+  return check_launch("attention backward");
 }
 
 }  // extern "C"

@@ -1,0 +1,388 @@
+// Differential attention, backward.
+//
+//   dP = dO v^T (both maps')   D_m = dO . o_m      dS_1 = P_1 (dP - D_1)   dS_2 = -lam P_2 (dP - D_2)
+//   dq_m = scale dS_m k_m      dk_m = scale dS_m^T q_m      dv = (P_1 - lam P_2)^T dO      dlam = -sum P_2 dP
+//
+// The maps share dP and one product for dv.  Two kernels make the scores again, one for a block of
+// queries (dq) and one for a block of keys (dk, dv), so that every sum stays in one wave's registers in
+// a fixed order: nothing is added by atomics.  Scores are made so that the index which is summed over
+// next is that of a lane's registers (keys x queries for dq, queries x keys for dk and dv), and P and dS,
+// rounded to bf16, are the next products' operands as they stand.  dlam takes P_2 dP in fp32 as dq's
+// kernel has them: o_2, from rounded probabilities, would give it their error.
+#include <algorithm>
+
+#include "attention_tile.hpp"
+#include "kernels.hpp"
+
+namespace mmuon {
+namespace {
+
+// For each query row (b, h, t): (lse_1, lse_2, D_1, D_2); and its part of dlam
+struct RowSpace {
+  float4* stats;
+  float* dlam;
+};
+
+// A wave to four rows' D: 16 lanes each
+__global__ __launch_bounds__(256) void attention_rows(mmuon_attention_args a, RowSpace space) {
+  const int64_t rows = int64_t(a.batch) * a.heads * a.queries;
+  const int64_t row = int64_t(blockIdx.x) * 16 + threadIdx.x / 16;
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 15, t = int(row % a.queries);
+  const int64_t bh = row / a.queries, b = bh / a.heads, h = bh - b * a.heads;
+  const int64_t at = ((b * a.queries + t) * a.heads + h) * 2 * a.dim;
+  float d1 = 0.f, d2 = 0.f;
+  for (int c = lane * 8; c < 2 * a.dim; c += 128) {
+    float g[8], x[8], y[8];
+    Vec8<BF16T>::load(static_cast<const uint16_t*>(a.dout) + at + c, g);
+    Vec8<F32T>::load(a.o1 + at + c, x);
+    Vec8<F32T>::load(a.o2 + at + c, y);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      d1 = fmaf(g[k], x[k], d1);
+      d2 = fmaf(g[k], y[k], d2);
+    }
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    d1 += __shfl_xor(d1, o, 64);
+    d2 += __shfl_xor(d2, o, 64);
+  }
+  if (lane == 0) space.stats[row] = make_float4(a.lse[2 * row], a.lse[2 * row + 1], d1, d2);
+}
+
+// dq and each row's part of dlam: 32 queries to a wave, over tiles of 32 keys
+template <int D, int WAVES, int SLOTS>
+__global__ __launch_bounds__(64 * WAVES) void attention_dq(mmuon_attention_args a, int tiles, int pinned, RowSpace space) {
+  constexpr int CA = D / 8, CB = D / 4, TK = 32;
+  using T = Tile<D, TK, WAVES>;
+  __shared__ __attribute__((aligned(1024))) char ring[SLOTS * T::BYTES];
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int groups = a.batch * a.kv_heads;
+  int group, rest;
+  if (pinned) {
+    const int local = blockIdx.x >> 3;
+    group = (blockIdx.x & 7) + 8 * (local / tiles);
+    rest = local % tiles;
+    if (group >= groups) return;
+  } else {
+    group = blockIdx.x / tiles;
+    rest = blockIdx.x % tiles;
+  }
+  const int tile = tiles - 1 - rest;
+  const int b = group / a.kv_heads, g = group % a.kv_heads, share = a.heads / a.kv_heads;
+  const int rows = share * a.queries, r0 = tile * 32 * WAVES;
+  const Span span = span_of(a, b);
+  const auto most_of = [&](int first, int n) {
+    if (first >= rows) return 0;
+    const int last = min(first + n, rows) - 1;
+    return seen(a, span, first / a.queries != last / a.queries ? a.queries - 1 : last % a.queries);
+  };
+  const int w0 = r0 + 32 * wave;
+  const int keys = most_of(r0, 32 * WAVES), mine = most_of(w0, 32);
+  const int row = w0 + (lane & 31);
+  const bool in = row < rows;
+  const int h = g * share + (in ? row : rows - 1) / a.queries, t = (in ? row : rows - 1) % a.queries;
+  const int limit = in ? seen(a, span, t) : keys;
+  int fewest = limit;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) fewest = min(fewest, __shfl_xor(fewest, o, 64));
+  fewest = __builtin_amdgcn_readfirstlane(fewest);
+
+  const char* k1 = static_cast<const char*>(a.k) + 2 * (b * a.k_stride[0] + 2 * g * a.k_stride[2]);
+  const char* v0 = static_cast<const char*>(a.v) + 2 * (b * a.v_stride[0] + g * a.v_stride[2]);
+  TileSource src;
+  src.a_stride = uint32_t(2 * a.k_stride[1]);
+  src.b_stride = uint32_t(2 * a.v_stride[1]);
+  src.a_last = a.dim / 8 - 1;
+  src.b_last = a.dim / 4 - 1;
+  const uint32_t lds = lds_addr(ring);
+  const auto load = [&](int i) {
+    const int64_t first = int64_t(i) * TK;
+    src.a1 = k1 + 2 * first * a.k_stride[1];
+    src.a2 = src.a1 + 2 * a.k_stride[2];
+    src.b = v0 + 2 * first * a.v_stride[1];
+    T::load(lds + (i % SLOTS) * T::BYTES, src, span.keys - int(first), wave, lane);
+  };
+
+  bf16x8 q[2][D / 16], dout[D / 8];
+  {
+    const uint16_t* p = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + 2 * h * a.q_stride[2];
+    load_operands(p, a.dim, half, q[0]);
+    load_operands(p + a.q_stride[2], a.dim, half, q[1]);
+    load_operands(static_cast<const uint16_t*>(a.dout) + ((int64_t(b) * a.queries + t) * a.heads + h) * 2 * a.dim, 2 * a.dim, half, dout);
+  }
+  const int64_t at = (int64_t(b) * a.heads + h) * a.queries + t;
+  const float4 st = space.stats[at];
+  const float scale = a.scale * LOG2E;
+  f32x16 acc[2][D / 32];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) acc[m][j] = f32x16{};
+  float along = 0.f;
+
+  const int n = (keys + TK - 1) / TK;
+#pragma unroll
+  for (int i = 0; i < SLOTS - 1; ++i)
+    if (i < n) load(i);
+  const uint32_t kbase = row_base<CA>(lane), vbase = row_base<CB>(lane), tbase = turned_base<CA>(lane);
+  for (int i = 0; i < n; ++i) {
+    if (i + SLOTS - 2 < n) wait_vm<(SLOTS - 2) * T::LOADS>();
+    else wait_vm<0>();
+    barrier_after_lds_writes();
+    if (i + SLOTS - 1 < n) load(i + SLOTS - 1);
+    const char* tile_at = ring + (i % SLOTS) * T::BYTES;
+    if (i * TK >= mine) continue;
+    f32x16 s[2] = {f32x16{}, f32x16{}}, dp = f32x16{};
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      s[0] = mfma(read_rows<CA>(tile_at, kbase, 0, kk), q[0][kk], s[0]);
+      s[1] = mfma(read_rows<CA>(tile_at + T::A2, kbase, 0, kk), q[1][kk], s[1]);
+    }
+#pragma unroll
+    for (int kk = 0; kk < D / 8; ++kk) dp = mfma(read_rows<CB>(tile_at + T::B, vbase, 0, kk), dout[kk], dp);
+    if (i * TK + TK > fewest) {
+      const int left = limit - i * TK - 4 * half;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (8 * (e / 4) + e % 4 >= left) {
+          s[0][e] = s[1][e] = -INFINITY;
+          dp[e] = 0.f;
+        }
+    }
+    float d1[16], d2[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][e], scale, -st.x));
+      const float p2 = __builtin_amdgcn_exp2f(fmaf(s[1][e], scale, -st.y));
+      along = fmaf(p2, dp[e], along);
+      d1[e] = p1 * (dp[e] - st.z);
+      d2[e] = p2 * (dp[e] - st.w);
+    }
+    const bf16x8 x1[2] = {operand(d1), operand(d1 + 8)}, x2[2] = {operand(d2), operand(d2 + 8)};
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        acc[0][j] = mfma(read_turned<CA>(tile_at, tbase, 16 * x, j), x1[x], acc[0][j]);
+        acc[1][j] = mfma(read_turned<CA>(tile_at + T::A2, tbase, 16 * x, j), x2[x], acc[1][j]);
+      }
+  }
+  const float lam = a.lam[int64_t(h) * a.lam_stride];
+  along += other_half(along);
+  if (in && half == 0) space.dlam[at] = -along;
+  uint16_t* dq = in ? static_cast<uint16_t*>(a.dq) + ((int64_t(b) * a.queries + t) * 2 * a.heads + 2 * h) * a.dim : nullptr;
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      acc[0][j][e] *= a.scale;
+      acc[1][j][e] *= -(lam * a.scale);
+    }
+    store_turned(dq, acc[0][j], j, a.dim, half);
+    store_turned(dq != nullptr ? dq + a.dim : nullptr, acc[1][j], j, a.dim, half);
+  }
+}
+
+// dlam[h]: its rows of all sequences, in order by thread and then in a tree
+__global__ __launch_bounds__(1024) void attention_dlam(mmuon_attention_args a, RowSpace space) {
+  __shared__ float sums[16];
+  const int h = blockIdx.x;
+  double s = 0.0;
+  for (int b = 0; b < a.batch; ++b) {
+    const float* from = space.dlam + (int64_t(b) * a.heads + h) * a.queries;
+    float r = 0.f;
+#pragma unroll 4
+    for (int t = threadIdx.x; t < a.queries; t += 1024) r += from[t];
+    s += r;
+  }
+  const float v = block_sum<1024>(float(s), sums);
+  if (threadIdx.x == 0) a.dlam[h] = v;
+}
+
+// dk and dv: 32 keys to a wave, over the query rows of the heads that share them, 32 at a time
+template <int D, int WAVES, int SLOTS>
+__global__ __launch_bounds__(64 * WAVES) void attention_dkv(mmuon_attention_args a, int tiles, int pinned, RowSpace space) {
+  constexpr int CA = D / 8, CB = D / 4, TQ = 32;
+  using T = Tile<D, TQ, WAVES>;
+  constexpr int BYTES = T::BYTES + 1024;  // and the rows' statistics
+  constexpr int LOADS = T::LOADS + 1;
+  __shared__ __attribute__((aligned(1024))) char ring[SLOTS * BYTES];
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int groups = a.batch * a.kv_heads;
+  int group, tile;  // the first keys are seen by the most queries: first
+  if (pinned) {
+    const int local = blockIdx.x >> 3;
+    group = (blockIdx.x & 7) + 8 * (local / tiles);
+    tile = local % tiles;
+    if (group >= groups) return;
+  } else {
+    group = blockIdx.x / tiles;
+    tile = blockIdx.x % tiles;
+  }
+  const int b = group / a.kv_heads, g = group % a.kv_heads, share = a.heads / a.kv_heads;
+  const Span span = span_of(a, b);
+  const int c0 = tile * 32 * WAVES, w0 = c0 + 32 * wave;  // first key of the workgroup, the wave
+  const int key = w0 + (lane & 31);
+  // the first query that sees a key
+  const auto first_of = [&](int k) -> int {
+    if (k >= span.keys) return a.queries;
+    if (!a.causal) return 0;
+    const int64_t t = k - span.first;
+    return t <= 0 ? 0 : t < a.queries ? int(t) : a.queries;
+  };
+  const int from = first_of(c0) / TQ * TQ, mine = first_of(w0), own = first_of(key);
+  const int full = first_of(w0 + 31);  // from here on every key of the wave is seen
+  const int steps = (a.queries - from + TQ - 1) / TQ, n = steps * share;
+
+  const char* q1 = static_cast<const char*>(a.q) + 2 * (b * a.q_stride[0] + 2 * g * share * a.q_stride[2]);
+  const char* g0 = static_cast<const char*>(a.dout) + 2 * (int64_t(b) * a.queries * a.heads + g * share) * 2 * a.dim;
+  TileSource src;
+  src.a_stride = uint32_t(2 * a.q_stride[1]);
+  src.b_stride = uint32_t(2) * a.heads * 2 * a.dim;
+  src.a_last = a.dim / 8 - 1;
+  src.b_last = a.dim / 4 - 1;
+  const uint32_t lds = lds_addr(ring);
+  const auto load = [&](int i) {
+    const int head = i / steps, first = from + (i - head * steps) * TQ;
+    src.a1 = q1 + 2 * (2 * head * a.q_stride[2] + first * a.q_stride[1]);
+    src.a2 = src.a1 + 2 * a.q_stride[2];
+    src.b = g0 + 2 * (int64_t(first) * a.heads + head) * 2 * a.dim;
+    const uint32_t to = lds + (i % SLOTS) * BYTES;
+    T::load(to, src, a.queries - first, wave, lane);
+    // (every wave loads them, so that each has as many loads)
+    const float4* stats = space.stats + (int64_t(b) * a.heads + g * share + head) * a.queries + first;
+    dma16(uniform_ptr(stats), uint32_t(min(lane, a.queries - first - 1)) * 16, to + T::BYTES);
+  };
+
+  bf16x8 k[2][D / 16], v[D / 8];
+  {
+    const int at = min(key, max(span.keys, 1) - 1);
+    const uint16_t* p = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + at * a.k_stride[1] + 2 * g * a.k_stride[2];
+    load_operands(p, a.dim, half, k[0]);
+    load_operands(p + a.k_stride[2], a.dim, half, k[1]);
+    load_operands(static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + at * a.v_stride[1] + g * a.v_stride[2], 2 * a.dim, half, v);
+  }
+  const float scale = a.scale * LOG2E;
+  f32x16 dv[D / 16], dk[2][D / 32];
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) dv[j] = f32x16{};
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) dk[m][j] = f32x16{};
+
+#pragma unroll
+  for (int i = 0; i < SLOTS - 1; ++i)
+    if (i < n) load(i);
+  const uint32_t abase = row_base<CA>(lane), bbase = row_base<CB>(lane), ta = turned_base<CA>(lane), tb = turned_base<CB>(lane);
+  for (int i = 0; i < n; ++i) {
+    if (i + SLOTS - 2 < n) wait_vm<(SLOTS - 2) * LOADS>();
+    else wait_vm<0>();
+    barrier_after_lds_writes();
+    if (i + SLOTS - 1 < n) load(i + SLOTS - 1);
+    const char* tile_at = ring + (i % SLOTS) * BYTES;
+    const int head = i / steps, first = from + (i - head * steps) * TQ;
+    if (first + TQ <= mine) continue;  // no key of this wave is seen
+    f32x16 s[2] = {f32x16{}, f32x16{}}, dp = f32x16{};
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      s[0] = mfma(read_rows<CA>(tile_at, abase, 0, kk), k[0][kk], s[0]);
+      s[1] = mfma(read_rows<CA>(tile_at + T::A2, abase, 0, kk), k[1][kk], s[1]);
+    }
+#pragma unroll
+    for (int kk = 0; kk < D / 8; ++kk) dp = mfma(read_rows<CB>(tile_at + T::B, bbase, 0, kk), v[kk], dp);
+    if (first < full || first + TQ > a.queries) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int t = first + 8 * (e / 4) + 4 * half + e % 4;
+        if (t < own || t >= a.queries) {
+          s[0][e] = s[1][e] = -INFINITY;
+          dp[e] = 0.f;
+        }
+      }
+    }
+    const float lam = a.lam[int64_t(g * share + head) * a.lam_stride];
+    const float4* stats = reinterpret_cast<const float4*>(tile_at + T::BYTES) + 4 * half;
+    float p[16], d1[16], d2[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float4 st = stats[8 * (e / 4) + e % 4];
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][e], scale, -st.x));
+      const float p2 = __builtin_amdgcn_exp2f(fmaf(s[1][e], scale, -st.y)) * lam;
+      p[e] = p1 - p2;
+      d1[e] = p1 * (dp[e] - st.z);
+      d2[e] = p2 * (st.w - dp[e]);
+    }
+    const bf16x8 x[2] = {operand(p), operand(p + 8)}, x1[2] = {operand(d1), operand(d1 + 8)}, x2[2] = {operand(d2), operand(d2 + 8)};
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) dv[j] = mfma(read_turned<CB>(tile_at + T::B, tb, 16 * y, j), x[y], dv[j]);
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        dk[0][j] = mfma(read_turned<CA>(tile_at, ta, 16 * y, j), x1[y], dk[0][j]);
+        dk[1][j] = mfma(read_turned<CA>(tile_at + T::A2, ta, 16 * y, j), x2[y], dk[1][j]);
+      }
+  }
+  const bool in = key < a.keys;
+  uint16_t* to_k = in ? static_cast<uint16_t*>(a.dk) + ((int64_t(b) * a.keys + key) * 2 * a.kv_heads + 2 * g) * a.dim : nullptr;
+  uint16_t* to_v = in ? static_cast<uint16_t*>(a.dv) + ((int64_t(b) * a.keys + key) * a.kv_heads + g) * 2 * a.dim : nullptr;
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) store_turned(to_v, dv[j], j, 2 * a.dim, half);
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dk[m][j][e] *= a.scale;
+      store_turned(in ? to_k + m * a.dim : nullptr, dk[m][j], j, a.dim, half);
+    }
+  }
+}
+
+RowSpace row_space(const mmuon_attention_args& a) {
+  const int64_t rows = int64_t(a.batch) * a.heads * a.queries;
+  return {static_cast<float4*>(a.workspace), static_cast<float*>(a.workspace) + 4 * rows};
+}
+
+template <int D>
+void backward_dim(const mmuon_attention_args& a, hipStream_t s) {
+  const int64_t rows = int64_t(a.batch) * a.heads * a.queries;
+  const int groups = a.batch * a.kv_heads, share = a.heads / a.kv_heads;
+  const int pinned = groups % 8 == 0 || groups >= 64;
+  const int64_t dealt = pinned ? (groups + 7) / 8 * 8 : groups;
+  const RowSpace space = row_space(a);
+  if (rows > 0) hipLaunchKernelGGL(attention_rows, dim3(unsigned((rows + 15) / 16)), dim3(256), 0, s, a, space);
+  if (a.dq != nullptr && rows > 0) {
+    constexpr int WAVES = 4;
+    const int tiles = int((int64_t(share) * a.queries + 32 * WAVES - 1) / (32 * WAVES));
+    hipLaunchKernelGGL((attention_dq<D, WAVES, 3>), dim3(unsigned(dealt * tiles)), dim3(64 * WAVES), 0, s, a, tiles, pinned, space);
+  }
+  if (a.dlam != nullptr && a.heads > 0) hipLaunchKernelGGL(attention_dlam, dim3(unsigned(a.heads)), dim3(1024), 0, s, a, space);
+  if (a.dk != nullptr && groups > 0 && a.keys > 0) {
+    constexpr int WAVES = 4;
+    const int tiles = (a.keys + 32 * WAVES - 1) / (32 * WAVES);
+    hipLaunchKernelGGL((attention_dkv<D, WAVES, 3>), dim3(unsigned(dealt * tiles)), dim3(64 * WAVES), 0, s, a, tiles, pinned, space);
+  }
+}
+
+}  // namespace
+
+size_t attention_backward_workspace(const mmuon_attention_args& a) {
+  return size_t(a.batch) * a.heads * a.queries * 5 * 4;
+}
+
+int launch_attention_bwd(const mmuon_attention_args& a, hipStream_t s) {
+  if (a.dim > 64) backward_dim<128>(a, s);
+  else if (a.dim > 32) backward_dim<64>(a, s);
+  else backward_dim<32>(a, s);
+  return 0;
+}
+
+}  // namespace mmuon

@@ -1,0 +1,161 @@
+// What the kernels of differential attention share: tiles of rows in LDS, loaded past the
+// registers, and the two ways in which they are read as MFMA operands.
+//
+// A tile has ROWS rows of three matrices: two of D columns (the two maps' queries or keys) and one
+// of 2 D (the values, or the output's gradient).  A row of CH 16-B chunks keeps chunk c at c ^ g(row):
+//   CH >= 16: g = 4 (r & 3) + (r >> 2 & 3);  CH = 8: 4 (r >> 1 & 1) + (r >> 2 & 3);  CH = 4: r >> 2 & 3.
+// So the 16 rows that a quarter-wave's ds_read_b128 takes of one chunk column, and the 4 rows of 64 B
+// that a half-wave's ds_read_b64_tr_b16 takes, each cover all 64 banks once.
+//
+// 32x32x16 products: a lane's accumulator i belongs to row 8 (i / 4) + 4 (lane / 32) + i % 4 and column
+// lane % 32.  A product's 16 consecutive values of a lane, rounded to bf16, are two operands of the
+// next one as they stand, if its other operand is read with the rows in that order: half h of a
+// 16-row step holds rows 4 h .. 4 h + 3 and 8 + 4 h .. 8 + 4 h + 3 (read_turned).
+#pragma once
+
+#include "mfma_tile.hpp"
+
+namespace mmuon {
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <int CH>
+__device__ __forceinline__ int chunk_mask(int r) {
+  static_assert(CH >= 4 && (CH & (CH - 1)) == 0, "rows of whole 64-B lines");
+  if constexpr (CH >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+  else if constexpr (CH == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  else return (r >> 2) & 3;
+}
+
+// A per-lane address of each reading; what depends on compile-time indexes is XORed or added.
+template <int CH>
+__device__ __forceinline__ uint32_t row_base(int lane) {
+  const int r = lane & 31;
+  return uint32_t((r * CH + ((lane >> 5) ^ chunk_mask<CH>(r))) * 16);
+}
+template <int CH>
+__device__ __forceinline__ uint32_t turned_base(int lane) {
+  const int l = lane & 15, r = 4 * (lane >> 5) + (l >> 2);
+  const int c = 2 * ((lane >> 4) & 1) + ((l & 3) >> 1);
+  return uint32_t((r * CH + (c ^ chunk_mask<CH>(r))) * 16 + (l & 1) * 8);
+}
+// Rows r0 + lane % 32 (r0 a multiple of 32), columns 16 kk + 8 (lane / 32) + [0, 8)
+template <int CH>
+__device__ __forceinline__ bf16x8 read_rows(const char* m, uint32_t base, int r0, int kk) {
+  return *reinterpret_cast<const bf16x8*>(m + r0 * CH * 16 + (base ^ uint32_t(kk * 32)));
+}
+// Column 32 jb + lane % 32, rows r0 + 4 (lane / 32) + [0, 4) and 8 more on (r0 a multiple of 16)
+template <int CH>
+__device__ __forceinline__ bf16x8 read_turned(const char* m, uint32_t base, int r0, int jb) {
+  const char* p = m + r0 * CH * 16;
+  const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p + (base ^ uint32_t(jb * 64))));
+  const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p + 8 * CH * 16 + (base ^ uint32_t(jb * 64 + 32))));
+  typedef short i16x8 __attribute__((ext_vector_type(8)));
+  const i16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  return __builtin_bit_cast(bf16x8, v);
+}
+
+// Values 8 s .. 8 s + 7 of a lane as an operand
+__device__ __forceinline__ bf16x8 operand(const float* v) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 u = {f2bf2(v[0], v[1]), f2bf2(v[2], v[3]), f2bf2(v[4], v[5]), f2bf2(v[6], v[7])};
+  return __builtin_bit_cast(bf16x8, u);
+}
+
+// c + the sum of an operand's eight values
+__device__ __forceinline__ float operand_sum(const bf16x8& v, float c) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 one = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) c = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{v[k], v[k + 1]}, one, c, false);
+  return c;
+}
+
+// The other half-wave's value for the same column
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+// Where a tile's rows come from
+struct TileSource {
+  const char* a1;  // the tile's first row in each matrix
+  const char* a2;
+  const char* b;
+  uint32_t a_stride, b_stride;  // bytes from one row to the next
+  int a_last, b_last;           // the last chunk of a row that is there
+};
+
+template <int D, int ROWS, int WAVES>
+struct Tile {
+  static constexpr int CA = D / 8, CB = D / 4;        // chunks of a row
+  static constexpr int NA = ROWS * CA / 64, NB = 2 * NA;  // loads of a wave that fill a matrix
+  static constexpr int LOADS = (2 * NA + NB) / WAVES;     // of each wave
+  static constexpr int A2 = ROWS * CA * 16, B = 2 * A2, BYTES = 4 * A2;
+  static_assert((2 * NA + NB) % WAVES == 0, "each wave has as many loads");
+
+  // Rows from `left` on repeat the last one there, and chunks a row does not have its last: what is
+  // read is always there, and what comes of it is masked, multiplied by zeros or not stored.
+  static __device__ __forceinline__ void load(uint32_t lds, const TileSource& s, int left, int wave, int lane) {
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) {
+      const int n = wave + WAVES * k;
+      if (n < 2 * NA) {
+        const int m = n >= NA ? 1 : 0, at = (n - m * NA) * 64 + lane;
+        const int r = at / CA, c = min((at % CA) ^ chunk_mask<CA>(r), s.a_last);
+        dma16(uniform_ptr(m ? s.a2 : s.a1), uint32_t(min(r, left - 1)) * s.a_stride + uint32_t(c) * 16, lds + m * A2 + (n - m * NA) * 1024);
+      } else {
+        const int at = (n - 2 * NA) * 64 + lane;
+        const int r = at / CB, c = min((at % CB) ^ chunk_mask<CB>(r), s.b_last);
+        dma16(uniform_ptr(s.b), uint32_t(min(r, left - 1)) * s.b_stride + uint32_t(c) * 16, lds + B + (n - 2 * NA) * 1024);
+      }
+    }
+  }
+};
+
+// A row of `dim` columns (a multiple of 8) as operands: columns 16 kk + 8 (lane / 32) + [0, 8), zeros behind the last
+template <int N>
+__device__ __forceinline__ void load_operands(const uint16_t* row, int dim, int half, bf16x8 (&v)[N]) {
+#pragma unroll
+  for (int kk = 0; kk < N; ++kk) {
+    const int col = 16 * kk + 8 * half;
+    v[kk] = bf16x8{};
+    if (col < dim) v[kk] = *reinterpret_cast<const bf16x8*>(row + col);
+  }
+}
+
+// Accumulators of 32 rows (columns of the output) and 32 columns (its rows) to bf16, a lane's row `out`
+// (null: none) from column 32 jb on: the half-waves exchange 4 values, so that each stores 16 B.
+__device__ __forceinline__ void store_turned(uint16_t* out, const f32x16& acc, int jb, int dim, int half) {
+#pragma unroll
+  for (int g = 0; g < 4; g += 2) {
+    uint32_t a0 = f2bf2(acc[4 * g], acc[4 * g + 1]), a1 = f2bf2(acc[4 * g + 2], acc[4 * g + 3]);
+    uint32_t b0 = f2bf2(acc[4 * g + 4], acc[4 * g + 5]), b1 = f2bf2(acc[4 * g + 6], acc[4 * g + 7]);
+    const auto x = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
+    const auto y = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+    const int col = 32 * jb + 8 * (g + half);
+    if (out != nullptr && col < dim) *reinterpret_cast<uint4*>(out + col) = make_uint4(x[0], y[0], x[1], y[1]);
+  }
+}
+
+// The sequence's keys and the place of its first query among them
+struct Span {
+  int keys;       // visible ones, of those there is room for
+  int64_t first;  // query t sees keys up to first + t, where the mask is causal
+};
+__device__ __forceinline__ Span span_of(const mmuon_attention_args& a, int b) {
+  constexpr int64_t FAR = int64_t(1) << 32;  // as good as any place farther off
+  const int64_t n = a.lengths != nullptr ? a.lengths[b] : a.keys;
+  Span s;
+  s.keys = int(n < 0 ? 0 : n > a.keys ? a.keys : n);
+  s.first = a.starts != nullptr ? a.starts[b] : s.keys - a.queries;
+  s.first = s.first < -FAR ? -FAR : s.first > FAR ? FAR : s.first;
+  return s;
+}
+// Keys that query t sees
+__device__ __forceinline__ int seen(const mmuon_attention_args& a, const Span& s, int t) {
+  if (!a.causal) return s.keys;
+  const int64_t n = s.first + t + 1;
+  return n <= 0 ? 0 : n < s.keys ? int(n) : s.keys;
+}
+
+}  // namespace
+}  // namespace mmuon

@@ -107,6 +107,12 @@ int launch_norm_fwd(const mmuon_norm_args& a, hipStream_t s);
 int launch_norm_bwd(const mmuon_norm_args& a, hipStream_t s);
 int launch_rotary(const mmuon_rotary_args& a, bool back, hipStream_t s);
 
+// Differential attention --------------------------------------------------------------
+size_t attention_forward_workspace(const mmuon_attention_args& a);
+size_t attention_backward_workspace(const mmuon_attention_args& a);
+int launch_attention_fwd(const mmuon_attention_args& a, hipStream_t s);
+int launch_attention_bwd(const mmuon_attention_args& a, hipStream_t s);
+
 // Gradient-clipping coefficient of a launch (gscale: device pointer, or null
 // when not clipping), read once per thread: the per-element form would test
 // the pointer in every element (a branch each) and, after the thread's first

@@ -33,6 +33,9 @@ struct Abi {
   int (*norm_bwd)(const mmuon_norm_args*, void*) = nullptr;
   size_t (*norm_workspace)(const mmuon_norm_args*) = nullptr;
   int (*rotary)(const mmuon_rotary_args*, int32_t, void*) = nullptr;
+  int (*attention_fwd)(const mmuon_attention_args*, void*) = nullptr;
+  int (*attention_bwd)(const mmuon_attention_args*, void*) = nullptr;
+  size_t (*attention_workspace)(const mmuon_attention_args*, int32_t) = nullptr;
   const char* (*last_error)() = nullptr;
 };
 extern Abi abi;

@@ -3,11 +3,14 @@
 //   mmuon::rms_norm(x, residual, weight, eps) -> (y, h, inv)
 //   mmuon::rms_norm_fp8(x, residual, weight, eps, dtype, group) -> (codes, scale, h)
 //   mmuon::rotary(q, k, table, positions, interleaved, back) -> (q, k)
-// over the C ABI's mmuon_norm_* and mmuon_rotary.
+//   mmuon::differential_attention(q, k, v, lam, lengths, starts, causal, scale, save) -> (o, o1, o2, lse)
+// over the C ABI's mmuon_norm_*, mmuon_rotary and mmuon_attention_*.
 //
-// The norm's gradient has no derivative of its own; the rotation's is a rotation, to any order.
+// The norm's and the attention's gradients have no derivative of their own; the rotation's is a
+// rotation, to any order.
 #include "torch_common.hpp"
 
+#include <array>
 #include <tuple>
 
 using namespace mmuon_torch;
@@ -28,6 +31,10 @@ void require_one_device(std::initializer_list<const Tensor*> ts) {
                 t->device());
   }
 }
+
+// The shape of a result that is not wanted
+const std::array<int64_t, 1> NOTHING = {0};
+const at::IntArrayRef NONE = NOTHING;
 
 const char* name_of(const Tensor& t) { return c10::getDtypeNames(t.scalar_type()).first.c_str(); }
 
@@ -79,7 +86,7 @@ Triple rms_norm_impl(const Tensor& x_, const OptionalTensor& residual, const Ten
   const c10::DeviceGuard guard(x_.device());
   const Tensor x = rows_of(x_), r = residual.has_value() ? rows_of(*residual) : Tensor(), w = weight.contiguous();
   Tensor y = at::empty(x_.sizes(), x.options());
-  Tensor h = at::empty(residual.has_value() ? x_.sizes() : at::IntArrayRef{0}, x.options());
+  Tensor h = at::empty(residual.has_value() ? x_.sizes() : NONE, x.options());
   Tensor inv = at::empty({a.rows}, x.options().dtype(at::kFloat));
   a.x_stride = row_stride(x);
   a.x = x.const_data_ptr();
@@ -110,7 +117,7 @@ Pair rms_norm_grad_impl(const Tensor& h_, const Tensor& inv, const Tensor& weigh
   const c10::DeviceGuard guard(h_.device());
   const Tensor h = rows_of(h_), dy = rows_of(dy_), dh = dh_.has_value() ? rows_of(*dh_) : Tensor(), w = weight.contiguous();
   Tensor dx = at::empty(h_.sizes(), h.options());
-  Tensor dw = at::empty(need_dw ? weight.sizes() : at::IntArrayRef{0}, w.options());
+  Tensor dw = at::empty(need_dw ? weight.sizes() : NONE, w.options());
   a.x = h.const_data_ptr();
   a.x_stride = row_stride(h);
   a.w = w.const_data_ptr();
@@ -146,7 +153,7 @@ Triple rms_norm_fp8_impl(const Tensor& x_, const OptionalTensor& residual, const
   shape.back() = group == 0 ? 1 : (a.width + 127) / 128;
   Tensor codes = at::empty(x_.sizes(), x.options().dtype(dtype));
   Tensor scale = at::empty(shape, x.options().dtype(at::kFloat));
-  Tensor h = at::empty(residual.has_value() ? x_.sizes() : at::IntArrayRef{0}, x.options());
+  Tensor h = at::empty(residual.has_value() ? x_.sizes() : NONE, x.options());
   a.out_dtype = dtype == at::kFloat8_e4m3fn ? MMUON_F8E4M3 : MMUON_F8E5M2;
   a.group = int32_t(group);
   a.x_stride = row_stride(x);
@@ -349,6 +356,235 @@ Pair rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& table, cons
   return call_rotary(q, k, table, positions, interleaved, back);
 }
 
+// ---------------------------------------------------------------------------
+// Differential attention
+// ---------------------------------------------------------------------------
+// Heads of 16-B chunks, tokens not too far apart for the kernels' offsets: the tensor itself where
+// it is such, else a copy
+Tensor aligned_heads(const Tensor& t) {
+  bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
+  ok = ok && (t.size(1) <= 1 || t.stride(1) < (int64_t(1) << 22));
+  return ok ? t : dense_aligned(t);
+}
+void take_strides(const Tensor& t, int64_t (&to)[3]) {
+  for (int i = 0; i < 3; ++i) to[i] = t.size(i) > 1 ? t.stride(i) : 0;
+}
+
+struct AttentionCall {
+  Tensor q, k, v, lam, lengths, starts, ws;
+  mmuon_attention_args a{};
+  c10::DeviceGuard guard;
+  AttentionCall(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& lam_, const OptionalTensor& lengths_,
+                const OptionalTensor& starts_, bool causal, double scale)
+      : guard((check(q_, k_, v_, lam_, lengths_, starts_, scale), q_.device())) {
+    q = aligned_heads(q_), k = aligned_heads(k_), v = aligned_heads(v_);
+    lam = lam_.size(0) <= 1 || lam_.stride(0) <= 1 ? lam_ : lam_.contiguous();
+    a.batch = int32_t(q.size(0));
+    a.queries = int32_t(q.size(1));
+    a.keys = int32_t(k.size(1));
+    a.heads = int32_t(q.size(2) / 2);
+    a.kv_heads = int32_t(v.size(2));
+    a.dim = int32_t(q.size(3));
+    a.dtype = MMUON_BF16;
+    a.causal = causal;
+    a.scale = float(scale);
+    a.lam_stride = a.heads > 1 ? int32_t(lam.stride(0)) : 0;
+    take_strides(q, a.q_stride);
+    take_strides(k, a.k_stride);
+    take_strides(v, a.v_stride);
+    a.q = q.const_data_ptr();
+    a.k = k.const_data_ptr();
+    a.v = v.const_data_ptr();
+    a.lam = static_cast<const float*>(lam.const_data_ptr());
+    if (lengths_.has_value()) {
+      lengths = lengths_->to(at::kLong).contiguous();
+      a.lengths = static_cast<const int64_t*>(lengths.const_data_ptr());
+    }
+    if (starts_.has_value()) {
+      starts = starts_->to(at::kLong).contiguous();
+      a.starts = static_cast<const int64_t*>(starts.const_data_ptr());
+    }
+  }
+  static void check(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const OptionalTensor& lengths,
+                    const OptionalTensor& starts, double scale) {
+    const char* names[3] = {"q", "k", "v"};
+    const Tensor* ts[3] = {&q, &k, &v};
+    for (int i = 0; i < 3; ++i)
+      TORCH_CHECK_TYPE(ts[i]->scalar_type() == at::kBFloat16, "differential_attention computes in bfloat16; ", names[i],
+                       " is torch.", name_of(*ts[i]), " (run under torch.autocast(dtype=torch.bfloat16) or pass bf16 tensors)");
+    TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && v.dim() == 4 && k.size(0) == q.size(0) && v.size(0) == q.size(0) &&
+                          v.size(1) == k.size(1) && k.size(3) == q.size(3) && v.size(3) == 2 * q.size(3) &&
+                          k.size(2) == 2 * v.size(2) && v.size(2) > 0 && q.size(2) % (2 * v.size(2)) == 0,
+                      "expected q (B, T, 2 H, D), k (B, S, 2 K, D) and v (B, S, K, 2 D) with H a multiple of K, got ",
+                      q.sizes(), ", ", k.sizes(), " and ", v.sizes());
+    TORCH_CHECK_VALUE(q.size(3) >= 8 && q.size(3) <= 128 && q.size(3) % 8 == 0,
+                      "differential_attention needs heads of a multiple of 8 columns, at most 128, got ", q.size(3));
+    for (int i = 0; i < 3; ++i)
+      TORCH_CHECK_VALUE(q.size(i) <= INT32_MAX && k.size(i) <= INT32_MAX, "differential_attention: sizes beyond 2^31");
+    TORCH_CHECK_TYPE(lam.scalar_type() == at::kFloat, "lam must be float32, got torch.", name_of(lam));
+    TORCH_CHECK_VALUE(lam.dim() == 1 && lam.size(0) == q.size(2) / 2, "lam must hold one value, or one for each of ",
+                      q.size(2) / 2, " heads, got ", lam.sizes());
+    TORCH_CHECK_VALUE(scale > 0 && scale <= 3.4e38, "scale must be positive and finite, got ", scale);
+    require_one_device({&q, &k, &v, &lam});
+    for (const OptionalTensor* t : {&lengths, &starts}) {
+      if (!t->has_value()) continue;
+      const char* name = t == &lengths ? "lengths" : "starts";
+      TORCH_CHECK_TYPE((*t)->scalar_type() == at::kLong || (*t)->scalar_type() == at::kInt, name,
+                       " must be int64 or int32, got torch.", name_of(**t));
+      TORCH_CHECK_VALUE((*t)->dim() == 1 && (*t)->size(0) == q.size(0), name, " must hold one value per sequence, got ",
+                        (*t)->sizes());
+      require_one_device({&q, &**t});
+    }
+    bind_library();
+  }
+  void workspace(bool backward) {
+    ws = at::empty({std::max<int64_t>(int64_t(abi.attention_workspace(&a, backward ? 1 : 0)), 256)}, q.options().dtype(at::kByte));
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = size_t(ws.numel());
+  }
+};
+
+using Quad = std::tuple<Tensor, Tensor, Tensor, Tensor>;
+
+Quad attention_impl(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const OptionalTensor& lengths,
+                    const OptionalTensor& starts, bool causal, double scale, bool save) {
+  AttentionCall call(q, k, v, lam, lengths, starts, causal, scale);
+  mmuon_attention_args& a = call.a;
+  const std::array<int64_t, 4> shape = {a.batch, a.queries, a.heads, 2 * a.dim};
+  const at::IntArrayRef kept = save ? at::IntArrayRef(shape) : NONE;
+  Tensor o = at::empty(shape, call.q.options()), o1 = at::empty(kept, call.q.options().dtype(at::kFloat)), o2 = at::empty(kept, o1.options());
+  Tensor lse = save ? at::empty({a.batch, a.heads, a.queries, 2}, call.q.options().dtype(at::kFloat))
+                    : at::empty(NONE, call.q.options().dtype(at::kFloat));
+  a.o = o.data_ptr();
+  if (save) {
+    a.o1 = static_cast<float*>(o1.data_ptr());
+    a.o2 = static_cast<float*>(o2.data_ptr());
+    a.lse = static_cast<float*>(lse.data_ptr());
+  }
+  call.workspace(false);
+  check_rc(abi.attention_fwd(&a, stream_of(call.q)), "mmuon_attention_fwd");
+  return {o, o1, o2, lse};
+}
+
+// need_q: dq and dlam; need_kv: dk and dv
+Quad attention_grad_impl(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const OptionalTensor& lengths,
+                         const OptionalTensor& starts, const Tensor& o1, const Tensor& o2, const Tensor& lse,
+                         const Tensor& dout_, bool causal, double scale, bool need_q, bool need_kv) {
+  AttentionCall call(q, k, v, lam, lengths, starts, causal, scale);
+  mmuon_attention_args& a = call.a;
+  const std::array<int64_t, 4> shape = {a.batch, a.queries, a.heads, 2 * a.dim}, two = {a.batch, a.heads, a.queries, 2};
+  TORCH_CHECK_VALUE(dout_.sizes() == at::IntArrayRef(shape) && dout_.scalar_type() == at::kBFloat16,
+                    "the gradient of differential_attention's output must be bfloat16 and of its shape, got ", dout_.sizes());
+  for (const Tensor* t : {&o1, &o2})
+    TORCH_CHECK_VALUE(t->sizes() == at::IntArrayRef(shape) && t->scalar_type() == at::kFloat, "o1 and o2 must be the forward's");
+  require_one_device({&q, &o1, &o2, &dout_});
+  TORCH_CHECK_VALUE(lse.sizes() == at::IntArrayRef(two) && lse.scalar_type() == at::kFloat && lse.is_contiguous(),
+                    "lse must be the forward's");
+  require_one_device({&q, &lse});
+  const Tensor dout = dense_aligned(dout_), p1 = dense_aligned(o1), p2 = dense_aligned(o2);
+  Tensor dq = at::empty(need_q ? q.sizes() : NONE, call.q.options());
+  Tensor dlam = at::empty(need_q ? lam.sizes() : NONE, lam.options());
+  Tensor dk = at::empty(need_kv ? k.sizes() : NONE, call.q.options());
+  Tensor dv = at::empty(need_kv ? v.sizes() : NONE, call.q.options());
+  a.o1 = const_cast<float*>(static_cast<const float*>(p1.const_data_ptr()));
+  a.o2 = const_cast<float*>(static_cast<const float*>(p2.const_data_ptr()));
+  a.lse = const_cast<float*>(static_cast<const float*>(lse.const_data_ptr()));
+  a.dout = dout.const_data_ptr();
+  if (need_q) {
+    a.dq = dq.data_ptr();
+    a.dlam = static_cast<float*>(dlam.data_ptr());
+  }
+  if (need_kv) {
+    a.dk = dk.data_ptr();
+    a.dv = dv.data_ptr();
+  }
+  call.workspace(true);
+  check_rc(abi.attention_bwd(&a, stream_of(call.q)), "mmuon_attention_bwd");
+  return {dq, dk, dv, dlam};
+}
+
+Quad call_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const OptionalTensor& lengths,
+                    const OptionalTensor& starts, bool causal, double scale, bool save) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("mmuon::differential_attention", "")
+                       .typed<Quad(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptionalTensor&,
+                                   const OptionalTensor&, bool, double, bool)>();
+  return op.call(q, k, v, lam, lengths, starts, causal, scale, save);
+}
+Quad call_attention_grad(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const OptionalTensor& lengths,
+                         const OptionalTensor& starts, const Tensor& o1, const Tensor& o2, const Tensor& lse,
+                         const Tensor& dout, bool causal, double scale, bool need_q, bool need_kv) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("mmuon::differential_attention_grad", "")
+                       .typed<Quad(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptionalTensor&,
+                                   const OptionalTensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, bool,
+                                   double, bool, bool)>();
+  return op.call(q, k, v, lam, lengths, starts, o1, o2, lse, dout, causal, scale, need_q, need_kv);
+}
+
+struct AttentionFn : torch::autograd::Function<AttentionFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam,
+                               const OptionalTensor& lengths, const OptionalTensor& starts, bool causal, double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [o, o1, o2, lse] = call_attention(q, k, v, lam, lengths, starts, causal, scale, true);
+    ctx->saved_data["q"] = q.requires_grad();
+    ctx->saved_data["k"] = k.requires_grad();
+    ctx->saved_data["v"] = v.requires_grad();
+    ctx->saved_data["lam"] = lam.requires_grad();
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    ctx->save_for_backward({q, k, v, lam, lengths.has_value() ? *lengths : Tensor(), starts.has_value() ? *starts : Tensor(),
+                            o1, o2, lse});
+    ctx->mark_non_differentiable({o1, o2, lse});
+    return {o, o1, o2, lse};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const auto given = [](const Tensor& t) { return t.defined() ? OptionalTensor(t) : c10::nullopt; };
+    const bool q = ctx->saved_data["q"].toBool(), k = ctx->saved_data["k"].toBool(), v = ctx->saved_data["v"].toBool(),
+               lam = ctx->saved_data["lam"].toBool();
+    auto [dq, dk, dv, dlam] = call_attention_grad(s[0], s[1], s[2], s[3], given(s[4]), given(s[5]), s[6], s[7], s[8], grads[0],
+                                                  ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(),
+                                                  q || lam, k || v);
+    return {q ? dq : Tensor(), k ? dk : Tensor(), v ? dv : Tensor(), lam ? dlam : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+struct AttentionGradFn : torch::autograd::Function<AttentionGradFn> {
+  static variable_list forward(AutogradContext*, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam,
+                               const OptionalTensor& lengths, const OptionalTensor& starts, const Tensor& o1, const Tensor& o2,
+                               const Tensor& lse, const Tensor& dout, bool causal, double scale, bool need_q, bool need_kv) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [dq, dk, dv, dlam] = call_attention_grad(q, k, v, lam, lengths, starts, o1, o2, lse, dout, causal, scale, need_q, need_kv);
+    return {dq, dk, dv, dlam};
+  }
+  static variable_list backward(AutogradContext*, const variable_list&) {
+    TORCH_CHECK(false, "Trying to backward through mmuon.differential_attention_grad.default but no autograd formula was "
+                "registered.");
+  }
+};
+
+Quad attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const OptionalTensor& lengths,
+                        const OptionalTensor& starts, bool causal, double scale, bool save) {
+  if (any_requires_grad({&q, &k, &v, &lam})) {
+    const variable_list r = AttentionFn::apply(q, k, v, lam, lengths, starts, causal, scale);
+    return {r[0], r[1], r[2], r[3]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_attention(q, k, v, lam, lengths, starts, causal, scale, save);
+}
+Quad attention_grad_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const OptionalTensor& lengths,
+                             const OptionalTensor& starts, const Tensor& o1, const Tensor& o2, const Tensor& lse,
+                             const Tensor& dout, bool causal, double scale, bool need_q, bool need_kv) {
+  if (any_requires_grad({&q, &k, &v, &lam, &o1, &o2, &lse, &dout})) {
+    const variable_list r = AttentionGradFn::apply(q, k, v, lam, lengths, starts, o1, o2, lse, dout, causal, scale, need_q, need_kv);
+    return {r[0], r[1], r[2], r[3]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_attention_grad(q, k, v, lam, lengths, starts, o1, o2, lse, dout, causal, scale, need_q, need_kv);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(mmuon, m) {
@@ -360,16 +596,25 @@ TORCH_LIBRARY_FRAGMENT(mmuon, m) {
         "Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
   m.def("rotary(Tensor q, Tensor k, Tensor table, Tensor? positions, bool interleaved, bool back) -> (Tensor, Tensor)",
         {at::Tag::pt2_compliant_tag});
+  m.def("differential_attention(Tensor q, Tensor k, Tensor v, Tensor lam, Tensor? lengths, Tensor? starts, bool causal, "
+        "float scale, bool save) -> (Tensor, Tensor, Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
+  m.def("differential_attention_grad(Tensor q, Tensor k, Tensor v, Tensor lam, Tensor? lengths, Tensor? starts, Tensor o1, "
+        "Tensor o2, Tensor lse, Tensor dout, bool causal, float scale, bool need_q, bool need_kv) -> (Tensor, Tensor, "
+        "Tensor, Tensor)", {at::Tag::pt2_compliant_tag});
 }
 TORCH_LIBRARY_IMPL(mmuon, CompositeExplicitAutograd, m) {
   m.impl("rms_norm", rms_norm_impl);
   m.impl("rms_norm_grad", rms_norm_grad_impl);
   m.impl("rms_norm_fp8", rms_norm_fp8_impl);
   m.impl("rotary", rotary_impl);
+  m.impl("differential_attention", attention_impl);
+  m.impl("differential_attention_grad", attention_grad_impl);
 }
 TORCH_LIBRARY_IMPL(mmuon, Autograd, m) {
   m.impl("rms_norm", norm_autograd);
   m.impl("rms_norm_grad", norm_grad_autograd);
   m.impl("rms_norm_fp8", norm_fp8_autograd);
   m.impl("rotary", rotary_autograd);
+  m.impl("differential_attention", attention_autograd);
+  m.impl("differential_attention_grad", attention_grad_autograd);
 }

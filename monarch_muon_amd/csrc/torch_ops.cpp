@@ -222,7 +222,8 @@ int mmuon_torch_bind_lm(int version, void* ce_fwd, void* ce_fwd_bwd, void* ce_wo
 }
 
 // The functions of the operators between a layer's projections (torch_layer.cpp), likewise.
-int mmuon_torch_bind_layer(int version, void* norm_fwd, void* norm_bwd, void* norm_workspace, void* rotary) {
+int mmuon_torch_bind_layer(int version, void* norm_fwd, void* norm_bwd, void* norm_workspace, void* rotary,
+                           void* attention_fwd, void* attention_bwd, void* attention_workspace) {
   if (version != MMUON_ABI_VERSION) return 0;
   const std::lock_guard<std::mutex> lock(binding);
   if (bound) return 0;
@@ -230,6 +231,9 @@ int mmuon_torch_bind_layer(int version, void* norm_fwd, void* norm_bwd, void* no
   abi.norm_bwd = reinterpret_cast<decltype(abi.norm_bwd)>(norm_bwd);
   abi.norm_workspace = reinterpret_cast<decltype(abi.norm_workspace)>(norm_workspace);
   abi.rotary = reinterpret_cast<decltype(abi.rotary)>(rotary);
+  abi.attention_fwd = reinterpret_cast<decltype(abi.attention_fwd)>(attention_fwd);
+  abi.attention_bwd = reinterpret_cast<decltype(abi.attention_bwd)>(attention_bwd);
+  abi.attention_workspace = reinterpret_cast<decltype(abi.attention_workspace)>(attention_workspace);
   return 0;
 }
 

@@ -2,8 +2,11 @@
 
 * ``rms_norm(x, weight, residual=r)``: the norm with the residual's addition; ``rms_norm_fp8`` with an output in 8 bits.
 * ``rotary(q, k, table)``: rotary positions of queries and keys, by a table that ``rotary_table`` makes.
+* ``differential_attention(q, k, v, lam)``: the difference of two softmax maps over shared values; for training, for
+  prompts, and for new tokens of a cache.
 
-The reference computes them with torch's ops (``pretrain/src/models/llama.py``: ``RMSNorm``, ``apply_rotary_emb``).  All
+The reference computes with torch's ops what it has of these (``pretrain/src/models/llama.py``: ``RMSNorm``,
+``apply_rotary_emb``, ``F.scaled_dot_product_attention``).  All
 are native torch operators (``csrc/torch_layer.cpp``), registered with fake implementations, on
 ``torch.cuda.current_stream()``; there is no fallback.
 """
@@ -13,16 +16,16 @@ import math
 
 import torch
 
-from . import _abi, butterfly  # noqa: F401
+from . import butterfly
 
-__all__ = ["rms_norm", "rms_norm_fp8", "rotary", "rotary_table"]
+__all__ = ["rms_norm", "rms_norm_fp8", "rotary", "rotary_table", "differential_attention"]
 
-_norm_op = _norm_fp8_op = _rotary_op = None
+_norm_op = _norm_fp8_op = _rotary_op = _attention_op = None
 
 
 def _load() -> None:
     """Register the operators' fakes; raises where the native library is not built."""
-    global _norm_op, _norm_fp8_op, _rotary_op
+    global _norm_op, _norm_fp8_op, _rotary_op, _attention_op
     if butterfly._linear_op is None:
         butterfly._load_linear()
 
@@ -45,9 +48,24 @@ def _load() -> None:
     def _(q, k, table, positions, interleaved, back):
         return q.new_empty(q.shape), k.new_empty(k.shape)
 
+    @torch.library.register_fake("mmuon::differential_attention")
+    def _(q, k, v, lam, lengths, starts, causal, scale, save):
+        B, T, heads = q.shape[:3]
+        o = q.new_empty(B, T, heads // 2, v.shape[3])
+        if not save:
+            return o, q.new_empty(0), q.new_empty(0), q.new_empty(0, dtype=torch.float32)
+        f32 = dict(dtype=torch.float32)
+        return o, torch.empty_like(o, **f32), torch.empty_like(o, **f32), q.new_empty(B, heads // 2, T, 2, dtype=torch.float32)
+
+    @torch.library.register_fake("mmuon::differential_attention_grad")
+    def _(q, k, v, lam, lengths, starts, o1, o2, lse, dout, causal, scale, need_q, need_kv):
+        return (q.new_empty(q.shape if need_q else (0,)), k.new_empty(k.shape if need_kv else (0,)),
+                v.new_empty(v.shape if need_kv else (0,)), lam.new_empty(lam.shape if need_q else (0,)))
+
     _norm_op = torch.ops.mmuon.rms_norm.default
     _norm_fp8_op = torch.ops.mmuon.rms_norm_fp8.default
     _rotary_op = torch.ops.mmuon.rotary.default
+    _attention_op = torch.ops.mmuon.differential_attention.default
 
 
 try:
@@ -145,3 +163,37 @@ def rotary(q: torch.Tensor, k: torch.Tensor, table: torch.Tensor, positions: tor
     if _rotary_op is None:
         _load()
     return _rotary_op(q, k, table, positions, bool(interleaved), False)
+
+
+def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, *, causal: bool = True,
+                           scale: float | None = None, lengths: torch.Tensor | None = None,
+                           starts: torch.Tensor | None = None) -> torch.Tensor:
+    """``(softmax(q1 k1^T scale) - lam softmax(q2 k2^T scale)) v`` for each head, (B, T, H, 2 D) bfloat16.
+
+    ``q`` (B, T, 2 H, D), ``k`` (B, S, 2 K, D) and ``v`` (B, S, K, 2 D) bfloat16 (cast under bf16 autocast) at any strides (copied
+    where rows of a head are no whole 16-byte chunks), D a multiple of 8 up to 128: query heads ``2 h`` and ``2 h + 1`` are head
+    ``h``'s two maps, key heads ``2 g`` and ``2 g + 1`` with value head ``g`` are shared by H / K heads.  ``lam``: one value or one for
+    each head (taken as float32).  ``scale`` is ``D ** -0.5`` by default.
+
+    ``lengths`` (B): the keys of each sequence that count; those behind are not read (a cache).  ``causal``: query ``t`` of
+    sequence ``b`` sees keys up to ``starts[b] + t``, by default ``lengths[b] - T + t``: the queries are the last ones of their
+    sequence.  A query that sees no key has zeros.  An infinity or a NaN in a key or value that ``causal`` alone hides may
+    show as NaN in the queries before it.
+
+    Differentiable in ``q``, ``k``, ``v`` and ``lam``; every sum has an order that depends on the sizes alone, so gradients are
+    the same bits every time.  Probabilities are rounded to bfloat16 before their products with the values, as are the
+    scores' gradients before theirs.  There is no second derivative.
+    """
+    if _attention_op is None:
+        _load()
+    if torch.is_autocast_enabled():
+        dt = torch.get_autocast_dtype("cuda")
+        q, k, v = q.to(dt), k.to(dt), v.to(dt)
+    if q.dim() != 4:
+        raise ValueError(f"expected q (B, T, 2 H, D), got {tuple(q.shape)}")
+    heads = q.shape[2] // 2
+    lam = lam.float()
+    if lam.numel() == 1 and lam.dim() <= 1:
+        lam = lam.reshape(1).expand(heads)
+    return _attention_op(q, k, v, lam, lengths, starts, bool(causal), float(q.shape[3] ** -0.5 if scale is None else scale),
+                         False)[0]

@@ -84,3 +84,83 @@ def rotary(x, angles, size=1.0, interleaved=False, back=False):
     tol[..., first] += half_step(x.dtype) * out[..., first].abs() + tiny(x.dtype)
     tol[..., second] += half_step(x.dtype) * out[..., second].abs() + tiny(x.dtype)
     return out, tol
+
+
+# ----- differential attention ------------------------------------------------------
+UBF = 2.0 ** -8
+
+
+def visible(Tq, Tk, causal, length=None, start=None):
+    """(queries, keys): which keys each query sees."""
+    n = Tk if length is None else min(max(int(length), 0), Tk)
+    j, t = torch.arange(Tk), torch.arange(Tq)
+    see = (j < n).expand(Tq, Tk)
+    if causal:
+        see = see & (j <= (n - Tq if start is None else int(start)) + t[:, None])
+    return see
+
+
+def attention(q, k, v, lam, causal=True, scale=None, lengths=None, starts=None, dout=None):
+    """((o, dq, dk, dv, dlam), bounds), float64; the gradients where ``dout`` is given.
+
+    Roundings: scores, their statistics and all sums in fp32; P, dS and P_1 - lam P_2 to bf16 before their products; results
+    once.  o_m, of which D_m = dO . o_m is made, has weights w = P (1 + e) / sum of P (1 + e) with |e| up to 2^-8 and stays in
+    fp32: o_m is off by sum of P e (v - o_m), D_m by sum of P e (dP - D_m)."""
+    B, Tq, H2, d = q.shape
+    H, Tk, K = H2 // 2, k.shape[1], v.shape[2]
+    scale = d ** -0.5 if scale is None else scale
+    f = torch.float64
+    dev = q.device
+    q, k, v, lam = q.double(), k.double(), v.double(), lam.double().to(dev).expand(H)
+    zero = lambda *s: torch.zeros(s, dtype=f, device=dev)  # noqa: E731
+    o, ot = zero(B, Tq, H, 2 * d), zero(B, Tq, H, 2 * d)
+    dq, dk, dv, dl = zero(*q.shape), zero(*k.shape), zero(*v.shape), zero(H)
+    qt, kt, vt, lt = zero(*q.shape), zero(*k.shape), zero(*v.shape), zero(H)
+    for b in range(B):
+        see = visible(Tq, Tk, causal, None if lengths is None else lengths[b], None if starts is None else starts[b]).to(dev)
+        kept = see.any(0)
+        for h in range(H):
+            g, L = h // (H // K), lam[h]
+            V = torch.where(kept[:, None], v[b, :, g], 0.0)
+            P, err, O, Ot = [], [], [], []
+            for m in (0, 1):
+                Q, Km = q[b, :, 2 * h + m], torch.where(kept[:, None], k[b, :, 2 * g + m], 0.0)
+                s = (Q @ Km.T * scale).masked_fill(~see, -float("inf"))
+                p = torch.softmax(s, 1).nan_to_num(0.0)
+                size = (Q.abs() @ Km.abs().T * scale).masked_fill(~see, 0.0)
+                top = size.amax(1, keepdim=True) if Tk else zero(Tq, 1)
+                # a probability's relative error: its score's, the reference's and the sum's; exp2 is good to 2^-22
+                e = U32 * (2 * (d + 6) * (size + top) + Tk + 40)
+                P.append(p)
+                err.append(e)
+                O.append(p @ V)
+                Ot.append(((1.01 * UBF + e + 2 * Tk * U32) * p) @ V.abs() + 1.01 * UBF * O[m].abs())
+            o[b, :, h] = O[0] - L * O[1]
+            ot[b, :, h] = Ot[0] + L.abs() * Ot[1] + half_step(torch.bfloat16) * o[b, :, h].abs() + 1e-37
+            if dout is None:
+                continue
+            G = dout[b, :, h].double()
+            both = P[0] - L * P[1]
+            dv[b, :, g] += both.T @ G
+            off = P[0] * err[0] + L.abs() * P[1] * err[1]
+            vt[b, :, g] += (off + UBF * both.abs() + 2 * H * Tq * U32 * (P[0] + L.abs() * P[1])).T @ G.abs()
+            dp = G @ V.T
+            dpt = 2 * (2 * d + 2) * U32 * (G.abs() @ V.abs().T)
+            for m, sign in ((0, 1.0), (1, -L)):
+                D = (P[m] * dp).sum(1, keepdim=True)
+                Dt = (P[m] * (dp - D).abs() * (1.01 * UBF + err[m])).sum(1, keepdim=True) + \
+                    (2 * Tk + 4 * d) * U32 * (P[m] * (G.abs() @ V.abs().T)).sum(1, keepdim=True)
+                ds = P[m] * (dp - D)
+                dst = P[m] * (dpt + Dt + 4 * U32 * (dp.abs() + D.abs())) + ds.abs() * (err[m] + UBF)
+                ds, dst = ds * sign * scale, dst * abs(sign) * scale
+                Q, Km = q[b, :, 2 * h + m], torch.where(kept[:, None], k[b, :, 2 * g + m], 0.0)
+                dq[b, :, 2 * h + m] = ds @ Km
+                qt[b, :, 2 * h + m] = (dst + 2 * Tk * U32 * ds.abs()) @ Km.abs()
+                dk[b, :, 2 * g + m] += ds.T @ Q
+                kt[b, :, 2 * g + m] += (dst + 2 * H * Tq * U32 * ds.abs()).T @ Q.abs()
+                if m:
+                    dl[h] -= D.sum()
+                    lt[h] += (P[1] * (dpt + dp.abs() * (err[1] + (Tk + B * Tq) * U32))).sum()
+    r = half_step(torch.bfloat16)
+    bounds = [ot, qt + r * dq.abs() + 1e-37, kt + r * dk.abs() + 1e-37, vt + r * dv.abs() + 1e-37, lt + U32 * dl.abs() + 1e-37]
+    return (o, dq, dk, dv, dl), bounds
