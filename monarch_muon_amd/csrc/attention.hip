@@ -17,8 +17,8 @@
 // a small part.  (Divided by the exact sum, the gradients of two queries were 0.65% off.)  o_m goes to the
 // backward in fp32 for the same reason; the backward's own probabilities are made with the exact sum.
 //
-// Rows are those of the query heads that share a key head, one head after the other, so that a single
-// token of several heads is one tile of rows and a cache is read once.  Where there are few rows the
+// Rows are the query heads that share a key head, token after token, so that single tokens of several
+// heads are one tile of rows and a cache is read once.  Where there are few rows the
 // keys are split over workgroups, and a second launch joins the parts in order.
 #include <algorithm>
 
@@ -37,7 +37,7 @@ struct Parts {
 
 // MAPS: maps of a wave
 template <int D, int TK, int WAVES, int MAPS, int SLOTS, bool SPLIT>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void attend(mmuon_attention_args a, int tiles, int splits, int pinned, Parts parts) {
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void attend(mmuon_attention_args a, int tiles, int splits, Dealing dealt, Parts parts) {
   constexpr int CA = D / 8, CB = D / 4, PANELS = D / 16;  // of the values: 2 D / 32
   using T = Tile<D, TK, WAVES>;
   __shared__ __attribute__((aligned(1024))) char ring[SLOTS * T::BYTES];
@@ -45,33 +45,23 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void attend(mmuon_a
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int PAIRS = WAVES * MAPS / 2;  // waves of 32 rows: one, or two that are a pair
   const int m0 = MAPS == 2 ? 0 : wave & 1;
-  const int each = tiles * splits, groups = a.batch * a.kv_heads;
-  int group, rest;
-  if (pinned) {  // a key head's workgroups on one XCD
-    const int local = blockIdx.x >> 3;
-    group = (blockIdx.x & 7) + 8 * (local / each);
-    rest = local % each;
-    if (group >= groups) return;
-  } else {
-    group = blockIdx.x / each;
-    rest = blockIdx.x % each;
-  }
+  int group, item;
+  if (!deal(dealt, a.batch * a.kv_heads, group, item)) return;
   // the last queries see the most keys: first
-  const int tile = tiles - 1 - rest / splits, split = rest % splits;
+  const int tile = tiles - 1 - item / splits, split = item % splits;
   const int b = group / a.kv_heads, g = group % a.kv_heads, share = a.heads / a.kv_heads;
   const int rows = share * a.queries, r0 = tile * 32 * PAIRS;
   const Span span = span_of(a, b);
   // keys that any row of the workgroup sees, and the wave's: most and fewest
   const auto most_of = [&](int first, int n) {  // rows first .. first + n - 1
     if (first >= rows) return 0;
-    const int last = min(first + n, rows) - 1;
-    return seen(a, span, first / a.queries != last / a.queries ? a.queries - 1 : last % a.queries);
+    return seen(a, span, (min(first + n, rows) - 1) / share);
   };
   const int w0 = r0 + 32 * (MAPS == 2 ? wave : wave >> 1);
   const int keys = most_of(r0, 32 * PAIRS), mine = most_of(w0, 32);
   const int row = w0 + (lane & 31);
   const bool in = row < rows;
-  const int h = g * share + (in ? row : rows - 1) / a.queries, t = (in ? row : rows - 1) % a.queries;
+  const int t = (in ? row : rows - 1) / share, h = g * share + (in ? row : rows - 1) - t * share;
   const int limit = in ? seen(a, span, t) : keys;
   int fewest = limit;
 #pragma unroll
@@ -121,6 +111,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void attend(mmuon_a
 #pragma unroll
   for (int i = 0; i < SLOTS - 1; ++i)
     if (i < n) load(i);
+  wait_loaded();
   const uint32_t kbase = row_base<CA>(lane), vbase = turned_base<CB>(lane);
   for (int i = 0; i < n; ++i) {
     // this wave's part of tile i is there; behind the barrier all of it, and tile i - 1 has been read
@@ -153,7 +144,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void attend(mmuon_a
         float top = s[m][0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) top = fmaxf(top, s[m][e]);
-        top = fmaxf(top, other_half(top));
+        top = half_max(top);
         if (__any(top * scale > shift[m] + 8.f || (ref[m] == -INFINITY && top > -INFINITY))) {
           const float next = fmaxf(ref[m], top);
           const float by = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((ref[m] - next) * scale);
@@ -188,8 +179,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void attend(mmuon_a
   }
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
-    sum[m] += other_half(sum[m]);
-    weight[m] += other_half(weight[m]);
+    sum[m] = half_sum(sum[m]);
+    weight[m] = half_sum(weight[m]);
   }
 
   if constexpr (SPLIT) {
@@ -326,7 +317,7 @@ __global__ __launch_bounds__(256) void attend_join(mmuon_attention_args a, int s
   n1 = found[0].z + found[1].z + found[2].z + found[3].z;
   n2 = found[0].w + found[1].w + found[2].w + found[3].w;
   const int b = group / a.kv_heads, g = group % a.kv_heads;
-  const int h = g * share + row / a.queries, t = row % a.queries;
+  const int t = row / share, h = g * share + row - t * share;
   const float lam = a.lam[int64_t(h) * a.lam_stride];
   const float i1 = n1 == 0.f ? 0.f : 1.f / n1, i2 = n2 == 0.f ? 0.f : 1.f / n2;
   const int64_t to = ((int64_t(b) * a.queries + t) * a.heads + h) * 2 * a.dim;
@@ -375,11 +366,9 @@ ForwardPlan forward_plan(const mmuon_attention_args& a) {
 
 template <int D, int TK, int WAVES, int MAPS, int SLOTS, bool SPLIT>
 void attend_launch(const mmuon_attention_args& a, const ForwardPlan& p, const Parts& parts, hipStream_t s) {
-  const int groups = a.batch * a.kv_heads;
-  const int pinned = groups % 8 == 0 || groups >= 64;
-  const int64_t blocks = int64_t(pinned ? (groups + 7) / 8 * 8 : groups) * p.tiles * p.splits;
-  hipLaunchKernelGGL((attend<D, TK, WAVES, MAPS, SLOTS, SPLIT>), dim3(unsigned(blocks)), dim3(64 * WAVES), 0, s, a, p.tiles, p.splits,
-                     pinned, parts);
+  const Dealing d = dealing(int64_t(a.batch) * a.kv_heads, int64_t(p.tiles) * p.splits);
+  hipLaunchKernelGGL((attend<D, TK, WAVES, MAPS, SLOTS, SPLIT>), dim3(blocks_of(d)), dim3(64 * WAVES), 0, s, a, p.tiles, p.splits, d,
+                     parts);
 }
 template <int D>
 void attend_dim(const mmuon_attention_args& a, hipStream_t s) {

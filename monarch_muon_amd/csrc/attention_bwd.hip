@@ -53,37 +53,27 @@ __global__ __launch_bounds__(256) void attention_rows(mmuon_attention_args a, Ro
 
 // dq and each row's part of dlam: 32 queries to a wave, over tiles of 32 keys
 template <int D, int WAVES, int SLOTS>
-__global__ __launch_bounds__(64 * WAVES) void attention_dq(mmuon_attention_args a, int tiles, int pinned, RowSpace space) {
+__global__ __launch_bounds__(64 * WAVES) void attention_dq(mmuon_attention_args a, Dealing dealt, RowSpace space) {
   constexpr int CA = D / 8, CB = D / 4, TK = 32;
   using T = Tile<D, TK, WAVES>;
   __shared__ __attribute__((aligned(1024))) char ring[SLOTS * T::BYTES];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int groups = a.batch * a.kv_heads;
-  int group, rest;
-  if (pinned) {
-    const int local = blockIdx.x >> 3;
-    group = (blockIdx.x & 7) + 8 * (local / tiles);
-    rest = local % tiles;
-    if (group >= groups) return;
-  } else {
-    group = blockIdx.x / tiles;
-    rest = blockIdx.x % tiles;
-  }
-  const int tile = tiles - 1 - rest;
+  int group, item;
+  if (!deal(dealt, a.batch * a.kv_heads, group, item)) return;
+  const int tile = dealt.each - 1 - item;
   const int b = group / a.kv_heads, g = group % a.kv_heads, share = a.heads / a.kv_heads;
   const int rows = share * a.queries, r0 = tile * 32 * WAVES;
   const Span span = span_of(a, b);
   const auto most_of = [&](int first, int n) {
     if (first >= rows) return 0;
-    const int last = min(first + n, rows) - 1;
-    return seen(a, span, first / a.queries != last / a.queries ? a.queries - 1 : last % a.queries);
+    return seen(a, span, (min(first + n, rows) - 1) / share);
   };
   const int w0 = r0 + 32 * wave;
   const int keys = most_of(r0, 32 * WAVES), mine = most_of(w0, 32);
   const int row = w0 + (lane & 31);
   const bool in = row < rows;
-  const int h = g * share + (in ? row : rows - 1) / a.queries, t = (in ? row : rows - 1) % a.queries;
+  const int t = (in ? row : rows - 1) / share, h = g * share + (in ? row : rows - 1) - t * share;
   const int limit = in ? seen(a, span, t) : keys;
   int fewest = limit;
 #pragma unroll
@@ -127,6 +117,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dq(mmuon_attention_args 
 #pragma unroll
   for (int i = 0; i < SLOTS - 1; ++i)
     if (i < n) load(i);
+  wait_loaded();
   const uint32_t kbase = row_base<CA>(lane), vbase = row_base<CB>(lane), tbase = turned_base<CA>(lane);
   for (int i = 0; i < n; ++i) {
     if (i + SLOTS - 2 < n) wait_vm<(SLOTS - 2) * T::LOADS>();
@@ -171,7 +162,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dq(mmuon_attention_args 
       }
   }
   const float lam = a.lam[int64_t(h) * a.lam_stride];
-  along += other_half(along);
+  along = half_sum(along);
   if (in && half == 0) space.dlam[at] = -along;
   uint16_t* dq = in ? static_cast<uint16_t*>(a.dq) + ((int64_t(b) * a.queries + t) * 2 * a.heads + 2 * h) * a.dim : nullptr;
 #pragma unroll
@@ -204,7 +195,7 @@ __global__ __launch_bounds__(1024) void attention_dlam(mmuon_attention_args a, R
 
 // dk and dv: 32 keys to a wave, over the query rows of the heads that share them, 32 at a time
 template <int D, int WAVES, int SLOTS>
-__global__ __launch_bounds__(64 * WAVES) void attention_dkv(mmuon_attention_args a, int tiles, int pinned, RowSpace space) {
+__global__ __launch_bounds__(64 * WAVES) void attention_dkv(mmuon_attention_args a, Dealing dealt, RowSpace space) {
   constexpr int CA = D / 8, CB = D / 4, TQ = 32;
   using T = Tile<D, TQ, WAVES>;
   constexpr int BYTES = T::BYTES + 1024;  // and the rows' statistics
@@ -212,17 +203,8 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dkv(mmuon_attention_args
   __shared__ __attribute__((aligned(1024))) char ring[SLOTS * BYTES];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int groups = a.batch * a.kv_heads;
   int group, tile;  // the first keys are seen by the most queries: first
-  if (pinned) {
-    const int local = blockIdx.x >> 3;
-    group = (blockIdx.x & 7) + 8 * (local / tiles);
-    tile = local % tiles;
-    if (group >= groups) return;
-  } else {
-    group = blockIdx.x / tiles;
-    tile = blockIdx.x % tiles;
-  }
+  if (!deal(dealt, a.batch * a.kv_heads, group, tile)) return;
   const int b = group / a.kv_heads, g = group % a.kv_heads, share = a.heads / a.kv_heads;
   const Span span = span_of(a, b);
   const int c0 = tile * 32 * WAVES, w0 = c0 + 32 * wave;  // first key of the workgroup, the wave
@@ -246,8 +228,11 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dkv(mmuon_attention_args
   src.a_last = a.dim / 8 - 1;
   src.b_last = a.dim / 4 - 1;
   const uint32_t lds = lds_addr(ring);
+  int next_head = 0, next_first = from;  // of the tile that is loaded next
   const auto load = [&](int i) {
-    const int head = i / steps, first = from + (i - head * steps) * TQ;
+    const int head = next_head, first = next_first;
+    next_first += TQ;
+    if (next_first >= a.queries) next_first = from, ++next_head;
     src.a1 = q1 + 2 * (2 * head * a.q_stride[2] + first * a.q_stride[1]);
     src.a2 = src.a1 + 2 * a.q_stride[2];
     src.b = g0 + 2 * (int64_t(first) * a.heads + head) * 2 * a.dim;
@@ -278,14 +263,17 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dkv(mmuon_attention_args
 #pragma unroll
   for (int i = 0; i < SLOTS - 1; ++i)
     if (i < n) load(i);
+  wait_loaded();
   const uint32_t abase = row_base<CA>(lane), bbase = row_base<CB>(lane), ta = turned_base<CA>(lane), tb = turned_base<CB>(lane);
+  int head = 0, first = from - TQ;
   for (int i = 0; i < n; ++i) {
+    first += TQ;
+    if (first >= a.queries) first = from, ++head;
     if (i + SLOTS - 2 < n) wait_vm<(SLOTS - 2) * LOADS>();
     else wait_vm<0>();
     barrier_after_lds_writes();
     if (i + SLOTS - 1 < n) load(i + SLOTS - 1);
     const char* tile_at = ring + (i % SLOTS) * BYTES;
-    const int head = i / steps, first = from + (i - head * steps) * TQ;
     if (first + TQ <= mine) continue;  // no key of this wave is seen
     f32x16 s[2] = {f32x16{}, f32x16{}}, dp = f32x16{};
 #pragma unroll
@@ -305,7 +293,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dkv(mmuon_attention_args
         }
       }
     }
-    const float lam = a.lam[int64_t(g * share + head) * a.lam_stride];
+    const float lam = load_uniform(a.lam + int64_t(g * share + head) * a.lam_stride);
     const float4* stats = reinterpret_cast<const float4*>(tile_at + T::BYTES) + 4 * half;
     float p[16], d1[16], d2[16];
 #pragma unroll
@@ -354,21 +342,19 @@ RowSpace row_space(const mmuon_attention_args& a) {
 template <int D>
 void backward_dim(const mmuon_attention_args& a, hipStream_t s) {
   const int64_t rows = int64_t(a.batch) * a.heads * a.queries;
-  const int groups = a.batch * a.kv_heads, share = a.heads / a.kv_heads;
-  const int pinned = groups % 8 == 0 || groups >= 64;
-  const int64_t dealt = pinned ? (groups + 7) / 8 * 8 : groups;
+  const int64_t groups = int64_t(a.batch) * a.kv_heads, share = a.heads / a.kv_heads;
   const RowSpace space = row_space(a);
   if (rows > 0) hipLaunchKernelGGL(attention_rows, dim3(unsigned((rows + 15) / 16)), dim3(256), 0, s, a, space);
   if (a.dq != nullptr && rows > 0) {
     constexpr int WAVES = 4;
-    const int tiles = int((int64_t(share) * a.queries + 32 * WAVES - 1) / (32 * WAVES));
-    hipLaunchKernelGGL((attention_dq<D, WAVES, 3>), dim3(unsigned(dealt * tiles)), dim3(64 * WAVES), 0, s, a, tiles, pinned, space);
+    const Dealing d = dealing(groups, (share * a.queries + 32 * WAVES - 1) / (32 * WAVES));
+    hipLaunchKernelGGL((attention_dq<D, WAVES, 3>), dim3(blocks_of(d)), dim3(64 * WAVES), 0, s, a, d, space);
   }
   if (a.dlam != nullptr && a.heads > 0) hipLaunchKernelGGL(attention_dlam, dim3(unsigned(a.heads)), dim3(1024), 0, s, a, space);
   if (a.dk != nullptr && groups > 0 && a.keys > 0) {
     constexpr int WAVES = 4;
-    const int tiles = (a.keys + 32 * WAVES - 1) / (32 * WAVES);
-    hipLaunchKernelGGL((attention_dkv<D, WAVES, 3>), dim3(unsigned(dealt * tiles)), dim3(64 * WAVES), 0, s, a, tiles, pinned, space);
+    const Dealing d = dealing(groups, (a.keys + 32 * WAVES - 1) / (32 * WAVES));
+    hipLaunchKernelGGL((attention_dkv<D, WAVES, 3>), dim3(blocks_of(d)), dim3(64 * WAVES), 0, s, a, d, space);
   }
 }
 

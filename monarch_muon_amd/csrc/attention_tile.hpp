@@ -72,8 +72,25 @@ __device__ __forceinline__ float operand_sum(const bf16x8& v, float c) {
   return c;
 }
 
-// The other half-wave's value for the same column
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+// Sum and maximum of a lane's and the other half-wave's value for the same column
+__device__ __forceinline__ float half_sum(float v) {
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+__device__ __forceinline__ float half_max(float v) {
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+
+// Wait for every load in flight, in a form that the compiler counts: registers that were loaded
+// before a loop would else be waited for inside it, and with them, in issue order, the tiles that
+// are on their way past the registers.
+__device__ __forceinline__ void wait_loaded() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0) alone
+
+// A uniform value by the scalar unit, whose loads do not queue behind the tiles'
+__device__ __forceinline__ float load_uniform(const float* p) {
+  return *(const __attribute__((address_space(4))) float*)(uintptr_t)p;
+}
 
 // Where a tile's rows come from
 struct TileSource {
@@ -135,6 +152,35 @@ __device__ __forceinline__ void store_turned(uint16_t* out, const f32x16& acc, i
     if (out != nullptr && col < dim) *reinterpret_cast<uint4*>(out + col) = make_uint4(x[0], y[0], x[1], y[1]);
   }
 }
+
+// Which group (sequence and key head) and which of its items a workgroup takes.  `across` 8: a group's
+// workgroups are on one XCD, whose L2 holds its keys and values; 1: groups are spread over all of them.
+// Items are in falling order of their work, and a block of groups is dealt item by item: the largest
+// first, so that the smallest fill the end, but no more groups at a time than that takes.
+struct Dealing {
+  int across;
+  int groups;  // of one XCD
+  int block;
+  int each;    // items of a group
+};
+__device__ __forceinline__ bool deal(const Dealing& d, int all, int& group, int& item) {
+  const int local = d.across == 8 ? blockIdx.x >> 3 : blockIdx.x;
+  const int full = d.block * d.each, at = local / full, rest = local - at * full;
+  const int n = min(d.block, d.groups - at * d.block);
+  item = rest / n;
+  const int of = at * d.block + rest - item * n;
+  group = d.across == 8 ? (blockIdx.x & 7) + 8 * of : of;
+  return group < all;
+}
+inline Dealing dealing(int64_t groups, int64_t each) {
+  Dealing d;
+  d.across = groups % 8 == 0 || groups >= 64 ? 8 : 1;
+  d.groups = int((groups + d.across - 1) / d.across);
+  d.each = int(each);
+  d.block = int(std::max<int64_t>(1, std::min<int64_t>(d.groups, 128 * (8 / d.across) / std::max<int64_t>(each, 1))));
+  return d;
+}
+inline unsigned blocks_of(const Dealing& d) { return unsigned(int64_t(d.across) * d.groups * d.each); }
 
 // The sequence's keys and the place of its first query among them
 struct Span {
