@@ -35,8 +35,8 @@ CFLAGS = [
 ]
 
 
-# The accumulators of these kernels' products are read by other instructions between the products: taken in VGPRs,
-# they are not copied from and to AGPRs (dk and dv of heads of 128 columns: 350 spilled registers without it, 26 with it).
+# The kernel of dk and dv has 256 accumulators that only products touch and others that are read between products: with
+# products in VGPR form the former are moved to AGPRs once, and nothing is spilled (in AGPR form 19 registers).
 FLAGS_OF = {"attention_bwd": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 

@@ -9,6 +9,12 @@
 // next is that of a lane's registers (keys x queries for dq, queries x keys for dk and dv), and P and dS,
 // rounded to bf16, are the next products' operands as they stand.  dlam takes P_2 dP in fp32 as dq's
 // kernel has them: o_2, from rounded probabilities, would give it their error.
+//
+// Two waves are a pair: each has one map's scores, half of dP's sum over the columns, and half of dv's
+// columns; the halves of dP, and the probabilities that dv needs of both maps, pass through LDS.  So no
+// product is made twice, and the sums leave room for two waves of registers on a SIMD, whose products
+// and exponentials run side by side.  (One wave for both maps, one to a SIMD: 16 x 1024 tokens, 8 heads
+// of 2 x 64, dk and dv 188 us; 4 x 1024, 16 heads of 2 x 128, dq 100, dk and dv 226.)
 #include <algorithm>
 
 #include "attention_tile.hpp"
@@ -17,7 +23,7 @@
 namespace mmuon {
 namespace {
 
-// For each query row (b, h, t): (lse_1, lse_2, D_1, D_2); and its part of dlam
+// For each query row (b, h, t): (lse_1, D_1, lse_2, D_2); and its part of dlam
 struct RowSpace {
   float4* stats;
   float* dlam;
@@ -48,29 +54,30 @@ __global__ __launch_bounds__(256) void attention_rows(mmuon_attention_args a, Ro
     d1 += __shfl_xor(d1, o, 64);
     d2 += __shfl_xor(d2, o, 64);
   }
-  if (lane == 0) space.stats[row] = make_float4(a.lse[2 * row], a.lse[2 * row + 1], d1, d2);
+  if (lane == 0) space.stats[row] = make_float4(a.lse[2 * row], d1, a.lse[2 * row + 1], d2);
 }
 
-// dq and each row's part of dlam: 32 queries to a wave, over tiles of 32 keys
-template <int D, int WAVES, int SLOTS>
-__global__ __launch_bounds__(64 * WAVES) void attention_dq(mmuon_attention_args a, Dealing dealt, RowSpace space) {
+// dq and each row's part of dlam: 32 queries to a pair, over tiles of 32 keys
+template <int D, int PAIRS, int SLOTS>
+__global__ __launch_bounds__(128 * PAIRS, 2) void attention_dq(mmuon_attention_args a, Dealing dealt, RowSpace space) {
   constexpr int CA = D / 8, CB = D / 4, TK = 32;
-  using T = Tile<D, TK, WAVES>;
+  using T = Tile<D, TK, 2 * PAIRS>;
   __shared__ __attribute__((aligned(1024))) char ring[SLOTS * T::BYTES];
+  __shared__ float4 passed[2 * PAIRS][4][64];
   const int lane = threadIdx.x & 63, half = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = wave & 1;
   int group, item;
   if (!deal(dealt, a.batch * a.kv_heads, group, item)) return;
   const int tile = dealt.each - 1 - item;
   const int b = group / a.kv_heads, g = group % a.kv_heads, share = a.heads / a.kv_heads;
-  const int rows = share * a.queries, r0 = tile * 32 * WAVES;
+  const int rows = share * a.queries, r0 = tile * 32 * PAIRS;
   const Span span = span_of(a, b);
   const auto most_of = [&](int first, int n) {
     if (first >= rows) return 0;
     return seen(a, span, (min(first + n, rows) - 1) / share);
   };
-  const int w0 = r0 + 32 * wave;
-  const int keys = most_of(r0, 32 * WAVES), mine = most_of(w0, 32);
+  const int w0 = r0 + 32 * (wave >> 1);
+  const int keys = most_of(r0, 32 * PAIRS), mine = most_of(w0, 32);
   const int row = w0 + (lane & 31);
   const bool in = row < rows;
   const int t = (in ? row : rows - 1) / share, h = g * share + (in ? row : rows - 1) - t * share;
@@ -96,21 +103,16 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dq(mmuon_attention_args 
     T::load(lds + (i % SLOTS) * T::BYTES, src, span.keys - int(first), wave, lane);
   };
 
-  bf16x8 q[2][D / 16], dout[D / 8];
-  {
-    const uint16_t* p = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + 2 * h * a.q_stride[2];
-    load_operands(p, a.dim, half, q[0]);
-    load_operands(p + a.q_stride[2], a.dim, half, q[1]);
-    load_operands(static_cast<const uint16_t*>(a.dout) + ((int64_t(b) * a.queries + t) * a.heads + h) * 2 * a.dim, 2 * a.dim, half, dout);
-  }
+  bf16x8 q[D / 16], dout[D / 16];
+  load_operands(static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + (2 * h + m) * a.q_stride[2], a.dim, half, q);
+  load_operands(static_cast<const uint16_t*>(a.dout) + ((int64_t(b) * a.queries + t) * a.heads + h) * 2 * a.dim, 2 * a.dim, half, dout,
+                m * D);
   const int64_t at = (int64_t(b) * a.heads + h) * a.queries + t;
-  const float4 st = space.stats[at];
+  const float2 st = reinterpret_cast<const float2*>(space.stats + at)[m];
   const float scale = a.scale * LOG2E;
-  f32x16 acc[2][D / 32];
+  f32x16 acc[D / 32];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) acc[m][j] = f32x16{};
+  for (int j = 0; j < D / 32; ++j) acc[j] = f32x16{};
   float along = 0.f;
 
   const int n = (keys + TK - 1) / TK;
@@ -118,62 +120,62 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dq(mmuon_attention_args 
   for (int i = 0; i < SLOTS - 1; ++i)
     if (i < n) load(i);
   wait_loaded();
-  const uint32_t kbase = row_base<CA>(lane), vbase = row_base<CB>(lane), tbase = turned_base<CA>(lane);
+  const uint32_t kbase = row_base<CA>(lane), vbase = row_base<CB>(lane) ^ uint32_t(m * 2 * D), tbase = turned_base<CA>(lane);
   for (int i = 0; i < n; ++i) {
     if (i + SLOTS - 2 < n) wait_vm<(SLOTS - 2) * T::LOADS>();
     else wait_vm<0>();
     barrier_after_lds_writes();
     if (i + SLOTS - 1 < n) load(i + SLOTS - 1);
     const char* tile_at = ring + (i % SLOTS) * T::BYTES;
-    if (i * TK >= mine) continue;
-    f32x16 s[2] = {f32x16{}, f32x16{}}, dp = f32x16{};
+    const bool active = i * TK < mine;  // the pair's
+    f32x16 dp = f32x16{};
+    float p[16];
+    if (active) {
+      f32x16 s = f32x16{};
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      s[0] = mfma(read_rows<CA>(tile_at, kbase, 0, kk), q[0][kk], s[0]);
-      s[1] = mfma(read_rows<CA>(tile_at + T::A2, kbase, 0, kk), q[1][kk], s[1]);
+      for (int kk = 0; kk < D / 16; ++kk) dp = mfma(read_rows<CB>(tile_at + T::B, vbase, 0, kk), dout[kk], dp);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) s = mfma(read_rows<CA>(tile_at + m * T::A2, kbase, 0, kk), q[kk], s);
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) passed[wave][e / 4][lane] = make_float4(dp[e], dp[e + 1], dp[e + 2], dp[e + 3]);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], scale, -st.x));
     }
+    barrier_after_lds_writes();
+    if (!active) continue;
+    float d[16];
 #pragma unroll
-    for (int kk = 0; kk < D / 8; ++kk) dp = mfma(read_rows<CB>(tile_at + T::B, vbase, 0, kk), dout[kk], dp);
+    for (int e = 0; e < 16; e += 4) {
+      const float4 x = passed[wave ^ 1][e / 4][lane];
+      dp[e] += x.x, dp[e + 1] += x.y, dp[e + 2] += x.z, dp[e + 3] += x.w;
+    }
     if (i * TK + TK > fewest) {
       const int left = limit - i * TK - 4 * half;
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        if (8 * (e / 4) + e % 4 >= left) {
-          s[0][e] = s[1][e] = -INFINITY;
-          dp[e] = 0.f;
-        }
+        if (8 * (e / 4) + e % 4 >= left) p[e] = dp[e] = 0.f;
     }
-    float d1[16], d2[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][e], scale, -st.x));
-      const float p2 = __builtin_amdgcn_exp2f(fmaf(s[1][e], scale, -st.y));
-      along = fmaf(p2, dp[e], along);
-      d1[e] = p1 * (dp[e] - st.z);
-      d2[e] = p2 * (dp[e] - st.w);
+      along = fmaf(p[e], dp[e], along);
+      d[e] = p[e] * (dp[e] - st.y);
     }
-    const bf16x8 x1[2] = {operand(d1), operand(d1 + 8)}, x2[2] = {operand(d2), operand(d2 + 8)};
+    const bf16x8 x[2] = {operand(d), operand(d + 8)};
 #pragma unroll
     for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        acc[0][j] = mfma(read_turned<CA>(tile_at, tbase, 16 * x, j), x1[x], acc[0][j]);
-        acc[1][j] = mfma(read_turned<CA>(tile_at + T::A2, tbase, 16 * x, j), x2[x], acc[1][j]);
-      }
+      for (int y = 0; y < 2; ++y) acc[j] = mfma(read_turned<CA>(tile_at + m * T::A2, tbase, 16 * y, j), x[y], acc[j]);
   }
   const float lam = a.lam[int64_t(h) * a.lam_stride];
   along = half_sum(along);
-  if (in && half == 0) space.dlam[at] = -along;
-  uint16_t* dq = in ? static_cast<uint16_t*>(a.dq) + ((int64_t(b) * a.queries + t) * 2 * a.heads + 2 * h) * a.dim : nullptr;
+  if (m == 1 && in && half == 0) space.dlam[at] = -along;
+  uint16_t* dq = in ? static_cast<uint16_t*>(a.dq) + ((int64_t(b) * a.queries + t) * 2 * a.heads + 2 * h + m) * a.dim : nullptr;
+  const float by = m ? -(lam * a.scale) : a.scale;
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      acc[0][j][e] *= a.scale;
-      acc[1][j][e] *= -(lam * a.scale);
-    }
-    store_turned(dq, acc[0][j], j, a.dim, half);
-    store_turned(dq != nullptr ? dq + a.dim : nullptr, acc[1][j], j, a.dim, half);
+    for (int e = 0; e < 16; ++e) acc[j][e] *= by;
+    store_turned(dq, acc[j], j, a.dim, half);
   }
 }
 
@@ -193,14 +195,16 @@ __global__ __launch_bounds__(1024) void attention_dlam(mmuon_attention_args a, R
   if (threadIdx.x == 0) a.dlam[h] = v;
 }
 
-// dk and dv: 32 keys to a wave, over the query rows of the heads that share them, 32 at a time
+// dk and dv: 32 keys to a wave, over the query rows of the heads that share them, 32 at a time.  The
+// keys are operands in registers, the values, whose product comes once for both maps, in LDS.
 template <int D, int WAVES, int SLOTS>
-__global__ __launch_bounds__(64 * WAVES) void attention_dkv(mmuon_attention_args a, Dealing dealt, RowSpace space) {
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_dkv(mmuon_attention_args a, Dealing dealt, RowSpace space) {
   constexpr int CA = D / 8, CB = D / 4, TQ = 32;
   using T = Tile<D, TQ, WAVES>;
   constexpr int BYTES = T::BYTES + 1024;  // and the rows' statistics
   constexpr int LOADS = T::LOADS + 1;
   __shared__ __attribute__((aligned(1024))) char ring[SLOTS * BYTES];
+  __shared__ __attribute__((aligned(1024))) char values[WAVES * 32 * CB * 16];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int group, tile;  // the first keys are seen by the most queries: first
@@ -243,13 +247,21 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dkv(mmuon_attention_args
     dma16(uniform_ptr(stats), uint32_t(min(lane, a.queries - first - 1)) * 16, to + T::BYTES);
   };
 
-  bf16x8 k[2][D / 16], v[D / 8];
+  // a sequence without keys reads its first row; nothing of it is stored
+  const int last = max(span.keys, 1) - 1;
+  bf16x8 k[2][D / 16];
   {
-    const int at = min(key, max(span.keys, 1) - 1);
-    const uint16_t* p = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + at * a.k_stride[1] + 2 * g * a.k_stride[2];
+    const uint16_t* p = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + min(key, last) * a.k_stride[1] + 2 * g * a.k_stride[2];
     load_operands(p, a.dim, half, k[0]);
     load_operands(p + a.k_stride[2], a.dim, half, k[1]);
-    load_operands(static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + at * a.v_stride[1] + g * a.v_stride[2], 2 * a.dim, half, v);
+    const uint16_t* v = static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + g * a.v_stride[2];
+#pragma unroll
+    for (int i = 0; i < CB / 2; ++i) {  // the wave's own rows
+      const int r = (i * 64 + lane) / CB, c = min(((i * 64 + lane) % CB) ^ chunk_mask<CB>(r), src.b_last);
+      const int row = min(w0 + r, last) - min(w0, last);
+      dma16(uniform_ptr(v + min(w0, last) * a.v_stride[1]), uint32_t(row) * uint32_t(2 * a.v_stride[1]) + uint32_t(c) * 16,
+            lds_addr(values) + (wave * (CB / 2) + i) * 1024);
+    }
   }
   const float scale = a.scale * LOG2E;
   f32x16 dv[D / 16], dk[2][D / 32];
@@ -264,7 +276,15 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dkv(mmuon_attention_args
   for (int i = 0; i < SLOTS - 1; ++i)
     if (i < n) load(i);
   wait_loaded();
-  const uint32_t abase = row_base<CA>(lane), bbase = row_base<CB>(lane), ta = turned_base<CA>(lane), tb = turned_base<CB>(lane);
+  const uint32_t abase0 = row_base<CA>(lane), bbase0 = row_base<CB>(lane), ta0 = turned_base<CA>(lane), tb0 = turned_base<CB>(lane);
+  char* mine_v = values + wave * (CB / 2) * 1024;
+  if (a.dim < D) {  // columns that are not there: the other operand's repeat its last ones
+#pragma unroll
+    for (int i = 0; i < CB / 2; ++i) {
+      const int r = (i * 64 + lane) / CB, c = ((i * 64 + lane) % CB) ^ chunk_mask<CB>(r);
+      if (c > src.b_last) *reinterpret_cast<uint4*>(mine_v + (i * 64 + lane) * 16) = make_uint4(0, 0, 0, 0);
+    }
+  }
   int head = 0, first = from - TQ;
   for (int i = 0; i < n; ++i) {
     first += TQ;
@@ -275,37 +295,36 @@ __global__ __launch_bounds__(64 * WAVES) void attention_dkv(mmuon_attention_args
     if (i + SLOTS - 1 < n) load(i + SLOTS - 1);
     const char* tile_at = ring + (i % SLOTS) * BYTES;
     if (first + TQ <= mine) continue;  // no key of this wave is seen
+    const float4* stats = reinterpret_cast<const float4*>(tile_at + T::BYTES) + 4 * half;
+    const float lam = load_uniform(a.lam + int64_t(g * share + head) * a.lam_stride);
     f32x16 s[2] = {f32x16{}, f32x16{}}, dp = f32x16{};
+    const uint32_t abase = fresh(abase0), bbase = fresh(bbase0);
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       s[0] = mfma(read_rows<CA>(tile_at, abase, 0, kk), k[0][kk], s[0]);
       s[1] = mfma(read_rows<CA>(tile_at + T::A2, abase, 0, kk), k[1][kk], s[1]);
     }
 #pragma unroll
-    for (int kk = 0; kk < D / 8; ++kk) dp = mfma(read_rows<CB>(tile_at + T::B, bbase, 0, kk), v[kk], dp);
-    if (first < full || first + TQ > a.queries) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int t = first + 8 * (e / 4) + 4 * half + e % 4;
-        if (t < own || t >= a.queries) {
-          s[0][e] = s[1][e] = -INFINITY;
-          dp[e] = 0.f;
-        }
-      }
-    }
-    const float lam = load_uniform(a.lam + int64_t(g * share + head) * a.lam_stride);
-    const float4* stats = reinterpret_cast<const float4*>(tile_at + T::BYTES) + 4 * half;
+    for (int kk = 0; kk < D / 8; ++kk) dp = mfma(read_rows<CB>(tile_at + T::B, bbase, 0, kk), read_rows<CB>(mine_v, bbase, 0, kk), dp);
     float p[16], d1[16], d2[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const float4 st = stats[8 * (e / 4) + e % 4];
       const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][e], scale, -st.x));
-      const float p2 = __builtin_amdgcn_exp2f(fmaf(s[1][e], scale, -st.y)) * lam;
+      const float p2 = __builtin_amdgcn_exp2f(fmaf(s[1][e], scale, -st.z)) * lam;
       p[e] = p1 - p2;
-      d1[e] = p1 * (dp[e] - st.z);
+      d1[e] = p1 * (dp[e] - st.y);
       d2[e] = p2 * (st.w - dp[e]);
     }
+    if (first < full || first + TQ > a.queries) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int t = first + 8 * (e / 4) + 4 * half + e % 4;
+        if (t < own || t >= a.queries) p[e] = d1[e] = d2[e] = 0.f;
+      }
+    }
     const bf16x8 x[2] = {operand(p), operand(p + 8)}, x1[2] = {operand(d1), operand(d1 + 8)}, x2[2] = {operand(d2), operand(d2 + 8)};
+    const uint32_t ta = fresh(ta0), tb = fresh(tb0);
 #pragma unroll
     for (int j = 0; j < D / 16; ++j)
 #pragma unroll
@@ -345,16 +364,16 @@ void backward_dim(const mmuon_attention_args& a, hipStream_t s) {
   const int64_t groups = int64_t(a.batch) * a.kv_heads, share = a.heads / a.kv_heads;
   const RowSpace space = row_space(a);
   if (rows > 0) hipLaunchKernelGGL(attention_rows, dim3(unsigned((rows + 15) / 16)), dim3(256), 0, s, a, space);
+  constexpr int PAIRS = 4;
   if (a.dq != nullptr && rows > 0) {
-    constexpr int WAVES = 4;
-    const Dealing d = dealing(groups, (share * a.queries + 32 * WAVES - 1) / (32 * WAVES));
-    hipLaunchKernelGGL((attention_dq<D, WAVES, 3>), dim3(blocks_of(d)), dim3(64 * WAVES), 0, s, a, d, space);
+    const Dealing d = dealing(groups, (share * a.queries + 32 * PAIRS - 1) / (32 * PAIRS));
+    hipLaunchKernelGGL((attention_dq<D, PAIRS, 3>), dim3(blocks_of(d)), dim3(128 * PAIRS), 0, s, a, d, space);
   }
   if (a.dlam != nullptr && a.heads > 0) hipLaunchKernelGGL(attention_dlam, dim3(unsigned(a.heads)), dim3(1024), 0, s, a, space);
   if (a.dk != nullptr && groups > 0 && a.keys > 0) {
-    constexpr int WAVES = 4;
+    constexpr int WAVES = D == 128 ? 4 : 8;
     const Dealing d = dealing(groups, (a.keys + 32 * WAVES - 1) / (32 * WAVES));
-    hipLaunchKernelGGL((attention_dkv<D, WAVES, 3>), dim3(blocks_of(d)), dim3(64 * WAVES), 0, s, a, d, space);
+    hipLaunchKernelGGL((attention_dkv<D, WAVES, (D == 128 ? 2 : 3)>), dim3(blocks_of(d)), dim3(64 * WAVES), 0, s, a, d, space);
   }
 }
 

@@ -92,6 +92,13 @@ __device__ __forceinline__ float load_uniform(const float* p) {
   return *(const __attribute__((address_space(4))) float*)(uintptr_t)p;
 }
 
+// A value that the compiler takes for new: what is formed from it is formed here, not before the loop,
+// where it would hold registers.
+__device__ __forceinline__ uint32_t fresh(uint32_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 // Where a tile's rows come from
 struct TileSource {
   const char* a1;  // the tile's first row in each matrix
@@ -128,12 +135,13 @@ struct Tile {
   }
 };
 
-// A row of `dim` columns (a multiple of 8) as operands: columns 16 kk + 8 (lane / 32) + [0, 8), zeros behind the last
+// A row of `dim` columns (a multiple of 8) as operands: columns first + 16 kk + 8 (lane / 32) + [0, 8), zeros
+// behind the last
 template <int N>
-__device__ __forceinline__ void load_operands(const uint16_t* row, int dim, int half, bf16x8 (&v)[N]) {
+__device__ __forceinline__ void load_operands(const uint16_t* row, int dim, int half, bf16x8 (&v)[N], int first = 0) {
 #pragma unroll
   for (int kk = 0; kk < N; ++kk) {
-    const int col = 16 * kk + 8 * half;
+    const int col = first + 16 * kk + 8 * half;
     v[kk] = bf16x8{};
     if (col < dim) v[kk] = *reinterpret_cast<const bf16x8*>(row + col);
   }
