@@ -76,19 +76,19 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void attend(mmuon_a
   }
 
   const char* k1 = static_cast<const char*>(a.k) + 2 * (b * a.k_stride[0] + 2 * g * a.k_stride[2]);
-  TileSource src;
+  TileRows src;
   src.a_stride = uint32_t(2 * a.k_stride[1]);
   src.b_stride = uint32_t(2 * a.v_stride[1]);
   src.a_last = a.dim / 8 - 1;
   src.b_last = a.dim / 4 - 1;
   const char* v0 = static_cast<const char*>(a.v) + 2 * (b * a.v_stride[0] + g * a.v_stride[2]);
   const uint32_t lds = lds_addr(ring);
+  uint32_t off[T::LOADS];
+  T::offsets(src, wave, lane, off);
   const auto load = [&](int i) {  // the i-th of this workgroup's tiles
     const int64_t first = int64_t(t0 + i) * TK;
-    src.a1 = k1 + 2 * first * a.k_stride[1];
-    src.a2 = src.a1 + 2 * a.k_stride[2];
-    src.b = v0 + 2 * first * a.v_stride[1];
-    T::load(lds + (i % SLOTS) * T::BYTES, src, span.keys - int(first), wave, lane);
+    const char* k = k1 + 2 * first * a.k_stride[1];
+    T::load(lds + (i % SLOTS) * T::BYTES, k, k + 2 * a.k_stride[2], v0 + 2 * first * a.v_stride[1], src, off, span.keys - int(first), wave, lane);
   };
 
   bf16x8 q[MAPS][D / 16];

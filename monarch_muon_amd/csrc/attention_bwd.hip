@@ -10,11 +10,10 @@
 // rounded to bf16, are the next products' operands as they stand.  dlam takes P_2 dP in fp32 as dq's
 // kernel has them: o_2, from rounded probabilities, would give it their error.
 //
-// Two waves are a pair: each has one map's scores, half of dP's sum over the columns, and half of dv's
-// columns; the halves of dP, and the probabilities that dv needs of both maps, pass through LDS.  So no
-// product is made twice, and the sums leave room for two waves of registers on a SIMD, whose products
-// and exponentials run side by side.  (One wave for both maps, one to a SIMD: 16 x 1024 tokens, 8 heads
-// of 2 x 64, dk and dv 188 us; 4 x 1024, 16 heads of 2 x 128, dq 100, dk and dv 226.)
+// Both kernels have both maps in a wave, which makes no product twice.  With heads of up to 64 columns
+// two waves fit a SIMD, whose products and exponentials run side by side; with more a wave's sums for dk
+// and dv alone are half of its registers.  (A map to each of two waves that pass dP and P through LDS:
+// 16 x 1024 tokens, 8 heads of 2 x 64, dq 123 us, dk and dv 186; 4 x 1024, 16 of 2 x 128, 92 and 210.)
 #include <algorithm>
 
 #include "attention_tile.hpp"
@@ -57,27 +56,26 @@ __global__ __launch_bounds__(256) void attention_rows(mmuon_attention_args a, Ro
   if (lane == 0) space.stats[row] = make_float4(a.lse[2 * row], d1, a.lse[2 * row + 1], d2);
 }
 
-// dq and each row's part of dlam: 32 queries to a pair, over tiles of 32 keys
-template <int D, int PAIRS, int SLOTS>
-__global__ __launch_bounds__(128 * PAIRS, 2) void attention_dq(mmuon_attention_args a, Dealing dealt, RowSpace space) {
+// dq and each row's part of dlam: 32 queries to a wave, over tiles of 32 keys
+template <int D, int WAVES, int SLOTS>
+__global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmuon_attention_args a, Dealing dealt, RowSpace space) {
   constexpr int CA = D / 8, CB = D / 4, TK = 32;
-  using T = Tile<D, TK, 2 * PAIRS>;
+  using T = Tile<D, TK, WAVES>;
   __shared__ __attribute__((aligned(1024))) char ring[SLOTS * T::BYTES];
-  __shared__ float4 passed[2 * PAIRS][4][64];
   const int lane = threadIdx.x & 63, half = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = wave & 1;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int group, item;
   if (!deal(dealt, a.batch * a.kv_heads, group, item)) return;
   const int tile = dealt.each - 1 - item;
   const int b = group / a.kv_heads, g = group % a.kv_heads, share = a.heads / a.kv_heads;
-  const int rows = share * a.queries, r0 = tile * 32 * PAIRS;
+  const int rows = share * a.queries, r0 = tile * 32 * WAVES;
   const Span span = span_of(a, b);
   const auto most_of = [&](int first, int n) {
     if (first >= rows) return 0;
     return seen(a, span, (min(first + n, rows) - 1) / share);
   };
-  const int w0 = r0 + 32 * (wave >> 1);
-  const int keys = most_of(r0, 32 * PAIRS), mine = most_of(w0, 32);
+  const int w0 = r0 + 32 * wave;
+  const int keys = most_of(r0, 32 * WAVES), mine = most_of(w0, 32);
   const int row = w0 + (lane & 31);
   const bool in = row < rows;
   const int t = (in ? row : rows - 1) / share, h = g * share + (in ? row : rows - 1) - t * share;
@@ -89,30 +87,35 @@ __global__ __launch_bounds__(128 * PAIRS, 2) void attention_dq(mmuon_attention_a
 
   const char* k1 = static_cast<const char*>(a.k) + 2 * (b * a.k_stride[0] + 2 * g * a.k_stride[2]);
   const char* v0 = static_cast<const char*>(a.v) + 2 * (b * a.v_stride[0] + g * a.v_stride[2]);
-  TileSource src;
+  TileRows src;
   src.a_stride = uint32_t(2 * a.k_stride[1]);
   src.b_stride = uint32_t(2 * a.v_stride[1]);
   src.a_last = a.dim / 8 - 1;
   src.b_last = a.dim / 4 - 1;
   const uint32_t lds = lds_addr(ring);
+  uint32_t off[T::LOADS];
+  T::offsets(src, wave, lane, off);
   const auto load = [&](int i) {
     const int64_t first = int64_t(i) * TK;
-    src.a1 = k1 + 2 * first * a.k_stride[1];
-    src.a2 = src.a1 + 2 * a.k_stride[2];
-    src.b = v0 + 2 * first * a.v_stride[1];
-    T::load(lds + (i % SLOTS) * T::BYTES, src, span.keys - int(first), wave, lane);
+    const char* k = k1 + 2 * first * a.k_stride[1];
+    T::load(lds + (i % SLOTS) * T::BYTES, k, k + 2 * a.k_stride[2], v0 + 2 * first * a.v_stride[1], src, off, span.keys - int(first), wave, lane);
   };
 
-  bf16x8 q[D / 16], dout[D / 16];
-  load_operands(static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + (2 * h + m) * a.q_stride[2], a.dim, half, q);
-  load_operands(static_cast<const uint16_t*>(a.dout) + ((int64_t(b) * a.queries + t) * a.heads + h) * 2 * a.dim, 2 * a.dim, half, dout,
-                m * D);
+  bf16x8 q[2][D / 16], dout[D / 8];
+  {
+    const uint16_t* p = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + 2 * h * a.q_stride[2];
+    load_operands(p, a.dim, half, q[0]);
+    load_operands(p + a.q_stride[2], a.dim, half, q[1]);
+    load_operands(static_cast<const uint16_t*>(a.dout) + ((int64_t(b) * a.queries + t) * a.heads + h) * 2 * a.dim, 2 * a.dim, half, dout);
+  }
   const int64_t at = (int64_t(b) * a.heads + h) * a.queries + t;
-  const float2 st = reinterpret_cast<const float2*>(space.stats + at)[m];
+  const float4 st = space.stats[at];
   const float scale = a.scale * LOG2E;
-  f32x16 acc[D / 32];
+  f32x16 acc[2][D / 32];
 #pragma unroll
-  for (int j = 0; j < D / 32; ++j) acc[j] = f32x16{};
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) acc[m][j] = f32x16{};
   float along = 0.f;
 
   const int n = (keys + TK - 1) / TK;
@@ -120,62 +123,66 @@ __global__ __launch_bounds__(128 * PAIRS, 2) void attention_dq(mmuon_attention_a
   for (int i = 0; i < SLOTS - 1; ++i)
     if (i < n) load(i);
   wait_loaded();
-  const uint32_t kbase = row_base<CA>(lane), vbase = row_base<CB>(lane) ^ uint32_t(m * 2 * D), tbase = turned_base<CA>(lane);
+  const uint32_t kbase0 = row_base<CA>(lane), vbase0 = row_base<CB>(lane), tbase0 = turned_base<CA>(lane);
   for (int i = 0; i < n; ++i) {
     if (i + SLOTS - 2 < n) wait_vm<(SLOTS - 2) * T::LOADS>();
     else wait_vm<0>();
     barrier_after_lds_writes();
     if (i + SLOTS - 1 < n) load(i + SLOTS - 1);
     const char* tile_at = ring + (i % SLOTS) * T::BYTES;
-    const bool active = i * TK < mine;  // the pair's
-    f32x16 dp = f32x16{};
-    float p[16];
-    if (active) {
-      f32x16 s = f32x16{};
+    if (i * TK >= mine) continue;
+    const uint32_t kbase = fresh(kbase0), vbase = fresh(vbase0), tbase = fresh(tbase0);
+    f32x16 s[2] = {f32x16{}, f32x16{}}, dp = f32x16{};
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) dp = mfma(read_rows<CB>(tile_at + T::B, vbase, 0, kk), dout[kk], dp);
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) s = mfma(read_rows<CA>(tile_at + m * T::A2, kbase, 0, kk), q[kk], s);
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) passed[wave][e / 4][lane] = make_float4(dp[e], dp[e + 1], dp[e + 2], dp[e + 3]);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], scale, -st.x));
-    }
-    barrier_after_lds_writes();
-    if (!active) continue;
-    float d[16];
-#pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      const float4 x = passed[wave ^ 1][e / 4][lane];
-      dp[e] += x.x, dp[e + 1] += x.y, dp[e + 2] += x.z, dp[e + 3] += x.w;
+    for (int kk = 0; kk < D / 16; ++kk) {
+      s[0] = mfma(read_rows<CA>(tile_at, kbase, 0, kk), q[0][kk], s[0]);
+      s[1] = mfma(read_rows<CA>(tile_at + T::A2, kbase, 0, kk), q[1][kk], s[1]);
     }
     if (i * TK + TK > fewest) {
       const int left = limit - i * TK - 4 * half;
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        if (8 * (e / 4) + e % 4 >= left) p[e] = dp[e] = 0.f;
+        if (8 * (e / 4) + e % 4 >= left) s[0][e] = s[1][e] = -INFINITY;
     }
 #pragma unroll
+    for (int kk = 0; kk < D / 8; ++kk) dp = mfma(read_rows<CB>(tile_at + T::B, vbase, 0, kk), dout[kk], dp);
+    float d1[16], d2[16];
+#pragma unroll
     for (int e = 0; e < 16; ++e) {
-      along = fmaf(p[e], dp[e], along);
-      d[e] = p[e] * (dp[e] - st.y);
+      d1[e] = __builtin_amdgcn_exp2f(fmaf(s[0][e], scale, -st.x));
+      d2[e] = __builtin_amdgcn_exp2f(fmaf(s[1][e], scale, -st.z));
     }
-    const bf16x8 x[2] = {operand(d), operand(d + 8)};
+#pragma unroll
+    for (int e = 0; e < 16; ++e) d1[e] *= dp[e] - st.y;
+    const bf16x8 x1[2] = {operand(d1), operand(d1 + 8)};
 #pragma unroll
     for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-      for (int y = 0; y < 2; ++y) acc[j] = mfma(read_turned<CA>(tile_at + m * T::A2, tbase, 16 * y, j), x[y], acc[j]);
+      for (int y = 0; y < 2; ++y) acc[0][j] = mfma(read_turned<CA>(tile_at, tbase, 16 * y, j), x1[y], acc[0][j]);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      along = fmaf(d2[e], dp[e], along);
+      d2[e] *= dp[e] - st.w;
+    }
+    const bf16x8 x2[2] = {operand(d2), operand(d2 + 8)};
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) acc[1][j] = mfma(read_turned<CA>(tile_at + T::A2, tbase, 16 * y, j), x2[y], acc[1][j]);
   }
   const float lam = a.lam[int64_t(h) * a.lam_stride];
   along = half_sum(along);
-  if (m == 1 && in && half == 0) space.dlam[at] = -along;
-  uint16_t* dq = in ? static_cast<uint16_t*>(a.dq) + ((int64_t(b) * a.queries + t) * 2 * a.heads + 2 * h + m) * a.dim : nullptr;
-  const float by = m ? -(lam * a.scale) : a.scale;
+  if (in && half == 0) space.dlam[at] = -along;
+  uint16_t* dq = in ? static_cast<uint16_t*>(a.dq) + ((int64_t(b) * a.queries + t) * 2 * a.heads + 2 * h) * a.dim : nullptr;
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[j][e] *= by;
-    store_turned(dq, acc[j], j, a.dim, half);
+    for (int e = 0; e < 16; ++e) {
+      acc[0][j][e] *= a.scale;
+      acc[1][j][e] *= -(lam * a.scale);
+    }
+    store_turned(dq, acc[0][j], j, a.dim, half);
+    store_turned(dq != nullptr ? dq + a.dim : nullptr, acc[1][j], j, a.dim, half);
   }
 }
 
@@ -198,7 +205,7 @@ __global__ __launch_bounds__(1024) void attention_dlam(mmuon_attention_args a, R
 // dk and dv: 32 keys to a wave, over the query rows of the heads that share them, 32 at a time.  The
 // keys are operands in registers, the values, whose product comes once for both maps, in LDS.
 template <int D, int WAVES, int SLOTS>
-__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_dkv(mmuon_attention_args a, Dealing dealt, RowSpace space) {
+__global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mmuon_attention_args a, Dealing dealt, RowSpace space) {
   constexpr int CA = D / 8, CB = D / 4, TQ = 32;
   using T = Tile<D, TQ, WAVES>;
   constexpr int BYTES = T::BYTES + 1024;  // and the rows' statistics
@@ -226,22 +233,22 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attention_dkv(mmuon_att
 
   const char* q1 = static_cast<const char*>(a.q) + 2 * (b * a.q_stride[0] + 2 * g * share * a.q_stride[2]);
   const char* g0 = static_cast<const char*>(a.dout) + 2 * (int64_t(b) * a.queries * a.heads + g * share) * 2 * a.dim;
-  TileSource src;
+  TileRows src;
   src.a_stride = uint32_t(2 * a.q_stride[1]);
   src.b_stride = uint32_t(2) * a.heads * 2 * a.dim;
   src.a_last = a.dim / 8 - 1;
   src.b_last = a.dim / 4 - 1;
   const uint32_t lds = lds_addr(ring);
+  uint32_t off[T::LOADS];
+  T::offsets(src, wave, lane, off);
   int next_head = 0, next_first = from;  // of the tile that is loaded next
   const auto load = [&](int i) {
     const int head = next_head, first = next_first;
     next_first += TQ;
     if (next_first >= a.queries) next_first = from, ++next_head;
-    src.a1 = q1 + 2 * (2 * head * a.q_stride[2] + first * a.q_stride[1]);
-    src.a2 = src.a1 + 2 * a.q_stride[2];
-    src.b = g0 + 2 * (int64_t(first) * a.heads + head) * 2 * a.dim;
+    const char* q = q1 + 2 * (2 * head * a.q_stride[2] + first * a.q_stride[1]);
     const uint32_t to = lds + (i % SLOTS) * BYTES;
-    T::load(to, src, a.queries - first, wave, lane);
+    T::load(to, q, q + 2 * a.q_stride[2], g0 + 2 * (int64_t(first) * a.heads + head) * 2 * a.dim, src, off, a.queries - first, wave, lane);
     // (every wave loads them, so that each has as many loads)
     const float4* stats = space.stats + (int64_t(b) * a.heads + g * share + head) * a.queries + first;
     dma16(uniform_ptr(stats), uint32_t(min(lane, a.queries - first - 1)) * 16, to + T::BYTES);
@@ -364,16 +371,16 @@ void backward_dim(const mmuon_attention_args& a, hipStream_t s) {
   const int64_t groups = int64_t(a.batch) * a.kv_heads, share = a.heads / a.kv_heads;
   const RowSpace space = row_space(a);
   if (rows > 0) hipLaunchKernelGGL(attention_rows, dim3(unsigned((rows + 15) / 16)), dim3(256), 0, s, a, space);
-  constexpr int PAIRS = 4;
   if (a.dq != nullptr && rows > 0) {
-    const Dealing d = dealing(groups, (share * a.queries + 32 * PAIRS - 1) / (32 * PAIRS));
-    hipLaunchKernelGGL((attention_dq<D, PAIRS, 3>), dim3(blocks_of(d)), dim3(128 * PAIRS), 0, s, a, d, space);
+    constexpr int WAVES = 4;
+    const Dealing d = dealing(groups, (share * a.queries + 32 * WAVES - 1) / (32 * WAVES));
+    hipLaunchKernelGGL((attention_dq<D, WAVES, 3>), dim3(blocks_of(d)), dim3(64 * WAVES), 0, s, a, d, space);
   }
   if (a.dlam != nullptr && a.heads > 0) hipLaunchKernelGGL(attention_dlam, dim3(unsigned(a.heads)), dim3(1024), 0, s, a, space);
   if (a.dk != nullptr && groups > 0 && a.keys > 0) {
-    constexpr int WAVES = D == 128 ? 4 : 8;
+    constexpr int WAVES = 4;
     const Dealing d = dealing(groups, (a.keys + 32 * WAVES - 1) / (32 * WAVES));
-    hipLaunchKernelGGL((attention_dkv<D, WAVES, (D == 128 ? 2 : 3)>), dim3(blocks_of(d)), dim3(64 * WAVES), 0, s, a, d, space);
+    hipLaunchKernelGGL((attention_dkv<D, WAVES, 2>), dim3(blocks_of(d)), dim3(64 * WAVES), 0, s, a, d, space);
   }
 }
 

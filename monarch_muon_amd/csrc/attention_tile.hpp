@@ -99,11 +99,8 @@ __device__ __forceinline__ uint32_t fresh(uint32_t v) {
   return v;
 }
 
-// Where a tile's rows come from
-struct TileSource {
-  const char* a1;  // the tile's first row in each matrix
-  const char* a2;
-  const char* b;
+// A tile's rows: of both kinds of matrix
+struct TileRows {
   uint32_t a_stride, b_stride;  // bytes from one row to the next
   int a_last, b_last;           // the last chunk of a row that is there
 };
@@ -116,21 +113,30 @@ struct Tile {
   static constexpr int A2 = ROWS * CA * 16, B = 2 * A2, BYTES = 4 * A2;
   static_assert((2 * NA + NB) % WAVES == 0, "each wave has as many loads");
 
-  // Rows from `left` on repeat the last one there, and chunks a row does not have its last: what is
-  // read is always there, and what comes of it is masked, multiplied by zeros or not stored.
-  static __device__ __forceinline__ void load(uint32_t lds, const TileSource& s, int left, int wave, int lane) {
+  // A wave's k-th load fills 1 KiB: its matrix, where in the tile, and each lane's offset in the
+  // matrix's rows.  Rows from `left` on repeat the last one there, and chunks a row does not have its
+  // last: what is read is always there, and what comes of it is masked, multiplied by zeros or not stored.
+  static __device__ __forceinline__ uint32_t offset(const TileRows& s, int n, int lane, int left) {
+    if (n < 2 * NA) {
+      const int at = (n >= NA ? n - NA : n) * 64 + lane, r = at / CA, c = min((at % CA) ^ chunk_mask<CA>(r), s.a_last);
+      return uint32_t(min(r, left - 1)) * s.a_stride + uint32_t(c) * 16;
+    }
+    const int at = (n - 2 * NA) * 64 + lane, r = at / CB, c = min((at % CB) ^ chunk_mask<CB>(r), s.b_last);
+    return uint32_t(min(r, left - 1)) * s.b_stride + uint32_t(c) * 16;
+  }
+  // (of whole tiles: made once, so that a load in the loop is a load and little else)
+  static __device__ __forceinline__ void offsets(const TileRows& s, int wave, int lane, uint32_t (&off)[LOADS]) {
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) off[k] = offset(s, wave + WAVES * k, lane, ROWS);
+  }
+  // a1, a2, b: the tile's first row in each matrix (values: a select between members of a struct goes through memory)
+  static __device__ __forceinline__ void load(uint32_t lds, const char* a1, const char* a2, const char* b, const TileRows& s,
+                                              const uint32_t (&off)[LOADS], int left, int wave, int lane) {
 #pragma unroll
     for (int k = 0; k < LOADS; ++k) {
       const int n = wave + WAVES * k;
-      if (n < 2 * NA) {
-        const int m = n >= NA ? 1 : 0, at = (n - m * NA) * 64 + lane;
-        const int r = at / CA, c = min((at % CA) ^ chunk_mask<CA>(r), s.a_last);
-        dma16(uniform_ptr(m ? s.a2 : s.a1), uint32_t(min(r, left - 1)) * s.a_stride + uint32_t(c) * 16, lds + m * A2 + (n - m * NA) * 1024);
-      } else {
-        const int at = (n - 2 * NA) * 64 + lane;
-        const int r = at / CB, c = min((at % CB) ^ chunk_mask<CB>(r), s.b_last);
-        dma16(uniform_ptr(s.b), uint32_t(min(r, left - 1)) * s.b_stride + uint32_t(c) * 16, lds + B + (n - 2 * NA) * 1024);
-      }
+      const char* from = uniform_ptr(n < NA ? a1 : n < 2 * NA ? a2 : b);
+      dma16(from, left >= ROWS ? off[k] : offset(s, n, lane, left), lds + n * 1024);
     }
   }
 };

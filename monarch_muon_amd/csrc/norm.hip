@@ -31,22 +31,24 @@ __device__ __forceinline__ void load_weight<F32T>(const mmuon_norm_args& a, int 
   load_chunk<F32T>(static_cast<const float*>(a.w) + col, left, v);
 }
 
-// A scale of 0, of values that are 0 or too small to have one, would be divided by
+// A scale that is no normal number, of values that are 0 or next to it, has no reciprocal.
 template <class F>
 __device__ __forceinline__ float code_scale(float most) {
   const float scale = most / F::MAX;
-  return scale > 0.f ? scale : 1.f;
+  return scale < 0x1p-126f ? 1.f : scale;
 }
 
+// y / scale as y (1 / scale): two roundings of 2^-24, where the code's own is 2^-4 or 2^-3
 template <class F, int N>
 __device__ __forceinline__ void store_codes(uint8_t* p, const float (&y)[N], float scale, int left) {
   uint32_t code[N / 4];
+  const float by = 1.f / scale;
 #pragma unroll
   for (int k = 0; k < N; k += 4) {
     float z[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      z[e] = y[k + e] / scale;
+      z[e] = y[k + e] * by;
       if (fabsf(z[e]) > F::MAX) z[e] = copysignf(F::MAX, z[e]);  // (a NaN stays one)
     }
     code[k / 4] = encode4<F>(z);
@@ -240,21 +242,26 @@ __global__ __launch_bounds__(1024) void norm_join(mmuon_norm_args a, int parts) 
   else static_cast<uint16_t*>(a.dw)[col] = f2bf(s);
 }
 
+// Lanes of a row and chunks of a lane.  Two chunks to a lane, or one where the rows are too few to fill
+// the chip's threads (2048 to a CU): many waves with little in flight each hide one another's latency
+// better than few with much.  16384 x 4096 in bf16 with a residual, 1, 2, 4 and 8 chunks: gradient 120,
+// 117, 147 and 221 us (512 MiB: 4.6 TB/s at best); forward, 2, 4 and 8: 85, 86 and 97 us (6.3 TB/s); 8-bit
+// output of 4096 x 4096: 23.3, 24.1 and 30 us (5.1 TB/s).  Rows of over 8192 bf16 columns take 4 and 8.
+constexpr int64_t FILL = 524288;
+constexpr int GRAD_BLOCK = 512;
 struct RowPlan {
-  int lanes, chunks;  // lanes of a row, chunks of a lane (1, 2, 4 or 8)
+  int lanes, chunks;
 };
-// One wave to a row where there are rows enough to fill the chip so, else as many lanes as the
-// row has chunks.
 RowPlan row_plan(int64_t rows, int width, int columns) {
   const int all = (width + columns - 1) / columns;
   int most = 1;
   while (most < all && most < 512) most *= 2;
   int lanes = std::min(most, 64);
-  while (lanes < 512 && lanes * 8 < all) lanes *= 2;
-  while (lanes < most && rows * lanes < 131072) lanes *= 2;
-  int chunks = 1;
-  while (chunks * lanes < all) chunks *= 2;
-  return {lanes, chunks};
+  while (lanes < 512 && lanes * 2 < all) lanes *= 2;
+  while (lanes < most && rows * lanes < FILL) lanes *= 2;
+  RowPlan p{lanes, 1};
+  while (p.chunks * lanes < all) p.chunks *= 2;
+  return p;
 }
 
 template <class T, int CPT, int OUT>
@@ -281,17 +288,16 @@ void norm_forward(const mmuon_norm_args& a, hipStream_t s) {
   else norm_forward<T, MMUON_BF16>(a, s);
 }
 
-// Workgroups of the gradient: each leaves a row of sums
+// Workgroups of the gradient: each leaves a row of sums.  Two to a CU, which their registers allow; a third
+// would wait for one of them (768: 132 us in place of 117), and 1024 leave twice the sums.
 int grad_parts(const mmuon_norm_args& a, int lanes) {
-  const int each = std::max(lanes, 256) / lanes;
+  const int each = GRAD_BLOCK / lanes;
   return int(std::min<int64_t>((a.rows + each - 1) / each, 512));
 }
 template <class T, int CPT>
 void grad_launch(const mmuon_norm_args& a, int lanes, hipStream_t s) {
-  const dim3 grid(unsigned(grad_parts(a, lanes)));
-  const size_t shared = lanes < 256 ? size_t(a.width) * 4 : 0;
-  if (lanes <= 256) hipLaunchKernelGGL((norm_grad<T, CPT, 256>), grid, dim3(256), shared, s, a, lanes);
-  else hipLaunchKernelGGL((norm_grad<T, CPT, 512>), grid, dim3(lanes), 0, s, a, lanes);
+  const size_t shared = lanes < GRAD_BLOCK ? size_t(a.width) * 4 : 0;
+  hipLaunchKernelGGL((norm_grad<T, CPT, GRAD_BLOCK>), dim3(unsigned(grad_parts(a, lanes))), dim3(GRAD_BLOCK), shared, s, a, lanes);
 }
 template <class T>
 void norm_backward(const mmuon_norm_args& a, hipStream_t s) {
