@@ -4,8 +4,9 @@
 //
 // One pass over the keys with a running reference and sum for each map.  A wave has 32 queries and
 // both maps, so that a value read from LDS serves two products; with heads of over 64 columns, whose
-// sums for both maps would be all of a SIMD's registers, two waves have a map each and join them at
-// the end (two waves to a SIMD either way, one's exponentials beside the other's products).  Scores are made transposed
+// sums for both maps would be all of a SIMD's registers, and where there are few rows, two waves have a
+// map each and join them at the end (two waves to a SIMD, one's exponentials beside the other's products;
+// 3 x 1001 tokens, 6 heads of 2 x 64: one wave for both maps 63 us, a pair 40).  Scores are made transposed
 // (keys x queries): a lane's values all belong to one query, the row's statistics are the lane's own
 // but for one exchange between the half-waves, and the probabilities are the next product's operand as
 // they stand.  The reference moves only where a score exceeds it by 2^8: what is exact needs no
@@ -257,81 +258,95 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void attend(mmuon_a
   }
 }
 
-// The parts of a row's keys: four waves take every fourth part each, and their sums are added in order.
-template <int D>
-__global__ __launch_bounds__(256) void attend_join(mmuon_attention_args a, int splits, Parts parts) {
-  constexpr int N = D / 32;  // columns of a lane, of each map
-  __shared__ float4 found[4];
-  __shared__ float sums[4][2][2 * D];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// The parts of a row's keys, joined by WAVES waves: each part's factor first, then the sums of every
+// WAVES-th part to a wave, which are added in order.
+constexpr int JOIN = 8;            // waves of a workgroup
+constexpr int ALONE_PARTS = 16;    // parts that a wave joins alone
+constexpr int MOST_PARTS = 1024;
+template <int D, int WAVES>
+__global__ __launch_bounds__(64 * JOIN) void attend_join(mmuon_attention_args a, int splits, Parts parts) {
+  constexpr int N = D / 32, ROWS = JOIN / WAVES;  // columns of a lane, of each map; rows of a workgroup
+  __shared__ float2 by[ROWS][WAVES == 1 ? ALONE_PARTS : MOST_PARTS];
+  __shared__ float found[2][JOIN];
+  __shared__ float4 total[JOIN];
+  __shared__ float sums[JOIN][2][2 * D];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part0 = wave % WAVES, mine = wave / WAVES;
   const int share = a.heads / a.kv_heads, rows = share * a.queries;
-  const int group = blockIdx.x / rows, row = blockIdx.x % rows;
+  const int64_t all = int64_t(a.batch) * a.kv_heads * rows, id = int64_t(blockIdx.x) * ROWS + mine;
+  const bool in = id < all;  // (a workgroup's waves meet at barriers)
+  const int group = int((in ? id : 0) / rows), row = int((in ? id : 0) - int64_t(group) * rows);
   const int64_t at = int64_t(group) * splits * rows + row;
-  // the parts' largest reference
-  float top1 = -INFINITY, top2 = -INFINITY;
   const float4* stats = parts.stats + 2 * at;
-  for (int p = threadIdx.x; p < splits; p += 256) {
+  const int step = 64 * WAVES, first = part0 * 64 + lane;
+  float top1 = -INFINITY, top2 = -INFINITY;
+  for (int p = first; p < splits; p += step) {
     const float4 s1 = stats[int64_t(p) * 2 * rows], s2 = stats[int64_t(p) * 2 * rows + 1];
     if (s1.y != 0.f) top1 = fmaxf(top1, s1.x);
     if (s2.y != 0.f) top2 = fmaxf(top2, s2.x);
   }
   top1 = wave_max(top1);
   top2 = wave_max(top2);
-  if (lane == 0) found[wave] = make_float4(top1, top2, 0.f, 0.f);
-  __syncthreads();
+  if constexpr (WAVES > 1) {
+    if (lane == 0) found[0][wave] = top1, found[1][wave] = top2;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    top1 = fmaxf(top1, found[w].x);
-    top2 = fmaxf(top2, found[w].y);
+    for (int w = 0; w < JOIN; ++w) top1 = fmaxf(top1, found[0][w]), top2 = fmaxf(top2, found[1][w]);
   }
-  float l1 = 0.f, l2 = 0.f, n1 = 0.f, n2 = 0.f, x1[N] = {}, x2[N] = {};
-#pragma unroll 4
-  for (int p = wave; p < splits; p += 4) {
+  float l1 = 0.f, l2 = 0.f, n1 = 0.f, n2 = 0.f;
+  for (int p = first; p < splits; p += step) {
     const float4 s1 = stats[int64_t(p) * 2 * rows], s2 = stats[int64_t(p) * 2 * rows + 1];
-    const float* from = parts.sums + (at + int64_t(p) * rows) * (4 * D) + lane * N;
-    if (s1.y != 0.f) {
-      const float w = __builtin_amdgcn_exp2f(s1.x - top1);
-      l1 = fmaf(s1.y, w, l1);
-      n1 = fmaf(s1.z, w, n1);
+    const float2 w = make_float2(s1.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(s1.x - top1),
+                                 s2.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(s2.x - top2));
+    by[mine][p] = w;
+    if (s1.y != 0.f) l1 = fmaf(s1.y, w.x, l1), n1 = fmaf(s1.z, w.x, n1);
+    if (s2.y != 0.f) l2 = fmaf(s2.y, w.y, l2), n2 = fmaf(s2.z, w.y, n2);
+  }
+  l1 = wave_sum(l1), l2 = wave_sum(l2), n1 = wave_sum(n1), n2 = wave_sum(n2);
+  if (lane == 0) total[wave] = make_float4(l1, l2, n1, n2);
+  __syncthreads();
+  float x1[N] = {}, x2[N] = {};
+  const float* from = parts.sums + at * (4 * D) + lane * N;
+#pragma unroll 8
+  for (int p = part0; p < splits; p += WAVES) {
+    const float2 w = by[mine][p];
+    const float* y = from + int64_t(p) * rows * (4 * D);
 #pragma unroll
-      for (int k = 0; k < N; ++k) x1[k] = fmaf(from[k], w, x1[k]);
-    }
-    if (s2.y != 0.f) {
-      const float w = __builtin_amdgcn_exp2f(s2.x - top2);
-      l2 = fmaf(s2.y, w, l2);
-      n2 = fmaf(s2.z, w, n2);
-#pragma unroll
-      for (int k = 0; k < N; ++k) x2[k] = fmaf(from[2 * D + k], w, x2[k]);
+    for (int k = 0; k < N; ++k) {  // (what a part did not write counts for nothing, whatever it holds)
+      const float y1 = y[k], y2 = y[2 * D + k];
+      x1[k] = fmaf(w.x == 0.f ? 0.f : y1, w.x, x1[k]);
+      x2[k] = fmaf(w.y == 0.f ? 0.f : y2, w.y, x2[k]);
     }
   }
-  __syncthreads();
-  if (lane == 0) found[wave] = make_float4(l1, l2, n1, n2);
+  if constexpr (WAVES > 1) {
+    l1 = l2 = n1 = n2 = 0.f;
+#pragma unroll
+    for (int w = 0; w < JOIN; ++w) l1 += total[w].x, l2 += total[w].y, n1 += total[w].z, n2 += total[w].w;
+  }
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     sums[wave][0][lane * N + k] = x1[k];
     sums[wave][1][lane * N + k] = x2[k];
   }
   __syncthreads();
-  l1 = found[0].x + found[1].x + found[2].x + found[3].x;
-  l2 = found[0].y + found[1].y + found[2].y + found[3].y;
-  n1 = found[0].z + found[1].z + found[2].z + found[3].z;
-  n2 = found[0].w + found[1].w + found[2].w + found[3].w;
   const int b = group / a.kv_heads, g = group % a.kv_heads;
   const int t = row / share, h = g * share + row - t * share;
   const float lam = a.lam[int64_t(h) * a.lam_stride];
   const float i1 = n1 == 0.f ? 0.f : 1.f / n1, i2 = n2 == 0.f ? 0.f : 1.f / n2;
   const int64_t to = ((int64_t(b) * a.queries + t) * a.heads + h) * 2 * a.dim;
-  const int c = threadIdx.x;
-  if (c < 2 * a.dim) {
-    const float y1 = (sums[0][0][c] + sums[1][0][c] + sums[2][0][c] + sums[3][0][c]) * i1;
-    const float y2 = (sums[0][1][c] + sums[1][1][c] + sums[2][1][c] + sums[3][1][c]) * i2;
+  if (!in) return;
+  for (int c = part0 * 64 + lane; c < 2 * a.dim; c += 64 * WAVES) {
+    float y1 = 0.f, y2 = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) y1 += sums[mine * WAVES + w][0][c], y2 += sums[mine * WAVES + w][1][c];
+    y1 *= i1;
+    y2 *= i2;
     static_cast<uint16_t*>(a.o)[to + c] = f2bf(fmaf(-lam, y2, y1));
     if (a.o1 != nullptr) {
       a.o1[to + c] = y1;
       a.o2[to + c] = y2;
     }
   }
-  if (a.lse != nullptr && c == 0) {
+  if (a.lse != nullptr && part0 == 0 && lane == 0) {
     float* lse = a.lse + ((int64_t(b) * a.heads + h) * a.queries + t) * 2;
     lse[0] = l1 == 0.f ? INFINITY : top1 + __builtin_amdgcn_logf(l1);
     lse[1] = l2 == 0.f ? INFINITY : top2 + __builtin_amdgcn_logf(l2);
@@ -339,7 +354,7 @@ __global__ __launch_bounds__(256) void attend_join(mmuon_attention_args a, int s
 }
 
 struct ForwardPlan {
-  bool wide;   // workgroups of several waves, else of one
+  bool wide;   // workgroups of eight waves, else of two that are a pair
   int tiles;   // of rows
   int splits;  // of the keys
 };
@@ -359,7 +374,7 @@ ForwardPlan forward_plan(const mmuon_attention_args& a) {
   }
   p.tiles = int((rows + 31) / 32);
   // as many workgroups as are resident, each of four tiles of keys at least
-  const int64_t resident = a.dim > 64 ? 512 : 1024, most = std::max(1, (a.keys + 127) / 128);
+  const int64_t resident = a.dim > 64 ? 512 : 1024, most = std::min<int64_t>(MOST_PARTS, std::max(1, (a.keys + 127) / 128));
   p.splits = int(std::max<int64_t>(1, std::min(most, resident / (groups * p.tiles))));
   return p;
 }
@@ -376,12 +391,14 @@ void attend_dim(const mmuon_attention_args& a, hipStream_t s) {
   Parts parts{};
   constexpr int MAPS = D == 128 ? 1 : 2;
   if (p.wide) return attend_launch<D, (D == 128 ? 32 : 64), 8, MAPS, 3, false>(a, p, parts, s);
-  if (p.splits == 1) return attend_launch<D, 32, 2 / MAPS, MAPS, 2, false>(a, p, parts, s);
+  if (p.splits == 1) return attend_launch<D, 32, 2, 1, 2, false>(a, p, parts, s);
   const int64_t rows = int64_t(a.heads / a.kv_heads) * a.queries * a.batch * a.kv_heads;
   parts.stats = static_cast<float4*>(a.workspace);
   parts.sums = static_cast<float*>(a.workspace) + rows * p.splits * 8;
-  attend_launch<D, 32, 2 / MAPS, MAPS, 2, true>(a, p, parts, s);
-  hipLaunchKernelGGL(attend_join<D>, dim3(unsigned(rows)), dim3(256), 0, s, a, p.splits, parts);
+  attend_launch<D, 32, 2, 1, 2, true>(a, p, parts, s);
+  if (p.splits <= ALONE_PARTS)
+    hipLaunchKernelGGL((attend_join<D, 1>), dim3(unsigned((rows + JOIN - 1) / JOIN)), dim3(64 * JOIN), 0, s, a, p.splits, parts);
+  else hipLaunchKernelGGL((attend_join<D, JOIN>), dim3(unsigned(rows)), dim3(64 * JOIN), 0, s, a, p.splits, parts);
 }
 
 }  // namespace

@@ -26,6 +26,7 @@ namespace {
 struct RowSpace {
   float4* stats;
   float* dlam;
+  float* sums;  // of the parts of dk and dv: (group, part, key, dv dk_1 dk_2)
 };
 
 // A wave to four rows' D: 16 lanes each
@@ -204,8 +205,9 @@ __global__ __launch_bounds__(1024) void attention_dlam(mmuon_attention_args a, R
 
 // dk and dv: 32 keys to a wave, over the query rows of the heads that share them, 32 at a time.  The
 // keys are operands in registers, the values, whose product comes once for both maps, in LDS.
-template <int D, int WAVES, int SLOTS>
-__global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mmuon_attention_args a, Dealing dealt, RowSpace space) {
+template <int D, int WAVES, int SLOTS, bool SPLIT>
+__global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mmuon_attention_args a, Dealing dealt, int parts,
+                                                                              RowSpace space) {
   constexpr int CA = D / 8, CB = D / 4, TQ = 32;
   using T = Tile<D, TQ, WAVES>;
   constexpr int BYTES = T::BYTES + 1024;  // and the rows' statistics
@@ -214,8 +216,10 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mm
   __shared__ __attribute__((aligned(1024))) char values[WAVES * 32 * CB * 16];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int group, tile;  // the first keys are seen by the most queries: first
-  if (!deal(dealt, a.batch * a.kv_heads, group, tile)) return;
+  int group, item;
+  if (!deal(dealt, a.batch * a.kv_heads, group, item)) return;
+  // the first keys are seen by the most queries: first
+  const int tile = SPLIT ? item / parts : item, part = SPLIT ? item % parts : 0;
   const int b = group / a.kv_heads, g = group % a.kv_heads, share = a.heads / a.kv_heads;
   const Span span = span_of(a, b);
   const int c0 = tile * 32 * WAVES, w0 = c0 + 32 * wave;  // first key of the workgroup, the wave
@@ -229,7 +233,9 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mm
   };
   const int from = first_of(c0) / TQ * TQ, mine = first_of(w0), own = first_of(key);
   const int full = first_of(w0 + 31);  // from here on every key of the wave is seen
-  const int steps = (a.queries - from + TQ - 1) / TQ, n = steps * share;
+  const int steps = (a.queries - from + TQ - 1) / TQ, all = steps * share;
+  const int i0 = SPLIT ? int(int64_t(all) * part / parts) : 0, n = (SPLIT ? int(int64_t(all) * (part + 1) / parts) : all) - i0;
+  const int head0 = SPLIT && n > 0 ? i0 / steps : 0, first0 = from + (i0 - head0 * steps) * TQ;
 
   const char* q1 = static_cast<const char*>(a.q) + 2 * (b * a.q_stride[0] + 2 * g * share * a.q_stride[2]);
   const char* g0 = static_cast<const char*>(a.dout) + 2 * (int64_t(b) * a.queries * a.heads + g * share) * 2 * a.dim;
@@ -241,7 +247,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mm
   const uint32_t lds = lds_addr(ring);
   uint32_t off[T::LOADS];
   T::offsets(src, wave, lane, off);
-  int next_head = 0, next_first = from;  // of the tile that is loaded next
+  int next_head = head0, next_first = first0;  // of the tile that is loaded next
   const auto load = [&](int i) {
     const int head = next_head, first = next_first;
     next_first += TQ;
@@ -292,7 +298,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mm
       if (c > src.b_last) *reinterpret_cast<uint4*>(mine_v + (i * 64 + lane) * 16) = make_uint4(0, 0, 0, 0);
     }
   }
-  int head = 0, first = from - TQ;
+  int head = head0, first = first0 - TQ;
   for (int i = 0; i < n; ++i) {
     first += TQ;
     if (first >= a.queries) first = from, ++head;
@@ -345,6 +351,18 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mm
       }
   }
   const bool in = key < a.keys;
+  if constexpr (SPLIT) {
+    if (!in) return;
+    float* to = space.sums + ((int64_t(group) * parts + part) * a.keys + key) * (4 * D) + 4 * half;
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {  // dv, dk of both maps
+      const f32x16& acc = j < D / 16 ? dv[j] : j < 3 * D / 32 ? dk[0][j - D / 16] : dk[1][j - 3 * D / 32];
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<float4*>(to + 32 * j + 2 * e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+    }
+    return;
+  }
   uint16_t* to_k = in ? static_cast<uint16_t*>(a.dk) + ((int64_t(b) * a.keys + key) * 2 * a.kv_heads + 2 * g) * a.dim : nullptr;
   uint16_t* to_v = in ? static_cast<uint16_t*>(a.dv) + ((int64_t(b) * a.keys + key) * a.kv_heads + g) * 2 * a.dim : nullptr;
 #pragma unroll
@@ -360,9 +378,45 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mm
   }
 }
 
+// dk and dv of the parts of the queries, in order: a thread to 4 columns of a key
+template <int D>
+__global__ __launch_bounds__(256) void attention_dkv_join(mmuon_attention_args a, int parts, RowSpace space) {
+  const int64_t id = int64_t(blockIdx.x) * 256 + threadIdx.x, row = id / D, all = int64_t(a.batch) * a.kv_heads * a.keys;
+  if (row >= all) return;
+  const int c = int(id - row * D) * 4, key = int(row % a.keys);
+  const int64_t group = row / a.keys, b = group / a.kv_heads, g = group - b * a.kv_heads;
+  const float* from = space.sums + (group * parts * a.keys + key) * (4 * D) + c;
+  float s[4] = {};
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p) {
+    const float4 x = *reinterpret_cast<const float4*>(from + int64_t(p) * a.keys * (4 * D));
+    s[0] += x.x, s[1] += x.y, s[2] += x.z, s[3] += x.w;
+  }
+  const bool is_v = c < 2 * D;
+  const int m = c >= 3 * D, col = is_v ? c : c - (2 + m) * D;
+  if (col >= (is_v ? 2 * a.dim : a.dim)) return;
+  const float by = is_v ? 1.f : a.scale;
+  const int64_t at = b * a.keys + key;
+  uint16_t* to = is_v ? static_cast<uint16_t*>(a.dv) + (at * a.kv_heads + g) * 2 * a.dim + col
+                      : static_cast<uint16_t*>(a.dk) + (at * 2 * a.kv_heads + 2 * g + m) * a.dim + col;
+  *reinterpret_cast<uint2*>(to) = make_uint2(f2bf2(s[0] * by, s[1] * by), f2bf2(s[2] * by, s[3] * by));
+}
+
+// Parts of the queries (of all heads that share the keys): where the keys' tiles fill less than half of the
+// chip, as many as fill it, each of eight tiles of queries at least.  3 x 1001 tokens, 6 heads of 2 x 64 on 2:
+// dk and dv 181 us in one part, 45 in ten.
+constexpr int KEY_WAVES = 4;
+int key_parts(const mmuon_attention_args& a) {
+  const int64_t tiles = int64_t(a.batch) * a.kv_heads * ((a.keys + 32 * KEY_WAVES - 1) / (32 * KEY_WAVES));
+  const int64_t resident = a.dim > 64 ? 256 : 512, steps = int64_t(a.heads / a.kv_heads) * ((a.queries + 31) / 32);
+  if (tiles == 0 || tiles * 2 > resident) return 1;
+  return int(std::max<int64_t>(1, std::min<int64_t>({resident / tiles, steps / 8, 16})));
+}
+
 RowSpace row_space(const mmuon_attention_args& a) {
   const int64_t rows = int64_t(a.batch) * a.heads * a.queries;
-  return {static_cast<float4*>(a.workspace), static_cast<float*>(a.workspace) + 4 * rows};
+  float* at = static_cast<float*>(a.workspace);
+  return {reinterpret_cast<float4*>(at), at + 4 * rows, at + 4 * rows + (rows + 63) / 64 * 64};
 }
 
 template <int D>
@@ -378,16 +432,25 @@ void backward_dim(const mmuon_attention_args& a, hipStream_t s) {
   }
   if (a.dlam != nullptr && a.heads > 0) hipLaunchKernelGGL(attention_dlam, dim3(unsigned(a.heads)), dim3(1024), 0, s, a, space);
   if (a.dk != nullptr && groups > 0 && a.keys > 0) {
-    constexpr int WAVES = 4;
-    const Dealing d = dealing(groups, (a.keys + 32 * WAVES - 1) / (32 * WAVES));
-    hipLaunchKernelGGL((attention_dkv<D, WAVES, 2>), dim3(blocks_of(d)), dim3(64 * WAVES), 0, s, a, d, space);
+    const int64_t tiles = (a.keys + 32 * KEY_WAVES - 1) / (32 * KEY_WAVES);
+    const int parts = key_parts(a);
+    const Dealing d = dealing(groups, tiles * parts);
+    const dim3 grid(blocks_of(d)), block(64 * KEY_WAVES);
+    if (parts == 1) {
+      hipLaunchKernelGGL((attention_dkv<D, KEY_WAVES, 2, false>), grid, block, 0, s, a, d, parts, space);
+    } else {
+      hipLaunchKernelGGL((attention_dkv<D, KEY_WAVES, 2, true>), grid, block, 0, s, a, d, parts, space);
+      hipLaunchKernelGGL(attention_dkv_join<D>, dim3(unsigned((groups * a.keys * D + 255) / 256)), dim3(256), 0, s, a, parts, space);
+    }
   }
 }
 
 }  // namespace
 
 size_t attention_backward_workspace(const mmuon_attention_args& a) {
-  return size_t(a.batch) * a.heads * a.queries * 5 * 4;
+  const size_t rows = size_t(a.batch) * a.heads * a.queries, d = a.dim > 64 ? 128 : a.dim > 32 ? 64 : 32;
+  const int parts = key_parts(a);
+  return (rows * 4 + (rows + 63) / 64 * 64 + (parts > 1 ? size_t(a.batch) * a.kv_heads * a.keys * parts * 4 * d : 0)) * 4;
 }
 
 int launch_attention_bwd(const mmuon_attention_args& a, hipStream_t s) {
