@@ -261,7 +261,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void attend(mmuon_a
 // The parts of a row's keys, joined by WAVES waves: each part's factor first, then the sums of every
 // WAVES-th part to a wave, which are added in order.
 constexpr int JOIN = 8;            // waves of a workgroup
-constexpr int ALONE_PARTS = 16;    // parts that a wave joins alone
+constexpr int ALONE_PARTS = 8;    // parts that a wave joins alone
 constexpr int MOST_PARTS = 1024;
 template <int D, int WAVES>
 __global__ __launch_bounds__(64 * JOIN) void attend_join(mmuon_attention_args a, int splits, Parts parts) {

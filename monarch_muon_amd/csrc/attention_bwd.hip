@@ -25,8 +25,8 @@ namespace {
 // For each query row (b, h, t): (lse_1, D_1, lse_2, D_2); and its part of dlam
 struct RowSpace {
   float4* stats;
-  float* dlam;
-  float* sums;  // of the parts of dk and dv: (group, part, key, dv dk_1 dk_2)
+  float* dlam;  // [part]
+  float* sums;  // of the parts: of dq (part, row, dq_1 dq_2), then of dk and dv (group, part, key, dv dk_1 dk_2)
 };
 
 // A wave to four rows' D: 16 lanes each
@@ -58,8 +58,9 @@ __global__ __launch_bounds__(256) void attention_rows(mmuon_attention_args a, Ro
 }
 
 // dq and each row's part of dlam: 32 queries to a wave, over tiles of 32 keys
-template <int D, int WAVES, int SLOTS>
-__global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmuon_attention_args a, Dealing dealt, RowSpace space) {
+template <int D, int WAVES, int SLOTS, bool SPLIT>
+__global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmuon_attention_args a, Dealing dealt, int parts,
+                                                                             RowSpace space) {
   constexpr int CA = D / 8, CB = D / 4, TK = 32;
   using T = Tile<D, TK, WAVES>;
   __shared__ __attribute__((aligned(1024))) char ring[SLOTS * T::BYTES];
@@ -67,7 +68,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmu
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int group, item;
   if (!deal(dealt, a.batch * a.kv_heads, group, item)) return;
-  const int tile = dealt.each - 1 - item;
+  const int tile = SPLIT ? dealt.each / parts - 1 - item / parts : dealt.each - 1 - item, part = SPLIT ? item % parts : 0;
   const int b = group / a.kv_heads, g = group % a.kv_heads, share = a.heads / a.kv_heads;
   const int rows = share * a.queries, r0 = tile * 32 * WAVES;
   const Span span = span_of(a, b);
@@ -96,8 +97,9 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmu
   const uint32_t lds = lds_addr(ring);
   uint32_t off[T::LOADS];
   T::offsets(src, wave, lane, off);
+  const int all = (keys + TK - 1) / TK, i0 = SPLIT ? int(int64_t(all) * part / parts) : 0;
   const auto load = [&](int i) {
-    const int64_t first = int64_t(i) * TK;
+    const int64_t first = int64_t(i0 + i) * TK;
     const char* k = k1 + 2 * first * a.k_stride[1];
     T::load(lds + (i % SLOTS) * T::BYTES, k, k + 2 * a.k_stride[2], v0 + 2 * first * a.v_stride[1], src, off, span.keys - int(first), wave, lane);
   };
@@ -119,7 +121,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmu
     for (int j = 0; j < D / 32; ++j) acc[m][j] = f32x16{};
   float along = 0.f;
 
-  const int n = (keys + TK - 1) / TK;
+  const int n = (SPLIT ? int(int64_t(all) * (part + 1) / parts) : all) - i0;
 #pragma unroll
   for (int i = 0; i < SLOTS - 1; ++i)
     if (i < n) load(i);
@@ -131,7 +133,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmu
     barrier_after_lds_writes();
     if (i + SLOTS - 1 < n) load(i + SLOTS - 1);
     const char* tile_at = ring + (i % SLOTS) * T::BYTES;
-    if (i * TK >= mine) continue;
+    const int key0 = (i0 + i) * TK;
+    if (key0 >= mine) continue;
     const uint32_t kbase = fresh(kbase0), vbase = fresh(vbase0), tbase = fresh(tbase0);
     f32x16 s[2] = {f32x16{}, f32x16{}}, dp = f32x16{};
 #pragma unroll
@@ -139,8 +142,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmu
       s[0] = mfma(read_rows<CA>(tile_at, kbase, 0, kk), q[0][kk], s[0]);
       s[1] = mfma(read_rows<CA>(tile_at + T::A2, kbase, 0, kk), q[1][kk], s[1]);
     }
-    if (i * TK + TK > fewest) {
-      const int left = limit - i * TK - 4 * half;
+    if (key0 + TK > fewest) {
+      const int left = limit - key0 - 4 * half;
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         if (8 * (e / 4) + e % 4 >= left) s[0][e] = s[1][e] = -INFINITY;
@@ -171,9 +174,23 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmu
 #pragma unroll
       for (int y = 0; y < 2; ++y) acc[1][j] = mfma(read_turned<CA>(tile_at + T::A2, tbase, 16 * y, j), x2[y], acc[1][j]);
   }
-  const float lam = a.lam[int64_t(h) * a.lam_stride];
   along = half_sum(along);
-  if (in && half == 0) space.dlam[at] = -along;
+  const int64_t total = int64_t(a.batch) * a.heads * a.queries;
+  if (in && half == 0) space.dlam[part * total + at] = -along;
+  if constexpr (SPLIT) {
+    if (!in) return;
+    float* to = space.sums + (part * total + at) * (2 * D) + 4 * half;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          *reinterpret_cast<float4*>(to + m * D + 32 * j + 2 * e) =
+              make_float4(acc[m][j][e], acc[m][j][e + 1], acc[m][j][e + 2], acc[m][j][e + 3]);
+    return;
+  }
+  const float lam = a.lam[int64_t(h) * a.lam_stride];
   uint16_t* dq = in ? static_cast<uint16_t*>(a.dq) + ((int64_t(b) * a.queries + t) * 2 * a.heads + 2 * h) * a.dim : nullptr;
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) {
@@ -187,13 +204,33 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmu
   }
 }
 
-// dlam[h]: its rows of all sequences, in order by thread and then in a tree
-__global__ __launch_bounds__(1024) void attention_dlam(mmuon_attention_args a, RowSpace space) {
+// dq of the parts of the keys, in order: a thread to 4 columns of a row
+template <int D>
+__global__ __launch_bounds__(256) void attention_dq_join(mmuon_attention_args a, int parts, RowSpace space) {
+  const int64_t id = int64_t(blockIdx.x) * 256 + threadIdx.x, row = id / (D / 2), all = int64_t(a.batch) * a.heads * a.queries;
+  if (row >= all) return;
+  const int c = int(id - row * (D / 2)) * 4, m = c >= D, col = c - m * D, t = int(row % a.queries);
+  const int64_t bh = row / a.queries, b = bh / a.heads, h = bh - b * a.heads;
+  const float* from = space.sums + row * (2 * D) + c;
+  float s[4] = {};
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p) {
+    const float4 x = *reinterpret_cast<const float4*>(from + p * all * (2 * D));
+    s[0] += x.x, s[1] += x.y, s[2] += x.z, s[3] += x.w;
+  }
+  if (col >= a.dim) return;
+  const float by = m ? -(a.lam[h * a.lam_stride] * a.scale) : a.scale;
+  uint16_t* to = static_cast<uint16_t*>(a.dq) + ((b * a.queries + t) * 2 * a.heads + 2 * h + m) * a.dim + col;
+  *reinterpret_cast<uint2*>(to) = make_uint2(f2bf2(s[0] * by, s[1] * by), f2bf2(s[2] * by, s[3] * by));
+}
+
+// dlam[h]: its rows of all sequences and parts, in order by thread and then in a tree
+__global__ __launch_bounds__(1024) void attention_dlam(mmuon_attention_args a, int parts, RowSpace space) {
   __shared__ float sums[16];
   const int h = blockIdx.x;
   double s = 0.0;
-  for (int b = 0; b < a.batch; ++b) {
-    const float* from = space.dlam + (int64_t(b) * a.heads + h) * a.queries;
+  for (int i = 0; i < parts * a.batch; ++i) {
+    const float* from = space.dlam + (int64_t(i) * a.heads + h) * a.queries;
     float r = 0.f;
 #pragma unroll 4
     for (int t = threadIdx.x; t < a.queries; t += 1024) r += from[t];
@@ -412,25 +449,43 @@ int key_parts(const mmuon_attention_args& a) {
   if (tiles == 0 || tiles * 2 > resident) return 1;
   return int(std::max<int64_t>(1, std::min<int64_t>({resident / tiles, steps / 8, 16})));
 }
+// Parts of the keys, likewise (4 heads of 2 x 128, 2000 tokens: dq 112 us in one part, 48 in four)
+constexpr int ROW_WAVES = 4;
+int64_t row_tiles(const mmuon_attention_args& a) {
+  return (int64_t(a.heads / a.kv_heads) * a.queries + 32 * ROW_WAVES - 1) / (32 * ROW_WAVES);
+}
+int row_parts(const mmuon_attention_args& a) {
+  const int64_t tiles = int64_t(a.batch) * a.kv_heads * row_tiles(a);
+  const int64_t resident = a.dim > 64 ? 256 : 512, steps = (a.keys + 31) / 32;
+  if (tiles == 0 || tiles * 2 > resident) return 1;
+  return int(std::max<int64_t>(1, std::min<int64_t>({resident / tiles, steps / 8, 16})));
+}
 
 RowSpace row_space(const mmuon_attention_args& a) {
   const int64_t rows = int64_t(a.batch) * a.heads * a.queries;
   float* at = static_cast<float*>(a.workspace);
-  return {reinterpret_cast<float4*>(at), at + 4 * rows, at + 4 * rows + (rows + 63) / 64 * 64};
+  return {reinterpret_cast<float4*>(at), at + 4 * rows, at + 4 * rows + (rows * row_parts(a) + 63) / 64 * 64};
 }
 
 template <int D>
 void backward_dim(const mmuon_attention_args& a, hipStream_t s) {
   const int64_t rows = int64_t(a.batch) * a.heads * a.queries;
-  const int64_t groups = int64_t(a.batch) * a.kv_heads, share = a.heads / a.kv_heads;
+  const int64_t groups = int64_t(a.batch) * a.kv_heads;
   const RowSpace space = row_space(a);
   if (rows > 0) hipLaunchKernelGGL(attention_rows, dim3(unsigned((rows + 15) / 16)), dim3(256), 0, s, a, space);
+  const int of_keys = row_parts(a);
   if (a.dq != nullptr && rows > 0) {
-    constexpr int WAVES = 4;
-    const Dealing d = dealing(groups, (share * a.queries + 32 * WAVES - 1) / (32 * WAVES));
-    hipLaunchKernelGGL((attention_dq<D, WAVES, 3>), dim3(blocks_of(d)), dim3(64 * WAVES), 0, s, a, d, space);
+    const Dealing d = dealing(groups, row_tiles(a) * of_keys);
+    const dim3 grid(blocks_of(d)), block(64 * ROW_WAVES);
+    if (of_keys == 1) {
+      hipLaunchKernelGGL((attention_dq<D, ROW_WAVES, 3, false>), grid, block, 0, s, a, d, of_keys, space);
+    } else {
+      hipLaunchKernelGGL((attention_dq<D, ROW_WAVES, 3, true>), grid, block, 0, s, a, d, of_keys, space);
+      hipLaunchKernelGGL(attention_dq_join<D>, dim3(unsigned((rows * (D / 2) + 255) / 256)), dim3(256), 0, s, a, of_keys, space);
+    }
   }
-  if (a.dlam != nullptr && a.heads > 0) hipLaunchKernelGGL(attention_dlam, dim3(unsigned(a.heads)), dim3(1024), 0, s, a, space);
+  if (a.dlam != nullptr && a.heads > 0)
+    hipLaunchKernelGGL(attention_dlam, dim3(unsigned(a.heads)), dim3(1024), 0, s, a, rows > 0 ? of_keys : 0, space);
   if (a.dk != nullptr && groups > 0 && a.keys > 0) {
     const int64_t tiles = (a.keys + 32 * KEY_WAVES - 1) / (32 * KEY_WAVES);
     const int parts = key_parts(a);
@@ -449,8 +504,10 @@ void backward_dim(const mmuon_attention_args& a, hipStream_t s) {
 
 size_t attention_backward_workspace(const mmuon_attention_args& a) {
   const size_t rows = size_t(a.batch) * a.heads * a.queries, d = a.dim > 64 ? 128 : a.dim > 32 ? 64 : 32;
-  const int parts = key_parts(a);
-  return (rows * 4 + (rows + 63) / 64 * 64 + (parts > 1 ? size_t(a.batch) * a.kv_heads * a.keys * parts * 4 * d : 0)) * 4;
+  const size_t of_keys = row_parts(a), of_rows = key_parts(a);
+  const size_t sums = std::max(of_keys > 1 ? rows * of_keys * 2 * d : 0,
+                               of_rows > 1 ? size_t(a.batch) * a.kv_heads * a.keys * of_rows * 4 * d : 0);
+  return (rows * 4 + (rows * of_keys + 63) / 64 * 64 + sums) * 4;
 }
 
 int launch_attention_bwd(const mmuon_attention_args& a, hipStream_t s) {
