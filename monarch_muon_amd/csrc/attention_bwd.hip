@@ -26,7 +26,8 @@ namespace {
 struct RowSpace {
   float4* stats;
   float* dlam;  // [part]
-  float* sums;  // of the parts: of dq (part, row, dq_1 dq_2), then of dk and dv (group, part, key, dv dk_1 dk_2)
+  float* dq;    // parts: (part, row, dq_1 dq_2)
+  float* dkv;   // (group, part, key, dv dk_1 dk_2)
 };
 
 // A wave to four rows' D: 16 lanes each
@@ -179,7 +180,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmu
   if (in && half == 0) space.dlam[part * total + at] = -along;
   if constexpr (SPLIT) {
     if (!in) return;
-    float* to = space.sums + (part * total + at) * (2 * D) + 4 * half;
+    float* to = space.dq + (part * total + at) * (2 * D) + 4 * half;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -204,14 +205,14 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmu
   }
 }
 
-// dq of the parts of the keys, in order: a thread to 4 columns of a row
+// dq of the parts of the keys, in order: 4 columns of a row
 template <int D>
-__global__ __launch_bounds__(256) void attention_dq_join(mmuon_attention_args a, int parts, RowSpace space) {
-  const int64_t id = int64_t(blockIdx.x) * 256 + threadIdx.x, row = id / (D / 2), all = int64_t(a.batch) * a.heads * a.queries;
+__device__ __forceinline__ void join_dq(const mmuon_attention_args& a, int parts, const RowSpace& space, int64_t id) {
+  const int64_t row = id / (D / 2), all = int64_t(a.batch) * a.heads * a.queries;
   if (row >= all) return;
   const int c = int(id - row * (D / 2)) * 4, m = c >= D, col = c - m * D, t = int(row % a.queries);
   const int64_t bh = row / a.queries, b = bh / a.heads, h = bh - b * a.heads;
-  const float* from = space.sums + row * (2 * D) + c;
+  const float* from = space.dq + row * (2 * D) + c;
   float s[4] = {};
 #pragma unroll 8
   for (int p = 0; p < parts; ++p) {
@@ -224,27 +225,30 @@ __global__ __launch_bounds__(256) void attention_dq_join(mmuon_attention_args a,
   *reinterpret_cast<uint2*>(to) = make_uint2(f2bf2(s[0] * by, s[1] * by), f2bf2(s[2] * by, s[3] * by));
 }
 
-// dlam[h]: its rows of all sequences and parts, in order by thread and then in a tree
-__global__ __launch_bounds__(1024) void attention_dlam(mmuon_attention_args a, int parts, RowSpace space) {
-  __shared__ float sums[16];
-  const int h = blockIdx.x;
-  double s = 0.0;
+// dlam[h]: its rows of all sequences and parts, in order by thread and then in a tree; 256 threads
+__device__ __forceinline__ void sum_dlam(const mmuon_attention_args& a, int parts, const RowSpace& space, int h, float* scratch) {
+  float s = 0.f;
   for (int i = 0; i < parts * a.batch; ++i) {
     const float* from = space.dlam + (int64_t(i) * a.heads + h) * a.queries;
     float r = 0.f;
 #pragma unroll 4
-    for (int t = threadIdx.x; t < a.queries; t += 1024) r += from[t];
+    for (int t = threadIdx.x; t < a.queries; t += 256) r += from[t];
     s += r;
   }
-  const float v = block_sum<1024>(float(s), sums);
-  if (threadIdx.x == 0) a.dlam[h] = v;
+  s = block_sum<256>(s, scratch);
+  if (threadIdx.x == 0) a.dlam[h] = s;
+}
+__global__ __launch_bounds__(256) void attention_dlam(mmuon_attention_args a, int parts, RowSpace space) {
+  __shared__ float scratch[4];
+  sum_dlam(a, parts, space, blockIdx.x, scratch);
 }
 
 // dk and dv: 32 keys to a wave, over the query rows of the heads that share them, 32 at a time.  The
-// keys are operands in registers, the values, whose product comes once for both maps, in LDS.
+// keys are operands in registers, the values, whose product comes once for both maps, in LDS.  The
+// workgroups from `dlam_at` on sum dlam, a head each, which would take a launch of its own (5 to 8 us).
 template <int D, int WAVES, int SLOTS, bool SPLIT>
 __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mmuon_attention_args a, Dealing dealt, int parts,
-                                                                              RowSpace space) {
+                                                                              int dlam_at, int of_keys, RowSpace space) {
   constexpr int CA = D / 8, CB = D / 4, TQ = 32;
   using T = Tile<D, TQ, WAVES>;
   constexpr int BYTES = T::BYTES + 1024;  // and the rows' statistics
@@ -253,6 +257,10 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mm
   __shared__ __attribute__((aligned(1024))) char values[WAVES * 32 * CB * 16];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (int(blockIdx.x) >= dlam_at) {
+    static_assert(WAVES == 4, "256 threads");
+    return sum_dlam(a, of_keys, space, blockIdx.x - dlam_at, reinterpret_cast<float*>(ring));
+  }
   int group, item;
   if (!deal(dealt, a.batch * a.kv_heads, group, item)) return;
   // the first keys are seen by the most queries: first
@@ -390,7 +398,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mm
   const bool in = key < a.keys;
   if constexpr (SPLIT) {
     if (!in) return;
-    float* to = space.sums + ((int64_t(group) * parts + part) * a.keys + key) * (4 * D) + 4 * half;
+    float* to = space.dkv + ((int64_t(group) * parts + part) * a.keys + key) * (4 * D) + 4 * half;
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) {  // dv, dk of both maps
       const f32x16& acc = j < D / 16 ? dv[j] : j < 3 * D / 32 ? dk[0][j - D / 16] : dk[1][j - 3 * D / 32];
@@ -415,14 +423,14 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mm
   }
 }
 
-// dk and dv of the parts of the queries, in order: a thread to 4 columns of a key
+// dk and dv of the parts of the queries, in order: 4 columns of a key
 template <int D>
-__global__ __launch_bounds__(256) void attention_dkv_join(mmuon_attention_args a, int parts, RowSpace space) {
-  const int64_t id = int64_t(blockIdx.x) * 256 + threadIdx.x, row = id / D, all = int64_t(a.batch) * a.kv_heads * a.keys;
+__device__ __forceinline__ void join_dkv(const mmuon_attention_args& a, int parts, const RowSpace& space, int64_t id) {
+  const int64_t row = id / D, all = int64_t(a.batch) * a.kv_heads * a.keys;
   if (row >= all) return;
   const int c = int(id - row * D) * 4, key = int(row % a.keys);
   const int64_t group = row / a.keys, b = group / a.kv_heads, g = group - b * a.kv_heads;
-  const float* from = space.sums + (group * parts * a.keys + key) * (4 * D) + c;
+  const float* from = space.dkv + (group * parts * a.keys + key) * (4 * D) + c;
   float s[4] = {};
 #pragma unroll 8
   for (int p = 0; p < parts; ++p) {
@@ -437,6 +445,12 @@ __global__ __launch_bounds__(256) void attention_dkv_join(mmuon_attention_args a
   uint16_t* to = is_v ? static_cast<uint16_t*>(a.dv) + (at * a.kv_heads + g) * 2 * a.dim + col
                       : static_cast<uint16_t*>(a.dk) + (at * 2 * a.kv_heads + 2 * g + m) * a.dim + col;
   *reinterpret_cast<uint2*>(to) = make_uint2(f2bf2(s[0] * by, s[1] * by), f2bf2(s[2] * by, s[3] * by));
+}
+// Both: the first `of_dq` workgroups dq's
+template <int D>
+__global__ __launch_bounds__(256) void attention_join(mmuon_attention_args a, int of_dq, int of_keys, int of_rows, RowSpace space) {
+  if (int(blockIdx.x) < of_dq) join_dq<D>(a, of_keys, space, int64_t(blockIdx.x) * 256 + threadIdx.x);
+  else join_dkv<D>(a, of_rows, space, int64_t(blockIdx.x - of_dq) * 256 + threadIdx.x);
 }
 
 // Parts of the queries (of all heads that share the keys): where the keys' tiles fill less than half of the
@@ -461,54 +475,55 @@ int row_parts(const mmuon_attention_args& a) {
   return int(std::max<int64_t>(1, std::min<int64_t>({resident / tiles, steps / 8, 16})));
 }
 
-RowSpace row_space(const mmuon_attention_args& a) {
-  const int64_t rows = int64_t(a.batch) * a.heads * a.queries;
-  float* at = static_cast<float*>(a.workspace);
-  return {reinterpret_cast<float4*>(at), at + 4 * rows, at + 4 * rows + (rows * row_parts(a) + 63) / 64 * 64};
+int template_dim(const mmuon_attention_args& a) { return a.dim > 64 ? 128 : a.dim > 32 ? 64 : 32; }
+struct BackwardLayout {
+  size_t dlam, dq, dkv, total;  // floats; the rows' statistics come first
+};
+BackwardLayout backward_layout(const mmuon_attention_args& a) {
+  const size_t rows = size_t(a.batch) * a.heads * a.queries, keys = size_t(a.batch) * a.kv_heads * a.keys;
+  const size_t d = template_dim(a), of_keys = row_parts(a), of_rows = key_parts(a);
+  const auto up = [](size_t n) { return (n + 63) / 64 * 64; };
+  BackwardLayout l;
+  l.dlam = up(rows * 4);
+  l.dq = l.dlam + up(rows * of_keys);
+  l.dkv = l.dq + (of_keys > 1 ? up(rows * of_keys * 2 * d) : 0);
+  l.total = l.dkv + (of_rows > 1 ? up(keys * of_rows * 4 * d) : 0);
+  return l;
 }
 
 template <int D>
 void backward_dim(const mmuon_attention_args& a, hipStream_t s) {
-  const int64_t rows = int64_t(a.batch) * a.heads * a.queries;
+  const int64_t rows = int64_t(a.batch) * a.heads * a.queries, keys = int64_t(a.batch) * a.kv_heads * a.keys;
   const int64_t groups = int64_t(a.batch) * a.kv_heads;
-  const RowSpace space = row_space(a);
+  const BackwardLayout l = backward_layout(a);
+  float* ws = static_cast<float*>(a.workspace);
+  const RowSpace space{reinterpret_cast<float4*>(ws), ws + l.dlam, ws + l.dq, ws + l.dkv};
+  const int of_keys = row_parts(a), of_rows = key_parts(a);
+  const bool dq = a.dq != nullptr && rows > 0, dkv = a.dk != nullptr && keys > 0;
   if (rows > 0) hipLaunchKernelGGL(attention_rows, dim3(unsigned((rows + 15) / 16)), dim3(256), 0, s, a, space);
-  const int of_keys = row_parts(a);
-  if (a.dq != nullptr && rows > 0) {
+  if (dq) {
     const Dealing d = dealing(groups, row_tiles(a) * of_keys);
     const dim3 grid(blocks_of(d)), block(64 * ROW_WAVES);
-    if (of_keys == 1) {
-      hipLaunchKernelGGL((attention_dq<D, ROW_WAVES, 3, false>), grid, block, 0, s, a, d, of_keys, space);
-    } else {
-      hipLaunchKernelGGL((attention_dq<D, ROW_WAVES, 3, true>), grid, block, 0, s, a, d, of_keys, space);
-      hipLaunchKernelGGL(attention_dq_join<D>, dim3(unsigned((rows * (D / 2) + 255) / 256)), dim3(256), 0, s, a, of_keys, space);
-    }
+    if (of_keys == 1) hipLaunchKernelGGL((attention_dq<D, ROW_WAVES, 3, false>), grid, block, 0, s, a, d, of_keys, space);
+    else hipLaunchKernelGGL((attention_dq<D, ROW_WAVES, 3, true>), grid, block, 0, s, a, d, of_keys, space);
   }
-  if (a.dlam != nullptr && a.heads > 0)
-    hipLaunchKernelGGL(attention_dlam, dim3(unsigned(a.heads)), dim3(1024), 0, s, a, rows > 0 ? of_keys : 0, space);
-  if (a.dk != nullptr && groups > 0 && a.keys > 0) {
-    const int64_t tiles = (a.keys + 32 * KEY_WAVES - 1) / (32 * KEY_WAVES);
-    const int parts = key_parts(a);
-    const Dealing d = dealing(groups, tiles * parts);
-    const dim3 grid(blocks_of(d)), block(64 * KEY_WAVES);
-    if (parts == 1) {
-      hipLaunchKernelGGL((attention_dkv<D, KEY_WAVES, 2, false>), grid, block, 0, s, a, d, parts, space);
-    } else {
-      hipLaunchKernelGGL((attention_dkv<D, KEY_WAVES, 2, true>), grid, block, 0, s, a, d, parts, space);
-      hipLaunchKernelGGL(attention_dkv_join<D>, dim3(unsigned((groups * a.keys * D + 255) / 256)), dim3(256), 0, s, a, parts, space);
-    }
+  const int heads = a.dlam != nullptr ? a.heads : 0, summed = rows > 0 ? of_keys : 0;
+  if (dkv) {
+    const Dealing d = dealing(groups, (a.keys + 32 * KEY_WAVES - 1) / (32 * KEY_WAVES) * int64_t(of_rows));
+    const unsigned blocks = blocks_of(d);
+    const dim3 grid(blocks + heads), block(64 * KEY_WAVES);
+    if (of_rows == 1) hipLaunchKernelGGL((attention_dkv<D, KEY_WAVES, 2, false>), grid, block, 0, s, a, d, of_rows, int(blocks), summed, space);
+    else hipLaunchKernelGGL((attention_dkv<D, KEY_WAVES, 2, true>), grid, block, 0, s, a, d, of_rows, int(blocks), summed, space);
+  } else if (heads > 0) {
+    hipLaunchKernelGGL(attention_dlam, dim3(unsigned(heads)), dim3(256), 0, s, a, summed, space);
   }
+  const int64_t q = dq && of_keys > 1 ? (rows * (D / 2) + 255) / 256 : 0, k = dkv && of_rows > 1 ? (keys * D + 255) / 256 : 0;
+  if (q + k > 0) hipLaunchKernelGGL(attention_join<D>, dim3(unsigned(q + k)), dim3(256), 0, s, a, int(q), of_keys, of_rows, space);
 }
 
 }  // namespace
 
-size_t attention_backward_workspace(const mmuon_attention_args& a) {
-  const size_t rows = size_t(a.batch) * a.heads * a.queries, d = a.dim > 64 ? 128 : a.dim > 32 ? 64 : 32;
-  const size_t of_keys = row_parts(a), of_rows = key_parts(a);
-  const size_t sums = std::max(of_keys > 1 ? rows * of_keys * 2 * d : 0,
-                               of_rows > 1 ? size_t(a.batch) * a.kv_heads * a.keys * of_rows * 4 * d : 0);
-  return (rows * 4 + (rows * of_keys + 63) / 64 * 64 + sums) * 4;
-}
+size_t attention_backward_workspace(const mmuon_attention_args& a) { return backward_layout(a).total * 4; }
 
 int launch_attention_bwd(const mmuon_attention_args& a, hipStream_t s) {
   if (a.dim > 64) backward_dim<128>(a, s);
