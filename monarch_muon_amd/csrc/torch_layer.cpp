@@ -11,6 +11,7 @@
 #include "torch_common.hpp"
 
 #include <array>
+#include <string>
 #include <tuple>
 
 using namespace mmuon_torch;
@@ -36,7 +37,7 @@ void require_one_device(std::initializer_list<const Tensor*> ts) {
 const std::array<int64_t, 1> NOTHING = {0};
 const at::IntArrayRef NONE = NOTHING;
 
-const char* name_of(const Tensor& t) { return c10::getDtypeNames(t.scalar_type()).first.c_str(); }
+std::string name_of(const Tensor& t) { return c10::getDtypeNames(t.scalar_type()).first; }
 
 int32_t float_code(const Tensor& t, const char* op, const char* name) {
   TORCH_CHECK_TYPE(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat, op, " takes bfloat16 or float32 "
@@ -66,13 +67,11 @@ mmuon_norm_args norm_args(const char* op, const Tensor& x, const OptionalTensor&
     TORCH_CHECK_VALUE(residual->sizes() == x.sizes(), "residual ", residual->sizes(), " is not of x's shape ", x.sizes());
     TORCH_CHECK_TYPE(residual->scalar_type() == x.scalar_type(), op, ": residual must be of x's type, got torch.",
                      name_of(*residual), " with torch.", name_of(x));
-    require_one_device({&x, &*residual, &w});
-  } else {
-    require_one_device({&x, &w});
   }
   TORCH_CHECK_VALUE(eps >= 0, "eps must not be negative, got ", eps);
   TORCH_CHECK_VALUE(x.size(-1) <= (a.dtype == MMUON_BF16 ? 32768 : 16384), op, ": width ", x.size(-1), " beyond ",
                     a.dtype == MMUON_BF16 ? 32768 : 16384);
+  require_one_device({&x, residual.has_value() ? &*residual : &x, &w});
   a.out_dtype = a.dtype;
   a.width = int32_t(x.size(-1));
   a.rows = x.numel() / a.width;
@@ -142,10 +141,10 @@ Pair rms_norm_grad_impl(const Tensor& h_, const Tensor& inv, const Tensor& weigh
 
 Triple rms_norm_fp8_impl(const Tensor& x_, const OptionalTensor& residual, const Tensor& weight, double eps,
                          at::ScalarType dtype, int64_t group) {
-  mmuon_norm_args a = norm_args("rms_norm_fp8", x_, residual, weight, eps);
   TORCH_CHECK_TYPE(dtype == at::kFloat8_e4m3fn || dtype == at::kFloat8_e5m2, "rms_norm_fp8 gives float8_e4m3fn or "
                    "float8_e5m2, not torch.", c10::getDtypeNames(dtype).first);
   TORCH_CHECK_VALUE(group == 128 || group == 0, "group must be 128 columns or None, got ", group);
+  mmuon_norm_args a = norm_args("rms_norm_fp8", x_, residual, weight, eps);
   bind_library();
   const c10::DeviceGuard guard(x_.device());
   const Tensor x = rows_of(x_), r = residual.has_value() ? rows_of(*residual) : Tensor(), w = weight.contiguous();
@@ -275,7 +274,6 @@ Pair rotary_impl(const Tensor& q_, const Tensor& k_, const Tensor& table_, const
                     "expected a table (positions, columns that are rotated) of an even number of at most ", q_.size(3),
                     " columns, got ", table_.sizes());
   TORCH_CHECK_VALUE(q_.numel() == 0 || table_.size(0) > 0, "rotary: a table of no positions");
-  require_one_device({&q_, &k_, &table_});
   const int64_t B = q_.size(0), T = q_.size(1);
   Tensor at_;
   if (positions.has_value()) {
@@ -284,8 +282,8 @@ Pair rotary_impl(const Tensor& q_, const Tensor& k_, const Tensor& table_, const
     TORCH_CHECK_VALUE((positions->dim() == 1 && positions->size(0) == T) ||
                           (positions->dim() == 2 && positions->size(0) == B && positions->size(1) == T),
                       "positions must be (T) or (B, T) = (", B, ", ", T, "), got ", positions->sizes());
-    require_one_device({&q_, &*positions});
   }
+  require_one_device({&q_, &k_, &table_, positions.has_value() ? &*positions : &table_});
   bind_library();
   const c10::DeviceGuard guard(q_.device());
   const auto heads = [](const Tensor& t) { return t.size(3) <= 1 || t.stride(3) == 1 ? t : t.contiguous(); };
@@ -426,7 +424,6 @@ struct AttentionCall {
     TORCH_CHECK_VALUE(lam.dim() == 1 && lam.size(0) == q.size(2) / 2, "lam must hold one value, or one for each of ",
                       q.size(2) / 2, " heads, got ", lam.sizes());
     TORCH_CHECK_VALUE(scale > 0 && scale <= 3.4e38, "scale must be positive and finite, got ", scale);
-    require_one_device({&q, &k, &v, &lam});
     for (const OptionalTensor* t : {&lengths, &starts}) {
       if (!t->has_value()) continue;
       const char* name = t == &lengths ? "lengths" : "starts";
@@ -434,8 +431,8 @@ struct AttentionCall {
                        " must be int64 or int32, got torch.", name_of(**t));
       TORCH_CHECK_VALUE((*t)->dim() == 1 && (*t)->size(0) == q.size(0), name, " must hold one value per sequence, got ",
                         (*t)->sizes());
-      require_one_device({&q, &**t});
     }
+    require_one_device({&q, &k, &v, &lam, lengths.has_value() ? &*lengths : &q, starts.has_value() ? &*starts : &q});
     bind_library();
   }
   void workspace(bool backward) {

@@ -2,9 +2,9 @@
 
     python -m monarch_muon_amd.example [steps]
 
-``embedding`` -> residual MLP blocks of Monarch projections (``butterfly_blk``) -> ``linear_cross_entropy`` ->
-backward -> ``MonarchMuonOptimizer`` (Monarch factors by Muon, the table, the norms and the head by AdamW), and then a
-few tokens sampled greedily, one at a time, and scored.
+``embedding`` -> decoder blocks (``rms_norm`` with the residual's addition, ``rotary``, ``differential_attention`` and an MLP
+between Monarch projections, ``butterfly_blk``) -> ``linear_cross_entropy`` -> backward -> ``MonarchMuonOptimizer`` (Monarch
+factors by Muon, the rest by AdamW), and then a few tokens sampled greedily, one at a time over a cache, and scored.
 """
 from __future__ import annotations
 
@@ -13,25 +13,52 @@ import sys
 import torch
 import torch.nn.functional as F
 
-from . import MonarchMuonOptimizer, butterfly_blk, embedding, linear_cross_entropy
+from . import (MonarchMuonOptimizer, butterfly_blk, differential_attention, embedding, linear_cross_entropy, rms_norm,
+               rotary, rotary_table)
 from .workloads import factor_shapes
 
 VOCAB, WIDTH, HIDDEN, NBLOCKS, LAYERS = 509, 256, 512, 2, 2
 PAD = 0
 BATCH, SEQ = 8, 96
+HEADS, DIM = 4, 32            # a head: two maps of DIM columns, values of twice as many
+
+
+def factors(*sizes):
+    return torch.nn.ParameterList(torch.randn(s) / s[2] ** 0.5 for din, dout in sizes for s in factor_shapes(din, dout, NBLOCKS))
+
+
+class Attention(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.w = factors(*[(WIDTH, WIDTH)] * 4)
+        self.lam = torch.nn.Parameter(torch.full((HEADS,), 0.3))
+        self.norm = torch.nn.Parameter(torch.ones(2 * DIM))
+
+    def forward(self, x, table, cache=None, at=0):
+        B, T, _ = x.shape
+        q, k, v = (butterfly_blk(x, self.w[i], self.w[i + 1]) for i in (0, 2, 4))
+        q, k, v = q.view(B, T, 2 * HEADS, DIM), k.view(B, T, 2 * HEADS, DIM), v.view(B, T, HEADS, 2 * DIM)
+        q, k = rotary(q, k, table, torch.arange(at, at + T, device=x.device))
+        lengths = None
+        if cache is not None:          # (keys, values) of the tokens before, with room for these
+            cache[0][:, at:at + T], cache[1][:, at:at + T] = k, v
+            (k, v), lengths = cache, torch.full((B,), at + T, device=x.device)
+        o = rms_norm(differential_attention(q, k, v, self.lam, lengths=lengths), self.norm)
+        return butterfly_blk(o.view(B, T, WIDTH), self.w[6], self.w[7])
 
 
 class Block(torch.nn.Module):
     def __init__(self):
         super().__init__()
-        self.norm = torch.nn.Parameter(torch.ones(WIDTH, dtype=torch.bfloat16))
-        self.w = torch.nn.ParameterList(torch.randn(s) / s[2] ** 0.5 for din, dout in ((WIDTH, HIDDEN), (HIDDEN, WIDTH))
-                                        for s in factor_shapes(din, dout, NBLOCKS))
+        self.norms = torch.nn.ParameterList(torch.ones(WIDTH) for _ in range(2))
+        self.attention = Attention()
+        self.w = factors((WIDTH, HIDDEN), (HIDDEN, WIDTH))
 
-    def forward(self, x):
-        h = F.rms_norm(x, (WIDTH,), self.norm)
-        h = F.silu(butterfly_blk(h, self.w[0], self.w[1]))
-        return x + butterfly_blk(h, self.w[2], self.w[3])
+    def forward(self, x, stream, table, cache=None, at=0):
+        """``x``: what the block before adds to the residual ``stream``, and so returned."""
+        x, stream = (rms_norm(x, self.norms[0]), x) if stream is None else rms_norm(x, self.norms[0], residual=stream)
+        x, stream = rms_norm(self.attention(x, table, cache, at), self.norms[1], residual=stream)
+        return butterfly_blk(F.silu(butterfly_blk(x, self.w[0], self.w[1])), self.w[2], self.w[3]), stream
 
 
 class TinyMonarchLM(torch.nn.Module):
@@ -39,15 +66,21 @@ class TinyMonarchLM(torch.nn.Module):
         super().__init__()
         self.wte = torch.nn.Parameter(torch.randn(VOCAB, WIDTH) * 0.02)
         self.blocks = torch.nn.ModuleList(Block() for _ in range(LAYERS))
-        self.ln_f = torch.nn.Parameter(torch.ones(WIDTH, dtype=torch.bfloat16))
+        self.ln_f = torch.nn.Parameter(torch.ones(WIDTH))
         self.lm_head = torch.nn.Parameter(torch.randn(VOCAB, WIDTH) * 0.02)
         self.to(torch.bfloat16)
+        self.register_buffer("table", rotary_table(DIM, SEQ), persistent=False)
 
-    def hidden(self, ids):
-        x = embedding(ids, self.wte, scale=WIDTH ** 0.5, padding_idx=PAD)
-        for b in self.blocks:
-            x = b(x)
-        return F.rms_norm(x, (WIDTH,), self.ln_f)
+    def hidden(self, ids, caches=None, at=0):
+        """Of ``ids`` (B, T), which stand at ``at`` on; ``caches``: one of each block for the tokens before."""
+        x, stream = embedding(ids, self.wte, scale=WIDTH ** 0.5, padding_idx=PAD), None
+        for i, b in enumerate(self.blocks):
+            x, stream = b(x, stream, self.table, None if caches is None else caches[i], at)
+        return rms_norm(x, self.ln_f, residual=stream)[0]
+
+    def caches(self, batch, length):
+        new = lambda heads, width: torch.empty(batch, length, heads, width, dtype=torch.bfloat16, device=self.wte.device)  # noqa: E731
+        return [(new(2 * HEADS, DIM), new(HEADS, 2 * DIM)) for _ in self.blocks]
 
     def loss(self, ids, targets, reduction="mean"):
         return linear_cross_entropy(self.hidden(ids), self.lm_head, targets, ignore_index=PAD, reduction=reduction)
@@ -90,9 +123,9 @@ def train(steps: int = 60, seed: int = 0, device: str = "cuda", verbose: bool = 
 def generate(model: TinyMonarchLM, token: int, count: int):
     """``count`` tokens after ``token``, the likeliest at each step, and the log-probability of each."""
     dev = model.wte.device
-    ids, scores = [token], []
-    for _ in range(count):
-        h = model.hidden(torch.tensor([ids[-1]], device=dev))
+    ids, scores, caches = [token], [], model.caches(1, count)
+    for at in range(count):
+        h = model.hidden(torch.tensor([[ids[-1]]], device=dev), caches, at)[0]
         best = (h.float() @ model.lm_head.float().T).argmax(-1)
         scores.append(-float(linear_cross_entropy(h, model.lm_head, best, reduction="sum")))
         ids.append(int(best))
