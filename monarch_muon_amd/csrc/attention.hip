@@ -366,7 +366,10 @@ ForwardPlan forward_plan(const mmuon_attention_args& a) {
   const int wide = wide_rows(a.dim);
   ForwardPlan p{false, 0, 1};
   if (rows == 0 || groups == 0) return p;
-  p.wide = groups * ((rows + wide - 1) / wide) >= 192;
+  // Workgroups of eight waves where they are enough.  us in turn, eight waves / pairs with split keys, heads
+  // of 2 x 64 (a wave for both maps against two): 96 workgroups 140 / 101, 128 185 / 136, 192 99 / 91,
+  // 256 188 / 185 and 32 / 35, 384 199 / 294; of 2 x 128 (pairs either way): 96 69 / 77, 192 53 / 57, 256 179 / 211.
+  p.wide = groups * ((rows + wide - 1) / wide) >= (a.dim > 64 ? 80 : 224);
   if (p.wide) {
     p.tiles = int((rows + wide - 1) / wide);
     p.splits = 1;
