@@ -813,10 +813,12 @@ int check_rotary(const mmuon_rotary_args* a) {
   return MMUON_OK;
 }
 
+// What a launch's threads and the kernels' indexes allow
 bool attention_sizes(const mmuon_attention_args* a) {
   return a != nullptr && a->batch >= 0 && a->queries >= 0 && a->keys >= 0 && a->heads >= 0 && a->kv_heads > 0 &&
          a->heads % a->kv_heads == 0 && a->dim >= 8 && a->dim <= 128 && a->dim % 8 == 0 &&
-         double(a->batch) * a->heads * a->queries < 2147483648.0 && double(a->batch) * a->kv_heads * a->keys < 2147483648.0;
+         a->heads < (1 << 22) && double(a->batch) * a->heads * a->queries < 1073741824.0 &&
+         double(a->batch) * a->kv_heads * a->keys < 2147482624.0 && double(a->batch) * a->kv_heads < 4194304.0;
 }
 
 int check_attention(const mmuon_attention_args* a, bool bwd) {
@@ -828,6 +830,11 @@ int check_attention(const mmuon_attention_args* a, bool bwd) {
     return fail(MMUON_EINVAL, "attention: heads (%d) must be a multiple of kv_heads (%d)", a->heads, a->kv_heads);
   if (!attention_sizes(a))
     return fail(MMUON_ERANGE, "attention: %d sequences of %d queries and %d keys are negative or too many", a->batch, a->queries, a->keys);
+  if (bwd && (double(a->batch) * a->heads * a->queries >= 268435456.0 || double(a->batch) * a->kv_heads * a->keys >= 1073741824.0))
+    return fail(MMUON_ERANGE, "attention: 2^28 query rows or 2^30 keys of all heads are too many for the backward");
+  if (bwd && a->queries > 1 && int64_t(a->heads) * 2 * a->dim >= (int64_t(1) << 22))
+    return fail(MMUON_ERANGE, "attention: output tokens %lld elements apart are beyond the kernels' tile offsets",
+                (long long)a->heads * 2 * a->dim);
   if (!(a->scale > 0.f) || !(a->scale <= 3.4e38f))
     return fail(MMUON_EINVAL, "attention: scale must be positive and finite (got %g)", a->scale);
   if (a->lam_stride != 0 && a->lam_stride != 1) return fail(MMUON_EINVAL, "attention: lam_stride must be 0 or 1");

@@ -225,15 +225,19 @@ __device__ __forceinline__ void join_dq(const mmuon_attention_args& a, int parts
   *reinterpret_cast<uint2*>(to) = make_uint2(f2bf2(s[0] * by, s[1] * by), f2bf2(s[2] * by, s[3] * by));
 }
 
-// dlam[h]: its rows of all sequences and parts, in order by thread and then in a tree; 256 threads
+// dlam[h]: its rows of all sequences and parts, in order by thread and then in a tree; 256 threads, each
+// with loads in flight also where sequences are short (a sequence after the other: SHORT)
 __device__ __forceinline__ void sum_dlam(const mmuon_attention_args& a, int parts, const RowSpace& space, int h, float* scratch) {
   float s = 0.f;
-  for (int i = 0; i < parts * a.batch; ++i) {
-    const float* from = space.dlam + (int64_t(i) * a.heads + h) * a.queries;
-    float r = 0.f;
-#pragma unroll 4
-    for (int t = threadIdx.x; t < a.queries; t += 256) r += from[t];
-    s += r;
+  const int64_t all = int64_t(parts) * a.batch * a.queries;
+  const int over = 256 / max(a.queries, 1), rest = 256 - over * a.queries;
+  int i = int(threadIdx.x) / max(a.queries, 1), t = int(threadIdx.x) - i * a.queries;
+#pragma unroll 8
+  for (int64_t n = threadIdx.x; n < all; n += 256) {
+    s += space.dlam[(int64_t(i) * a.heads + h) * a.queries + t];
+    i += over;
+    t += rest;
+    if (t >= a.queries) t -= a.queries, ++i;
   }
   s = block_sum<256>(s, scratch);
   if (threadIdx.x == 0) a.dlam[h] = s;

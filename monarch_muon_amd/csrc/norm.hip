@@ -265,11 +265,25 @@ RowPlan row_plan(int64_t rows, int width, int columns) {
 }
 
 template <class T, int CPT, int OUT>
-void norm_launch(const mmuon_norm_args& a, int lanes, hipStream_t s) {
+void norm_launch(const mmuon_norm_args& all, int lanes, hipStream_t s) {
+  using S = typename T::storage;
   const int block = std::max(lanes, 256), each = block / lanes;
-  const dim3 grid(unsigned((a.rows + each - 1) / each));
-  if (block == 256) hipLaunchKernelGGL((norm_rows<T, CPT, 256, OUT>), grid, dim3(256), 0, s, a, lanes);
-  else hipLaunchKernelGGL((norm_rows<T, CPT, 512, OUT>), grid, dim3(block), 0, s, a, lanes);
+  // a launch holds fewer than 2^32 threads: more rows take several
+  const int64_t most = (int64_t(1) << 31) / lanes;
+  for (int64_t r = 0; r < all.rows; r += most) {
+    mmuon_norm_args a = all;
+    a.rows = std::min(all.rows - r, most);
+    a.x = static_cast<const S*>(all.x) + r * all.x_stride;
+    if (all.residual != nullptr) a.residual = static_cast<const S*>(all.residual) + r * all.residual_stride;
+    if (all.h != nullptr) a.h = static_cast<S*>(all.h) + r * all.width;
+    if (all.inv != nullptr) a.inv = all.inv + r;
+    constexpr bool codes = OUT == MMUON_F8E4M3 || OUT == MMUON_F8E5M2;
+    a.y = static_cast<char*>(all.y) + r * all.width * int64_t(codes ? 1 : sizeof(S));
+    if (codes) a.scale = all.scale + r * (all.group > 0 ? (all.width + 127) / 128 : 1);
+    const dim3 grid(unsigned((a.rows + each - 1) / each));
+    if (block == 256) hipLaunchKernelGGL((norm_rows<T, CPT, 256, OUT>), grid, dim3(256), 0, s, a, lanes);
+    else hipLaunchKernelGGL((norm_rows<T, CPT, 512, OUT>), grid, dim3(block), 0, s, a, lanes);
+  }
 }
 template <class T, int OUT>
 void norm_forward(const mmuon_norm_args& a, hipStream_t s) {

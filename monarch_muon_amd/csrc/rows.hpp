@@ -35,27 +35,21 @@ __device__ __forceinline__ u32x4_v pack_chunk(const float (&v)[4]) {
 }
 
 // A chunk's bits: `left` elements of the row from p on are there (left >= N: the whole chunk; the
-// others are 0).  NT: not kept in the caches.
-template <class T, bool NT = false>
+// others are 0).
+template <class T>
 __device__ __forceinline__ u32x4_v load_bits(const typename T::storage* p, int left) {
   constexpr int N = ROW_CHUNK<T>;
-  if (left >= N) {
-    const auto* q = reinterpret_cast<const u32x4_any*>(p);
-    if constexpr (NT) return __builtin_nontemporal_load(q);
-    else return *q;
-  }
+  if (left >= N) return *reinterpret_cast<const u32x4_any*>(p);
   float v[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) v[k] = k < left ? T::load(p, k) : 0.f;
   return pack_chunk(v);
 }
-template <class T, bool NT = false>
+template <class T>
 __device__ __forceinline__ void store_bits(typename T::storage* p, const u32x4_v& u, int left) {
   constexpr int N = ROW_CHUNK<T>;
   if (left >= N) {
-    auto* q = reinterpret_cast<u32x4_any*>(p);
-    if constexpr (NT) __builtin_nontemporal_store(u, q);
-    else *q = u;
+    *reinterpret_cast<u32x4_any*>(p) = u;
     return;
   }
   float v[N];
@@ -64,13 +58,13 @@ __device__ __forceinline__ void store_bits(typename T::storage* p, const u32x4_v
   for (int k = 0; k < N; ++k)
     if (k < left) T::store(p, k, v[k]);
 }
-template <class T, bool NT = false>
+template <class T>
 __device__ __forceinline__ void load_chunk(const typename T::storage* p, int left, float (&v)[ROW_CHUNK<T>]) {
-  unpack_chunk(load_bits<T, NT>(p, left), v);
+  unpack_chunk(load_bits<T>(p, left), v);
 }
-template <class T, bool NT = false>
+template <class T>
 __device__ __forceinline__ void store_chunk(typename T::storage* p, const float (&v)[ROW_CHUNK<T>], int left) {
-  store_bits<T, NT>(p, pack_chunk(v), left);
+  store_bits<T>(p, pack_chunk(v), left);
 }
 // N floats (2, or a multiple of 4), `left` of them there
 template <int N>

@@ -77,6 +77,27 @@ def test_many_rows(d):
     check(*inputs(24, 70, 333, 16, 8, d, seed=4), causal=False)
 
 
+@pytest.mark.parametrize("d", [24, 32, 40, 64])
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_workgroups_of_both_maps(d, causal):
+    """Workgroups whose waves have both maps: 256 of them, rows that end inside a wave, keys that end inside a tile."""
+    check(*inputs(16, 300, 333, 8, 8, d, seed=13), causal=causal)
+
+
+@pytest.mark.parametrize("d", [24, 64, 128])
+@pytest.mark.parametrize("B, T, H, K", [(1, 700, 1, 1), (2, 517, 4, 2), (1, 1100, 6, 1)])
+def test_gradients_in_parts(d, B, T, H, K):
+    """Few tiles of queries and of keys: both are split, parts of a triangle among them."""
+    q, k, v, lam = inputs(B, T, T, H, K, d, seed=14)
+    check(q, k, v, lam)
+    check(q, k, v, lam, lengths=torch.tensor([T - 40, 0])[:B])
+
+
+@pytest.mark.parametrize("B, T", [(700, 1), (300, 3), (90, 17), (9, 257)])
+def test_many_short_sequences(B, T):
+    check(*inputs(B, T, T, 4, 2, 64, seed=15))
+
+
 @pytest.mark.parametrize("d", [40, 64, 128])
 @pytest.mark.parametrize("Tq, lengths", [(1, [0, 1, 31, 32, 33, 200]), (7, [5, 7, 8, 64, 199, 200]), (200, [0, 3, 150, 199, 200, 64])])
 @pytest.mark.parametrize("causal", [True, False])

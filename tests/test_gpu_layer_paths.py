@@ -302,6 +302,25 @@ def test_norm_beyond_32_bit_offsets():
     assert ((gx[-5:].double() - dx).abs() <= xt).all() and ((gw.double() - dw).abs() <= wt).all()
 
 
+@pytest.mark.parametrize("codes", [False, True])
+def test_norm_of_more_rows_than_a_launch_holds(codes):
+    rows, width, each = (1 << 27) + 70, 65, 1 << 27    # 16 lanes of a row: 2^27 rows are 2^31 threads
+    if torch.cuda.get_device_properties(0).total_memory < 100 << 30:
+        pytest.skip("needs 40 GB")
+    x = randn(width, seed=4).expand(rows, width)
+    at = torch.tensor([0, 1, each - 1, each, each + 1, rows - 1], device=DEV)
+    w = randn(width, seed=5)
+    if codes:
+        y, scale = rms_norm_fp8(x, w)
+        one, s1 = rms_norm_fp8(x[:1], w)
+        assert torch.equal(y.view(torch.uint8)[at], one.view(torch.uint8).expand(6, width)) and torch.equal(scale[at], s1.expand(6, 1))
+        return
+    y = rms_norm(x, w)
+    ref, _, _, tol = oracle.norm(x[:1], w)
+    assert ((y[at].double() - ref).abs() <= tol).all() and torch.equal(y[at], y[:1].expand(6, width))
+    assert torch.equal(y[each:], y[:70])
+
+
 def test_rotary_beyond_32_bit_offsets():
     q = torch.zeros(40, 20000, 64, 128, dtype=torch.bfloat16, device=DEV)   # 6.6e9 elements
     q[-1, -1] = randn(64, 128, seed=1)

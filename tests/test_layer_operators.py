@@ -282,6 +282,17 @@ def test_attention_entry_points_validate(change, code, match):
         assert rc == code and match in why, why
 
 
+@pytest.mark.parametrize("change, forward", [
+    (dict(heads=1 << 22, kv_heads=1), True), (dict(batch=1 << 22), True), (dict(batch=1 << 18, queries=1 << 12), True),
+    (dict(batch=1 << 16, queries=1 << 12), False), (dict(batch=1 << 16, keys=1 << 15), True), (dict(batch=1 << 16, keys=1 << 14), False),
+    (dict(heads=1 << 14, kv_heads=1, dim=128, queries=2), False)])
+def test_attention_entry_points_refuse_what_a_launch_cannot_hold(change, forward):
+    sizes = {**ATTENTION, "heads": 1, "kv_heads": 1, "batch": 1, "queries": 1, "keys": 1, **change}
+    for fn in ("mmuon_attention_fwd",) * forward + ("mmuon_attention_bwd",):
+        rc, why = refusal(fn, _abi.AttentionArgs(**sizes))
+        assert rc == -3 and ("too many" in why or "tile offsets" in why), why
+
+
 def test_workspaces_of_sizes_at_the_ends():
     """No size makes the plans divide by zero, and none that is refused has a workspace."""
     lib = _abi.lib()
