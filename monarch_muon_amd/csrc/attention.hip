@@ -370,6 +370,11 @@ ForwardPlan forward_plan(const mmuon_attention_args& a) {
   // of 2 x 64 (a wave for both maps against two): 96 workgroups 140 / 101, 128 185 / 136, 192 99 / 91,
   // 256 188 / 185 and 32 / 35, 384 199 / 294; of 2 x 128 (pairs either way): 96 69 / 77, 192 53 / 57, 256 179 / 211.
   p.wide = groups * ((rows + wide - 1) / wide) >= (a.dim > 64 ? 80 : 224);
+  // But not where most of those waves would have no rows.  512 groups over 4096 keys, heads of 2 x 64: 1 row
+  // 296 / 193, 64 rows 305 / 220, 100 rows 340 / 518; of 2 x 128: 1 row 361 / 351, 64 rows 361 / 710; 16384 groups
+  // of 16 rows and keys 341 / 105 and 502 / 279.  One row of 2 x 128: 128 groups 136 / 112, 192 140 / 159, 256 183 / 196
+  // (one such workgroup to a CU has as many loads on their way as two pairs, and needs no join), 320 310 / 251.
+  if (rows * 4 <= wide) p.wide = a.dim > 64 && groups > 160 && groups <= 256;
   if (p.wide) {
     p.tiles = int((rows + wide - 1) / wide);
     p.splits = 1;
