@@ -261,7 +261,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void attend(mmuon_a
 // The parts of a row's keys, joined by WAVES waves: each part's factor first, then the sums of every
 // WAVES-th part to a wave, which are added in order.
 constexpr int JOIN = 8;            // waves of a workgroup
-constexpr int ALONE_PARTS = 8;    // parts that a wave joins alone
+constexpr int ALONE_PARTS = 32;  // parts that a wave can join alone
 constexpr int MOST_PARTS = 1024;
 template <int D, int WAVES>
 __global__ __launch_bounds__(64 * JOIN) void attend_join(mmuon_attention_args a, int splits, Parts parts) {
@@ -366,24 +366,35 @@ ForwardPlan forward_plan(const mmuon_attention_args& a) {
   const int wide = wide_rows(a.dim);
   ForwardPlan p{false, 0, 1};
   if (rows == 0 || groups == 0) return p;
-  // Workgroups of eight waves where they are enough.  us in turn, eight waves / pairs with split keys, heads
-  // of 2 x 64 (a wave for both maps against two): 96 workgroups 140 / 101, 128 185 / 136, 192 99 / 91,
-  // 256 188 / 185 and 32 / 35, 384 199 / 294; of 2 x 128 (pairs either way): 96 69 / 77, 192 53 / 57, 256 179 / 211.
-  p.wide = groups * ((rows + wide - 1) / wide) >= (a.dim > 64 ? 80 : 224);
-  // But not where most of those waves would have no rows.  512 groups over 4096 keys, heads of 2 x 64: 1 row
-  // 296 / 193, 64 rows 305 / 220, 100 rows 340 / 518; of 2 x 128: 1 row 361 / 351, 64 rows 361 / 710; 16384 groups
-  // of 16 rows and keys 341 / 105 and 502 / 279.  One row of 2 x 128: 128 groups 136 / 112, 192 140 / 159, 256 183 / 196
-  // (one such workgroup to a CU has as many loads on their way as two pairs, and needs no join), 320 310 / 251.
-  if (rows * 4 <= wide) p.wide = a.dim > 64 && groups > 160 && groups <= 256;
-  if (p.wide) {
-    p.tiles = int((rows + wide - 1) / wide);
-    p.splits = 1;
+  // Pairs: as many workgroups as are resident, each of four tiles of keys at least
+  p.tiles = int((rows + 31) / 32);
+  const Pace pair = a.dim > 64 ? Pace{512, 0.049, 0.049, 5, 4e6} : Pace{1024, 0.050, 0.030, 5, 4e6};
+  const int64_t most = std::min<int64_t>(MOST_PARTS, std::max(1, (a.keys + 127) / 128));
+  p.splits = int(std::max<int64_t>(1, std::min(most, pair.resident / (groups * p.tiles))));
+  const int64_t wide_tiles = (rows + wide - 1) / wide, wides = groups * wide_tiles;
+  if (rows * 4 <= wide) {
+    // Few rows of a group, over which eight waves would not be spread, are bound by the loads.  512 groups over
+    // 4096 keys, heads of 2 x 64, eight waves / pairs: 1 row 296 / 193 us, 64 rows 305 / 220; of 2 x 128: 1 row 361 / 351;
+    // 16384 groups of 16 rows and keys 341 / 105 and 502 / 279.  One row of 2 x 128: 128 groups 136 / 112, 192 140 / 159,
+    // 256 183 / 196 (eight waves to a CU have as many loads on their way as two pairs, and need no join), 320 310 / 251.
+    p.wide = a.dim > 64 && groups > 160 && groups <= 256;
+    if (p.wide) p.tiles = int(wide_tiles), p.splits = 1;
     return p;
   }
-  p.tiles = int((rows + 31) / 32);
-  // as many workgroups as are resident, each of four tiles of keys at least
-  const int64_t resident = a.dim > 64 ? 512 : 1024, most = std::min<int64_t>(MOST_PARTS, std::max(1, (a.keys + 127) / 128));
-  p.splits = int(std::max<int64_t>(1, std::min(most, resident / (groups * p.tiles))));
+  // More are bound by products and exponentials: what the estimate finds shortest.  us measured, pairs / eight waves in
+  // one part / in the parts that it takes: heads of 2 x 128, 1 x 8192 tokens, 1 head 212 / 334 / 104 (6), 4 heads 402 /
+  // 342 / 272 (2); 4096, 4 heads 197 / 174 / 106 (3); 1024, 4 heads 34 / 50 / -; of 2 x 64, 8192, 4 heads 243 / 354 / 173 (4);
+  // 2048, 8 heads 61 / 94 / -; 3 x 1001, 6 heads on 2 36 / 51 / -; 2 x 128, 3 x 208 over 5102, 12 heads on 6 143 / 211 / 111 (3).
+  const double fewest = a.causal ? std::max(0, a.keys - a.queries) : a.keys, mean = 0.5 * (a.keys + fewest);
+  const double part = double(groups) * rows * (4 * (a.dim > 64 ? 128 : a.dim > 32 ? 64 : 32) + 8) * 4;
+  double best = 0.95 * estimate({groups * p.tiles, double(a.keys), mean, fewest}, pair, p.splits, part);  // pairs where the two are near
+  const Pace eight = a.dim > 64 ? Pace{256, 0.042, 0.042, 5, 4e6} : Pace{256, 0.0435, 0.0435, 5, 4e6};
+  for (int splits = 1; splits <= ALONE_PARTS && (splits == 1 || (wides * splits <= 512 && splits * 64 <= a.keys)); ++splits) {
+    const double t = estimate({wides, double(a.keys), mean, fewest}, eight, splits, part);
+    if (t >= best) continue;
+    best = t;
+    p = {true, int(wide_tiles), splits};
+  }
   return p;
 }
 
@@ -398,13 +409,17 @@ void attend_dim(const mmuon_attention_args& a, hipStream_t s) {
   const ForwardPlan p = forward_plan(a);
   Parts parts{};
   constexpr int MAPS = D == 128 ? 1 : 2;
-  if (p.wide) return attend_launch<D, (D == 128 ? 32 : 64), 8, MAPS, 3, false>(a, p, parts, s);
+  constexpr int TK = D == 128 ? 32 : 64;
+  if (p.wide && p.splits == 1) return attend_launch<D, TK, 8, MAPS, 3, false>(a, p, parts, s);
   if (p.splits == 1) return attend_launch<D, 32, 2, 1, 2, false>(a, p, parts, s);
   const int64_t rows = int64_t(a.heads / a.kv_heads) * a.queries * a.batch * a.kv_heads;
   parts.stats = static_cast<float4*>(a.workspace);
   parts.sums = static_cast<float*>(a.workspace) + rows * p.splits * 8;
-  attend_launch<D, 32, 2, 1, 2, true>(a, p, parts, s);
-  if (p.splits <= ALONE_PARTS)
+  if (p.wide) attend_launch<D, TK, 8, MAPS, 3, true>(a, p, parts, s);
+  else attend_launch<D, 32, 2, 1, 2, true>(a, p, parts, s);
+  // A wave to a row where the parts are few or the rows alone fill the chip (8192 rows of 2 x 64, 9 parts: forward 120
+  // us with eight waves to a row, 82 with one)
+  if (p.splits <= 8 || (p.splits <= ALONE_PARTS && rows >= 2048))
     hipLaunchKernelGGL((attend_join<D, 1>), dim3(unsigned((rows + JOIN - 1) / JOIN)), dim3(64 * JOIN), 0, s, a, p.splits, parts);
   else hipLaunchKernelGGL((attend_join<D, JOIN>), dim3(unsigned(rows)), dim3(64 * JOIN), 0, s, a, p.splits, parts);
 }

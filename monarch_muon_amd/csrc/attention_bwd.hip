@@ -457,29 +457,50 @@ __global__ __launch_bounds__(256) void attention_join(mmuon_attention_args a, in
   else join_dkv<D>(a, of_rows, space, int64_t(blockIdx.x - of_dq) * 256 + threadIdx.x);
 }
 
-// Parts of the queries (of all heads that share the keys): where the keys' tiles fill less than half of the
-// chip, as many as fill it, each of eight tiles of queries at least.  3 x 1001 tokens, 6 heads of 2 x 64 on 2:
-// dk and dv 181 us in one part, 45 in ten.
-constexpr int KEY_WAVES = 4;
+int template_dim(const mmuon_attention_args& a) { return a.dim > 64 ? 128 : a.dim > 32 ? 64 : 32; }
+// Parts of a loop of `most` steps that the estimate finds shortest, each of eight steps at least
+int fewest_us(const Items& n, const Pace& p, double part_bytes) {
+  int best = 1;
+  double least = estimate(n, p, 1, part_bytes);
+  for (int splits = 2; splits <= 16 && splits * 8 <= n.most; ++splits) {
+    const double t = estimate(n, p, splits, part_bytes);
+    if (t < least) least = t, best = splits;
+  }
+  return best;
+}
+// Pairs of a query and a key that it sees, of one head
+double seen_pairs(const mmuon_attention_args& a) {
+  const double q = a.queries, k = a.keys;
+  return !a.causal ? q * k : k >= q ? q * k - q * q / 2 : k * k / 2;
+}
+constexpr int KEY_WAVES = 4, ROW_WAVES = 4;
+// Parts of the queries (of all heads that share the keys).  Units of the estimate are steps of 32 queries.  us
+// of all launches of a pass, dk and dv in one part / in as many as fill the chip / in those that the estimate takes:
+// heads of 2 x 64, 3 x 1001 tokens, 6 heads on 2 231 / 86 / 86 (10); 1 x 8192, 4 heads 670 / 433 / 385 (3), 1 head 534 / 149 /
+// 149; of 2 x 128, 8192, 4 heads 1192 / 1192 / 910 (2), 4096, 16 heads on 4 1772 / 1071 / 751 (4): under a causal mask
+// the first keys' workgroups are much longer than the mean.
 int key_parts(const mmuon_attention_args& a) {
   const int64_t tiles = int64_t(a.batch) * a.kv_heads * ((a.keys + 32 * KEY_WAVES - 1) / (32 * KEY_WAVES));
-  const int64_t resident = a.dim > 64 ? 256 : 512, steps = int64_t(a.heads / a.kv_heads) * ((a.queries + 31) / 32);
-  if (tiles == 0 || tiles * 2 > resident) return 1;
-  return int(std::max<int64_t>(1, std::min<int64_t>({resident / tiles, steps / 8, 16})));
+  if (tiles == 0 || a.queries == 0 || a.heads == 0) return 1;
+  const double share = a.heads / a.kv_heads / 32.0;
+  const Items n{tiles, share * (a.causal ? std::min(a.queries, a.keys) : a.queries), share * seen_pairs(a) / a.keys,
+                share * (!a.causal || a.keys / 2 >= a.queries ? a.queries : 0)};
+  const Pace p = a.dim > 64 ? Pace{256, 2.7, 2.7, 22, 8e6} : Pace{512, 2.3, 1.7, 20, 8e6};
+  return fewest_us(n, p, double(a.batch) * a.kv_heads * a.keys * 4 * template_dim(a) * 4);
 }
-// Parts of the keys, likewise (4 heads of 2 x 128, 2000 tokens: dq 112 us in one part, 48 in four)
-constexpr int ROW_WAVES = 4;
+// Parts of the keys, likewise.  8192 tokens, 4 heads of 2 x 128: dq in one part 1192 us, in two 1036; 4096 tokens,
+// 4 heads of 2 x 64: one 233, four 148.
 int64_t row_tiles(const mmuon_attention_args& a) {
   return (int64_t(a.heads / a.kv_heads) * a.queries + 32 * ROW_WAVES - 1) / (32 * ROW_WAVES);
 }
 int row_parts(const mmuon_attention_args& a) {
   const int64_t tiles = int64_t(a.batch) * a.kv_heads * row_tiles(a);
-  const int64_t resident = a.dim > 64 ? 256 : 512, steps = (a.keys + 31) / 32;
-  if (tiles == 0 || tiles * 2 > resident) return 1;
-  return int(std::max<int64_t>(1, std::min<int64_t>({resident / tiles, steps / 8, 16})));
+  if (tiles == 0 || a.keys == 0) return 1;
+  const Items n{tiles, a.keys / 32.0, seen_pairs(a) / a.queries / 32, (a.causal ? std::max(0, a.keys - a.queries) : a.keys) / 32.0};
+  const Pace p = a.dim > 64 ? Pace{256, 1.6, 1.6, 20, 8e6} : Pace{512, 1.45, 0.95, 18, 8e6};
+  return fewest_us(n, p, double(a.batch) * a.heads * a.queries * 2 * template_dim(a) * 4);
 }
 
-int template_dim(const mmuon_attention_args& a) { return a.dim > 64 ? 128 : a.dim > 32 ? 64 : 32; }
 struct BackwardLayout {
   size_t dlam, dq, dkv, total;  // floats; the rows' statistics come first
 };

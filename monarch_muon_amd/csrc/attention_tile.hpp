@@ -13,6 +13,8 @@
 // 16-row step holds rows 4 h .. 4 h + 3 and 8 + 4 h .. 8 + 4 h + 3 (read_turned).
 #pragma once
 
+#include <algorithm>
+
 #include "mfma_tile.hpp"
 
 namespace mmuon {
@@ -195,6 +197,26 @@ inline Dealing dealing(int64_t groups, int64_t each) {
   return d;
 }
 inline unsigned blocks_of(const Dealing& d) { return unsigned(int64_t(d.across) * d.groups * d.each); }
+
+// Workgroups of a launch, and the length of the longest, the mean and the shortest one's loop
+struct Items {
+  int64_t count;
+  double most, mean, fewest;
+};
+// us of a unit of that length: with as many workgroups resident as there is room for, and by itself where
+// others are through; of a workgroup beside its loop; bytes a us at which parts are written and joined
+struct Pace {
+  int64_t resident;
+  double full, alone, beside, parts;
+};
+// us of a launch with its loops in `splits` parts, and of joining them: the longest workgroup, all of them over
+// those that are resident, or rounds of the shortest
+inline double estimate(const Items& n, const Pace& p, int64_t splits, double part_bytes) {
+  const double rounds = double((n.count * splits + p.resident - 1) / p.resident);
+  const double t = std::max({n.most * p.alone / splits + p.beside, double(n.count) * splits * (n.mean * p.full / splits + p.beside) / p.resident,
+                             rounds * (n.fewest * p.full / splits + p.beside)});
+  return splits == 1 ? t : t + 5 + 2 * splits * part_bytes / p.parts;
+}
 
 // The sequence's keys and the place of its first query among them
 struct Span {

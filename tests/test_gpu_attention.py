@@ -142,6 +142,18 @@ def test_starts(d):
     check(q, k, v, lam, starts=torch.tensor([0, -100, 10, 30]), lengths=torch.tensor([0, 20, 30, 30]))
 
 
+@pytest.mark.parametrize("d, B, H, K, Tk, Tq", [(64, 1, 8, 2, 16384, 300), (32, 1, 8, 2, 9001, 300), (128, 3, 12, 6, 5102, 208),
+                                                (104, 1, 4, 4, 4099, 1023), (48, 2, 2, 2, 3333, 3333), (128, 1, 1, 1, 4200, 4200)])
+def test_split_keys_of_many_rows(d, B, H, K, Tk, Tq):
+    """A prompt of few heads: workgroups of eight waves over parts of the keys."""
+    q, k, v, lam = inputs(B, Tq, Tk, H, K, d, seed=16)
+    check(q, k, v, lam)
+    check(q, k, v, lam, causal=False, grads=False)
+    lengths = torch.tensor([Tk - 700, 0, 3000])[:B]
+    check(q, k, v, lam, lengths=lengths, grads=False)
+    check(q, k, v, lam, lengths=lengths, starts=torch.tensor([3, 0, -100])[:B], grads=False)
+
+
 @pytest.mark.parametrize("d, B, H, K, Tk, Tq", [(64, 1, 1, 1, 5000, 1), (128, 1, 2, 1, 3001, 1), (128, 3, 8, 2, 777, 1), (32, 2, 4, 4, 4097, 2),
                                                 (64, 2, 6, 2, 1025, 5), (128, 1, 4, 1, 600, 33), (96, 1, 1, 1, 20000, 1), (64, 5, 2, 2, 129, 1)])
 def test_split_keys(d, B, H, K, Tk, Tq):
