@@ -566,7 +566,7 @@ typedef struct mmuon_attention_args {
   void* o;                /* out (batch, queries, heads, 2 dim), contiguous */
   float* o1;              /* out, or null: of o's shape, contiguous; backward in */
   float* o2;
-  float* lse;             /* out, or null: (batch, heads, queries, 2); backward in */
+  float* lse;             /* out, or null: (batch, heads, queries, 4), 16-B aligned; backward in */
   const void* dout;       /* backward in: of o's shape, contiguous */
   void* dq;               /* backward out, contiguous; dq and dlam, or dk and dv, may both be null */
   void* dk;

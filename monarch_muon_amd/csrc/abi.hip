@@ -852,7 +852,7 @@ int check_attention(const mmuon_attention_args* a, bool bwd) {
   if ((queries && a->lam == nullptr) || misplaced(a->lam, MMUON_F32)) return fail(MMUON_EINVAL, "attention: null or unaligned lam");
   if (((reinterpret_cast<uintptr_t>(a->lengths) | reinterpret_cast<uintptr_t>(a->starts)) & 7) != 0)
     return fail(MMUON_EINVAL, "attention: unaligned lengths or starts");
-  if (bad(a->o1, bwd && queries) || bad(a->o2, bwd && queries) || (bwd && queries && a->lse == nullptr) || misplaced(a->lse, MMUON_F32) ||
+  if (bad(a->o1, bwd && queries) || bad(a->o2, bwd && queries) || bad(a->lse, bwd && queries) ||
       (a->o1 == nullptr) != (a->o2 == nullptr))
     return fail(MMUON_EINVAL, "attention: o1, o2 and lse go together, aligned");
   if (bwd) {

@@ -36,6 +36,14 @@ struct Parts {
   float4* stats;  // [row][map]
 };
 
+// log2 of the sum of a row's 2^(s - shift), shift still on it, and what 2^(s - that) is to be multiplied by
+// for what the logarithm's rounding took (up to 1e-6 of it, the same for all of the row).  Of a row that sees nothing
+// +inf, so that its probabilities are 0.
+__device__ __forceinline__ void store_lse(float* to, float shift, float sum) {
+  const float lse = sum == 0.f ? INFINITY : shift + __builtin_amdgcn_logf(sum);
+  *reinterpret_cast<float2*>(to) = make_float2(lse, sum == 0.f ? 1.f : __builtin_amdgcn_exp2f(lse - shift) / sum);
+}
+
 // MAPS: maps of a wave
 template <int D, int TK, int WAVES, int MAPS, int SLOTS, bool SPLIT>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void attend(mmuon_attention_args a, int tiles, int splits, Dealing dealt, Parts parts) {
@@ -106,7 +114,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void attend(mmuon_a
   float ref[MAPS], shift[MAPS], sum[MAPS], weight[MAPS];  // sum: of exact probabilities; weight: of the rounded ones
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) ref[m] = -INFINITY, shift[m] = sum[m] = weight[m] = 0.f;
-  const float scale = a.scale * LOG2E;
+  const float scale = scale_of(a);
 
   const int n = t1 - t0;
 #pragma unroll
@@ -219,9 +227,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void attend(mmuon_a
         }
       }
     }
-    if (a.lse != nullptr && in && half == 0)  // base 2; of a row that sees nothing +inf, so that its probabilities are 0
-      a.lse[((int64_t(b) * a.heads + h) * a.queries + t) * 2 + m0 + m] =
-          sum[m] == 0.f ? INFINITY : shift[m] + __builtin_amdgcn_logf(sum[m]);
+    if (a.lse != nullptr && in && half == 0)
+      store_lse(a.lse + ((int64_t(b) * a.heads + h) * a.queries + t) * 4 + 2 * (m0 + m), shift[m], sum[m]);
   }
   const float lam = a.lam[int64_t(h) * a.lam_stride];
   uint16_t* o = in ? static_cast<uint16_t*>(a.o) + at * 2 * a.dim : nullptr;
@@ -347,9 +354,9 @@ __global__ __launch_bounds__(64 * JOIN) void attend_join(mmuon_attention_args a,
     }
   }
   if (a.lse != nullptr && part0 == 0 && lane == 0) {
-    float* lse = a.lse + ((int64_t(b) * a.heads + h) * a.queries + t) * 2;
-    lse[0] = l1 == 0.f ? INFINITY : top1 + __builtin_amdgcn_logf(l1);
-    lse[1] = l2 == 0.f ? INFINITY : top2 + __builtin_amdgcn_logf(l2);
+    float* lse = a.lse + ((int64_t(b) * a.heads + h) * a.queries + t) * 4;
+    store_lse(lse, top1, l1);
+    store_lse(lse + 2, top2, l2);
   }
 }
 

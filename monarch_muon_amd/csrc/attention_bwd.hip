@@ -10,6 +10,11 @@
 // rounded to bf16, are the next products' operands as they stand.  dlam takes P_2 dP in fp32 as dq's
 // kernel has them: o_2, from rounded probabilities, would give it their error.
 //
+// dq's dS goes in as two bf16 terms (dS and what its rounding left): D's error, from rounded weights, and dS's
+// rounding together would make it 2.4e-3 to 2.6e-3 off, where rounding the result alone makes 1.7e-3; so it is 1.7e-3 to
+// 1.8e-3, for 10 us of 85 to 95 (16 x 1024 tokens, 8 heads of 2 x 64: 88 -> 99; 4 x 1024, 16 of 2 x 128: 94 -> 105).
+// dk and dv, 2.4e-3 off, have one.
+//
 // Both kernels have both maps in a wave, which makes no product twice.  With heads of up to 64 columns
 // two waves fit a SIMD, whose products and exponentials run side by side; with more a wave's sums for dk
 // and dv alone are half of its registers.  (A map to each of two waves that pass dP and P through LDS:
@@ -55,7 +60,7 @@ __global__ __launch_bounds__(256) void attention_rows(mmuon_attention_args a, Ro
     d1 += __shfl_xor(d1, o, 64);
     d2 += __shfl_xor(d2, o, 64);
   }
-  if (lane == 0) space.stats[row] = make_float4(a.lse[2 * row], d1, a.lse[2 * row + 1], d2);
+  if (lane == 0) space.stats[row] = make_float4(a.lse[4 * row], d1, a.lse[4 * row + 2], d2);
 }
 
 // dq and each row's part of dlam: 32 queries to a wave, over tiles of 32 keys
@@ -114,7 +119,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmu
   }
   const int64_t at = (int64_t(b) * a.heads + h) * a.queries + t;
   const float4 st = space.stats[at];
-  const float scale = a.scale * LOG2E;
+  const float by1 = a.lse[4 * at + 1], by2 = a.lse[4 * at + 3];
+  const float scale = scale_of(a);
   f32x16 acc[2][D / 32];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -159,23 +165,33 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmu
     }
 #pragma unroll
     for (int e = 0; e < 16; ++e) d1[e] *= dp[e] - st.y;
-    const bf16x8 x1[2] = {operand(d1), operand(d1 + 8)};
+    const bf16x8 x1[2] = {operand(d1), operand(d1 + 8)}, y1[2] = {operand_rest(d1, x1[0]), operand_rest(d1 + 8, x1[1])};
 #pragma unroll
     for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-      for (int y = 0; y < 2; ++y) acc[0][j] = mfma(read_turned<CA>(tile_at, tbase, 16 * y, j), x1[y], acc[0][j]);
+      for (int y = 0; y < 2; ++y) {
+        const bf16x8 k = read_turned<CA>(tile_at, tbase, 16 * y, j);
+        acc[0][j] = mfma(k, x1[y], acc[0][j]);
+        acc[0][j] = mfma(k, y1[y], acc[0][j]);
+      }
+    float tile_along = 0.f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      along = fmaf(d2[e], dp[e], along);
+      tile_along = fmaf(d2[e], dp[e], tile_along);
       d2[e] *= dp[e] - st.w;
     }
-    const bf16x8 x2[2] = {operand(d2), operand(d2 + 8)};
+    along += tile_along;
+    const bf16x8 x2[2] = {operand(d2), operand(d2 + 8)}, y2[2] = {operand_rest(d2, x2[0]), operand_rest(d2 + 8, x2[1])};
 #pragma unroll
     for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-      for (int y = 0; y < 2; ++y) acc[1][j] = mfma(read_turned<CA>(tile_at + T::A2, tbase, 16 * y, j), x2[y], acc[1][j]);
+      for (int y = 0; y < 2; ++y) {
+        const bf16x8 k = read_turned<CA>(tile_at + T::A2, tbase, 16 * y, j);
+        acc[1][j] = mfma(k, x2[y], acc[1][j]);
+        acc[1][j] = mfma(k, y2[y], acc[1][j]);
+      }
   }
-  along = half_sum(along);
+  along = half_sum(along) * by2;
   const int64_t total = int64_t(a.batch) * a.heads * a.queries;
   if (in && half == 0) space.dlam[part * total + at] = -along;
   if constexpr (SPLIT) {
@@ -186,9 +202,11 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmu
 #pragma unroll
       for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-        for (int e = 0; e < 16; e += 4)
+        for (int e = 0; e < 16; e += 4) {
+          const float by = m ? by2 : by1;
           *reinterpret_cast<float4*>(to + m * D + 32 * j + 2 * e) =
-              make_float4(acc[m][j][e], acc[m][j][e + 1], acc[m][j][e + 2], acc[m][j][e + 3]);
+              make_float4(acc[m][j][e] * by, acc[m][j][e + 1] * by, acc[m][j][e + 2] * by, acc[m][j][e + 3] * by);
+        }
     return;
   }
   const float lam = a.lam[int64_t(h) * a.lam_stride];
@@ -197,8 +215,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmu
   for (int j = 0; j < D / 32; ++j) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      acc[0][j][e] *= a.scale;
-      acc[1][j][e] *= -(lam * a.scale);
+      acc[0][j][e] *= a.scale * by1;
+      acc[1][j][e] *= -(lam * a.scale) * by2;
     }
     store_turned(dq, acc[0][j], j, a.dim, half);
     store_turned(dq != nullptr ? dq + a.dim : nullptr, acc[1][j], j, a.dim, half);
@@ -225,10 +243,11 @@ __device__ __forceinline__ void join_dq(const mmuon_attention_args& a, int parts
   *reinterpret_cast<uint2*>(to) = make_uint2(f2bf2(s[0] * by, s[1] * by), f2bf2(s[2] * by, s[3] * by));
 }
 
-// dlam[h]: its rows of all sequences and parts, in order by thread and then in a tree; 256 threads, each
-// with loads in flight also where sequences are short (a sequence after the other: SHORT)
-__device__ __forceinline__ void sum_dlam(const mmuon_attention_args& a, int parts, const RowSpace& space, int h, float* scratch) {
-  float s = 0.f;
+// dlam[h]: its rows of all sequences and parts, which may cancel, in 64 bits, in order by thread and then in a
+// tree; 256 threads, each with loads in flight also where sequences are short (4096 x 4 tokens, 8 heads: a pass
+// 2800 us with a sequence after the other, 1610 so)
+__device__ __forceinline__ void sum_dlam(const mmuon_attention_args& a, int parts, const RowSpace& space, int h, double* scratch) {
+  double s = 0.0;
   const int64_t all = int64_t(parts) * a.batch * a.queries;
   const int over = 256 / max(a.queries, 1), rest = 256 - over * a.queries;
   int i = int(threadIdx.x) / max(a.queries, 1), t = int(threadIdx.x) - i * a.queries;
@@ -239,11 +258,13 @@ __device__ __forceinline__ void sum_dlam(const mmuon_attention_args& a, int part
     t += rest;
     if (t >= a.queries) t -= a.queries, ++i;
   }
-  s = block_sum<256>(s, scratch);
-  if (threadIdx.x == 0) a.dlam[h] = s;
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if (threadIdx.x % 64 == 0) scratch[threadIdx.x / 64] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) a.dlam[h] = float(scratch[0] + scratch[1] + scratch[2] + scratch[3]);
 }
 __global__ __launch_bounds__(256) void attention_dlam(mmuon_attention_args a, int parts, RowSpace space) {
-  __shared__ float scratch[4];
+  __shared__ double scratch[4];
   sum_dlam(a, parts, space, blockIdx.x, scratch);
 }
 
@@ -263,7 +284,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mm
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (int(blockIdx.x) >= dlam_at) {
     static_assert(WAVES == 4, "256 threads");
-    return sum_dlam(a, of_keys, space, blockIdx.x - dlam_at, reinterpret_cast<float*>(ring));
+    return sum_dlam(a, of_keys, space, blockIdx.x - dlam_at, reinterpret_cast<double*>(ring));
   }
   int group, item;
   if (!deal(dealt, a.batch * a.kv_heads, group, item)) return;
@@ -325,7 +346,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mm
             lds_addr(values) + (wave * (CB / 2) + i) * 1024);
     }
   }
-  const float scale = a.scale * LOG2E;
+  const float scale = scale_of(a);
   f32x16 dv[D / 16], dk[2][D / 32];
 #pragma unroll
   for (int j = 0; j < D / 16; ++j) dv[j] = f32x16{};

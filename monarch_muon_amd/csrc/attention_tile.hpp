@@ -20,7 +20,9 @@
 namespace mmuon {
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f;
+// The scores' factor, for powers of 2: rounded once, since what it is off by is the same for all scores and
+// shows in dlam, a sum that cancels
+__device__ __forceinline__ float scale_of(const mmuon_attention_args& a) { return float(double(a.scale) * 1.4426950408889634); }
 
 template <int CH>
 __device__ __forceinline__ int chunk_mask(int r) {
@@ -63,6 +65,19 @@ __device__ __forceinline__ bf16x8 operand(const float* v) {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   const u32x4 u = {f2bf2(v[0], v[1]), f2bf2(v[2], v[3]), f2bf2(v[4], v[5]), f2bf2(v[6], v[7])};
   return __builtin_bit_cast(bf16x8, u);
+}
+
+// What the rounding of those values to the operand left
+__device__ __forceinline__ bf16x8 operand_rest(const float* v, const bf16x8& rounded) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 u = __builtin_bit_cast(u32x4, rounded);
+  float r[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    r[2 * k] = v[2 * k] - __uint_as_float(u[k] << 16);
+    r[2 * k + 1] = v[2 * k + 1] - __uint_as_float(u[k] & 0xffff0000u);
+  }
+  return operand(r);
 }
 
 // c + the sum of an operand's eight values

@@ -451,7 +451,7 @@ Quad attention_impl(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
   const std::array<int64_t, 4> shape = {a.batch, a.queries, a.heads, 2 * a.dim};
   const at::IntArrayRef kept = save ? at::IntArrayRef(shape) : NONE;
   Tensor o = at::empty(shape, call.q.options()), o1 = at::empty(kept, call.q.options().dtype(at::kFloat)), o2 = at::empty(kept, o1.options());
-  Tensor lse = save ? at::empty({a.batch, a.heads, a.queries, 2}, call.q.options().dtype(at::kFloat))
+  Tensor lse = save ? at::empty({a.batch, a.heads, a.queries, 4}, call.q.options().dtype(at::kFloat))
                     : at::empty(NONE, call.q.options().dtype(at::kFloat));
   a.o = o.data_ptr();
   if (save) {
@@ -470,13 +470,13 @@ Quad attention_grad_impl(const Tensor& q, const Tensor& k, const Tensor& v, cons
                          const Tensor& dout_, bool causal, double scale, bool need_q, bool need_kv) {
   AttentionCall call(q, k, v, lam, lengths, starts, causal, scale);
   mmuon_attention_args& a = call.a;
-  const std::array<int64_t, 4> shape = {a.batch, a.queries, a.heads, 2 * a.dim}, two = {a.batch, a.heads, a.queries, 2};
+  const std::array<int64_t, 4> shape = {a.batch, a.queries, a.heads, 2 * a.dim}, four = {a.batch, a.heads, a.queries, 4};
   TORCH_CHECK_VALUE(dout_.sizes() == at::IntArrayRef(shape) && dout_.scalar_type() == at::kBFloat16,
                     "the gradient of differential_attention's output must be bfloat16 and of its shape, got ", dout_.sizes());
   for (const Tensor* t : {&o1, &o2})
     TORCH_CHECK_VALUE(t->sizes() == at::IntArrayRef(shape) && t->scalar_type() == at::kFloat, "o1 and o2 must be the forward's");
   require_one_device({&q, &o1, &o2, &dout_});
-  TORCH_CHECK_VALUE(lse.sizes() == at::IntArrayRef(two) && lse.scalar_type() == at::kFloat && lse.is_contiguous(),
+  TORCH_CHECK_VALUE(lse.sizes() == at::IntArrayRef(four) && lse.scalar_type() == at::kFloat && lse.is_contiguous(),
                     "lse must be the forward's");
   require_one_device({&q, &lse});
   const Tensor dout = dense_aligned(dout_), p1 = dense_aligned(o1), p2 = dense_aligned(o2);

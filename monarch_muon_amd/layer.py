@@ -55,7 +55,7 @@ def _load() -> None:
         if not save:
             return o, q.new_empty(0), q.new_empty(0), q.new_empty(0, dtype=torch.float32)
         f32 = dict(dtype=torch.float32)
-        return o, torch.empty_like(o, **f32), torch.empty_like(o, **f32), q.new_empty(B, heads // 2, T, 2, dtype=torch.float32)
+        return o, torch.empty_like(o, **f32), torch.empty_like(o, **f32), q.new_empty(B, heads // 2, T, 4, dtype=torch.float32)
 
     @torch.library.register_fake("mmuon::differential_attention_grad")
     def _(q, k, v, lam, lengths, starts, o1, o2, lse, dout, causal, scale, need_q, need_kv):

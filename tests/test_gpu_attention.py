@@ -231,6 +231,17 @@ def test_gradients_that_are_wanted():
         assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("d, B, T, H, K", [(16, 5, 531, 6, 6), (32, 1, 1431, 4, 4), (64, 2, 300, 24, 6), (128, 4, 229, 4, 4)])
+def test_queries_gradient_is_rounded_once(d, B, T, H, K):
+    """dq is its rounding away from the exact one, and little else: a uniform rounding to bf16 has 2^-8 / sqrt(3) at most."""
+    q, k, v, lam = inputs(B, T, T, H, K, d, seed=17)
+    dout = randn(B, T, H, 2 * d, seed=18)
+    refs, _ = oracle.attention(q, k, v, lam, dout=dout)
+    q.requires_grad_()
+    dq, = torch.autograd.grad(differential_attention(q, k, v, lam), q, dout)
+    assert float((dq.double() - refs[1]).norm() / refs[1].norm()) <= 2 ** -8 / 3 ** 0.5
+
+
 @pytest.mark.parametrize("d", [32, 128])
 def test_gradients_against_differences(d):
     """The directional derivative by differences of the float64 form; bf16 leaves its roundings."""
