@@ -817,7 +817,7 @@ int check_rotary(const mmuon_rotary_args* a) {
 bool attention_sizes(const mmuon_attention_args* a) {
   return a != nullptr && a->batch >= 0 && a->queries >= 0 && a->keys >= 0 && a->heads >= 0 && a->kv_heads > 0 &&
          a->heads % a->kv_heads == 0 && a->dim >= 8 && a->dim <= 128 && a->dim % 8 == 0 &&
-         a->heads < (1 << 22) && double(a->batch) * a->heads * a->queries < 1073741824.0 &&
+         a->heads < (1 << 22) && double(a->batch) * a->heads * a->queries < 536870912.0 &&
          double(a->batch) * a->kv_heads * a->keys < 2147482624.0 && double(a->batch) * a->kv_heads < 4194304.0;
 }
 

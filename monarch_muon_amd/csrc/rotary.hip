@@ -6,9 +6,10 @@
 // the others are copied.  The gradient's rotation is by -s.  The table holds cosines and sines (times
 // the scaling's factor) in fp32, made once in 64 bits, where the angles of far positions need them.
 //
-// A lane takes one chunk of 16 B (or two that are pairs) of a few heads of a token, with the cosines
-// and sines of the chunk in registers.  Bound by HBM: queries and keys are read and written once,
-// both in one launch; the table comes from the caches.
+// A lane takes one chunk of 16 B (or two that are pairs) of a head.  Bound by HBM: queries and keys are
+// read and written once, both in one launch (16384 tokens x 64 heads of 128, bf16: 92 us, 5.8 TB/s); the
+// table comes from the caches, so that four heads to a lane, which read it once, are no faster (in graphs of ten
+// calls 107 us, one head 98; 2048 tokens 13.1 one head, 12.6 four; 1024 7.5, 8.1; 256 5.0, 5.6).
 #include <algorithm>
 
 #include "common.hpp"
@@ -18,15 +19,16 @@
 namespace mmuon {
 namespace {
 
-template <class T, bool INTERLEAVED, int HEADS>
-__global__ __launch_bounds__(256) void rotary_rows(mmuon_rotary_args a, int turned, int items, int groups, float sign) {
+template <class T, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void rotary_rows(mmuon_rotary_args a, int turned, int items, float sign) {
   using S = typename T::storage;
   constexpr int N = ROW_CHUNK<T>, M = INTERLEAVED ? N / 2 : N;
-  const int64_t all = int64_t(a.batch) * a.tokens * groups * items;
+  const int heads = a.q_heads + a.k_heads;
+  const int64_t all = int64_t(a.batch) * a.tokens * heads * items;
   const int64_t id = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (id >= all) return;
-  const int64_t token = id / (groups * items);
-  const int rest = int(id - token * (groups * items)), group = rest / items, item = rest - group * items;
+  const int64_t token = id / (heads * items);
+  const int rest = int(id - token * (heads * items)), h = rest / items, item = rest - h * items;
   const int64_t b = token / a.tokens, t = token - b * a.tokens;
   const int half = a.part / 2;
   const bool turn = item < turned;
@@ -45,59 +47,42 @@ __global__ __launch_bounds__(256) void rotary_rows(mmuon_rotary_args a, int turn
       s[k] *= sign;
     }
   }
-  u32x4_v u[HEADS], v[HEADS];
-  const int heads = a.q_heads + a.k_heads;
-  const auto in_of = [&](int h) {
-    return h < a.q_heads ? static_cast<const S*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + h * a.q_stride[2]
-                         : static_cast<const S*>(a.k) + b * a.k_stride[0] + t * a.k_stride[1] + (h - a.q_heads) * a.k_stride[2];
-  };
+  const S* from = h < a.q_heads ? static_cast<const S*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + h * a.q_stride[2]
+                                : static_cast<const S*>(a.k) + b * a.k_stride[0] + t * a.k_stride[1] + (h - a.q_heads) * a.k_stride[2];
+  S* to = h < a.q_heads ? static_cast<S*>(a.q_out) + (token * a.q_heads + h) * a.dim
+                        : static_cast<S*>(a.k_out) + (token * a.k_heads + h - a.q_heads) * a.dim;
+  u32x4_v u = load_bits<T>(from + col, left);
+  if (turn) {
+    float x[N], y[N];
+    unpack_chunk(u, x);
+    if constexpr (INTERLEAVED) {
 #pragma unroll
-  for (int j = 0; j < HEADS; ++j) {
-    const int h = group + j * groups;
-    if (h >= heads) break;
-    const S* p = in_of(h) + col;
-    u[j] = load_bits<T>(p, left);
-    if (!INTERLEAVED && turn) v[j] = load_bits<T>(p + half, left);
-  }
-#pragma unroll
-  for (int j = 0; j < HEADS; ++j) {
-    const int h = group + j * groups;
-    if (h >= heads) break;
-    S* p = h < a.q_heads ? static_cast<S*>(a.q_out) + (token * a.q_heads + h) * a.dim
-                         : static_cast<S*>(a.k_out) + (token * a.k_heads + h - a.q_heads) * a.dim;
-    if (turn) {
-      float x[N], y[N];
-      unpack_chunk(u[j], x);
-      if constexpr (INTERLEAVED) {
-#pragma unroll
-        for (int k = 0; k < N; k += 2) {
-          y[k] = fmaf(x[k], c[k / 2], -(x[k + 1] * s[k / 2]));
-          y[k + 1] = fmaf(x[k], s[k / 2], x[k + 1] * c[k / 2]);
-        }
-        u[j] = pack_chunk(y);
-      } else {
-        float z[N];
-        unpack_chunk(v[j], z);
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-          y[k] = fmaf(x[k], s[k], z[k] * c[k]);
-          x[k] = fmaf(x[k], c[k], -(z[k] * s[k]));
-        }
-        u[j] = pack_chunk(x);
-        store_chunk<T>(p + col + half, y, left);
+      for (int k = 0; k < N; k += 2) {
+        y[k] = fmaf(x[k], c[k / 2], -(x[k + 1] * s[k / 2]));
+        y[k + 1] = fmaf(x[k], s[k / 2], x[k + 1] * c[k / 2]);
       }
+      u = pack_chunk(y);
+    } else {
+      float z[N];
+      load_chunk<T>(from + col + half, left, z);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        y[k] = fmaf(x[k], s[k], z[k] * c[k]);
+        x[k] = fmaf(x[k], c[k], -(z[k] * s[k]));
+      }
+      u = pack_chunk(x);
+      store_chunk<T>(to + col + half, y, left);
     }
-    store_bits<T>(p + col, u[j], left);
   }
+  store_bits<T>(to + col, u, left);
 }
 
-template <class T, bool INTERLEAVED, int HEADS>
+template <class T, bool INTERLEAVED>
 void rotary_launch(const mmuon_rotary_args& a, bool back, hipStream_t s) {
   constexpr int N = ROW_CHUNK<T>;
   const int rotated = INTERLEAVED ? a.part : a.part / 2;
   const int turned = (rotated + N - 1) / N, items = turned + (a.dim - a.part + N - 1) / N;
-  const int groups = (a.q_heads + a.k_heads + HEADS - 1) / HEADS;
-  const int64_t each = int64_t(groups) * items;
+  const int64_t each = int64_t(a.q_heads + a.k_heads) * items;
   // a launch holds fewer than 2^32 threads: more sequences take several
   const int64_t most = std::max<int64_t>(1, (int64_t(1) << 31) / (each * a.tokens));
   for (int64_t b = 0; b < a.batch; b += most) {
@@ -110,21 +95,14 @@ void rotary_launch(const mmuon_rotary_args& a, bool back, hipStream_t s) {
     p.k_out = static_cast<S*>(a.k_out) + b * a.tokens * a.k_heads * a.dim;
     if (a.positions != nullptr) p.positions = a.positions + b * a.tokens;
     const int64_t n = p.batch * a.tokens * each;
-    hipLaunchKernelGGL((rotary_rows<T, INTERLEAVED, HEADS>), dim3(unsigned((n + 255) / 256)), dim3(256), 0, s, p, turned,
-                       items, groups, back ? -1.f : 1.f);
+    hipLaunchKernelGGL((rotary_rows<T, INTERLEAVED>), dim3(unsigned((n + 255) / 256)), dim3(256), 0, s, p, turned,
+                       items, back ? -1.f : 1.f);
   }
-}
-template <class T, bool INTERLEAVED>
-void rotary_heads(const mmuon_rotary_args& a, bool back, hipStream_t s) {
-  // Four heads of a lane share its cosines and sines where that leaves the chip full
-  const int64_t chunks = a.batch * a.tokens * (a.q_heads + a.k_heads) * ((a.dim + ROW_CHUNK<T> - 1) / ROW_CHUNK<T>);
-  if (chunks >= 4 * 262144) rotary_launch<T, INTERLEAVED, 4>(a, back, s);
-  else rotary_launch<T, INTERLEAVED, 1>(a, back, s);
 }
 template <class T>
 void rotary(const mmuon_rotary_args& a, bool back, hipStream_t s) {
-  if (a.interleaved) rotary_heads<T, true>(a, back, s);
-  else rotary_heads<T, false>(a, back, s);
+  if (a.interleaved) rotary_launch<T, true>(a, back, s);
+  else rotary_launch<T, false>(a, back, s);
 }
 
 }  // namespace
