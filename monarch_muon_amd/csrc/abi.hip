@@ -847,7 +847,9 @@ int check_attention(const mmuon_attention_args* a, bool bwd) {
   }
   const bool queries = a->batch > 0 && a->queries > 0 && a->heads > 0, keys = a->batch > 0 && a->keys > 0;
   const auto bad = [](const void* p, bool needed) { return (needed && p == nullptr) || !aligned16(p); };
-  if (bad(a->q, queries) || bad(a->k, keys && queries) || bad(a->v, keys && queries))
+  // (the kernel that makes dk and dv reads the keys also where there is no query, whose zeros it stores)
+  const bool read = keys && (queries || (bwd && a->dk != nullptr));
+  if (bad(a->q, queries) || bad(a->k, read) || bad(a->v, read))
     return fail(MMUON_EINVAL, "attention: null or unaligned q, k or v");
   if ((queries && a->lam == nullptr) || misplaced(a->lam, MMUON_F32)) return fail(MMUON_EINVAL, "attention: null or unaligned lam");
   if (((reinterpret_cast<uintptr_t>(a->lengths) | reinterpret_cast<uintptr_t>(a->starts)) & 7) != 0)

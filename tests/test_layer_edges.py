@@ -1,0 +1,24 @@
+"""The operators between a layer's projections without a GPU, at the ends of what their entry points allow."""
+import ctypes as C
+
+import pytest
+
+from monarch_muon_amd import _abi
+
+ATTENTION = dict(batch=1, queries=4, keys=4, heads=2, kv_heads=1, dim=64, dtype=_abi.BF16, scale=1.0, q=4096, k=8192, v=12288,
+                 lam=16384, o=20480, o1=24576, o2=28672, lse=32768, dout=36864, dq=40960, dk=45056, dv=49152, dlam=53248,
+                 workspace=65536, workspace_bytes=1 << 40)
+
+
+def refusal(fn, args, *more):
+    lib = _abi.lib()
+    rc = getattr(lib, fn)(C.byref(args), *more, None)
+    return rc, lib.mmuon_last_error().decode()
+
+
+@pytest.mark.parametrize("none", [dict(queries=0), dict(heads=0)])
+@pytest.mark.parametrize("missing", [dict(k=0), dict(v=0), dict(k=0, v=0), dict(k=8194)])
+def test_keys_gradients_of_no_query_need_keys(none, missing):
+    """Their zeros come from a kernel that reads the keys first."""
+    rc, why = refusal("mmuon_attention_bwd", _abi.AttentionArgs(**{**ATTENTION, **none, **missing}))
+    assert rc == -1 and "q, k or v" in why, why
