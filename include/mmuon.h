@@ -545,7 +545,7 @@ int mmuon_rotary(const mmuon_rotary_args* a, int32_t back, void* stream);
    Backward (mmuon_attention_bwd), from the same inputs, o1, o2, lse and dout: dq, dk, dv (zeros
    where nothing reaches) and dlam, sums in fp32 in an order of the sizes alone. */
 typedef struct mmuon_attention_args {
-  int32_t batch;          /* batch * heads * queries < 2^29 (backward: 2^28), batch * kv_heads * keys < 2^31 - 1024
+  int32_t batch;          /* batch * heads * queries < 2^29 (backward: <= 2^28 - 16), batch * kv_heads * keys < 2^31 - 1024
                              (backward: 2^30), batch * kv_heads < 2^22 */
   int32_t queries, keys;
   int32_t heads, kv_heads;  /* heads a multiple of kv_heads, < 2^22; backward of over one query: heads * dim < 2^21 */

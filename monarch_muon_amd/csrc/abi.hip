@@ -830,8 +830,8 @@ int check_attention(const mmuon_attention_args* a, bool bwd) {
     return fail(MMUON_EINVAL, "attention: heads (%d) must be a multiple of kv_heads (%d)", a->heads, a->kv_heads);
   if (!attention_sizes(a))
     return fail(MMUON_ERANGE, "attention: %d sequences of %d queries and %d keys are negative or too many", a->batch, a->queries, a->keys);
-  if (bwd && (double(a->batch) * a->heads * a->queries >= 268435456.0 || double(a->batch) * a->kv_heads * a->keys >= 1073741824.0))
-    return fail(MMUON_ERANGE, "attention: 2^28 query rows or 2^30 keys of all heads are too many for the backward");
+  if (bwd && (double(a->batch) * a->heads * a->queries > 268435440.0 || double(a->batch) * a->kv_heads * a->keys >= 1073741824.0))
+    return fail(MMUON_ERANGE, "attention: more than 2^28 - 16 query rows, or 2^30 keys of all heads, are too many for the backward");
   if (bwd && a->queries > 1 && int64_t(a->heads) * 2 * a->dim >= (int64_t(1) << 22))
     return fail(MMUON_ERANGE, "attention: output tokens %lld elements apart are beyond the kernels' tile offsets",
                 (long long)a->heads * 2 * a->dim);

@@ -22,3 +22,12 @@ def test_keys_gradients_of_no_query_need_keys(none, missing):
     """Their zeros come from a kernel that reads the keys first."""
     rc, why = refusal("mmuon_attention_bwd", _abi.AttentionArgs(**{**ATTENTION, **none, **missing}))
     assert rc == -1 and "q, k or v" in why, why
+
+
+@pytest.mark.parametrize("rows, code, match", [((1 << 28) - 8, -3, "too many"), ((1 << 28) - 15, -3, "too many"),
+                                               ((1 << 28) - 16, -1, "unaligned gradients")])
+def test_rows_of_the_backwards_largest_launch(rows, code, match):
+    """16 threads to a row, 256 to a workgroup: fewer than 2^32 in all.  (The last case goes on to dk's address.)"""
+    sizes = dict(heads=1, keys=1, queries=rows, dk=45058)
+    rc, why = refusal("mmuon_attention_bwd", _abi.AttentionArgs(**{**ATTENTION, **sizes}))
+    assert rc == code and match in why, why
