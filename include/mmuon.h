@@ -515,7 +515,7 @@ size_t mmuon_norm_workspace(const mmuon_norm_args* a);
    in fp32 with one rounding; the other columns are copied.  p = positions[b][t], or t; a position
    outside the table gives NaN.  back: by -s, which is the gradient. */
 typedef struct mmuon_rotary_args {
-  int64_t batch;          /* batch * tokens * (q_heads + k_heads) * dim < 2^40, of one sequence < 2^31 */
+  int64_t batch;          /* batch * tokens * (q_heads + k_heads) * dim < 2^40, of one token < 2^31 */
   int64_t tokens;
   int32_t q_heads, k_heads;
   int32_t dim;            /* 1 <= dim <= 65536 */

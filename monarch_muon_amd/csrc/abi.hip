@@ -798,9 +798,9 @@ int check_rotary(const mmuon_rotary_args* a) {
     return fail(MMUON_EINVAL, "rotary: dim (%d) must be in [1, 65536], part (%d) even and in [2, dim]", a->dim, a->part);
   if (a->batch < 0 || a->tokens < 0 || a->q_heads < 0 || a->k_heads < 0 || a->table_rows < 0)
     return fail(MMUON_EINVAL, "rotary: negative size");
-  const double one = double(a->tokens) * (double(a->q_heads) + a->k_heads) * a->dim;
-  if (one >= 2147483648.0 || one * double(a->batch) >= 1099511627776.0 || a->batch >= (int64_t(1) << 31))
-    return fail(MMUON_ERANGE, "rotary: 2^31 elements of a sequence or 2^40 of all are too many");
+  const double one = (double(a->q_heads) + a->k_heads) * a->dim;
+  if (one >= 2147483648.0 || one * double(a->batch) * double(a->tokens) >= 1099511627776.0)
+    return fail(MMUON_ERANGE, "rotary: 2^31 elements of a token or 2^40 of all are too many");
   if (a->batch == 0 || a->tokens == 0) return MMUON_OK;
   if (a->table_rows == 0) return fail(MMUON_EINVAL, "rotary: a table of no positions");
   for (int i = 0; i < 3; ++i)

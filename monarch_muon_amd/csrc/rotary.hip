@@ -20,15 +20,14 @@ namespace mmuon {
 namespace {
 
 template <class T, bool INTERLEAVED>
-__global__ __launch_bounds__(256) void rotary_rows(mmuon_rotary_args a, int turned, int items, float sign) {
+__global__ __launch_bounds__(256) void rotary_rows(mmuon_rotary_args a, int64_t first, int64_t tokens, int turned, int items, float sign) {
   using S = typename T::storage;
   constexpr int N = ROW_CHUNK<T>, M = INTERLEAVED ? N / 2 : N;
   const int heads = a.q_heads + a.k_heads;
-  const int64_t all = int64_t(a.batch) * a.tokens * heads * items;
   const int64_t id = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (id >= all) return;
-  const int64_t token = id / (heads * items);
-  const int rest = int(id - token * (heads * items)), h = rest / items, item = rest - h * items;
+  if (id >= tokens * (heads * items)) return;
+  const int64_t of = id / (heads * items), token = first + of;
+  const int rest = int(id - of * (heads * items)), h = rest / items, item = rest - h * items;
   const int64_t b = token / a.tokens, t = token - b * a.tokens;
   const int half = a.part / 2;
   const bool turn = item < turned;
@@ -83,20 +82,12 @@ void rotary_launch(const mmuon_rotary_args& a, bool back, hipStream_t s) {
   const int rotated = INTERLEAVED ? a.part : a.part / 2;
   const int turned = (rotated + N - 1) / N, items = turned + (a.dim - a.part + N - 1) / N;
   const int64_t each = int64_t(a.q_heads + a.k_heads) * items;
-  // a launch holds fewer than 2^32 threads: more sequences take several
-  const int64_t most = std::max<int64_t>(1, (int64_t(1) << 31) / (each * a.tokens));
-  for (int64_t b = 0; b < a.batch; b += most) {
-    mmuon_rotary_args p = a;
-    p.batch = std::min(a.batch - b, most);
-    using S = typename T::storage;
-    p.q = static_cast<const S*>(a.q) + b * a.q_stride[0];
-    p.k = static_cast<const S*>(a.k) + b * a.k_stride[0];
-    p.q_out = static_cast<S*>(a.q_out) + b * a.tokens * a.q_heads * a.dim;
-    p.k_out = static_cast<S*>(a.k_out) + b * a.tokens * a.k_heads * a.dim;
-    if (a.positions != nullptr) p.positions = a.positions + b * a.tokens;
-    const int64_t n = p.batch * a.tokens * each;
-    hipLaunchKernelGGL((rotary_rows<T, INTERLEAVED>), dim3(unsigned((n + 255) / 256)), dim3(256), 0, s, p, turned,
-                       items, back ? -1.f : 1.f);
+  // a launch holds fewer than 2^32 threads: more tokens, of one sequence or several, take several
+  const int64_t all = a.batch * a.tokens, most = std::max<int64_t>(1, (int64_t(1) << 31) / each);
+  for (int64_t first = 0; first < all; first += most) {
+    const int64_t tokens = std::min(all - first, most);
+    hipLaunchKernelGGL((rotary_rows<T, INTERLEAVED>), dim3(unsigned((tokens * each + 255) / 256)), dim3(256), 0, s, a, first, tokens,
+                       turned, items, back ? -1.f : 1.f);
   }
 }
 template <class T>

@@ -31,3 +31,17 @@ def test_rows_of_the_backwards_largest_launch(rows, code, match):
     sizes = dict(heads=1, keys=1, queries=rows, dk=45058)
     rc, why = refusal("mmuon_attention_bwd", _abi.AttentionArgs(**{**ATTENTION, **sizes}))
     assert rc == code and match in why, why
+
+
+ROTARY = dict(batch=1, tokens=4, q_heads=32, k_heads=32, dim=128, part=128, dtype=_abi.BF16, table_rows=9, q=4096, k=8192,
+              table=12289, q_out=16384, k_out=20480)
+
+
+@pytest.mark.parametrize("change, code, match", [
+    (dict(tokens=1 << 18), -1, "unaligned table"), (dict(tokens=1 << 26), -1, "unaligned table"),
+    (dict(tokens=1 << 27), -3, "too many"), (dict(batch=1 << 27, tokens=1), -3, "too many"),
+    (dict(q_heads=1 << 24, dim=256, part=2), -3, "too many"), (dict(q_heads=1 << 22, part=2), -1, "unaligned table")])
+def test_rotary_takes_long_sequences(change, code, match):
+    """2^40 elements of all, and one token's 2^31.  (What is taken goes on to the table's address, which is none.)"""
+    rc, why = refusal("mmuon_rotary", _abi.RotaryArgs(**{**ROTARY, **change}), 0)
+    assert rc == code and match in why, why
