@@ -212,12 +212,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void attend(mmuon_a
   const int64_t at = (int64_t(b) * a.queries + t) * a.heads + h;
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
-    const float inv = weight[m] == 0.f ? 0.f : 1.f / weight[m];
+    const float inv = 1.f / weight[m];
     float* own = in && a.o1 != nullptr ? (m0 + m ? a.o2 : a.o1) + at * 2 * a.dim : nullptr;
 #pragma unroll
     for (int j = 0; j < PANELS; ++j) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[m][j][e] *= inv;
+      for (int e = 0; e < 16; ++e) acc[m][j][e] = weight[m] == 0.f ? 0.f : acc[m][j][e] * inv;  // (0 * NaN of a hidden key is NaN)
       if (own != nullptr) {
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {

@@ -192,6 +192,13 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dq(mmu
       }
   }
   along = half_sum(along) * by2;
+  if (limit == 0) {  // nothing is seen: 0, where the products have 0 * NaN if a hidden key, q or dO holds one
+    along = 0.f;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) acc[m][j] = f32x16{};
+  }
   const int64_t total = int64_t(a.batch) * a.heads * a.queries;
   if (in && half == 0) space.dlam[part * total + at] = -along;
   if constexpr (SPLIT) {

@@ -3,7 +3,7 @@ elements than 31 bits count, and more threads than one launch holds."""
 import pytest
 import torch
 
-from monarch_muon_amd import rotary, rotary_table
+from monarch_muon_amd import differential_attention, rotary, rotary_table
 from oracle import layer as oracle
 
 pytestmark = pytest.mark.gpu
@@ -50,3 +50,35 @@ def test_rotary_of_a_sequence_of_more_threads_than_a_launch():
     whole = T // cycle * cycle
     assert torch.equal(out[:whole].view(-1, cycle), ref.expand(T // cycle, cycle))
     assert torch.equal(out[whole:], ref[:T - whole])
+
+
+# ----- attention: rows and keys that nothing reaches ---------------------------------
+BAD = (float("nan"), float("inf"), float("-inf"))
+
+
+def attend(q, k, v, lam, dout, **kw):
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, lam)]
+    out = differential_attention(*leaves, **kw)
+    return (out.detach(), *torch.autograd.grad(out, leaves, dout))
+
+
+def inputs(B, Tq, Tk, H, K, d, seed):
+    return (randn(B, Tq, 2 * H, d, seed=seed, size=1.5), randn(B, Tk, 2 * K, d, seed=seed + 1), randn(B, Tk, K, 2 * d, seed=seed + 2),
+            torch.linspace(0.2, 0.8, H, device=DEV), randn(B, Tq, H, 2 * d, seed=seed + 3))
+
+
+# (of one tile; of several; keys in parts; queries and keys in parts; many sequences, eight waves)
+SIZES = [(2, 40, 40, 2, 1), (1, 150, 150, 2, 2), (1, 3, 2000, 2, 1), (1, 700, 700, 1, 1), (12, 300, 300, 8, 8)]
+
+
+@pytest.mark.parametrize("d", [24, 64, 128])
+@pytest.mark.parametrize("B, Tq, Tk, H, K", SIZES)
+def test_queries_that_see_nothing_are_zero_beside_any_key(B, Tq, Tk, H, K, d):
+    """A key that is no number reaches the queries that see it; those before every key have zeros all the same."""
+    q, k, v, lam, dout = inputs(B, Tq, Tk, H, K, d, 41)
+    none = (Tq + 1) // 2
+    for bad in BAD:
+        k[:, 0], v[:, 0] = bad, bad
+        o, dq, *_ = attend(q, k, v, lam, dout, starts=torch.full((B,), -none, device=DEV))
+        assert not o[:, :none].any() and not dq[:, :none].any()
+        assert none == Tq or o[:, none:].isnan().any(-1).all()
