@@ -427,6 +427,14 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mm
         dk[1][j] = mfma(read_turned<CA>(tile_at + T::A2, ta, 16 * y, j), x2[y], dk[1][j]);
       }
   }
+  if (own >= a.queries) {  // nobody sees the key: 0, where the products have 0 * NaN if a query or its dO holds one
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) dv[j] = f32x16{};
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) dk[m][j] = f32x16{};
+  }
   const bool in = key < a.keys;
   if constexpr (SPLIT) {
     if (!in) return;

@@ -82,3 +82,21 @@ def test_queries_that_see_nothing_are_zero_beside_any_key(B, Tq, Tk, H, K, d):
         o, dq, *_ = attend(q, k, v, lam, dout, starts=torch.full((B,), -none, device=DEV))
         assert not o[:, :none].any() and not dq[:, :none].any()
         assert none == Tq or o[:, none:].isnan().any(-1).all()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", [24, 64, 128])
+@pytest.mark.parametrize("B, Tq, Tk, H, K", SIZES)
+def test_keys_that_nobody_sees_have_zeros_beside_any_query(B, Tq, Tk, H, K, d, causal):
+    """Behind a sequence's length, and behind the last query's place: zeros, whatever the queries hold."""
+    q, k, v, lam, dout = inputs(B, Tq, Tk, H, K, d, 51)
+    n = Tk - 5
+    for bad in BAD:
+        q[:, -1], dout[:, -1] = bad, bad
+        cases = [dict(lengths=torch.full((B,), n, device=DEV))]
+        if causal and n >= Tq:
+            cases.append(dict(starts=torch.full((B,), n - Tq, device=DEV)))
+        for kw in cases:
+            _, _, dk, dv, _ = attend(q, k, v, lam, dout, causal=causal, **kw)
+            assert not dk[:, n:].any() and not dv[:, n:].any()
+            assert dv[:, n - 1].isnan().all()
