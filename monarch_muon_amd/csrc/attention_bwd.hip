@@ -310,6 +310,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mm
   };
   const int from = first_of(c0) / TQ * TQ, mine = first_of(w0), own = first_of(key);
   const int full = first_of(w0 + 31);  // from here on every key of the wave is seen
+  const int none = first_of(0);        // the queries before see nothing, and their rows may hold anything
   const int steps = (a.queries - from + TQ - 1) / TQ, all = steps * share;
   const int i0 = SPLIT ? int(int64_t(all) * part / parts) : 0, n = (SPLIT ? int(int64_t(all) * (part + 1) / parts) : all) - i0;
   const int head0 = SPLIT && n > 0 ? i0 / steps : 0, first0 = from + (i0 - head0 * steps) * TQ;
@@ -331,7 +332,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mm
     if (next_first >= a.queries) next_first = from, ++next_head;
     const char* q = q1 + 2 * (2 * head * a.q_stride[2] + first * a.q_stride[1]);
     const uint32_t to = lds + (i % SLOTS) * BYTES;
-    T::load(to, q, q + 2 * a.q_stride[2], g0 + 2 * (int64_t(first) * a.heads + head) * 2 * a.dim, src, off, a.queries - first, wave, lane);
+    T::load(to, q, q + 2 * a.q_stride[2], g0 + 2 * (int64_t(first) * a.heads + head) * 2 * a.dim, src, off, a.queries - first, wave, lane, none - first);
     // (every wave loads them, so that each has as many loads)
     const float4* stats = space.stats + (int64_t(b) * a.heads + g * share + head) * a.queries + first;
     dma16(uniform_ptr(stats), uint32_t(min(lane, a.queries - first - 1)) * 16, to + T::BYTES);

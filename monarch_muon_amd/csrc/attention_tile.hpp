@@ -131,15 +131,16 @@ struct Tile {
   static_assert((2 * NA + NB) % WAVES == 0, "each wave has as many loads");
 
   // A wave's k-th load fills 1 KiB: its matrix, where in the tile, and each lane's offset in the
-  // matrix's rows.  Rows from `left` on repeat the last one there, and chunks a row does not have its
-  // last: what is read is always there, and what comes of it is masked, multiplied by zeros or not stored.
-  static __device__ __forceinline__ uint32_t offset(const TileRows& s, int n, int lane, int left) {
+  // matrix's rows.  Rows from `left` on repeat the last one there, rows before `skip` that one, and chunks a
+  // row does not have its last: what is read is always there, and what comes of it is masked, multiplied by
+  // zeros or not stored.
+  static __device__ __forceinline__ uint32_t offset(const TileRows& s, int n, int lane, int left, int skip = 0) {
     if (n < 2 * NA) {
       const int at = (n >= NA ? n - NA : n) * 64 + lane, r = at / CA, c = min((at % CA) ^ chunk_mask<CA>(r), s.a_last);
-      return uint32_t(min(r, left - 1)) * s.a_stride + uint32_t(c) * 16;
+      return uint32_t(min(max(r, skip), left - 1)) * s.a_stride + uint32_t(c) * 16;
     }
     const int at = (n - 2 * NA) * 64 + lane, r = at / CB, c = min((at % CB) ^ chunk_mask<CB>(r), s.b_last);
-    return uint32_t(min(r, left - 1)) * s.b_stride + uint32_t(c) * 16;
+    return uint32_t(min(max(r, skip), left - 1)) * s.b_stride + uint32_t(c) * 16;
   }
   // (of whole tiles: made once, so that a load in the loop is a load and little else)
   static __device__ __forceinline__ void offsets(const TileRows& s, int wave, int lane, uint32_t (&off)[LOADS]) {
@@ -148,12 +149,12 @@ struct Tile {
   }
   // a1, a2, b: the tile's first row in each matrix (values: a select between members of a struct goes through memory)
   static __device__ __forceinline__ void load(uint32_t lds, const char* a1, const char* a2, const char* b, const TileRows& s,
-                                              const uint32_t (&off)[LOADS], int left, int wave, int lane) {
+                                              const uint32_t (&off)[LOADS], int left, int wave, int lane, int skip = 0) {
 #pragma unroll
     for (int k = 0; k < LOADS; ++k) {
       const int n = wave + WAVES * k;
       const char* from = uniform_ptr(n < NA ? a1 : n < 2 * NA ? a2 : b);
-      dma16(from, left >= ROWS ? off[k] : offset(s, n, lane, left), lds + n * 1024);
+      dma16(from, left >= ROWS && skip <= 0 ? off[k] : offset(s, n, lane, left, skip), lds + n * 1024);
     }
   }
 };

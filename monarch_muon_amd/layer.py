@@ -177,8 +177,9 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
 
     ``lengths`` (B): the keys of each sequence that count; those behind are not read (a cache).  ``causal``: query ``t`` of
     sequence ``b`` sees keys up to ``starts[b] + t``, by default ``lengths[b] - T + t``: the queries are the last ones of their
-    sequence.  A query that sees no key has zeros.  An infinity or a NaN in a key or value that ``causal`` alone hides may
-    show as NaN in the queries before it.
+    sequence.  A query that sees no key has zeros and reaches nothing, whatever it holds; a key that no query sees has zeros
+    for gradients.  Between a query and a later key that ``causal`` alone hides an infinity or a NaN may show as NaN: of the key
+    or its value in the query's output and gradient, of the query or its output's gradient in the key's and the value's.
 
     Differentiable in ``q``, ``k``, ``v`` and ``lam``; every sum has an order that depends on the sizes alone, so gradients are
     the same bits every time.  Probabilities are rounded to bfloat16 before their products with the values, as are the

@@ -73,6 +73,22 @@ SIZES = [(2, 40, 40, 2, 1), (1, 150, 150, 2, 2), (1, 3, 2000, 2, 1), (1, 700, 70
 
 @pytest.mark.parametrize("d", [24, 64, 128])
 @pytest.mark.parametrize("B, Tq, Tk, H, K", SIZES)
+def test_queries_that_see_nothing_reach_nothing(B, Tq, Tk, H, K, d):
+    """Whatever the queries before the first key hold, and their output's gradients: the others have the same bits, they zeros."""
+    q, k, v, lam, dout = inputs(B, Tq, Tk, H, K, d, 31)
+    for none in (1, Tq // 2, Tq):            # so many queries see no key
+        starts = torch.full((B,), -none, device=DEV)
+        ref = attend(q, k, v, lam, dout, starts=starts)
+        assert not ref[0][:, :none].any() and not ref[1][:, :none].any()
+        for bad in BAD:
+            q[:, :none], dout[:, :none] = bad, bad
+            for x, y in zip(attend(q, k, v, lam, dout, starts=starts), ref):
+                assert torch.equal(x, y)
+        q[:, :none], dout[:, :none] = 0.5, 0.25
+
+
+@pytest.mark.parametrize("d", [24, 64, 128])
+@pytest.mark.parametrize("B, Tq, Tk, H, K", SIZES)
 def test_queries_that_see_nothing_are_zero_beside_any_key(B, Tq, Tk, H, K, d):
     """A key that is no number reaches the queries that see it; those before every key have zeros all the same."""
     q, k, v, lam, dout = inputs(B, Tq, Tk, H, K, d, 41)
