@@ -72,11 +72,14 @@ class TinyMonarchLM(torch.nn.Module):
         self.register_buffer("table", rotary_table(DIM, SEQ), persistent=False)
 
     def hidden(self, ids, caches=None, at=0):
-        """Of ``ids`` (B, T), which stand at ``at`` on; ``caches``: one of each block for the tokens before."""
-        x, stream = embedding(ids, self.wte, scale=WIDTH ** 0.5, padding_idx=PAD), None
+        """Of ``ids`` (..., T), which stand at ``at`` on; ``caches``: one of each block for the tokens before."""
+        end = at + ids.shape[-1]
+        if end > self.table.shape[0]:
+            self.table = rotary_table(DIM, 2 * end, device=self.table.device)
+        x, stream = embedding(ids.reshape(-1, ids.shape[-1]), self.wte, scale=WIDTH ** 0.5, padding_idx=PAD), None
         for i, b in enumerate(self.blocks):
             x, stream = b(x, stream, self.table, None if caches is None else caches[i], at)
-        return rms_norm(x, self.ln_f, residual=stream)[0]
+        return rms_norm(x, self.ln_f, residual=stream)[0].view(*ids.shape, WIDTH)
 
     def caches(self, batch, length):
         new = lambda heads, width: torch.empty(batch, length, heads, width, dtype=torch.bfloat16, device=self.wte.device)  # noqa: E731

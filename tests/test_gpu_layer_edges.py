@@ -116,3 +116,44 @@ def test_keys_that_nobody_sees_have_zeros_beside_any_query(B, Tq, Tk, H, K, d, c
             _, _, dk, dv, _ = attend(q, k, v, lam, dout, causal=causal, **kw)
             assert not dk[:, n:].any() and not dv[:, n:].any()
             assert dv[:, n - 1].isnan().all()
+
+
+# ----- the example -------------------------------------------------------------------
+def tiny_model(seed=3):
+    from monarch_muon_amd import example
+    torch.manual_seed(seed)
+    return example, example.TinyMonarchLM().to(DEV)
+
+
+def test_the_example_goes_beyond_a_training_sequence():
+    """Tokens one by one and sequences in one call, longer than those that it is trained on."""
+    example, model = tiny_model()
+    count = 2 * example.SEQ + 5
+    tokens, scores = example.generate(model, 7, count)
+    assert len(tokens) == count and all(0 <= t < example.VOCAB for t in tokens)
+    assert all(-50 < s <= 0 for s in scores)             # log-probabilities of a fresh model: about -ln 509 at most
+    assert example.generate(model, 7, 20)[0] == tokens[:20]
+    ids = torch.tensor([[7, *tokens[:-1]]], device=DEV)
+    with torch.no_grad():
+        fresh = tiny_model()[1]
+        whole = fresh.hidden(ids)
+        assert whole.isfinite().all() and torch.equal(whole, model.hidden(ids))
+        # one call or one by one: the sums of the projections and of attention's parts are of other orders
+        caches = fresh.caches(1, count)
+        last = [fresh.hidden(ids[:, t:t + 1], caches, t) for t in range(count)][-1]
+    assert float((last - whole[:, -1:]).float().norm() / whole[:, -1:].float().norm()) < 12 * 2 ** -9
+    assert model.loss(ids[:, :-1], ids[:, 1:]).isfinite()
+
+
+def test_the_example_takes_ids_of_any_shape():
+    example, model = tiny_model()
+    ids, targets = example.text(torch.Generator().manual_seed(4), DEV)
+    with torch.no_grad():
+        h = model.hidden(ids)
+        assert h.shape == (*ids.shape, example.WIDTH)
+        assert torch.equal(model.hidden(ids.view(2, 4, -1)), h.view(2, 4, *h.shape[1:]))
+        one = model.hidden(ids[0])
+        assert one.shape == h[0].shape
+        # (one sequence's products are split otherwise than eight's)
+        assert float((one - h[0]).float().norm() / h[0].float().norm()) < 12 * 2 ** -9
+        assert abs(float(model.loss(ids[0], targets[0])) - float(model.loss(ids[:1], targets[:1]))) == 0
