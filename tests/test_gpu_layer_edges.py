@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from monarch_muon_amd import differential_attention, rotary, rotary_table
+from oracle import butterfly
 from oracle import layer as oracle
 
 pytestmark = pytest.mark.gpu
@@ -157,3 +158,84 @@ def test_the_example_takes_ids_of_any_shape():
         # (one sequence's products are split otherwise than eight's)
         assert float((one - h[0]).float().norm() / h[0].float().norm()) < 12 * 2 ** -9
         assert abs(float(model.loss(ids[0], targets[0])) - float(model.loss(ids[:1], targets[:1]))) == 0
+
+
+class Rounded(torch.autograd.Function):
+    """To bf16's values and back, the gradient too."""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.bfloat16().to(x.dtype)
+
+    @staticmethod
+    def backward(ctx, g):
+        return g.bfloat16().to(g.dtype)
+
+
+def plain_model(example, p, ids, targets, r):
+    """The example's loss in 64 bits, its results through ``r``."""
+    p = {n: r(t) for n, t in p.items()}
+    H, D, W = example.HEADS, example.DIM, example.WIDTH
+    B, T = ids.shape
+    angle = torch.arange(T, dtype=torch.float64)[:, None, None] * 10000.0 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)
+    hidden = torch.ones(T, T, dtype=torch.bool).triu(1)
+
+    def norm(h, w):
+        return r(h / (h.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w)
+
+    def monarch(x, w1, w2):
+        x2 = x.reshape(B * T, -1)
+        y = r(x2.view(B * T, w1.shape[0], -1).transpose(0, 1) @ w1.transpose(1, 2))
+        y = r(butterfly.riffle(y, w2.shape[0]) @ w2.transpose(1, 2))
+        return y.permute(1, 2, 0).reshape(B, T, -1)
+
+    def turn(x):
+        a, b = x[..., :D // 2], x[..., D // 2:]
+        return r(torch.cat([a * angle.cos() - b * angle.sin(), a * angle.sin() + b * angle.cos()], -1))
+
+    x, stream = r(p["wte"][ids] * W ** 0.5), None
+    x = torch.where((ids == example.PAD)[..., None], x.detach(), x)   # the padding's row takes no gradient
+    for i in range(example.LAYERS):
+        at = lambda n: p[f"blocks.{i}.{n}"]  # noqa: E731
+        stream = x if stream is None else r(x + stream)
+        y = norm(stream, at("norms.0"))
+        q, k, v = (monarch(y, at(f"attention.w.{j}"), at(f"attention.w.{j + 1}")) for j in (0, 2, 4))
+        q, k, v = turn(q.view(B, T, 2 * H, D)).view(B, T, H, 2, D), turn(k.view(B, T, 2 * H, D)).view(B, T, H, 2, D), v.view(B, T, H, 2 * D)
+        s = torch.einsum("bthmd,bshmd->bhmts", q, k) * D ** -0.5
+        s = r(s.masked_fill(hidden, -float("inf")).softmax(-1))
+        o = r(torch.einsum("bhts,bshd->bthd", s[:, :, 0] - at("attention.lam")[:, None, None] * s[:, :, 1], v))
+        x = monarch(norm(o, at("attention.norm")), at("attention.w.6"), at("attention.w.7"))
+        stream = r(x + stream)
+        y = monarch(norm(stream, at("norms.1")), at("w.0"), at("w.1"))
+        x = monarch(r(y * y.sigmoid()), at("w.2"), at("w.3"))
+    logits = norm(r(x + stream), p["ln_f"]) @ p["lm_head"].t()
+    return torch.nn.functional.cross_entropy(logits.flatten(0, 1), targets.flatten(), ignore_index=example.PAD)
+
+
+def test_the_examples_gradients_against_differences():
+    """Each parameter's gradient against that of the model in 64 bits, which differences of its loss confirm.  The same
+    model with its results and their gradients rounded to bf16 says how far those roundings take each gradient: the
+    kernels' are as many or fewer and independent of these, so four times as far is beyond what they explain."""
+    from monarch_muon_amd import example
+    torch.manual_seed(3)
+    model = example.TinyMonarchLM()
+    ids, targets = example.text(torch.Generator().manual_seed(4), "cpu")
+    p = {n: t.detach().double().requires_grad_() for n, t in model.named_parameters()}
+    loss = plain_model(example, p, ids, targets, lambda t: t)
+    exact = dict(zip(p, torch.autograd.grad(loss, list(p.values()))))
+    rounded = dict(zip(p, torch.autograd.grad(plain_model(example, p, ids, targets, Rounded.apply), list(p.values()))))
+    g = torch.Generator().manual_seed(5)
+    along = {n: torch.randn(t.shape, generator=g, dtype=torch.float64) * t.detach().norm() / t.numel() ** 0.5 for n, t in p.items()}
+    e = 1e-5
+    with torch.no_grad():
+        ends = [plain_model(example, {n: t + s * e * along[n] for n, t in p.items()}, ids, targets, lambda t: t) for s in (1, -1)]
+    slope = sum(float((exact[n] * along[n]).sum()) for n in p)
+    # the differences' own error: the third derivative's e^2, and 64 bits' rounding of the loss over e
+    size = sum(float((exact[n] * along[n]).norm()) for n in p)
+    assert abs(float(ends[0] - ends[1]) / (2 * e) - slope) <= 1e-6 * size
+    model.to(DEV)
+    got = model.loss(ids.to(DEV), targets.to(DEV))
+    assert abs(float(got.detach()) - float(loss.detach())) <= 0.01 * float(loss.detach())
+    for (name, _), grad in zip(model.named_parameters(), torch.autograd.grad(got, list(model.parameters()))):
+        off, room = (float((t.double().cpu() - exact[name]).norm()) for t in (grad, rounded[name]))
+        assert off <= 4 * room, (name, off / float(exact[name].norm()), room / float(exact[name].norm()))
