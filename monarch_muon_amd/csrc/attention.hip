@@ -37,8 +37,10 @@ struct Parts {
 };
 
 // log2 of the sum of a row's 2^(s - shift), shift still on it, and what 2^(s - that) is to be multiplied by
-// for what the logarithm's rounding took (up to 1e-6 of it, the same for all of the row).  Of a row that sees nothing
-// +inf, so that its probabilities are 0.
+// for what the logarithm's rounding took: half of its last place, 2^(e - 24) ln 2 of each probability of the row for one
+// of 2^e and more (1.3e-6 from 32 on, 4e-5 from 1024 on; the scores' own fp32 sums are off by as much).  dq and dlam, where
+// rows cancel, take that factor; dk and dv, whose P and dS are rounded to bf16 (2^-9), do not.  Of a row that sees
+// nothing +inf, so that its probabilities are 0.
 __device__ __forceinline__ void store_lse(float* to, float shift, float sum) {
   const float lse = sum == 0.f ? INFINITY : shift + __builtin_amdgcn_logf(sum);
   *reinterpret_cast<float2*>(to) = make_float2(lse, sum == 0.f ? 1.f : __builtin_amdgcn_exp2f(lse - shift) / sum);

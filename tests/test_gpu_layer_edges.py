@@ -239,3 +239,22 @@ def test_the_examples_gradients_against_differences():
     for (name, _), grad in zip(model.named_parameters(), torch.autograd.grad(got, list(model.parameters()))):
         off, room = (float((t.double().cpu() - exact[name]).norm()) for t in (grad, rounded[name]))
         assert off <= 4 * room, (name, off / float(exact[name].norm()), room / float(exact[name].norm()))
+
+
+# ----- attention: scores far from zero -----------------------------------------------
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", [24, 32, 64, 128])
+def test_gradients_of_large_scores(d, causal):
+    """Scores of up to some thousands, within the bounds of fp32 scores: a row's log-sum-exp is rounded like they are."""
+    q, k, v, lam, dout = inputs(2, 150, 150, 2, 2, d, 61)
+    k = (k.float() * torch.linspace(0.01, 6, 150, device=DEV)[None, :, None, None]).bfloat16()
+    q = (q.float() * 30).bfloat16()
+    refs, bounds = oracle.attention(q, k, v, lam, causal=causal, dout=dout)
+    # A probability or a dS below fp32's 2^-126 is lost, where the form in 64 bits has it: in each of the 300 terms of an
+    # element (150 rows or keys, two heads at most) under 2^-126 of P, times |dP| + |D| <= 2 max |dO| . |v|, or 2^-126 of dS
+    # itself; times an element of q, k, dO or v.
+    largest = max(float(t.abs().max()) for t in (q, k, v, dout))
+    lost = 300 * 2.0 ** -126 * (1 + 2 * 2 * d * float(dout.abs().max()) * float(v.abs().max())) * largest
+    for name, x, ref, bound in zip(("o", "dq", "dk", "dv", "dlam"), attend(q, k, v, lam, dout, causal=causal), refs, bounds):
+        worst, bad = float(((x.double() - ref).abs() - bound).max()), bool(x.isnan().any())
+        assert not bad and worst <= lost, (name, worst)
