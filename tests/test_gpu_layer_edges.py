@@ -6,6 +6,7 @@ import torch
 from monarch_muon_amd import differential_attention, rotary, rotary_table
 from oracle import butterfly
 from oracle import layer as oracle
+from test_gpu_attention import check
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -258,3 +259,22 @@ def test_gradients_of_large_scores(d, causal):
     for name, x, ref, bound in zip(("o", "dq", "dk", "dv", "dlam"), attend(q, k, v, lam, dout, causal=causal), refs, bounds):
         worst, bad = float(((x.double() - ref).abs() - bound).max()), bool(x.isnan().any())
         assert not bad and worst <= lost, (name, worst)
+
+
+# ----- attention: far offsets, exactly -----------------------------------------------
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("apart", [(1 << 21) + 8, (1 << 22) - 8, 1 << 22])
+def test_tokens_far_apart(apart, d):
+    """Queries, keys and values of one buffer whose tokens stand up to the kernels' largest stride apart, and beyond it, where
+    they are copied: offsets of over 2^32 bytes, and each output and gradient within the bounds of near ones."""
+    room_for(60)
+    T, H, K = (5 << 30) // (2 * apart) + 40, 4, 2
+    buffer = torch.empty(1, T, apart, device=DEV, dtype=torch.bfloat16)
+    sizes = (2 * H * d, 2 * K * d, 2 * K * d)
+    parts = buffer[..., -sum(sizes):].split(sizes, -1)
+    for i, part in enumerate(parts):
+        part.copy_(randn(*part.shape, seed=71 + i))
+    q, k, v = (part.unflatten(-1, (-1, w)) for part, w in zip(parts, (d, d, 2 * d)))
+    lam = torch.linspace(0.1, 0.9, H, device=DEV)
+    check(q, k, v, lam)
+    check(q[:, -3:], k, v, lam, lengths=torch.tensor([T - 1]), grads=False)
