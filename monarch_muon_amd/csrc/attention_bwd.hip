@@ -495,13 +495,16 @@ __global__ __launch_bounds__(256) void attention_join(mmuon_attention_args a, in
 }
 
 int template_dim(const mmuon_attention_args& a) { return a.dim > 64 ? 128 : a.dim > 32 ? 64 : 32; }
-// Parts of a loop of `most` steps that the estimate finds shortest, each of eight steps at least
+// Parts of a loop of `most` steps that the estimate finds shortest, each of eight steps at least.  Parts whose sums take
+// over 4 GiB have to make it 5% shorter: rounds of hundreds of workgroups that end a little earlier do not (no mask, 1 x 52858
+// tokens, 22 heads of 2 x 112: two parts 292 ms and 15.6 GB held in a pass, one 290 and 10.8; 35 x 10013, 16 of 2 x 96 on 2: three
+// 279 and 31.5, one 282 and 27.2; 4 x 222563, 96 of 2 x 72 on 24 would have taken 89 GB for them).
 int fewest_us(const Items& n, const Pace& p, double part_bytes) {
   int best = 1;
   double least = estimate(n, p, 1, part_bytes);
   for (int splits = 2; splits <= 16 && splits * 8 <= n.most; ++splits) {
     const double t = estimate(n, p, splits, part_bytes);
-    if (t < least) least = t, best = splits;
+    if (t < (splits * part_bytes > 4294967296.0 ? 0.95 : 1.0) * least) least = t, best = splits;
   }
   return best;
 }

@@ -45,3 +45,11 @@ def test_rotary_takes_long_sequences(change, code, match):
     """2^40 elements of all, and one token's 2^31.  (What is taken goes on to the table's address, which is none.)"""
     rc, why = refusal("mmuon_rotary", _abi.RotaryArgs(**{**ROTARY, **change}), 0)
     assert rc == code and match in why, why
+
+
+@pytest.mark.parametrize("B, T, H, K, d", [(4, 222563, 96, 24, 72), (2, 259541, 148, 37, 96), (253, 128675, 16, 2, 16), (9, 269351, 100, 25, 8)])
+def test_workspace_of_many_keys(B, T, H, K, d):
+    """Queries and keys in parts are for calls of few tiles: rounds of workgroups that end a little earlier are not worth
+    tens of gigabytes.  What is left are the rows' statistics and their parts of dlam."""
+    a = _abi.AttentionArgs(**{**ATTENTION, "batch": B, "queries": T, "keys": T, "heads": H, "kv_heads": K, "dim": d})
+    assert _abi.lib().mmuon_attention_workspace(C.byref(a), 1) <= 20 * B * H * T + 4096
