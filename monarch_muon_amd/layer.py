@@ -129,6 +129,12 @@ def rotary_table(dim: int, length: int, *, base: float = 10000.0, scaling: str |
         raise ValueError(f"base and factor must be positive, not {base} and {factor}")
     if scaling in ("yarn", "llama") and (trained is None or trained < 1):
         raise ValueError(f"scaling {scaling!r} needs the trained length")
+    if scaling in ("yarn", "llama"):
+        fast = {"yarn": 32.0, "llama": 4.0}[scaling] if fast is None else fast
+        if not 0 < slow < fast:
+            raise ValueError(f"scaling {scaling!r} needs 0 < slow < fast, not {slow} and {fast}")
+    if scaling == "yarn" and not base > 1:
+        raise ValueError(f"scaling 'yarn' needs a base above 1, not {base}")
     i = torch.arange(0, dim, 2, dtype=torch.float64, device=device)
     if scaling == "ntk":
         base = base * factor ** (dim / max(dim - 2, 1))
@@ -139,13 +145,12 @@ def rotary_table(dim: int, length: int, *, base: float = 10000.0, scaling: str |
     elif scaling == "yarn":
         def pair(turns):   # that takes so many turns within the trained length
             return dim * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))
-        lo, hi = max(math.floor(pair(32.0 if fast is None else fast)), 0), min(math.ceil(pair(slow)), dim - 1)
+        lo, hi = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), dim - 1)
         ramp = ((i / 2 - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
         f = f / factor * ramp + f * (1 - ramp)
         size = (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0) if attention_factor is None else attention_factor
     elif scaling == "llama":
-        most = 4.0 if fast is None else fast
-        keep = ((trained * f / (2 * math.pi) - slow) / (most - slow)).clamp(0, 1)
+        keep = ((trained * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
         f = f * keep + f / factor * (1 - keep)
     a = torch.arange(length, dtype=torch.float64, device=device).unsqueeze(1) * f
     return (torch.cat([a.cos(), a.sin()], 1) * size).float()

@@ -1,9 +1,10 @@
 """The operators between a layer's projections without a GPU, at the ends of what their entry points allow."""
 import ctypes as C
+import math
 
 import pytest
 
-from monarch_muon_amd import _abi
+from monarch_muon_amd import _abi, rotary_table
 
 ATTENTION = dict(batch=1, queries=4, keys=4, heads=2, kv_heads=1, dim=64, dtype=_abi.BF16, scale=1.0, q=4096, k=8192, v=12288,
                  lam=16384, o=20480, o1=24576, o2=28672, lse=32768, dout=36864, dq=40960, dk=45056, dv=49152, dlam=53248,
@@ -53,3 +54,16 @@ def test_workspace_of_many_keys(B, T, H, K, d):
     tens of gigabytes.  What is left are the rows' statistics and their parts of dlam."""
     a = _abi.AttentionArgs(**{**ATTENTION, "batch": B, "queries": T, "keys": T, "heads": H, "kv_heads": K, "dim": d})
     assert _abi.lib().mmuon_attention_workspace(C.byref(a), 1) <= 20 * B * H * T + 4096
+
+
+@pytest.mark.parametrize("kw", [
+    dict(scaling="llama", fast=1.0), dict(scaling="llama", fast=4.0, slow=4.0), dict(scaling="llama", fast=1.0, slow=4.0),
+    dict(scaling="llama", slow=0.0), dict(scaling="llama", slow=math.nan), dict(scaling="yarn", fast=1.0, slow=1.0),
+    dict(scaling="yarn", fast=1.0, slow=32.0), dict(scaling="yarn", slow=0.0), dict(scaling="yarn", fast=math.nan),
+    dict(scaling="yarn", base=1.0), dict(scaling="yarn", base=0.5)])
+def test_a_ramp_over_no_turns_is_refused(kw):
+    """A ramp needs turns that it rises over (0 / 0 where a pair stands at both its ends), and one by pairs falling angles."""
+    with pytest.raises(ValueError, match="fast|base"):
+        rotary_table(64, 128, **{"factor": 2.0, "trained": 512, **kw})
+    if "base" not in kw:                       # who has no ramp takes no notice
+        assert not rotary_table(64, 128, **{"trained": 512, **kw, "scaling": None}).isnan().any()
