@@ -131,8 +131,8 @@ def rotary_table(dim: int, length: int, *, base: float = 10000.0, scaling: str |
         raise ValueError(f"scaling {scaling!r} needs the trained length")
     if scaling in ("yarn", "llama"):
         fast = {"yarn": 32.0, "llama": 4.0}[scaling] if fast is None else fast
-        if not 0 < slow < fast:
-            raise ValueError(f"scaling {scaling!r} needs 0 < slow < fast, not {slow} and {fast}")
+        if not (slow < fast if scaling == "llama" else 0 < slow <= fast):
+            raise ValueError(f"scaling {scaling!r} needs {'slow < fast' if scaling == 'llama' else '0 < slow <= fast'}, not {slow} and {fast}")
     if scaling == "yarn" and not base > 1:
         raise ValueError(f"scaling 'yarn' needs a base above 1, not {base}")
     i = torch.arange(0, dim, 2, dtype=torch.float64, device=device)

@@ -3,6 +3,7 @@ import ctypes as C
 import math
 
 import pytest
+import torch
 
 from monarch_muon_amd import _abi, rotary_table
 
@@ -58,12 +59,18 @@ def test_workspace_of_many_keys(B, T, H, K, d):
 
 @pytest.mark.parametrize("kw", [
     dict(scaling="llama", fast=1.0), dict(scaling="llama", fast=4.0, slow=4.0), dict(scaling="llama", fast=1.0, slow=4.0),
-    dict(scaling="llama", slow=0.0), dict(scaling="llama", slow=math.nan), dict(scaling="yarn", fast=1.0, slow=1.0),
-    dict(scaling="yarn", fast=1.0, slow=32.0), dict(scaling="yarn", slow=0.0), dict(scaling="yarn", fast=math.nan),
-    dict(scaling="yarn", base=1.0), dict(scaling="yarn", base=0.5)])
+    dict(scaling="llama", slow=math.nan), dict(scaling="yarn", fast=1.0, slow=32.0), dict(scaling="yarn", slow=0.0),
+    dict(scaling="yarn", fast=math.nan), dict(scaling="yarn", base=1.0), dict(scaling="yarn", base=0.5)])
 def test_a_ramp_over_no_turns_is_refused(kw):
     """A ramp needs turns that it rises over (0 / 0 where a pair stands at both its ends), and one by pairs falling angles."""
     with pytest.raises(ValueError, match="fast|base"):
         rotary_table(64, 128, **{"factor": 2.0, "trained": 512, **kw})
     if "base" not in kw:                       # who has no ramp takes no notice
         assert not rotary_table(64, 128, **{"trained": 512, **kw, "scaling": None}).isnan().any()
+
+
+@pytest.mark.parametrize("kw", [dict(scaling="llama", slow=0.0), dict(scaling="yarn", fast=1.0, slow=1.0)])
+def test_the_narrowest_ramps(kw):
+    """From no turn at all, and a step between one pair and the next."""
+    table = rotary_table(64, 128, factor=2.0, trained=512, **kw)
+    assert table.isfinite().all() and not torch.equal(table, rotary_table(64, 128))
