@@ -474,8 +474,8 @@ size_t mmuon_embedding_workspace(const mmuon_embedding_args* a);
      h = residual given ? x + residual rounded to dtype : x;
      y = h * inv * w,  inv = 1 / sqrt(mean of h^2 + eps), fp32, one rounding.
    With an 8-bit out_dtype, y is codes and scale: for each 128 columns (group 128) or the row
-   (group 0) scale = max |y| / (448 or 57344), 1 where that is 0, and code = y / scale to the
-   nearest even.
+   (group 0) scale = max |y| / (448 or 57344), 1 where that is no normal number (the codes are
+   then 0), and code = y / scale to the nearest even.
    Backward, from x (the forward's h), inv and dy:
      dx = inv w dy - h inv^3 mean(w dy h) + dh (of x and of residual alike; dh null: none);
      dw = sum over rows of dy h inv, fp32 in an order of the sizes alone, one rounding. */

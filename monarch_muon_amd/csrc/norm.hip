@@ -8,7 +8,7 @@
 // 16-B chunks each, so each input is read once and each output written once: bound by HBM.
 //
 // Output in 8 bits: a scale for each `group` columns (or the row), scale = max |y| / MAX (1 where
-// that is 0), code = y / scale to the nearest even; y goes from fp32 to its code in one rounding.
+// that is no normal number), code = y / scale to the nearest even; y goes from fp32 to its code in one rounding.
 #include <algorithm>
 #include <type_traits>
 

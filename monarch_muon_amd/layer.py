@@ -79,10 +79,12 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | 
 
     Without ``residual``, ``h`` is ``x`` and the result ``y``.  With it, ``h = x + residual`` rounded to their type, which
     is what the residual stream keeps, and the result is ``(y, h)``.  ``x`` (..., D) bfloat16 or float32 at any row
-    stride, D at most 32768 (bfloat16) or 16384; ``residual`` of its shape and type; ``weight`` (D) of its type or float32.
+    stride, D at most 32768 (bfloat16) or 16384, fewer than 2 ** 31 rows; ``residual`` of its shape and type; ``weight`` (D) of its
+    type or float32.
 
     Differentiable in all three; ``weight``'s gradient is the fp32 sum over the rows in an order that depends on the
-    sizes alone.  There is no second derivative.  A row with a NaN or an infinity has NaN in ``y``.
+    sizes alone.  There is no second derivative.  A row with a NaN or an infinity has NaN in ``y``; one whose squares' sum
+    is beyond float32 (magnitudes around 1e19) has zeros.
     """
     if _norm_op is None:
         _load()
@@ -95,7 +97,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tenso
     """``rms_norm`` with ``y`` in 8 bits: ``(codes, scale)``, or ``(codes, scale, h)`` with ``residual``.
 
     ``y ~ codes.float() * scale``, a float32 scale for each 128 columns, (..., ceil(D / 128)), or with ``group=None`` for the
-    row, (..., 1): the largest magnitude over 448 (``float8_e4m3fn``) or 57344 (``float8_e5m2``), 1 where that is zero.
+    row, (..., 1): the largest magnitude over 448 (``float8_e4m3fn``) or 57344 (``float8_e5m2``), 1 where that is zero or
+    below float32's normal numbers (the codes are then zeros).
     A code is ``y / scale`` rounded once, from fp32, to the nearest even.  It has no gradient: inputs that require one
     raise.
     """
@@ -176,7 +179,7 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     """``(softmax(q1 k1^T scale) - lam softmax(q2 k2^T scale)) v`` for each head, (B, T, H, 2 D) bfloat16.
 
     ``q`` (B, T, 2 H, D), ``k`` (B, S, 2 K, D) and ``v`` (B, S, K, 2 D) bfloat16 (cast under bf16 autocast) at any strides (copied
-    where rows of a head are no whole 16-byte chunks), D a multiple of 8 up to 128: query heads ``2 h`` and ``2 h + 1`` are head
+    where rows of a head are no whole 16-byte chunks or tokens stand 2 ** 22 elements apart), D a multiple of 8 up to 128: query heads ``2 h`` and ``2 h + 1`` are head
     ``h``'s two maps, key heads ``2 g`` and ``2 g + 1`` with value head ``g`` are shared by H / K heads.  ``lam``: one value or one for
     each head (taken as float32).  ``scale`` is ``D ** -0.5`` by default.
 
@@ -185,6 +188,9 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     sequence.  A query that sees no key has zeros and reaches nothing, whatever it holds; a key that no query sees has zeros
     for gradients.  Between a query and a later key that ``causal`` alone hides an infinity or a NaN may show as NaN: of the key
     or its value in the query's output and gradient, of the query or its output's gradient in the key's and the value's.
+
+    B H T is below 2 ** 29 and B K S below 2 ** 31 - 1024; with gradients B H T is at most 2 ** 28 - 16, B K S below 2 ** 30 and, for
+    T > 1, H D below 2 ** 21.
 
     Differentiable in ``q``, ``k``, ``v`` and ``lam``; every sum has an order that depends on the sizes alone, so gradients are
     the same bits every time.  Probabilities are rounded to bfloat16 before their products with the values, as are the

@@ -3,7 +3,7 @@ elements than 31 bits count, and more threads than one launch holds."""
 import pytest
 import torch
 
-from monarch_muon_amd import differential_attention, rotary, rotary_table
+from monarch_muon_amd import differential_attention, rms_norm, rms_norm_fp8, rotary, rotary_table
 from oracle import butterfly
 from oracle import layer as oracle
 from test_gpu_attention import check
@@ -278,3 +278,29 @@ def test_tokens_far_apart(apart, d):
     lam = torch.linspace(0.1, 0.9, H, device=DEV)
     check(q, k, v, lam)
     check(q[:, -3:], k, v, lam, lengths=torch.tensor([T - 1]), grads=False)
+
+
+# ----- norm: the ends of float32 -----------------------------------------------------
+def test_norm_where_squares_leave_float32():
+    """Sums of squares beyond float32: zeros, and beside them what there is; below it, eps alone counts."""
+    x, w = randn(4, 200, seed=81, dtype=torch.float32), randn(200, seed=82, dtype=torch.float32)
+    x[1] *= 1e20
+    x[2] *= 1e-30
+    y = rms_norm(x, w)
+    assert not y[1].any()
+    keep = [0, 2, 3]
+    ref, _, _, tol = oracle.norm(x[keep], w)
+    assert ((y[keep].double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("fmt", [torch.float8_e4m3fn, torch.float8_e5m2])
+@pytest.mark.parametrize("group", [128, None])
+def test_scales_below_the_normal_numbers(group, fmt):
+    most = torch.finfo(fmt).max * 2.0 ** -126              # the least of a group's largest that has a scale
+    x = torch.zeros(3, 256, device=DEV)
+    x[:, 0], x[:, 128] = 1.0, -1.0
+    inv = (128 ** -1 + 1e-6) ** -0.5                        # two ones of 256
+    for size, seen in ((4.0, True), (0.25, False)):
+        codes, scale = rms_norm_fp8(x, torch.full((256,), size * most / inv, device=DEV), dtype=fmt, group=group)
+        assert bool((codes.float() != 0).any()) == seen
+        assert (scale == 1).all() if not seen else (scale < 1e-36).all() and (codes.float()[:, 0] == torch.finfo(fmt).max).all()
