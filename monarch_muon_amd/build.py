@@ -35,8 +35,9 @@ CFLAGS = [
 ]
 
 
-# The kernel of dk and dv has 256 accumulators that only products touch and others that are read between products: with
-# products in VGPR form the former are moved to AGPRs once, and nothing is spilled (in AGPR form 19 registers).
+# The kernel of dk and dv with heads of over 64 columns has 256 accumulators that only products touch and others that are
+# read between products: with products in VGPR form the former are moved to AGPRs once and nothing is spilled (in AGPR form 192
+# registers, in parts 179).  With heads of 33 to 64 columns, two waves to a SIMD, it spills 14 (in parts 13) in either form.
 FLAGS_OF = {"attention_bwd": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 

@@ -46,7 +46,7 @@ __device__ __forceinline__ void store_lse(float* to, float shift, float sum) {
   *reinterpret_cast<float2*>(to) = make_float2(lse, sum == 0.f ? 1.f : __builtin_amdgcn_exp2f(lse - shift) / sum);
 }
 
-// MAPS: maps of a wave
+// MAPS: maps of a wave.  (Heads of over 64 columns, eight waves, keys in parts: 2 registers go to scratch.)
 template <int D, int TK, int WAVES, int MAPS, int SLOTS, bool SPLIT>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void attend(mmuon_attention_args a, int tiles, int splits, Dealing dealt, Parts parts) {
   constexpr int CA = D / 8, CB = D / 4, PANELS = D / 16;  // of the values: 2 D / 32

@@ -276,7 +276,9 @@ __global__ __launch_bounds__(256) void attention_dlam(mmuon_attention_args a, in
 }
 
 // dk and dv: 32 keys to a wave, over the query rows of the heads that share them, 32 at a time.  The
-// keys are operands in registers, the values, whose product comes once for both maps, in LDS.  The
+// keys are operands in registers, the values, whose product comes once for both maps, in LDS.  With heads of
+// 2 x 64 a lane has 14 registers too few for two waves to a SIMD, 60 B of scratch (16 x 1024 tokens, 8 heads: 20
+// of the 88 MB that are written); two waves are worth it (188 -> 128 us).  The
 // workgroups from `dlam_at` on sum dlam, a head each, which would take a launch of its own (5 to 8 us).
 template <int D, int WAVES, int SLOTS, bool SPLIT>
 __global__ __launch_bounds__(64 * WAVES, D == 128 ? 1 : 2) void attention_dkv(mmuon_attention_args a, Dealing dealt, int parts,
