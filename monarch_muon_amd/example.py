@@ -76,7 +76,8 @@ class TinyMonarchLM(torch.nn.Module):
         end = at + ids.shape[-1]
         if end > self.table.shape[0]:
             self.table = rotary_table(DIM, 2 * end, device=self.table.device)
-        x, stream = embedding(ids.reshape(-1, ids.shape[-1]), self.wte, scale=WIDTH ** 0.5, padding_idx=PAD), None
+        rows = ids.reshape(ids.shape[:-1].numel(), ids.shape[-1])
+        x, stream = embedding(rows, self.wte, scale=WIDTH ** 0.5, padding_idx=PAD), None
         for i, b in enumerate(self.blocks):
             x, stream = b(x, stream, self.table, None if caches is None else caches[i], at)
         return rms_norm(x, self.ln_f, residual=stream)[0].view(*ids.shape, WIDTH)

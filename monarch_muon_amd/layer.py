@@ -179,9 +179,9 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     """``(softmax(q1 k1^T scale) - lam softmax(q2 k2^T scale)) v`` for each head, (B, T, H, 2 D) bfloat16.
 
     ``q`` (B, T, 2 H, D), ``k`` (B, S, 2 K, D) and ``v`` (B, S, K, 2 D) bfloat16 (cast under bf16 autocast) at any strides (copied
-    where rows of a head are no whole 16-byte chunks or tokens stand 2 ** 22 elements apart), D a multiple of 8 up to 128: query heads ``2 h`` and ``2 h + 1`` are head
-    ``h``'s two maps, key heads ``2 g`` and ``2 g + 1`` with value head ``g`` are shared by H / K heads.  ``lam``: one value or one for
-    each head (taken as float32).  ``scale`` is ``D ** -0.5`` by default.
+    where rows of a head are no whole 16-byte chunks or tokens stand 2 ** 22 elements apart), D a multiple of 8 up to 128: query
+    heads ``2 h`` and ``2 h + 1`` are head ``h``'s two maps, key heads ``2 g`` and ``2 g + 1`` with value head ``g`` are shared by
+    H / K heads.  ``lam``: one value or one for each head (taken as float32).  ``scale`` is ``D ** -0.5`` by default.
 
     ``lengths`` (B): the keys of each sequence that count; those behind are not read (a cache).  ``causal``: query ``t`` of
     sequence ``b`` sees keys up to ``starts[b] + t``, by default ``lengths[b] - T + t``: the queries are the last ones of their

@@ -154,6 +154,8 @@ def test_the_example_takes_ids_of_any_shape():
         h = model.hidden(ids)
         assert h.shape == (*ids.shape, example.WIDTH)
         assert torch.equal(model.hidden(ids.view(2, 4, -1)), h.view(2, 4, *h.shape[1:]))
+        for none in (ids[:, :0], ids[:0], ids[0, :0]):
+            assert model.hidden(none).shape == (*none.shape, example.WIDTH)
         one = model.hidden(ids[0])
         assert one.shape == h[0].shape
         # (one sequence's products are split otherwise than eight's)
